@@ -1,0 +1,243 @@
+// Host side of include/bz_long_cache.h's attention: argument checks, workspace layout, split counts, launches. The device
+// code is in long_cache.cuh.
+#include <hip/hip_runtime.h>
+
+#include <stdint.h>
+
+#include "bz_long_cache.h"
+#include "long_cache.cuh"
+
+namespace bz {
+int device_cu_count(int* cus);  // gqa_decode.hip
+}
+
+namespace {
+
+constexpr int kKv4Tokens = 16;  // most query tokens per row over a 4-bit cache
+
+bool dim_ok(int D) { return D == 64 || D == 128; }
+bool group_ok(int G) { return G == 1 || G == 2 || G == 4 || G == 8; }
+size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+// What a call's sizes determine: the column tiles, the splits and where things lie in the workspace (its arrival
+// counters first, one 256-byte line per (row, column tile, kv head); they are zero between calls, everything else is
+// written before it is read).
+struct Plan {
+  int G, gshift, tpt, tiles, splits, min_tiles, one_split, score_stride;
+  int64_t units;
+  size_t ml, acc, head_ml, scores, total;
+};
+
+int make_plan(int kind, int B, int NH, int NKV, int D, int cap, int T, int window, int sinks, int num_splits, int max_seq_len,
+              Plan* pl) {
+  if (B <= 0 || NH <= 0 || NKV <= 0 || cap <= 0 || T <= 0 || NH % NKV != 0 || window < 0 || sinks < 0) return BZ_ERR_SHAPE;
+  if (num_splits < 0 || num_splits > kMaxSplits) return BZ_ERR_SHAPE;
+  if (!dim_ok(D) || !group_ok(NH / NKV)) return BZ_ERR_UNSUPPORTED;
+  if (kind == BZ_LONG_KV4 && T > kKv4Tokens) return BZ_ERR_UNSUPPORTED;
+  if (kind == BZ_LONG_TRACKED && T != 1) return BZ_ERR_UNSUPPORTED;
+  const bool kv4 = kind == BZ_LONG_KV4;
+  pl->G = NH / NKV;
+  pl->gshift = __builtin_ctz(pl->G);
+  pl->tpt = kLongCols / pl->G < T ? kLongCols / pl->G : T;
+  pl->tiles = (T + pl->tpt - 1) / pl->tpt;
+  if ((int64_t)B * pl->tiles > 65535 || NKV > 65535) return BZ_ERR_SHAPE;  // grid limits
+  pl->units = (int64_t)B * pl->tiles * NKV;
+
+  // positions a column tile attends, in wave tiles
+  int64_t len = max_seq_len > 0 && max_seq_len < cap ? max_seq_len : cap;
+  if (window > 0 && (int64_t)window + pl->tpt + sinks < len) len = (int64_t)window + pl->tpt + sinks;
+  const int P = kv4 ? 32 : 16;
+  const int n = (int)((len + P - 1) / P) + 1;
+  pl->min_tiles = kLongWaves;
+  pl->one_split = (kOneSplitBytes / (kv4 ? D + D / 16 : 4 * D)) / P;
+  int splits = num_splits;
+  if (splits == 0) {
+    int cus = 0;
+    const int rc = bz::device_cu_count(&cus);
+    if (rc != BZ_OK) return rc;
+    splits = (int)(2 * cus / pl->units);
+    const int most = (n + pl->min_tiles - 1) / pl->min_tiles;
+    if (splits > most) splits = most;
+    if (splits > 64) splits = 64;
+    if (n <= pl->one_split || splits < 1) splits = 1;
+  }
+  pl->splits = splits;
+
+  const size_t cols = (size_t)pl->units * splits * pl->tpt * pl->G;
+  const bool merged = splits > 1;
+  pl->ml = merged ? (size_t)pl->units * kCounterStride * sizeof(int) : 0;
+  pl->acc = up256(pl->ml + (merged ? cols * sizeof(float2) : 0));
+  pl->head_ml = up256(pl->acc + (merged ? cols * D * sizeof(float) : 0));
+  pl->total = pl->head_ml;
+  pl->scores = 0;
+  pl->score_stride = 0;
+  if (kind == BZ_LONG_TRACKED) {
+    const int64_t longest = cap;  // rows may be longer than max_seq_len, which only steers the tiling
+    pl->score_stride = (int)((longest + 31) & ~(int64_t)31);
+    pl->scores = up256(pl->head_ml + (size_t)B * NH * sizeof(float2));
+    pl->total = up256(pl->scores + (size_t)B * NH * pl->score_stride * sizeof(float));
+  }
+  return BZ_OK;
+}
+
+int check_base(const bz_gqa_decode_args* a) {
+  if (a->q == nullptr || a->k_cache == nullptr || a->v_cache == nullptr || a->out == nullptr || a->seq_lens == nullptr)
+    return BZ_ERR_NULL;
+  if (a->mask != nullptr || a->mask_dtype != BZ_MASK_NONE) return BZ_ERR_UNSUPPORTED;
+  if (a->tokens_per_row < 0) return BZ_ERR_SHAPE;
+  if ((reinterpret_cast<uintptr_t>(a->q) & 15) || ((a->q_stride_b | a->q_stride_h) & 7) ||
+      (a->tokens_per_row > 1 && (a->q_stride_t & 7)))
+    return BZ_ERR_ALIGNMENT;
+  if ((reinterpret_cast<uintptr_t>(a->out) & 1) || (reinterpret_cast<uintptr_t>(a->seq_lens) & 3) ||
+      (reinterpret_cast<uintptr_t>(a->kv_start) & 3))
+    return BZ_ERR_ALIGNMENT;
+  return BZ_OK;
+}
+
+int check_bf16_cache(const bz_gqa_decode_args* a) {
+  if ((reinterpret_cast<uintptr_t>(a->k_cache) | reinterpret_cast<uintptr_t>(a->v_cache)) & 15) return BZ_ERR_ALIGNMENT;
+  if ((a->kv_stride_b | a->kv_stride_h | a->kv_stride_s) & 7) return BZ_ERR_ALIGNMENT;
+  if (a->kv_stride_s < a->head_dim) return BZ_ERR_SHAPE;
+  if (((int64_t)a->capacity + 1024) * a->kv_stride_s * 2 > INT32_MAX) return BZ_ERR_SHAPE;  // 32-bit byte offsets
+  return BZ_OK;
+}
+
+int check_kv4_cache(const bz_kv4_cache* c) {
+  if (c->k == nullptr || c->v == nullptr || c->k_scale == nullptr || c->v_scale == nullptr) return BZ_ERR_NULL;
+  if (c->batch <= 0 || c->num_kv_heads <= 0 || c->capacity <= 0) return BZ_ERR_SHAPE;
+  if (!dim_ok(c->head_dim)) return BZ_ERR_UNSUPPORTED;
+  const int D = c->head_dim, code_align = D / 8 - 1, scale_align = D / 32 - 1;
+  if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & code_align) return BZ_ERR_ALIGNMENT;
+  if ((c->stride_b | c->stride_h | c->stride_s) & code_align) return BZ_ERR_ALIGNMENT;
+  if ((reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale) | (uintptr_t)c->scale_stride_b |
+       (uintptr_t)c->scale_stride_h) &
+      scale_align)
+    return BZ_ERR_ALIGNMENT;
+  if (c->stride_s < D / 2) return BZ_ERR_SHAPE;
+  if (((int64_t)c->capacity + 1024) * c->stride_s > INT32_MAX) return BZ_ERR_SHAPE;
+  return BZ_OK;
+}
+
+int check_workspace(const bz_gqa_decode_args* a, const Plan& pl) {
+  if (pl.total == 0) return BZ_OK;
+  if (a->workspace == nullptr || a->workspace_bytes < pl.total) return BZ_ERR_WORKSPACE;
+  return (reinterpret_cast<uintptr_t>(a->workspace) & 255) ? BZ_ERR_ALIGNMENT : BZ_OK;
+}
+
+LongParams long_params(const bz_gqa_decode_args* a, const Plan& pl, int window, int sinks) {
+  LongParams p{};
+  p.q = static_cast<const uint16_t*>(a->q);
+  p.q_sb = a->q_stride_b, p.q_sh = a->q_stride_h, p.q_st = a->q_stride_t;
+  p.k = static_cast<const char*>(a->k_cache);
+  p.v = static_cast<const char*>(a->v_cache);
+  p.kv_sb = 2 * a->kv_stride_b, p.kv_sh = 2 * a->kv_stride_h, p.kv_ss = 2 * a->kv_stride_s;
+  p.window = window > 0 ? window : INT32_MAX;
+  p.sinks = sinks;
+  p.scale_log2 = a->scale * kLog2e;
+  p.out = static_cast<uint16_t*>(a->out);
+  p.o_sb = a->out_stride_b, p.o_sh = a->out_stride_h, p.o_st = a->out_stride_t;
+  p.NKV = a->num_kv_heads, p.G = pl.G, p.gshift = pl.gshift, p.T = a->tokens_per_row > 1 ? a->tokens_per_row : 1;
+  p.cap = a->capacity;
+  p.tiles = pl.tiles, p.tpt = pl.tpt;
+  p.splits = pl.splits, p.min_tiles = pl.min_tiles, p.one_split = pl.one_split;
+  char* const ws = static_cast<char*>(a->workspace);
+  p.counters = reinterpret_cast<int*>(ws);
+  p.part_ml = reinterpret_cast<float2*>(ws + pl.ml);
+  p.part_acc = reinterpret_cast<float*>(ws + pl.acc);
+  p.head_ml = reinterpret_cast<float2*>(ws + pl.head_ml);
+  p.scores = reinterpret_cast<float*>(ws + pl.scores);
+  p.score_stride = pl.score_stride;
+  return p;
+}
+
+template <bool KV4, bool TRACK>
+int launch_split(const bz_gqa_decode_args* a, int D, const LongParams& p, const Plan& pl, int B, hipStream_t stream) {
+  const dim3 grid(pl.splits, p.NKV, B * pl.tiles);
+  if (D == 128)
+    hipLaunchKernelGGL((long_split_kernel<128, KV4, TRACK>), grid, dim3(kLongThreads), 0, stream, a->seq_lens, a->kv_start, p);
+  else
+    hipLaunchKernelGGL((long_split_kernel<64, KV4, TRACK>), grid, dim3(kLongThreads), 0, stream, a->seq_lens, a->kv_start, p);
+  return hipGetLastError() == hipSuccess ? BZ_OK : BZ_ERR_LAUNCH;
+}
+
+int tokens_in(const bz_gqa_decode_args* a) { return a->tokens_per_row > 1 ? a->tokens_per_row : 1; }
+
+}  // namespace
+
+#define BZ_EXPORT __attribute__((visibility("default")))
+
+extern "C" {
+
+BZ_EXPORT int bz_long_workspace_size(int32_t kind, int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                     int32_t capacity, int32_t tokens_per_row, int32_t window, int32_t sinks,
+                                     int32_t num_splits, int32_t max_seq_len, size_t* bytes) {
+  if (bytes == nullptr) return BZ_ERR_NULL;
+  if (kind < BZ_LONG_WINDOW || kind > BZ_LONG_TRACKED) return BZ_ERR_SHAPE;
+  Plan pl;
+  const int rc = make_plan(kind, batch, num_q_heads, num_kv_heads, head_dim, capacity, tokens_per_row > 1 ? tokens_per_row : 1,
+                           window, sinks, num_splits, max_seq_len, &pl);
+  if (rc != BZ_OK) return rc;
+  *bytes = pl.total;
+  return BZ_OK;
+}
+
+BZ_EXPORT int bz_gqa_window(const bz_gqa_window_args* wa, hipStream_t stream) {
+  if (wa == nullptr) return BZ_ERR_NULL;
+  const bz_gqa_decode_args* a = &wa->base;
+  int rc = check_base(a);
+  if (rc != BZ_OK) return rc;
+  Plan pl;
+  rc = make_plan(BZ_LONG_WINDOW, a->batch, a->num_q_heads, a->num_kv_heads, a->head_dim, a->capacity, tokens_in(a), wa->window,
+                 wa->sinks, a->num_splits, a->max_seq_len, &pl);
+  if (rc == BZ_OK) rc = check_bf16_cache(a);
+  if (rc == BZ_OK) rc = check_workspace(a, pl);
+  if (rc != BZ_OK) return rc;
+  return launch_split<false, false>(a, a->head_dim, long_params(a, pl, wa->window, wa->sinks), pl, a->batch, stream);
+}
+
+BZ_EXPORT int bz_gqa_decode_kv4(const bz_gqa_kv4_args* ka, hipStream_t stream) {
+  if (ka == nullptr) return BZ_ERR_NULL;
+  bz_gqa_decode_args a = ka->base;
+  const bz_kv4_cache* c = &ka->cache;
+  int rc = check_kv4_cache(c);
+  if (rc != BZ_OK) return rc;
+  a.k_cache = c->k, a.v_cache = c->v;
+  a.batch = c->batch, a.num_kv_heads = c->num_kv_heads, a.capacity = c->capacity, a.head_dim = c->head_dim;
+  rc = check_base(&a);
+  if (rc != BZ_OK) return rc;
+  Plan pl;
+  rc = make_plan(BZ_LONG_KV4, a.batch, a.num_q_heads, a.num_kv_heads, a.head_dim, a.capacity, tokens_in(&a), ka->window,
+                 ka->sinks, a.num_splits, a.max_seq_len, &pl);
+  if (rc == BZ_OK) rc = check_workspace(&a, pl);
+  if (rc != BZ_OK) return rc;
+  LongParams p = long_params(&a, pl, ka->window, ka->sinks);
+  p.kv_sb = c->stride_b, p.kv_sh = c->stride_h, p.kv_ss = c->stride_s;
+  p.k_scale = static_cast<const uint8_t*>(c->k_scale);
+  p.v_scale = static_cast<const uint8_t*>(c->v_scale);
+  p.sc_sb = c->scale_stride_b, p.sc_sh = c->scale_stride_h;
+  return launch_split<true, false>(&a, a.head_dim, p, pl, a.batch, stream);
+}
+
+BZ_EXPORT int bz_gqa_decode_tracked(const bz_gqa_tracked_args* ta, hipStream_t stream) {
+  if (ta == nullptr) return BZ_ERR_NULL;
+  const bz_gqa_decode_args* a = &ta->base;
+  int rc = check_base(a);
+  if (rc != BZ_OK) return rc;
+  if (ta->weights == nullptr || ta->weights_out == nullptr) return BZ_ERR_NULL;
+  if ((reinterpret_cast<uintptr_t>(ta->weights) | reinterpret_cast<uintptr_t>(ta->weights_out)) & 3) return BZ_ERR_ALIGNMENT;
+  Plan pl;
+  rc = make_plan(BZ_LONG_TRACKED, a->batch, a->num_q_heads, a->num_kv_heads, a->head_dim, a->capacity, tokens_in(a), 0, 0,
+                 a->num_splits, a->max_seq_len, &pl);
+  if (rc == BZ_OK) rc = check_bf16_cache(a);
+  if (rc == BZ_OK) rc = check_workspace(a, pl);
+  if (rc != BZ_OK) return rc;
+  const LongParams p = long_params(a, pl, 0, 0);
+  rc = launch_split<false, true>(a, a->head_dim, p, pl, a->batch, stream);
+  if (rc != BZ_OK) return rc;
+  const dim3 grid((a->capacity + 4 * kLongThreads - 1) / (4 * kLongThreads), a->num_kv_heads, a->batch);
+  hipLaunchKernelGGL(track_apply_kernel, grid, dim3(kLongThreads), 0, stream, a->seq_lens, a->kv_start, ta->weights,
+                     ta->weights_out, ta->w_stride_b, ta->w_stride_h, ta->wo_stride_b, ta->wo_stride_h, ta->decay, p);
+  return hipGetLastError() == hipSuccess ? BZ_OK : BZ_ERR_LAUNCH;
+}
+
+}  // extern "C"

@@ -23,8 +23,9 @@ REPO_DIR = PKG_DIR.parent
 INCLUDE = REPO_DIR / "include"
 LIB_NAME = "libbz_gqa_decode.so"
 LIB_PATH = PKG_DIR / LIB_NAME
-SOURCES = ["gqa_decode.hip", "gqa_fused.hip", "gemv.hip"]  # translation units, compiled in parallel
-HEADERS = ["gqa_kernels.cuh", "gqa_wave.cuh", "device_common.cuh"]
+SOURCES = ["gqa_decode.hip", "gqa_fused.hip", "gemv.hip", "long_cache.hip", "kv4_store.hip",
+           "kv_evict.hip"]  # translation units, compiled in parallel
+HEADERS = ["gqa_kernels.cuh", "gqa_wave.cuh", "device_common.cuh", "long_cache.cuh"]
 ARCH = "gfx950"
 # -packed-fp32-ops: keep hipcc from emitting packed fp32 VALU ops (v_pk_*_f32)
 # -falign-loops=64: loop heads on 64-byte boundaries (instruction fetch); the split kernels measured 1-4% faster with
@@ -38,14 +39,15 @@ HIPCC_FLAGS = [
     "-mllvm", "-amdgpu-kernarg-preload-count=14",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
-ABI_VERSION = 9
+ABI_VERSION = 10
 
-# exported symbols and their ctypes signatures (include/bz_gqa_decode.h)
+# exported symbols and their ctypes signatures (include/*.h)
 EXPORTS = (
     "bz_gqa_decode", "bz_gqa_decode_masked", "bz_gqa_decode_fused", "bz_gqa_decode_workspace_size",
     "bz_gqa_decode_default_splits", "bz_status_string", "bz_gqa_decode_abi_version", "bz_gemv", "bz_rmsnorm",
     "bz_mask_interval", "bz_gqa_decode_wave", "bz_gqa_decode_build_id", "bz_gqa_decode_noalloc",
-    "bz_gqa_decode_probs", "bz_gqa_decode_fused_probs",
+    "bz_gqa_decode_probs", "bz_gqa_decode_fused_probs", "bz_gqa_window", "bz_gqa_decode_kv4", "bz_gqa_decode_tracked",
+    "bz_long_workspace_size", "bz_kv4_store", "bz_kv4_load", "bz_kv_select", "bz_kv_compact",
 )
 
 
@@ -109,6 +111,64 @@ class GemvArgs(ctypes.Structure):
         ("y", ctypes.c_void_p), ("y_stride", ctypes.c_int64),
         ("m", ctypes.c_int32), ("k", ctypes.c_int32), ("epilogue", ctypes.c_int32),
     ]
+
+
+class GqaWindowArgs(ctypes.Structure):
+    """Mirror of struct bz_gqa_window_args (include/bz_long_cache.h)."""
+    _fields_ = [("base", GqaDecodeArgs), ("window", ctypes.c_int32), ("sinks", ctypes.c_int32)]
+
+
+class Kv4CacheArgs(ctypes.Structure):
+    """Mirror of struct bz_kv4_cache."""
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("stride_b", ctypes.c_int64), ("stride_h", ctypes.c_int64), ("stride_s", ctypes.c_int64),
+        ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+        ("scale_stride_b", ctypes.c_int64), ("scale_stride_h", ctypes.c_int64),
+        ("batch", ctypes.c_int32), ("num_kv_heads", ctypes.c_int32), ("capacity", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+    ]
+
+
+class GqaKv4Args(ctypes.Structure):
+    """Mirror of struct bz_gqa_kv4_args."""
+    _fields_ = [("base", GqaDecodeArgs), ("cache", Kv4CacheArgs), ("window", ctypes.c_int32), ("sinks", ctypes.c_int32)]
+
+
+class GqaTrackedArgs(ctypes.Structure):
+    """Mirror of struct bz_gqa_tracked_args."""
+    _fields_ = [
+        ("base", GqaDecodeArgs),
+        ("weights", ctypes.c_void_p), ("w_stride_b", ctypes.c_int64), ("w_stride_h", ctypes.c_int64),
+        ("weights_out", ctypes.c_void_p), ("wo_stride_b", ctypes.c_int64), ("wo_stride_h", ctypes.c_int64),
+        ("decay", ctypes.c_float),
+    ]
+
+
+class KvSelectArgs(ctypes.Structure):
+    """Mirror of struct bz_kv_select_args."""
+    _fields_ = [
+        ("weights", ctypes.c_void_p), ("w_stride_b", ctypes.c_int64), ("w_stride_h", ctypes.c_int64),
+        ("seq_lens", ctypes.c_void_p), ("kv_start", ctypes.c_void_p), ("index", ctypes.c_void_p),
+        ("lens", ctypes.c_void_p),
+        ("weights_out", ctypes.c_void_p), ("wo_stride_b", ctypes.c_int64), ("wo_stride_h", ctypes.c_int64),
+        ("batch", ctypes.c_int32), ("num_kv_heads", ctypes.c_int32), ("capacity", ctypes.c_int32),
+        ("keep", ctypes.c_int32), ("sinks", ctypes.c_int32), ("recent", ctypes.c_int32),
+    ]
+
+
+class KvTensor(ctypes.Structure):
+    """Mirror of struct bz_kv_tensor."""
+    _fields_ = [
+        ("src", ctypes.c_void_p), ("dst", ctypes.c_void_p),
+        ("src_stride_b", ctypes.c_int64), ("src_stride_h", ctypes.c_int64), ("src_stride_s", ctypes.c_int64),
+        ("dst_stride_b", ctypes.c_int64), ("dst_stride_h", ctypes.c_int64), ("dst_stride_s", ctypes.c_int64),
+        ("row_bytes", ctypes.c_int32),
+    ]
+
+
+KV_TENSORS = 4  # BZ_KV_TENSORS
+LONG_WINDOW, LONG_KV4, LONG_TRACKED = 0, 1, 2
 
 
 _LOCK = threading.Lock()
@@ -239,6 +299,20 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.bz_gqa_decode_probs.restype = ctypes.c_int
     lib.bz_gqa_decode_fused_probs.argtypes = [P(GqaDecodeFusedArgs), ctypes.c_void_p, ctypes.c_void_p]
     lib.bz_gqa_decode_fused_probs.restype = ctypes.c_int
+    lib.bz_gqa_window.argtypes = [P(GqaWindowArgs), ctypes.c_void_p]
+    lib.bz_gqa_decode_kv4.argtypes = [P(GqaKv4Args), ctypes.c_void_p]
+    lib.bz_gqa_decode_tracked.argtypes = [P(GqaTrackedArgs), ctypes.c_void_p]
+    lib.bz_long_workspace_size.argtypes = [ctypes.c_int32] * 11 + [P(ctypes.c_size_t)]
+    lib.bz_kv4_store.argtypes = [ctypes.c_void_p] * 2 + [ctypes.c_int64] * 3 + [
+        ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, P(Kv4CacheArgs), ctypes.c_void_p]
+    lib.bz_kv4_load.argtypes = [P(Kv4CacheArgs), ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p] + [
+        ctypes.c_int64] * 3 + [ctypes.c_void_p]
+    lib.bz_kv_select.argtypes = [P(KvSelectArgs), ctypes.c_void_p]
+    lib.bz_kv_compact.argtypes = [P(KvTensor), ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p] + [
+        ctypes.c_int32] * 4 + [ctypes.c_void_p]
+    for name in ("bz_gqa_window", "bz_gqa_decode_kv4", "bz_gqa_decode_tracked", "bz_long_workspace_size", "bz_kv4_store",
+                 "bz_kv4_load", "bz_kv_select", "bz_kv_compact"):
+        getattr(lib, name).restype = ctypes.c_int
     lib.bz_gqa_decode_build_id.argtypes = []
     lib.bz_gqa_decode_build_id.restype = ctypes.c_char_p
 

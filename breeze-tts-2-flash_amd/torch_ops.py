@@ -22,7 +22,7 @@ from __future__ import annotations
 
 import torch
 
-from . import attention, gemv
+from . import attention, gemv, long_cache
 
 _LIB = torch.library.Library("bz", "DEF")  # kept alive for the process: dropping it would unregister the ops
 
@@ -44,6 +44,20 @@ _SCHEMAS = {
     "gemv_resid": "(Tensor x, Tensor W, Tensor res, Tensor(a!) y) -> ()",
     "gemv_gateup": "(Tensor x, Tensor nw, float eps, Tensor Wg, Tensor Wu, Tensor(a!) y) -> ()",
     "rmsnorm": "(Tensor x, Tensor w, float eps, Tensor(a!) y) -> ()",
+    "gqa_window": "(Tensor q, Tensor k_cache, Tensor v_cache, Tensor seq_lens, float scale, SymInt window, Tensor(a!) out, "
+                  "SymInt sinks, Tensor? kv_start, SymInt num_splits, SymInt max_seq_len, Tensor(b!)? workspace) -> ()",
+    "kv4_store": "(Tensor k, Tensor v, Tensor(a!) ck, Tensor(b!) cv, Tensor(c!) k_scale, Tensor(d!) v_scale, Tensor slots, "
+                 "Tensor? counts) -> ()",
+    "kv4_load": "(Tensor ck, Tensor cv, Tensor k_scale, Tensor v_scale, Tensor slots, Tensor(a!) k, Tensor(b!) v) -> ()",
+    "gqa_decode_kv4": "(Tensor q, Tensor ck, Tensor cv, Tensor k_scale, Tensor v_scale, Tensor seq_lens, float scale, "
+                      "Tensor(a!) out, Tensor? kv_start, SymInt window, SymInt sinks, SymInt num_splits, SymInt max_seq_len, "
+                      "Tensor(b!)? workspace) -> ()",
+    "gqa_decode_tracked": "(Tensor q, Tensor k_cache, Tensor v_cache, Tensor seq_lens, float scale, Tensor weights, "
+                          "Tensor(a!) out, float decay, Tensor(b!) weights_out, Tensor? kv_start, SymInt num_splits, "
+                          "SymInt max_seq_len, Tensor(c!)? workspace) -> ()",
+    "kv_select": "(Tensor weights, Tensor seq_lens, SymInt keep, SymInt sinks, SymInt recent, Tensor? kv_start, "
+                 "Tensor(a!) index, Tensor(b!) lens, Tensor(c!)? weights_out) -> ()",
+    "kv_compact": "(Tensor[] tensors, Tensor index, Tensor lens, Tensor(a!)[] outs) -> ()",
 }
 
 
@@ -88,6 +102,39 @@ def _rmsnorm(x, w, eps, y):
     gemv._rmsnorm(x, w, eps, y)
 
 
+def _gqa_window(q, k_cache, v_cache, seq_lens, scale, window, out, sinks, kv_start, num_splits, max_seq_len, workspace):
+    long_cache._gqa_window(q, k_cache, v_cache, seq_lens, scale, window, out, sinks, kv_start, num_splits, max_seq_len,
+                           workspace)
+
+
+def _kv4_store(k, v, ck, cv, k_scale, v_scale, slots, counts):
+    long_cache._kv4_store(k, v, long_cache.Kv4Cache(ck, cv, k_scale, v_scale), slots, counts)
+
+
+def _kv4_load(ck, cv, k_scale, v_scale, slots, k, v):
+    long_cache._kv4_load(long_cache.Kv4Cache(ck, cv, k_scale, v_scale), slots, k, v)
+
+
+def _gqa_decode_kv4(q, ck, cv, k_scale, v_scale, seq_lens, scale, out, kv_start, window, sinks, num_splits, max_seq_len,
+                    workspace):
+    long_cache._gqa_decode_kv4(q, long_cache.Kv4Cache(ck, cv, k_scale, v_scale), seq_lens, scale, out, kv_start, window, sinks,
+                               num_splits, max_seq_len, workspace)
+
+
+def _gqa_decode_tracked(q, k_cache, v_cache, seq_lens, scale, weights, out, decay, weights_out, kv_start, num_splits,
+                        max_seq_len, workspace):
+    long_cache._gqa_decode_tracked(q, k_cache, v_cache, seq_lens, scale, weights, out, decay, weights_out, kv_start,
+                                   num_splits, max_seq_len, workspace)
+
+
+def _kv_select(weights, seq_lens, keep, sinks, recent, kv_start, index, lens, weights_out):
+    long_cache._kv_select(weights, seq_lens, keep, sinks, recent, kv_start, index, lens, weights_out)
+
+
+def _kv_compact(tensors, index, lens, outs):
+    long_cache._kv_compact(tensors, index, lens, outs)
+
+
 _KERNELS = {
     "gqa_decode": _gqa_decode,
     "gqa_decode_wave": _gqa_decode_wave,
@@ -98,6 +145,13 @@ _KERNELS = {
     "gemv_resid": _gemv_resid,
     "gemv_gateup": _gemv_gateup,
     "rmsnorm": _rmsnorm,
+    "gqa_window": _gqa_window,
+    "kv4_store": _kv4_store,
+    "kv4_load": _kv4_load,
+    "gqa_decode_kv4": _gqa_decode_kv4,
+    "gqa_decode_tracked": _gqa_decode_tracked,
+    "kv_select": _kv_select,
+    "kv_compact": _kv_compact,
 }
 
 

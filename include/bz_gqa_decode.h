@@ -35,7 +35,7 @@
 extern "C" {
 #endif
 
-#define BZ_GQA_DECODE_ABI_VERSION 9
+#define BZ_GQA_DECODE_ABI_VERSION 10
 
 typedef enum bz_status {
   BZ_OK = 0,
