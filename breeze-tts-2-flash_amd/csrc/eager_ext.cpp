@@ -7,6 +7,8 @@
 // registers it here and launches. Every attention check and error message is the Python path's, so both raise the
 // same RuntimeError for the same arguments. The GEMVs need no workspace and go through this module alone.
 //
+// The long-cache operators (eager_long.hpp) go through it alone as well; Python only makes their workspaces.
+//
 // The C ABI functions come as addresses (bind), taken from the library the package has already loaded and checked,
 // so this module never loads a second copy of it. Host code only: compiled with g++ against torch's headers.
 #include <Python.h>
@@ -17,6 +19,7 @@
 #include <hip/hip_runtime_api.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cmath>
 #include <map>
 #include <string>
@@ -628,6 +631,12 @@ PyObject* register_workspace(PyObject*, PyObject* args) {
   Py_RETURN_NONE;
 }
 
+}  // namespace
+
+#include "eager_long.hpp"
+
+namespace {
+
 PyObject* build_id(PyObject*, PyObject*) { return PyUnicode_FromString(BZ_EAGER_BUILD_ID); }
 
 PyMethodDef kMethods[] = {
@@ -642,13 +651,31 @@ PyMethodDef kMethods[] = {
      "gemv_seg / gemv_resid / gemv_gateup through the C ABI"},
     {"rmsnorm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(rmsnorm)), METH_FASTCALL,
      "rmsnorm through the C ABI"},
+    {"window", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(window)), METH_FASTCALL,
+     "gqa_window through the C ABI"},
+    {"kv4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(kv4)), METH_FASTCALL,
+     "gqa_decode_kv4 through the C ABI"},
+    {"tracked", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(tracked)), METH_FASTCALL,
+     "gqa_decode_tracked through the C ABI"},
+    {"kv4_store", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(kv4_store)), METH_FASTCALL,
+     "kv4_store through the C ABI"},
+    {"kv4_load", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(kv4_load)), METH_FASTCALL,
+     "kv4_load through the C ABI"},
+    {"select", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(select)), METH_FASTCALL,
+     "kv_select through the C ABI"},
+    {"compact", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(compact)), METH_FASTCALL,
+     "kv_compact through the C ABI"},
+    {"evict", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(evict)), METH_FASTCALL,
+     "kv_evict through the C ABI"},
     {"bind", bind, METH_VARARGS, "the C ABI functions' addresses"},
+    {"bind_long", bind_long, METH_VARARGS, "the long-cache functions' addresses"},
+    {"register_long_workspace", register_long_workspace, METH_VARARGS, "a workspace made for a long-cache call's key"},
     {"register_workspace", register_workspace, METH_VARARGS, "a workspace made for (device, stream, groups)"},
     {"build_id", build_id, METH_NOARGS, "hash of the sources this module was built from"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_bz_eager",
-                       "native eager binding of the decode-attention entries and the backbone GEMVs", -1, kMethods};
+                       "native eager binding of the decode-attention and long-cache entries and the backbone GEMVs", -1, kMethods};
 
 }  // namespace
 

@@ -199,7 +199,7 @@ STAMP_PATH = PKG_DIR / "libbz_bench_stamp.so"  # bench.py's GPU timestamp kernel
 
 # The native eager binding (csrc/eager_ext.cpp): a CPython extension module built with g++ against torch's headers,
 # host code only, which calls the C ABI functions of the loaded library (eager()).
-EAGER_SOURCE = "eager_ext.cpp"
+EAGER_SOURCE, EAGER_HEADER = "eager_ext.cpp", "eager_long.hpp"
 EAGER_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM"]
 
 
@@ -210,9 +210,9 @@ def eager_path() -> Path:
 
 
 def eager_id() -> str:
-    """Hash of what the eager module is built from: its source, the C ABI headers and its flags."""
+    """Hash of what the eager module is built from: its sources, the C ABI headers and its flags."""
     h = hashlib.sha256()
-    for f in [CSRC / EAGER_SOURCE] + sorted(INCLUDE.glob("*.h")):
+    for f in [CSRC / EAGER_SOURCE, CSRC / EAGER_HEADER] + sorted(INCLUDE.glob("*.h")):
         h.update(f.name.encode() + b"\0" + f.read_bytes() + b"\0")
     h.update(" ".join(EAGER_FLAGS).encode())
     return h.hexdigest()[:16]
@@ -373,6 +373,9 @@ def eager():
     mod.bind(addr(lib.bz_gqa_decode), addr(lib.bz_gqa_decode_masked), addr(lib.bz_gqa_decode_noalloc),
              addr(lib.bz_gqa_decode_fused), addr(lib.bz_status_string), addr(lib.bz_gqa_decode_workspace_size),
              addr(lib.bz_gemv), addr(lib.bz_rmsnorm))
+    mod.bind_long(addr(lib.bz_gqa_window), addr(lib.bz_gqa_decode_kv4), addr(lib.bz_gqa_decode_tracked),
+                  addr(lib.bz_long_workspace_size), addr(lib.bz_kv4_store), addr(lib.bz_kv4_load), addr(lib.bz_kv_select),
+                  addr(lib.bz_kv_compact))
     with _LOCK:
         if _EAGER is None:
             _EAGER = mod

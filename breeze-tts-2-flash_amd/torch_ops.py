@@ -22,7 +22,7 @@ from __future__ import annotations
 
 import torch
 
-from . import attention, gemv, long_cache
+from . import attention, gemv, kernels, long_cache
 
 _LIB = torch.library.Library("bz", "DEF")  # kept alive for the process: dropping it would unregister the ops
 
@@ -48,7 +48,8 @@ _SCHEMAS = {
                   "SymInt sinks, Tensor? kv_start, SymInt num_splits, SymInt max_seq_len, Tensor(b!)? workspace) -> ()",
     "kv4_store": "(Tensor k, Tensor v, Tensor(a!) ck, Tensor(b!) cv, Tensor(c!) k_scale, Tensor(d!) v_scale, Tensor slots, "
                  "Tensor? counts) -> ()",
-    "kv4_load": "(Tensor ck, Tensor cv, Tensor k_scale, Tensor v_scale, Tensor slots, Tensor(a!) k, Tensor(b!) v) -> ()",
+    "kv4_load": "(Tensor ck, Tensor cv, Tensor k_scale, Tensor v_scale, Tensor slots, SymInt tokens, "
+                "Tensor(a!) k, Tensor(b!) v) -> ()",
     "gqa_decode_kv4": "(Tensor q, Tensor ck, Tensor cv, Tensor k_scale, Tensor v_scale, Tensor seq_lens, float scale, "
                       "Tensor(a!) out, Tensor? kv_start, SymInt window, SymInt sinks, SymInt num_splits, SymInt max_seq_len, "
                       "Tensor(b!)? workspace) -> ()",
@@ -111,8 +112,8 @@ def _kv4_store(k, v, ck, cv, k_scale, v_scale, slots, counts):
     long_cache._kv4_store(k, v, long_cache.Kv4Cache(ck, cv, k_scale, v_scale), slots, counts)
 
 
-def _kv4_load(ck, cv, k_scale, v_scale, slots, k, v):
-    long_cache._kv4_load(long_cache.Kv4Cache(ck, cv, k_scale, v_scale), slots, k, v)
+def _kv4_load(ck, cv, k_scale, v_scale, slots, tokens, k, v):
+    kernels.eager().kv4_load(ck, cv, k_scale, v_scale, slots, tokens, k, v)
 
 
 def _gqa_decode_kv4(q, ck, cv, k_scale, v_scale, seq_lens, scale, out, kv_start, window, sinks, num_splits, max_seq_len,
@@ -128,11 +129,11 @@ def _gqa_decode_tracked(q, k_cache, v_cache, seq_lens, scale, weights, out, deca
 
 
 def _kv_select(weights, seq_lens, keep, sinks, recent, kv_start, index, lens, weights_out):
-    long_cache._kv_select(weights, seq_lens, keep, sinks, recent, kv_start, index, lens, weights_out)
+    kernels.eager().select(weights, seq_lens, keep, sinks, recent, kv_start, index, lens, weights_out)
 
 
 def _kv_compact(tensors, index, lens, outs):
-    long_cache._kv_compact(tensors, index, lens, outs)
+    kernels.eager().compact(tensors, index, lens, outs)
 
 
 _KERNELS = {
