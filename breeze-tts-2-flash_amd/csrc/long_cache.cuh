@@ -27,6 +27,7 @@ struct LongParams {
   float scale_log2;             // scale * log2(e)
   uint16_t* out;
   int64_t o_sb, o_sh, o_st;
+  int out_wide;                 // out and its strides are multiples of 8 bytes
   int NKV, G, gshift, T, cap;   // G = 1 << gshift q heads per kv head
   int tiles, tpt;               // column tiles per row, tokens per column tile (16 / G)
   int splits, min_tiles, one_split;  // a split takes at least min_tiles wave tiles; up to one_split in all are not split
@@ -52,8 +53,8 @@ __device__ __forceinline__ int clamp_int(int x, int lo, int hi) { return min(max
 
 // [start, end) of row b, clamped to the cache as clamp_range does.
 __device__ __forceinline__ void long_range(int e_raw, int s_raw, bool has_start, int cap, int& start, int& end) {
-  end = clamp_int(e_raw, 0, cap);
-  start = has_start ? clamp_int(s_raw, 0, end) : 0;
+  end = wave_uniform(clamp_int(e_raw, 0, cap));
+  start = has_start ? wave_uniform(clamp_int(s_raw, 0, end)) : 0;
 }
 
 // What one column (query token) attends: [lo, lo + len) and [s, s + sink).

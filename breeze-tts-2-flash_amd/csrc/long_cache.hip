@@ -6,6 +6,7 @@
 
 #include "bz_long_cache.h"
 #include "long_cache.cuh"
+#include "window_prefill.cuh"
 
 namespace bz {
 int device_cu_count(int* cus);  // gqa_decode.hip
@@ -15,6 +16,9 @@ namespace {
 
 constexpr int kKv4Tokens = 16;  // most query tokens per row over a 4-bit cache
 
+// Columns (tokens times q heads of a kv head) from which a chunk takes the kernel of window_prefill.cuh.
+constexpr int64_t kPrefillCols = 64;
+
 bool dim_ok(int D) { return D == 64 || D == 128; }
 bool group_ok(int G) { return G == 1 || G == 2 || G == 4 || G == 8; }
 size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -23,6 +27,7 @@ size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 // counters first, one 256-byte line per (row, column tile, kv head); they are zero between calls, everything else is
 // written before it is read).
 struct Plan {
+  bool prefill;  // gqa_window: the chunk kernel, which needs no workspace
   int G, gshift, tpt, tiles, splits, min_tiles, one_split, score_stride;
   int64_t units;
   size_t ml, acc, head_ml, scores, total;
@@ -40,8 +45,15 @@ int make_plan(int kind, int B, int NH, int NKV, int D, int cap, int T, int windo
   pl->gshift = __builtin_ctz(pl->G);
   pl->tpt = kLongCols / pl->G < T ? kLongCols / pl->G : T;
   pl->tiles = (T + pl->tpt - 1) / pl->tpt;
-  if ((int64_t)B * pl->tiles > 65535 || NKV > 65535) return BZ_ERR_SHAPE;  // grid limits
   pl->units = (int64_t)B * pl->tiles * NKV;
+  pl->prefill = kind == BZ_LONG_WINDOW && (int64_t)T * pl->G >= kPrefillCols;
+  if (pl->prefill) {
+    pl->tiles = (int)(((int64_t)T * pl->G + kPreCols - 1) / kPreCols);
+    pl->splits = 1;
+    pl->ml = pl->acc = pl->head_ml = pl->scores = pl->total = 0;
+    return pl->tiles <= 65535 && B <= 65535 ? BZ_OK : BZ_ERR_SHAPE;
+  }
+  if ((int64_t)B * pl->tiles > 65535 || NKV > 65535) return BZ_ERR_SHAPE;  // grid limits
 
   // positions a column tile attends, in wave tiles
   int64_t len = max_seq_len > 0 && max_seq_len < cap ? max_seq_len : cap;
@@ -136,6 +148,7 @@ LongParams long_params(const bz_gqa_decode_args* a, const Plan& pl, int window, 
   p.scale_log2 = a->scale * kLog2e;
   p.out = static_cast<uint16_t*>(a->out);
   p.o_sb = a->out_stride_b, p.o_sh = a->out_stride_h, p.o_st = a->out_stride_t;
+  p.out_wide = !((reinterpret_cast<uintptr_t>(a->out) & 7) || ((p.o_sb | p.o_sh | p.o_st) & 3));
   p.NKV = a->num_kv_heads, p.G = pl.G, p.gshift = pl.gshift, p.T = a->tokens_per_row > 1 ? a->tokens_per_row : 1;
   p.cap = a->capacity;
   p.tiles = pl.tiles, p.tpt = pl.tpt;
@@ -192,7 +205,14 @@ BZ_EXPORT int bz_gqa_window(const bz_gqa_window_args* wa, hipStream_t stream) {
   if (rc == BZ_OK) rc = check_bf16_cache(a);
   if (rc == BZ_OK) rc = check_workspace(a, pl);
   if (rc != BZ_OK) return rc;
-  return launch_split<false, false>(a, a->head_dim, long_params(a, pl, wa->window, wa->sinks), pl, a->batch, stream);
+  const LongParams p = long_params(a, pl, wa->window, wa->sinks);
+  if (!pl.prefill) return launch_split<false, false>(a, a->head_dim, p, pl, a->batch, stream);
+  const dim3 grid(a->num_kv_heads, pl.tiles, a->batch);
+  if (a->head_dim == 128)
+    hipLaunchKernelGGL(window_prefill_kernel<128>, grid, dim3(kPreThreads), 0, stream, a->seq_lens, a->kv_start, p);
+  else
+    hipLaunchKernelGGL(window_prefill_kernel<64>, grid, dim3(kPreThreads), 0, stream, a->seq_lens, a->kv_start, p);
+  return hipGetLastError() == hipSuccess ? BZ_OK : BZ_ERR_LAUNCH;
 }
 
 BZ_EXPORT int bz_gqa_decode_kv4(const bz_gqa_kv4_args* ka, hipStream_t stream) {

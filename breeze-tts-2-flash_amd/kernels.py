@@ -25,7 +25,7 @@ LIB_NAME = "libbz_gqa_decode.so"
 LIB_PATH = PKG_DIR / LIB_NAME
 SOURCES = ["gqa_decode.hip", "gqa_fused.hip", "gemv.hip", "long_cache.hip", "kv4_store.hip",
            "kv_evict.hip"]  # translation units, compiled in parallel
-HEADERS = ["gqa_kernels.cuh", "gqa_wave.cuh", "device_common.cuh", "long_cache.cuh"]
+HEADERS = ["gqa_kernels.cuh", "gqa_wave.cuh", "device_common.cuh", "long_cache.cuh", "window_prefill.cuh"]
 ARCH = "gfx950"
 # -packed-fp32-ops: keep hipcc from emitting packed fp32 VALU ops (v_pk_*_f32)
 # -falign-loops=64: loop heads on 64-byte boundaries (instruction fetch); the split kernels measured 1-4% faster with

@@ -42,13 +42,14 @@ def window_attention(q, k, v, lens, scale, window=0, sinks=0, kv_start=None):
     return out, spread, reach
 
 
-def attention_bound(out, spread, reach, scale, D):
+def attention_bound(out, spread, reach, scale, D, one_term=False):
     """How far a kernel's bf16 output may lie from out: half a bf16 step (2^-8 of the value), and the terms' own error times
     sum p |v|. A score is a sum of D products of bf16 values in fp32, D + 2 roundings of at most 2^-23 of sum |q_i k_i|
     each; it enters a term and the sum that divides it (twice), with the same again for the shift by the maximum; two bf16
-    terms hold p to 2^-17, and the sums and exponentials add a few 2^-23."""
+    terms hold p to 2^-17, and the sums and exponentials add a few 2^-23. one_term: p is rounded to a single bf16 before it
+    meets V (a chunk of many tokens), half a bf16 step of each term: 2^-8 of sum p |v| more."""
     ds = scale * reach * (D + 2) * 2.0 ** -23
-    return 2.0 ** -8 * np.abs(out) + (4 * ds + 2.0 ** -15)[..., None] * spread + 1e-30
+    return 2.0 ** -8 * np.abs(out) + (4 * ds + 2.0 ** -15 + one_term * 2.0 ** -8)[..., None] * spread + 1e-30
 
 
 def kv4_round(x):
