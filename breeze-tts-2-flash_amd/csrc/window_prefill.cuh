@@ -2,8 +2,8 @@
 //
 // A workgroup of four waves takes 128 columns: (token, q head) pairs of one kv head, 128 / G tokens of a row times its G
 // heads, 32 a wave, so K and V are fetched once for the whole group. It walks the positions any of its tokens attends (the
-// sinks' tiles, then the window's; tile_range) in tiles of 64 staged in LDS, two buffers, the next tile's loads in flight
-// while one is worked on.
+// sinks' tiles, then the window's; tile_range) in tiles of 64 staged in LDS, two buffers each of K and V, the next loads in
+// flight while a tile is worked on.
 //   S^T = K Q^T   mfma 32x32x16: A = K rows, B = Q^T (registers, loaded once). A lane then holds 32 scores of one column, the
 //                 rows 8 (v / 4) + 4 half + v % 4 of each block of 32 positions, so the softmax is within a lane but for one
 //                 swap with lane ^ 32.
@@ -21,7 +21,7 @@ namespace {
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef short s16x4_lds __attribute__((ext_vector_type(4)));
 
-constexpr int kPreThreads = 256, kPreCols = 128, kPreTile = 64;
+constexpr int kPreThreads = 256, kPreCols = 128, kPreTile = 64, kPreRows = kPreTile / 4;
 
 // LDS of one buffer: K, then V, 64 rows of D bf16 each, in 16-byte chunks. Chunk c of row r lies in slot c ^ swizzle(r), so
 // that the lanes of one read, which take the same chunk of different rows, fall into different banks.
@@ -34,20 +34,16 @@ struct PreLds {
 
 // Loads the 64 rows from pos0 on (clamped to `last`: a row past it holds a copy of that one, and no column attends it) into
 // LDS at base: 64 lanes write 1 KB in lane order, so the swizzle is in which chunk each lane fetches.
-template <int D>
-__device__ __forceinline__ void stage_tile(char* base, const Rsrc& rk, const Rsrc& rv, int pos0, int last, uint32_t row_bytes,
-                                           int w, int lane) {
+template <int D, bool V>
+__device__ __forceinline__ void stage_tile(char* base, const Rsrc& rsrc, int pos0, int last, uint32_t row_bytes, int w, int lane) {
   using L = PreLds<D>;
   constexpr int RPI = 1024 / L::kRow, CH = D / 8;  // rows an instruction, chunks a row
 #pragma unroll
-  for (int u = 0; u < 16 / RPI; ++u) {
-    const int row = 16 * w + RPI * u + lane / CH, c = lane % CH;
-    const uint32_t off = (uint32_t)min(pos0 + row, last) * row_bytes;
-    char* const to = base + (16 * w + RPI * u) * L::kRow;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (__attribute__((address_space(3))) void*)to, 16,
-                                             off + 16 * (c ^ L::k_swz(row)), 0, 0, 0);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (__attribute__((address_space(3))) void*)(to + L::kBytes), 16,
-                                             off + 16 * (c ^ L::v_swz(row)), 0, 0, 0);
+  for (int u = 0; u < kPreRows / RPI; ++u) {
+    const int row = kPreRows * w + RPI * u + lane / CH, c = lane % CH;
+    const uint32_t off = (uint32_t)min(pos0 + row, last) * row_bytes + 16 * (c ^ (V ? L::v_swz(row) : L::k_swz(row)));
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        rsrc, (__attribute__((address_space(3))) void*)(base + (kPreRows * w + RPI * u) * L::kRow), 16, off, 0, 0, 0);
   }
 }
 
@@ -140,9 +136,11 @@ __global__ void __launch_bounds__(kPreThreads, 2)
   // of this wave's tokens: the first one's end, and the last one's window start and end
   const int wt0 = t0 + min((32 * w) >> p.gshift, ntok - 1), wt1 = t0 + min((32 * w + 31) >> p.gshift, ntok - 1);
   const int we0 = token_end(wt0), we1 = token_end(wt1);
-  const int wlo0 = max(s, we0 - p.window), wlo1 = max(s, we1 - p.window), wsink = s + min(p.sinks, we1 - s);
+  const int wlo1 = max(s, we1 - p.window);
 
-  __shared__ __align__(16) char lds[2][2 * L::kBytes];
+  // arrays of their own, and the tiles' parity known at compile time: the compiler then sees that the reads of one do not
+  // depend on the loads in flight to another (it would wait for all of them)
+  __shared__ __align__(16) char k_even[L::kBytes], k_odd[L::kBytes], v_even[L::kBytes], v_odd[L::kBytes];
   const int64_t head = (int64_t)b * p.kv_sb + (int64_t)h * p.kv_sh;
   const uint32_t row_bytes = (uint32_t)p.kv_ss;
   const Rsrc rk = span_rsrc(p.k + head, e1 * (int)p.kv_ss), rv = span_rsrc(p.v + head, e1 * (int)p.kv_ss);
@@ -153,7 +151,7 @@ __global__ void __launch_bounds__(kPreThreads, 2)
   int v_addr[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d)
-    v_addr[d] = L::kBytes + v_row * L::kRow + 16 * ((4 * d + 2 * ((lane / 16) % 2) + (l16 % 4) / 2) ^ L::v_swz(v_row)) + 8 * (l16 % 2);
+    v_addr[d] = v_row * L::kRow + 16 * ((4 * d + 2 * ((lane / 16) % 2) + (l16 % 4) / 2) ^ L::v_swz(v_row)) + 8 * (l16 % 2);
 
   float m = -INFINITY, l = 0.f;
   f32x16_t acc[ND];
@@ -162,26 +160,37 @@ __global__ void __launch_bounds__(kPreThreads, 2)
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
 
-  if (n > 0) stage_tile<D>(lds[0], rk, rv, pos_of(0), e1 - 1, row_bytes, w, lane);
-  for (int j = 0; j < n; ++j) {
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // this wave's loads of tile j are in LDS
-    __syncthreads();                     // everyone's are, and nobody reads the other buffer any more
-    if (j + 1 < n) stage_tile<D>(lds[(j + 1) & 1], rk, rv, pos_of(j + 1), e1 - 1, row_bytes, w, lane);
+  // K operand i of the tile in buf: positions 32 (i % 2) .., contraction step i / 2 (the two blocks' products alternate, since
+  // one that adds to the product before it waits for it)
+  auto k_read = [&](const char* buf, int i) __attribute__((always_inline)) {
+    return *reinterpret_cast<const bf16x8_t*>(buf + k_addr + 32 * (i % 2) * L::kRow + 16 * ((2 * (i / 2) + half) ^ k_sw));
+  };
+  // V^T operand d of 16 positions: the lane's 8, in two reads
+  auto v_read = [&](const char* buf, int ut, int d) __attribute__((always_inline)) {
+    using Tr = __attribute__((address_space(3))) s16x4_lds*;
+    const char* const at = buf + v_addr[d] + 16 * ut * L::kRow;
+    const uint2 a = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Tr)(at)));
+    const uint2 b = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Tr)(at + 8 * L::kRow)));
+    return __builtin_bit_cast(bf16x8_t, make_uint4(a.x, a.y, b.x, b.y));
+  };
+  constexpr int NK = 2 * NQ, PG = 16 / NK;  // products of K q, and pairs of terms worked out beside each
+  // Tile j: its scores x into the running maximum, sum and accumulators, and the scores of tile j + 1 (next; unused after the
+  // last). A wave has the matrix unit, the vector unit and LDS at work at once only if its instructions alternate, and an
+  // operand read just before its product costs the LDS latency each time: so the first 8 K operands are read before the
+  // maximum is taken, each product of K q is followed by the read 8 products ahead (or of V) and a share of the
+  // exponentials, and each product of V p by the read 4 ahead. The scheduling barriers keep that order.
+  auto step = [&](auto odd, int j, f32x16_t (&x)[2], f32x16_t (&next)[2]) __attribute__((always_inline)) {
+    constexpr bool kOdd = decltype(odd)::value;
+    const char *const kbuf = kOdd ? k_even : k_odd, *const vbuf = kOdd ? v_odd : v_even;
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // this wave's loads of K j + 1 and V j are in LDS
+    __syncthreads();                     // everyone's are, and nobody reads K j or V j - 1 any more
+    bf16x8_t kf[8], vf[2][ND];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) kf[i] = k_read(kbuf, i);
+    __builtin_amdgcn_sched_barrier(0);
+    if (j + 2 < n) stage_tile<D, false>(kOdd ? k_odd : k_even, rk, pos_of(j + 2), e1 - 1, row_bytes, w, lane);
+    if (j + 1 < n) stage_tile<D, true>(kOdd ? v_even : v_odd, rv, pos_of(j + 1), e1 - 1, row_bytes, w, lane);
     const int p0 = pos_of(j);
-    if (p0 >= we1 || (p0 + kPreTile <= wlo0 && p0 >= wsink)) continue;  // this wave attends nothing here
-    const char* const buf = lds[j & 1];
-
-    f32x16_t x[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x[u][i] = 0.f;
-#pragma unroll
-      for (int k = 0; k < NQ; ++k) {
-        const bf16x8_t kf = *reinterpret_cast<const bf16x8_t*>(buf + k_addr + 32 * u * L::kRow + 16 * ((2 * k + half) ^ k_sw));
-        x[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[k], x[u], 0, 0, 0);
-      }
-    }
     if (!(p0 + kPreTile <= we0 && p0 >= wlo1)) {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
@@ -208,31 +217,47 @@ __global__ void __launch_bounds__(kPreThreads, 2)
     }
     const float base = m == -INFINITY ? 0.f : m;
     uint32_t pk[2][8];
+    const f32x16_t zero = {};
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int i = 0; i < NK; ++i) {
+      next[i % 2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i % 8], qf[i / 2], i < 2 ? zero : next[i % 2], 0, 0, 0);
+      if (i + 8 < NK) kf[i % 8] = k_read(kbuf, i + 8);
+      else if (i - (NK - 8) < ND) vf[0][i - (NK - 8)] = v_read(vbuf, 0, i - (NK - 8));
 #pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        const float a = fast_exp2(fmaf(x[u][i], scale, -base)), a1 = fast_exp2(fmaf(x[u][i + 1], scale, -base));
-        l += a + a1;
-        pk[u][i / 2] = pack_bf16x2(a, a1);
+      for (int g = PG * i; g < PG * (i + 1); ++g) {
+        const int u = g / 8, v = 2 * (g % 8);
+        pk[u][g % 8] = pack_bf16x2(fast_exp2(fmaf(x[u][v], scale, -base)), fast_exp2(fmaf(x[u][v + 1], scale, -base)));
+        l = dot2_bf16(pk[u][g % 8], 0x3f803f80u, l);  // the sum of the rounded terms, the ones that meet V
       }
+      __builtin_amdgcn_sched_barrier(0);
+    }
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int ut = 0; ut < 4; ++ut) {
+      const uint32_t* const q = &pk[ut / 2][4 * (ut % 2)];
+      const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, make_uint4(q[0], q[1], q[2], q[3]));
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const bf16x8_t pf =
-            __builtin_bit_cast(bf16x8_t, make_uint4(pk[u][4 * t], pk[u][4 * t + 1], pk[u][4 * t + 2], pk[u][4 * t + 3]));
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          using Tr = __attribute__((address_space(3))) s16x4_lds*;
-          const char* const at = buf + v_addr[d] + (32 * u + 16 * t) * L::kRow;
-          const auto v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Tr)(at));
-          const auto v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Tr)(at + 8 * L::kRow));
-          const uint2 a = __builtin_bit_cast(uint2, v0), a1 = __builtin_bit_cast(uint2, v1);
-          acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, make_uint4(a.x, a.y, a1.x, a1.y)), pf,
-                                                           acc[d], 0, 0, 0);
-        }
+      for (int d = 0; d < ND; ++d) {
+        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[ut % 2][d], pf, acc[d], 0, 0, 0);
+        if (ut < 3) vf[(ut + 1) % 2][d] = v_read(vbuf, ut + 1, d);
+        __builtin_amdgcn_sched_barrier(0);
       }
+    }
+  };
+  if (n > 0) {
+    stage_tile<D, false>(k_even, rk, pos_of(0), e1 - 1, row_bytes, w, lane);
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    __syncthreads();
+    if (n > 1) stage_tile<D, false>(k_odd, rk, pos_of(1), e1 - 1, row_bytes, w, lane);
+    stage_tile<D, true>(v_even, rv, pos_of(0), e1 - 1, row_bytes, w, lane);
+    f32x16_t xa[2], xb[2];
+#pragma unroll
+    for (int i = 0; i < NK; ++i)
+      xa[i % 2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_read(k_even, i), qf[i / 2], i < 2 ? f32x16_t{} : xa[i % 2], 0, 0, 0);
+    for (int j = 0; j < n; j += 2) {
+      step(std::false_type{}, j, xa, xb);
+      if (j + 1 < n) step(std::true_type{}, j + 1, xb, xa);
+    }
   }
 
   float other = l;
