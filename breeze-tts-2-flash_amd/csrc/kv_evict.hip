@@ -14,8 +14,12 @@ namespace {
 // One workgroup per (row, kv head). The threshold is the m-th largest key of the middle positions (m = keep - sinks -
 // recent), found by a radix selection from the top digit down (11 + 11 + 10 bits: a histogram in LDS, then the digit
 // that holds the m-th key); every key above it stays, and as many equal ones, from the lowest position on, as are still
-// missing. Each thread owns one run of consecutive positions, so one scan over the threads gives every kept position its
-// place in ascending order.
+// missing. The kept positions' places in ascending order come from ballots: one count per wave and strip of 1024
+// positions, one scan over those.
+//
+// A row's bytes are few (4 a position) and one workgroup reads them all, so its latencies are the bound: a row of up to
+// 1024 IPT positions is loaded once, all loads at a time, and everything after works from registers. A longer one goes
+// through in chunks of that many, loaded again for each pass.
 
 constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / kWave;
@@ -28,129 +32,170 @@ struct SelectParams {
   int32_t *index, *lens;
   float* wo;
   int64_t wo_sb, wo_sh;
-  int NKV, cap, keep, sinks, recent;
+  int NKV, cap, keep, sinks, recent, write_lens;
 };
 
 // Order-preserving map of float to uint32; NaN above everything, -0 as 0.
 __device__ __forceinline__ uint32_t weight_key(float f) {
   const uint32_t u = __float_as_uint(f);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
-  if ((u & 0x7fffffffu) == 0) return 0x80000000u;
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  const uint32_t k = u & 0x80000000u ? ~u : u | 0x80000000u;
+  return (u & 0x7fffffffu) > 0x7f800000u ? 0xffffffffu : (u & 0x7fffffffu) == 0 ? 0x80000000u : k;
 }
 
-// Exclusive sum of x over the workgroup's threads; total: the sum over all. s: kSelWaves + 1 words of LDS.
-__device__ __forceinline__ uint64_t block_scan(uint64_t x, uint64_t* s, uint64_t* total) {
-  const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
-  uint64_t v = x;
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) {
-    const uint64_t y = __shfl_up(v, d);
-    if (lane >= d) v += y;
-  }
-  __syncthreads();  // s may still be read from an earlier scan
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t scan_step(uint32_t x) {  // x of the lane that CTRL names, 0 where there is none
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+}
+// Inclusive sum of x over the lanes of a 16-lane row up to this one, and over those of the wave: DPP row_shr by 1, 2, 4 and
+// 8, then the last lanes of the rows before (row_bcast:15 into rows 1 and 3, row_bcast:31 into rows 2 and 3). (Six
+// ds_bpermutes and 16 LDS reads a thread in their place: 12.1 -> 10.7 us for 32 rows of 8192.)
+__device__ __forceinline__ uint32_t row_scan(uint32_t x) {
+  x += scan_step<0x111, 0xf>(x);
+  x += scan_step<0x112, 0xf>(x);
+  x += scan_step<0x114, 0xf>(x);
+  return x + scan_step<0x118, 0xf>(x);
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  x = row_scan(x);
+  x += scan_step<0x142, 0xa>(x);
+  return x + scan_step<0x143, 0xc>(x);
+}
+// Exclusive sum of x over the workgroup's threads. s: kSelWaves words of LDS that no earlier read is still at.
+__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* s) {
+  static_assert(kSelWaves == 16, "one row of lanes scans the waves' sums");
+  const int lane = threadIdx.x % kWave, w = wave_uniform((int)threadIdx.x / kWave);
+  const uint32_t v = wave_scan(x);
   if (lane == kWave - 1) s[w] = v;
   __syncthreads();
-  uint64_t before = 0, all = 0;
-#pragma unroll
-  for (int u = 0; u < kSelWaves; ++u) {
-    before += u < w ? s[u] : 0;
-    all += s[u];
-  }
-  *total = all;
-  return before + v - x;
+  const uint32_t sums = row_scan(s[lane % 16]);
+  return (w > 0 ? (uint32_t)__builtin_amdgcn_readlane((int)sums, w - 1) : 0u) + v - x;
 }
 
+template <int IPT>
 __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const SelectParams p) {
+  constexpr int kCounts = IPT * kSelWaves, kChunk = IPT * kSelThreads;
   __shared__ uint32_t s_hist[kBins];
-  __shared__ uint64_t s_scan[kSelWaves];
-  __shared__ uint32_t s_found[2];
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+  __shared__ uint32_t s_scan[3][kSelWaves];
+  __shared__ uint32_t s_found[3][2];
+  __shared__ uint32_t s_count[kCounts];  // positions that stay (low half) and that are at the threshold (high half)
+  __shared__ uint32_t s_base[2];
+  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid % kWave, wv = tid / kWave;
   const int e = min(max(p.seq_lens[b], 0), p.cap);
   const int s = p.kv_start ? min(max(p.kv_start[b], 0), e) : 0;
   const int n = e - s, kept = min(n, p.keep);
   const float* const w = p.w + (int64_t)b * p.w_sb + (int64_t)h * p.w_sh;
+  float* const wo = p.wo ? p.wo + (int64_t)b * p.wo_sb + (int64_t)h * p.wo_sh : nullptr;
   int32_t* const index = p.index + ((int64_t)b * p.NKV + h) * p.keep;
 
-  if (n <= p.keep) {
-    for (int d = tid; d < p.keep; d += kSelThreads) index[d] = d < n ? s + d : -1;
-  } else {
-    const int lo = s + p.sinks, hi = e - p.recent;  // hi - lo > m >= 0
-    const uint32_t m = (uint32_t)(p.keep - p.sinks - p.recent);
-    uint32_t prefix = 0, left = m;  // the threshold's known top bits; how many of the keys with those bits stay
-    int known = 0;                  // bits known
-    if (m > 0) {
-      for (int pass = 0; pass < 3; ++pass) {
-        const int bits = pass < 2 ? 11 : 10, shift = 32 - known - bits;
-        for (int i = tid; i < kBins; i += kSelThreads) s_hist[i] = 0;
-        __syncthreads();
-        for (int i = lo + tid; i < hi; i += kSelThreads) {
-          const uint32_t k = weight_key(w[i]);
-          if (known == 0 || k >> (32 - known) == prefix) atomicAdd(&s_hist[(k >> shift) & ((1u << bits) - 1)], 1u);
+  // a chunk's weights: strip i holds the positions c0 + 1024 i .. + 1023, one a thread
+  float x[IPT];
+  auto load = [&](int c0) {
+#pragma unroll
+    for (int i = 0; i < IPT; ++i) x[i] = w[max(min(c0 + i * kSelThreads + tid, e - 1), 0)];  // past the row: unused
+  };
+  load(s);
+  const int lo = s + p.sinks, hi = e - p.recent;  // the middle, of which m positions stay
+  const uint32_t m = n > p.keep ? (uint32_t)(p.keep - p.sinks - p.recent) : 0u;
+  uint32_t prefix = 0, left = m;  // the threshold's top bits; how many of the keys with those bits stay
+  if (m > 0) {                    // then hi - lo > m
+    for (int i = tid; i < kBins; i += kSelThreads) s_hist[i] = 0;
+    int known = 0;
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+      const int bits = pass < 2 ? 11 : 10, shift = 32 - known - bits;
+      __syncthreads();
+      for (int c0 = s; c0 < e; c0 += kChunk) {
+        if (n > kChunk && (pass > 0 || c0 > s)) load(c0);
+#pragma unroll
+        for (int i = 0; i < IPT; ++i) {
+          const int pos = c0 + i * kSelThreads + tid;
+          const uint32_t k = weight_key(x[i]);
+          if (pos >= lo && pos < hi && (pass == 0 || k >> (32 - known) == prefix))
+            atomicAdd(&s_hist[(k >> shift) & ((1u << bits) - 1)], 1u);
         }
-        __syncthreads();
-        // the digit with fewer than `left` keys above it and at least `left` from it on: thread t sums bins from the top
-        uint64_t total;
-        const int bin = kBins - 2 - 2 * tid;  // this thread's two bins: bin + 1, then bin
-        const uint32_t c1 = s_hist[bin + 1], c0 = s_hist[bin];
-        const uint32_t above = (uint32_t)block_scan(c0 + c1, s_scan, &total);
-        if (above < left && above + c1 >= left) s_found[0] = bin + 1, s_found[1] = left - above;
-        else if (above + c1 < left && above + c1 + c0 >= left) s_found[0] = bin, s_found[1] = left - above - c1;
-        __syncthreads();
-        prefix = (prefix << bits) | s_found[0];
-        left = s_found[1];
-        known += bits;
       }
-    }
-    // this thread's run of positions
-    const int run = (n + kSelThreads - 1) / kSelThreads, r0 = s + min(n, tid * run), r1 = s + min(n, (tid + 1) * run);
-    uint32_t above = 0, equal = 0;
-    for (int i = r0; i < r1; ++i) {
-      if (i < lo || i >= hi) {
-        ++above;
-      } else if (m > 0) {
-        const uint32_t k = weight_key(w[i]);
-        above += k > prefix;
-        equal += k == prefix;
-      }
-    }
-    uint64_t total;
-    const uint64_t before = block_scan((uint64_t)equal << 32 | above, s_scan, &total);
-    uint32_t at_above = (uint32_t)before, at_equal = (uint32_t)(before >> 32);
-    for (int i = r0; i < r1; ++i) {
-      bool stays = i < lo || i >= hi, same = false;
-      if (!stays && m > 0) {
-        const uint32_t k = weight_key(w[i]);
-        stays = k > prefix;
-        same = k == prefix;
-      }
-      if (stays || (same && at_equal < left)) index[at_above + min(at_equal, left)] = i;
-      at_above += stays;
-      at_equal += same;
+      __syncthreads();
+      // the digit with fewer than `left` keys above it and at least `left` from it on: thread t sums two bins from the top
+      const int bin = kBins - 2 - 2 * tid;
+      const uint32_t c1 = s_hist[bin + 1], c0 = s_hist[bin];
+      s_hist[bin + 1] = s_hist[bin] = 0;
+      const uint32_t above = block_scan(c0 + c1, s_scan[pass]);
+      if (above < left && above + c1 >= left) s_found[pass][0] = bin + 1, s_found[pass][1] = left - above;
+      else if (above + c1 < left && above + c1 + c0 >= left) s_found[pass][0] = bin, s_found[pass][1] = left - above - c1;
+      __syncthreads();
+      prefix = (prefix << bits) | s_found[pass][0];
+      left = s_found[pass][1];
+      known += bits;
     }
   }
-  // Every workgroup of the row has to see seq_lens before one of them may write lens over it: lens of a row is written by
-  // kv_lens_kernel, after this launch.
-  if (p.wo == nullptr) return;
-  float* const wo = p.wo + (int64_t)b * p.wo_sb + (int64_t)h * p.wo_sh;
-  // index[d] >= d and ascends, so a chunk that is read whole before it is written never overwrites what a later one reads
-  for (int d0 = 0; d0 < kept; d0 += kSelThreads) {
-    __syncthreads();  // index is written (first chunk); the chunk before is read
-    const int d = d0 + tid;
-    const float x = d < kept ? w[index[d]] : 0.f;
-    __builtin_amdgcn_s_waitcnt(0x0f70);
+  // Each strip's places. A chunk writes at most up to its own first positions, so wo may be w: what a later chunk reads lies
+  // behind, and this one has been read before the barriers.
+  uint32_t before = 0, ties_before = 0;  // in the chunks before
+  for (int c0 = s; c0 < e; c0 += kChunk) {
+    if (n > kChunk && (m > 0 || c0 > s)) load(c0);
+    uint32_t above = 0, equal = 0;  // bit i: strip i's position stays, or is at the threshold
+#pragma unroll
+    for (int i = 0; i < IPT; ++i) {
+      const int pos = c0 + i * kSelThreads + tid;
+      const uint32_t k = weight_key(x[i]);
+      const bool ends = n <= p.keep || pos < lo || pos >= hi;
+      const bool stays = pos < e && (ends || (m > 0 && k > prefix)), ties = pos < e && !ends && m > 0 && k == prefix;
+      above |= stays ? 1u << i : 0u;
+      equal |= ties ? 1u << i : 0u;
+      const uint32_t c = (uint32_t)__popcll(__ballot(stays)) | (uint32_t)__popcll(__ballot(ties)) << 16;
+      if (lane == 0) s_count[i * kSelWaves + wv] = c;
+    }
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // the chunk's weights are here before anyone writes wo
     __syncthreads();
-    if (d < kept) wo[d] = x;
+    if (wv == 0) {  // exclusive sums over the counts, kCounts / 64 a lane; the halves stay below 2^16 (a chunk has 2^15)
+      constexpr int PER = kCounts / kWave;
+      uint32_t c[PER], sum = 0;
+#pragma unroll
+      for (int q = 0; q < PER; ++q) c[q] = s_count[PER * lane + q], sum += c[q];
+      uint32_t acc = wave_scan(sum) - sum;
+#pragma unroll
+      for (int q = 0; q < PER; ++q) s_count[PER * lane + q] = acc, acc += c[q];
+      if (lane == kWave - 1) s_base[0] = acc & 0xffffu, s_base[1] = acc >> 16;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < IPT; ++i) {
+      const bool stays = (above >> i) & 1, ties = (equal >> i) & 1;
+      const uint64_t bs = __ballot(stays), bt = __ballot(ties), below = (1ull << lane) - 1;
+      const uint32_t c = s_count[i * kSelWaves + wv];
+      const uint32_t at = before + (c & 0xffffu) + (uint32_t)__popcll(bs & below);
+      const uint32_t tie = ties_before + (c >> 16) + (uint32_t)__popcll(bt & below);
+      if (stays || (ties && tie < left)) {
+        const int d = (int)(at + min(tie, left));
+        index[d] = c0 + i * kSelThreads + tid;
+        if (wo != nullptr) wo[d] = x[i];
+      }
+    }
+    before += s_base[0], ties_before += s_base[1];
+    __syncthreads();
   }
-  for (int d = kept + tid; d < e; d += kSelThreads) wo[d] = 0.f;
+  for (int d = kept + tid; d < p.keep; d += kSelThreads) index[d] = -1;
+  if (p.write_lens && h == 0 && tid == 0) p.lens[b] = kept;
+  if (wo != nullptr)
+    for (int d = kept + tid; d < e; d += kSelThreads) wo[d] = 0.f;
 }
 
+// lens of a call that writes it over seq_lens: after every workgroup of the launch before has read those.
 __global__ void __launch_bounds__(kWave) kv_lens_kernel(const SelectParams p, int batch) {
   const int b = blockIdx.x * kWave + threadIdx.x;
   if (b >= batch) return;
   const int e = min(max(p.seq_lens[b], 0), p.cap);
   const int s = p.kv_start ? min(max(p.kv_start[b], 0), e) : 0;
   p.lens[b] = min(e - s, p.keep);
+}
+
+using SelectFn = void (*)(const SelectParams);
+// The fewest registers that hold a row of the capacity (of the first 32768 positions of a longer one).
+SelectFn pick_select(int cap) {
+  if (cap <= 4 * kSelThreads) return kv_select_kernel<4>;
+  if (cap <= 8 * kSelThreads) return kv_select_kernel<8>;
+  if (cap <= 16 * kSelThreads) return kv_select_kernel<16>;
+  return kv_select_kernel<32>;
 }
 
 // ---------------------------------------------------------------------------------------------------- compaction
@@ -161,6 +206,8 @@ __global__ void __launch_bounds__(kWave) kv_lens_kernel(const SelectParams p, in
 // workgroups too.
 
 constexpr int kMoveThreads = 256, kMoveU = 8;
+typedef uint32_t vec8 __attribute__((ext_vector_type(2)));
+typedef uint32_t vec16 __attribute__((ext_vector_type(4)));
 
 struct MoveParams {
   bz_kv_tensor t[BZ_KV_TENSORS];
@@ -174,32 +221,33 @@ struct MoveParams {
 };
 
 template <class V>
-__device__ void move_rows(const MoveParams& p, const bz_kv_tensor& t, const char* src, char* dst, const int32_t* index,
-                          int len, int slice, int lanes, bool in_place) {
+__device__ __forceinline__ void move_rows(const bz_kv_tensor& t, const char* src, char* dst, const int32_t* index, int cap,
+                                          int len, int slice, int lanes, bool in_place) {
   const int rows = kMoveThreads / lanes, r = threadIdx.x / lanes, c = slice * lanes + (int)threadIdx.x % lanes;
-  const bool mine = r < rows && (int64_t)c * (int)sizeof(V) < t.row_bytes;
+  const int64_t col = (int64_t)c * (int)sizeof(V);
+  const bool mine = col < t.row_bytes;
   const int step = rows * kMoveU;
   const int d_begin = in_place ? 0 : (int)blockIdx.y * step, d_end = in_place ? len : min(len, d_begin + step);
   for (int d0 = d_begin; d0 < d_end; d0 += step) {
     V x[kMoveU];
-    bool put[kMoveU];
+    int from[kMoveU];
 #pragma unroll
-    for (int u = 0; u < kMoveU; ++u) {
-      const int d = d0 + u * rows + r;
-      put[u] = false;
-      if (mine && d < len) {
-        const int i = index[d];
-        put[u] = i >= 0 && i < p.cap && !(in_place && i == d);
-        if (put[u]) x[u] = *reinterpret_cast<const V*>(src + i * t.src_stride_s + c * (int64_t)sizeof(V));
-      }
+    for (int u = 0; u < kMoveU; ++u) from[u] = index[min(d0 + u * rows + r, len - 1)];
+#pragma unroll
+    for (int u = 0; u < kMoveU; ++u) {  // every load without a condition; an index that is none reads row 0, unused
+      const int64_t i = from[u] >= 0 && from[u] < cap ? from[u] : 0;
+      x[u] = __builtin_nontemporal_load(reinterpret_cast<const V*>(src + i * t.src_stride_s + (mine ? col : 0)));
     }
     if (in_place) {
       __builtin_amdgcn_s_waitcnt(0x0f70);
       __syncthreads();
     }
 #pragma unroll
-    for (int u = 0; u < kMoveU; ++u)
-      if (put[u]) *reinterpret_cast<V*>(dst + (int64_t)(d0 + u * rows + r) * t.dst_stride_s + c * (int64_t)sizeof(V)) = x[u];
+    for (int u = 0; u < kMoveU; ++u) {
+      const int d = d0 + u * rows + r;
+      if (mine && d < len && from[u] >= 0 && from[u] < cap && !(in_place && from[u] == d))
+        __builtin_nontemporal_store(x[u], reinterpret_cast<V*>(dst + d * t.dst_stride_s + col));
+    }
   }
 }
 
@@ -216,11 +264,11 @@ __global__ void __launch_bounds__(kMoveThreads) kv_compact_kernel(const MovePara
   const int32_t* const index = p.index + ((int64_t)b * p.NKV + h) * p.keep;
   const int slice = blockIdx.x - p.first[k], lanes = p.lanes[k];
   switch (p.vec[k]) {
-    case 16: move_rows<uint4>(p, t, src, dst, index, len, slice, lanes, in_place); break;
-    case 8: move_rows<uint2>(p, t, src, dst, index, len, slice, lanes, in_place); break;
-    case 4: move_rows<uint32_t>(p, t, src, dst, index, len, slice, lanes, in_place); break;
-    case 2: move_rows<uint16_t>(p, t, src, dst, index, len, slice, lanes, in_place); break;
-    default: move_rows<uint8_t>(p, t, src, dst, index, len, slice, lanes, in_place); break;
+    case 16: move_rows<vec16>(t, src, dst, index, p.cap, len, slice, lanes, in_place); break;
+    case 8: move_rows<vec8>(t, src, dst, index, p.cap, len, slice, lanes, in_place); break;
+    case 4: move_rows<uint32_t>(t, src, dst, index, p.cap, len, slice, lanes, in_place); break;
+    case 2: move_rows<uint16_t>(t, src, dst, index, p.cap, len, slice, lanes, in_place); break;
+    default: move_rows<uint8_t>(t, src, dst, index, p.cap, len, slice, lanes, in_place); break;
   }
 }
 
@@ -246,8 +294,12 @@ BZ_EXPORT int bz_kv_select(const bz_kv_select_args* a, hipStream_t stream) {
   p.index = a->index, p.lens = a->lens;
   p.wo = a->weights_out, p.wo_sb = a->wo_stride_b, p.wo_sh = a->wo_stride_h;
   p.NKV = a->num_kv_heads, p.cap = a->capacity, p.keep = a->keep, p.sinks = a->sinks, p.recent = a->recent;
-  hipLaunchKernelGGL(kv_select_kernel, dim3(a->num_kv_heads, a->batch), dim3(kSelThreads), 0, stream, p);
+  // workgroups of a row read seq_lens and kv_start; lens that lies on either is written by a launch of its own
+  auto apart = [&](const int32_t* x) { return x == nullptr || a->lens + a->batch <= x || x + a->batch <= a->lens; };
+  p.write_lens = apart(a->seq_lens) && apart(a->kv_start);
+  hipLaunchKernelGGL(pick_select(a->capacity), dim3(a->num_kv_heads, a->batch), dim3(kSelThreads), 0, stream, p);
   if (hipGetLastError() != hipSuccess) return BZ_ERR_LAUNCH;
+  if (p.write_lens) return BZ_OK;
   hipLaunchKernelGGL(kv_lens_kernel, dim3((a->batch + kWave - 1) / kWave), dim3(kWave), 0, stream, p, a->batch);
   return hipGetLastError() == hipSuccess ? BZ_OK : BZ_ERR_LAUNCH;
 }

@@ -317,7 +317,7 @@ def heavy(rng, shape):
 @pytest.mark.parametrize("cap,lens,starts,keep,sinks,recent", [
     (50, [50, 7, 0], None, 20, 2, 5), (300, [300, 250, 64], [0, 33, 0], 64, 4, 60), (2100, [2100, 1030], [5, 0], 1024, 0, 0),
     (5000, [5000, 4097], None, 1, 0, 0), (1111, [1111], None, 1110, 3, 100), (700, [700, 400], [0, 1], 399, 0, 399),
-    (9000, [9000], None, 4000, 8, 128), (64, [64], None, 64, 1, 1),
+    (9000, [9000], None, 4000, 8, 128), (64, [64], None, 64, 1, 1), (70000, [70000, 40001], [0, 3], 33000, 4, 100), (40000, [39999], None, 20000, 0, 0),
 ])
 def test_select(device, cap, lens, starts, keep, sinks, recent):
     rng = np.random.default_rng(cap)
