@@ -162,6 +162,15 @@ __device__ __forceinline__ uint32_t finite_pair(uint32_t w) {
   return lo | hi;
 }
 
+// Scores are taken times a positive scale, which a maximum may be taken before; the query carries the sign. (1e-30 stands for
+// a scale of 0, whose product with an excluded position's -inf would be NaN.)
+__device__ __forceinline__ float positive_scale(float scale_log2) { return fmaxf(fabsf(scale_log2), 1e-30f); }
+__device__ __forceinline__ bf16x8_t signed_q(uint4 q, float scale_log2) {
+  const uint32_t flip = scale_log2 < 0.f ? 0x80008000u : 0u;
+  q.x ^= flip, q.y ^= flip, q.z ^= flip, q.w ^= flip;
+  return __builtin_bit_cast(bf16x8_t, q);
+}
+
 // The running state of one wave: column r's max (the same in the column's four lanes) and sum (over the lane's own
 // positions), and acc[n][i]: dim (D / 16)(4 g + i) + n of column r.
 template <int D>
@@ -170,24 +179,28 @@ struct LongState {
   f32x4_t acc[D / 16];
 };
 
-// One wave tile's scores x (times log2 e, -inf where not attended) folded into the running max and sum; x becomes the
-// softmax terms 2^(x - m).
+// One wave tile's products x (q . k times a positive scale is the score in base 2; -inf where not attended) folded into the
+// running max and sum; x becomes the softmax terms 2^(scale x - m). The running maximum moves only when a column's has grown
+// by more than 2^8, so that the accumulators are rarely rescaled: until then its terms stay below 2^8, and what rounds them
+// is relative.
 template <int D, int N>
-__device__ __forceinline__ void fold_scores(LongState<D>& st, float (&x)[N]) {
+__device__ __forceinline__ void fold_scores(LongState<D>& st, float (&x)[N], float scale) {
   float mt[1] = {x[0]};
 #pragma unroll
   for (int i = 1; i < N; ++i) mt[0] = fmaxf(mt[0], x[i]);
   rows_max<1>(mt);
-  const float mn = fmaxf(st.m, mt[0]);
-  const float mu = (mn == -INFINITY) ? 0.f : mn;
-  const float alpha = fast_exp2(st.m - mu);
-  st.m = mn;
-  st.l *= alpha;
+  const float top = mt[0] * scale;
+  if (__ballot(top > st.m + 8.f) != 0) {
+    const float mn = fmaxf(st.m, top), mu = (mn == -INFINITY) ? 0.f : mn, alpha = fast_exp2(st.m - mu);
+    st.m = mn;
+    st.l *= alpha;
 #pragma unroll
-  for (int n = 0; n < D / 16; ++n) st.acc[n] *= alpha;
+    for (int n = 0; n < D / 16; ++n) st.acc[n] *= alpha;
+  }
+  const float base = st.m == -INFINITY ? 0.f : st.m;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    x[i] = fast_exp2(x[i] - mu);
+    x[i] = fast_exp2(fmaf(x[i], scale, -base));
     st.l += x[i];
   }
 }
@@ -315,8 +328,9 @@ __global__ void __launch_bounds__(kLongThreads, 2)
     const uint16_t* qsrc = p.q + (int64_t)b * p.q_sb + (int64_t)tok * p.q_st + (int64_t)hq * p.q_sh;
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
-      qf[j] = __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const uint4*>(qsrc + (KV4 ? (D / 4) * g + 8 * j : 32 * j + 8 * g)));
+      qf[j] = signed_q(*reinterpret_cast<const uint4*>(qsrc + (KV4 ? (D / 4) * g + 8 * j : 32 * j + 8 * g)), p.scale_log2);
   }
+  const float scale = positive_scale(p.scale_log2);
 
   int s, e;
   long_range(e_raw, s_raw, starts != nullptr, p.cap, s, e);
@@ -330,6 +344,8 @@ __global__ void __launch_bounds__(kLongThreads, 2)
   if (split >= nact) return;
   const int j0 = split * per, j1 = min(n, j0 + per);
   const int e1 = token_end(t0 + ntok - 1);
+  // every column attends the whole of [whole_lo, whole_end)
+  const int whole_end = token_end(t0), whole_lo = max(s, e1 - p.window);
   const int past = (e1 + P - 1) & ~(P - 1);  // a tile here lies outside the spans: its loads touch no memory
   auto pos_of = [&](int j) { return j >= j1 ? past : j < tr.na ? tr.fa + P * j : tr.fb + P * (j - tr.na); };
 
@@ -383,15 +399,19 @@ __global__ void __launch_bounds__(kLongThreads, 2)
         d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[k], d, 0, 0, 0);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[4 * u + i] = attends(mine, s, pos(4 * u + i)) ? d[i] * p.scale_log2 : -INFINITY;
+      for (int i = 0; i < 4; ++i) x[4 * u + i] = d[i];
+    }
+    if (!(pos0 + P <= whole_end && pos0 >= whole_lo)) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = attends(mine, s, pos(i)) ? x[i] : -INFINITY;
     }
     if constexpr (TRACK) {
       if (r < ncol) {
         float* const row = p.scores + ((int64_t)b * p.NKV * p.G + hq) * p.score_stride;
-        *reinterpret_cast<f32x4_t*>(row + pos0 + 4 * g) = f32x4_t{x[0], x[1], x[2], x[3]};
+        *reinterpret_cast<f32x4_t*>(row + pos0 + 4 * g) = f32x4_t{x[0], x[1], x[2], x[3]} * scale;
       }
     }
-    fold_scores<D, N>(st, x);
+    fold_scores<D, N>(st, x, scale);
     if constexpr (KV4) {
       uint32_t v[N][NJ];
       uint32_t emax = 0;

@@ -112,17 +112,12 @@ __global__ void __launch_bounds__(kPreThreads, 2)
   const int t0 = tile * (kPreCols >> p.gshift), ntok = min(kPreCols >> p.gshift, p.T - t0);
   const int mine = 32 * w + c, tok = t0 + min(mine >> p.gshift, ntok - 1), hq = (h << p.gshift) + (mine & (p.G - 1));
 
-  const float scale = fmaxf(fabsf(p.scale_log2), 1e-30f);  // scores are taken times a positive scale: q carries the sign
-  const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
+  const float scale = positive_scale(p.scale_log2);
   bf16x8_t qf[NQ];
   {
     const uint16_t* src = p.q + (int64_t)b * p.q_sb + (int64_t)tok * p.q_st + (int64_t)hq * p.q_sh + 8 * half;
 #pragma unroll
-    for (int j = 0; j < NQ; ++j) {
-      uint4 x = *reinterpret_cast<const uint4*>(src + 16 * j);
-      x.x ^= flip, x.y ^= flip, x.z ^= flip, x.w ^= flip;
-      qf[j] = __builtin_bit_cast(bf16x8_t, x);
-    }
+    for (int j = 0; j < NQ; ++j) qf[j] = signed_q(*reinterpret_cast<const uint4*>(src + 16 * j), p.scale_log2);
   }
 
   int s, e;

@@ -48,7 +48,7 @@ def attention_bound(out, spread, reach, scale, D, one_term=False):
     each; it enters a term and the sum that divides it (twice), with the same again for the shift by the maximum; two bf16
     terms hold p to 2^-17, and the sums and exponentials add a few 2^-23. one_term: p is rounded to a single bf16 before it
     meets V (a chunk of many tokens), half a bf16 step of each term: 2^-8 of sum p |v| more."""
-    ds = scale * reach * (D + 2) * 2.0 ** -23
+    ds = abs(scale) * reach * (D + 2) * 2.0 ** -23
     return 2.0 ** -8 * np.abs(out) + (4 * ds + 2.0 ** -15 + one_term * 2.0 ** -8)[..., None] * spread + 1e-30
 
 

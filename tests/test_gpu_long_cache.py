@@ -155,6 +155,21 @@ def test_unattended_values_do_not_reach_a_token(device, T, value):
     assert torch.isnan(out[0, T - 1].float()).all() and torch.isfinite(out[0, :T - 1].float()).all()
 
 
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 3.0])
+@pytest.mark.parametrize("T", [1, 64])
+def test_scales(device, T, scale):
+    """A negative scale, none, and one that leaves a single position."""
+    rng = np.random.default_rng(T)
+    NKV, G, D, n = 2, 2, 128, 150
+    q, k, v = randn(rng, 1, NKV * G, T, D), randn(rng, 1, NKV, n, D), randn(rng, 1, NKV, n, D)
+    out = pkg.gqa_window(q.to(device), k.to(device), v.to(device), ints([n], device), scale, 60, sinks=3)
+    check_attention(out, q.float(), k.float(), v.float(), [n], scale, 60, 3)
+    if T == 1:
+        cache = pkg.kv4_store(k.to(device), v.to(device), pkg.kv4_cache(1, NKV, n, D, device), ints([0], device))
+        out = pkg.gqa_decode_kv4(q.to(device), cache, ints([n], device), scale)
+        check_attention(out, q.float(), kv4_round(k.float().numpy())[0], kv4_round(v.float().numpy())[0], [n], scale)
+
+
 def test_window_equals_plain_decode(device):
     """Without a window it is gqa_decode's attention."""
     rng = np.random.default_rng(5)
