@@ -45,8 +45,7 @@ namespace {
 
 using bz::LongParams;
 
-constexpr int kLongThreads = 256;
-constexpr int kLongWaves = kLongThreads / kWave;
+constexpr int kApplyThreads = 256;
 constexpr int kLongCols = 16;
 
 __device__ __forceinline__ int clamp_int(int x, int lo, int hi) { return min(max(x, lo), hi); }
@@ -227,58 +226,68 @@ __device__ __forceinline__ f32x4_t mfma_pv(const uint32_t (&v)[N / 2], const uin
                                                    __builtin_bit_cast(bf16x8_t, make_uint4(p[0], p[1], p[2], p[3])), acc, 0, 0, 0);
 }
 
+// The pair with finite halves replaced by 0.
+__device__ __forceinline__ uint32_t odd_pair(uint32_t w) { return w & ~finite_pair(w); }
+
 // st.acc += V^T P. v[i][m]: bf16 dims 2 m and 2 m + 1 of this lane's dims at its i-th position; pos(i): that position.
 // Where V holds an infinity or NaN (bad, any lane of the wave), 0 times it must not reach the columns that do not attend
-// its position: each column then takes a product of its own with the positions it does not attend cleared (and the
-// lower terms leave non-finite values out: p times an infinity is the infinity).
+// its position: each column then takes a product of its own with the non-finite values of the positions it attends (in the
+// higher terms alone: p times an infinity is the infinity), and the product of all columns what is left.
 template <int D, int N, class Pos>
-__device__ __forceinline__ void accumulate(LongState<D>& st, const uint32_t (&v)[N][D / 32], const float (&p)[N], bool bad,
+__device__ __forceinline__ void accumulate(LongState<D>& st, uint32_t (&v)[N][D / 32], const float (&p)[N], bool bad,
                                            int col, int ncol, const Reach& mine, int s, Pos pos) {
   uint32_t hi[N / 2], lo[N / 2];
   split_terms(p, hi, lo);
-  if (__builtin_expect(__ballot(bad) == 0, 1)) {
+  auto operand = [](const uint32_t (&x)[N][D / 32], int n, uint32_t (&vt)[N / 2]) {
 #pragma unroll
-    for (int n = 0; n < D / 16; ++n) {
-      uint32_t vt[N / 2];
+    for (int a = 0; a < N / 2; ++a)
+      vt[a] = n % 2 ? pair_hi(x[2 * a][n / 2], x[2 * a + 1][n / 2]) : pair_lo(x[2 * a][n / 2], x[2 * a + 1][n / 2]);
+  };
+  if (__builtin_expect(__ballot(bad) != 0, 0)) {
+    for (int c = 0; c < ncol; ++c) {
+      const Reach rc{__builtin_amdgcn_readlane(mine.lo, c), __builtin_amdgcn_readlane(mine.len, c),
+                     __builtin_amdgcn_readlane(mine.sink, c)};
+      uint32_t keep[N / 2];  // the halves of each operand word whose positions the column attends
 #pragma unroll
       for (int a = 0; a < N / 2; ++a)
-        vt[a] = n % 2 ? pair_hi(v[2 * a][n / 2], v[2 * a + 1][n / 2]) : pair_lo(v[2 * a][n / 2], v[2 * a + 1][n / 2]);
-      st.acc[n] = mfma_pv<N>(vt, hi, st.acc[n]);
-      st.acc[n] = mfma_pv<N>(vt, lo, st.acc[n]);
-    }
-    return;
-  }
-  for (int c = 0; c < ncol; ++c) {
-    const Reach rc{__builtin_amdgcn_readlane(mine.lo, c), __builtin_amdgcn_readlane(mine.len, c),
-                   __builtin_amdgcn_readlane(mine.sink, c)};
-    uint32_t keep = 0;
+        keep[a] = (attends(rc, s, pos(2 * a)) ? 0xffffu : 0u) | (attends(rc, s, pos(2 * a + 1)) ? 0xffff0000u : 0u);
 #pragma unroll
-    for (int i = 0; i < N; ++i) keep |= attends(rc, s, pos(i)) ? 1u << i : 0u;
+      for (int n = 0; n < D / 16; ++n) {
+        uint32_t vt[N / 2];
+        operand(v, n, vt);
 #pragma unroll
-    for (int n = 0; n < D / 16; ++n) {
-      uint32_t vt[N / 2], vf[N / 2];
+        for (int a = 0; a < N / 2; ++a) {
+          vt[a] = odd_pair(vt[a]) & keep[a];
+          asm volatile("" : "+v"(vt[a]));  // worked out here, not for all columns before the loop (registers)
+        }
+        const f32x4_t t = mfma_pv<N>(vt, hi, f32x4_t{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-      for (int a = 0; a < N / 2; ++a) {
-        const uint32_t x = (keep >> (2 * a)) & 1 ? v[2 * a][n / 2] : 0u, y = (keep >> (2 * a + 1)) & 1 ? v[2 * a + 1][n / 2] : 0u;
-        vt[a] = n % 2 ? pair_hi(x, y) : pair_lo(x, y);
-        vf[a] = finite_pair(vt[a]);
+        for (int i = 0; i < 4; ++i) st.acc[n][i] += col == c ? t[i] : 0.f;
       }
-      const f32x4_t t = mfma_pv<N>(vf, lo, mfma_pv<N>(vt, hi, st.acc[n]));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) st.acc[n][i] = col == c ? t[i] : st.acc[n][i];
     }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int m = 0; m < D / 32; ++m) v[i][m] = finite_pair(v[i][m]);
+  }
+#pragma unroll
+  for (int n = 0; n < D / 16; ++n) {
+    uint32_t vt[N / 2];
+    operand(v, n, vt);
+    st.acc[n] = mfma_pv<N>(vt, hi, st.acc[n]);
+    st.acc[n] = mfma_pv<N>(vt, lo, st.acc[n]);
   }
 }
 
 // Merges nact partials of ncol columns in split order and writes out (and, tracked, each head's max and 1 / sum). Each
 // thread owns 4 consecutive values of one column; the weights of 16 splits at a time are worked out by the lanes of a
 // 16-lane row and handed round by DPP, as in merge_many. write(column, dim, values, max, sum).
-template <int D, class Write>
+template <int D, int NT, class Write>
 __device__ __forceinline__ void merge_columns(const float* part_acc, const float2* part_ml, int ncols_max, int ncol, int nact,
                                               Write write) {
   const Rsrc racc = span_rsrc(part_acc, nact * ncols_max * D * 4), rml = span_rsrc(part_ml, nact * ncols_max * 8);
   const int lane16 = threadIdx.x % 16;
-  for (int o = threadIdx.x; o < ncol * D / 4; o += kLongThreads) {
+  for (int o = threadIdx.x; o < ncol * D / 4; o += NT) {
     const int c = o / (D / 4);
     float m = -INFINITY, l = 0.f;
     f32x4_t a = {0.f, 0.f, 0.f, 0.f};
@@ -309,10 +318,10 @@ __device__ __forceinline__ void merge_columns(const float* part_acc, const float
 // ------------------------------------------------------------------------------------------------ split kernel
 
 // grid (splits, kv heads, rows * column tiles). KV4: a 4-bit cache. TRACK: also writes the scores (one token per row).
-template <int D, bool KV4, bool TRACK>
-__global__ void __launch_bounds__(kLongThreads, 2)
+template <int D, bool KV4, bool TRACK, int NT>
+__global__ void __launch_bounds__(NT, 2)
     long_split_kernel(const int32_t* lens, const int32_t* starts, const LongParams p) {
-  constexpr int P = KV4 ? 32 : 16, NS = P / 16, N = 4 * NS, NJ = D / 32;
+  constexpr int NW = NT / kWave, P = KV4 ? 32 : 16, NS = P / 16, N = 4 * NS, NJ = D / 32;
   const int split = blockIdx.x, h = blockIdx.y, z = blockIdx.z;
   const int b = p.tiles == 1 ? z : z / p.tiles, t0 = (z - b * p.tiles) * p.tpt;
   const int e_raw = lens[b], s_raw = (starts ? starts : lens)[b];
@@ -339,7 +348,7 @@ __global__ void __launch_bounds__(kLongThreads, 2)
   const TileRange tr = tile_range<P>(s, token_end(t0), token_end(t0 + ntok - 1), p.window, p.sinks);
   const int n = tr.na + tr.nb;
   int per = n <= p.one_split ? n : max(p.min_tiles, (n + p.splits - 1) / p.splits);
-  per = max(kLongWaves, (per + kLongWaves - 1) / kLongWaves * kLongWaves);
+  per = max(NW, (per + NW - 1) / NW * NW);
   const int nact = max(1, (n + per - 1) / per);
   if (split >= nact) return;
   const int j0 = split * per, j1 = min(n, j0 + per);
@@ -435,14 +444,14 @@ __global__ void __launch_bounds__(kLongThreads, 2)
 
   int j = j0 + w;
   load(ta, j);
-  load(tb, j + kLongWaves);
+  load(tb, j + NW);
   __builtin_amdgcn_sched_barrier(0);
-  for (; j < j1; j += 2 * kLongWaves) {
+  for (; j < j1; j += 2 * NW) {
     consume(ta, j);
-    if (j + kLongWaves >= j1) break;
-    load(ta, j + 2 * kLongWaves);
-    consume(tb, j + kLongWaves);
-    load(tb, j + 3 * kLongWaves);
+    if (j + NW >= j1) break;
+    load(ta, j + 2 * NW);
+    consume(tb, j + NW);
+    load(tb, j + 3 * NW);
   }
 
   // the columns are complete over the wave's positions; only the sums are still one per lane group
@@ -454,8 +463,8 @@ __global__ void __launch_bounds__(kLongThreads, 2)
   st.l += y;
 
   constexpr int PD = D + 4;  // keeps the 16-byte stores free of bank conflicts
-  __shared__ __align__(16) float s_acc[kLongWaves][kLongCols][PD];
-  __shared__ float s_m[kLongWaves][kLongCols], s_l[kLongWaves][kLongCols];
+  __shared__ __align__(16) float s_acc[NW][kLongCols][PD];
+  __shared__ float s_m[NW][kLongCols], s_l[NW][kLongCols];
   if (r < ncol) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -481,16 +490,16 @@ __global__ void __launch_bounds__(kLongThreads, 2)
 
   const int ncols_max = p.tpt << p.gshift;
   const int64_t unit = (int64_t)z * p.NKV + h;
-  for (int o = tid; o < ncol * D / 4; o += kLongThreads) {
+  for (int o = tid; o < ncol * D / 4; o += NT) {
     const int c = o / (D / 4), d = 4 * (o % (D / 4));
     float M = s_m[0][c];
 #pragma unroll
-    for (int u = 1; u < kLongWaves; ++u) M = fmaxf(M, s_m[u][c]);
+    for (int u = 1; u < NW; ++u) M = fmaxf(M, s_m[u][c]);
     const float mu = (M == -INFINITY) ? 0.f : M;
     float L = 0.f;
     f32x4_t A = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int u = 0; u < kLongWaves; ++u) {
+    for (int u = 0; u < NW; ++u) {
       const float f = fast_exp2(s_m[u][c] - mu);
       L = fmaf(f, s_l[u][c], L);
       const f32x4_t a = *reinterpret_cast<const f32x4_t*>(&s_acc[u][c][d]);
@@ -524,20 +533,20 @@ __global__ void __launch_bounds__(kLongThreads, 2)
   }
   __syncthreads();
   if (!s_last) return;
-  merge_columns<D>(p.part_acc + unit * p.splits * ncols_max * D, p.part_ml + unit * p.splits * ncols_max, ncols_max, ncol, nact,
+  merge_columns<D, NT>(p.part_acc + unit * p.splits * ncols_max * D, p.part_ml + unit * p.splits * ncols_max, ncols_max, ncol, nact,
                    write);
 }
 
 // weights_out[b, h, pos] = decay * weights[b, h, pos] + sum_g 2^(score - max_g) / sum_g over the row's range; grid (chunks of
-// kLongThreads * 4 positions, kv heads, rows), after the split kernel that wrote the scores. Four consecutive positions a
+// kApplyThreads * 4 positions, kv heads, rows), after the split kernel that wrote the scores. Four consecutive positions a
 // thread (16-byte score loads).
-__global__ void __launch_bounds__(kLongThreads)
+__global__ void __launch_bounds__(kApplyThreads)
     track_apply_kernel(const int32_t* lens, const int32_t* starts, const float* weights, float* weights_out, int64_t w_sb,
                        int64_t w_sh, int64_t wo_sb, int64_t wo_sh, float decay, const LongParams p) {
   const int h = blockIdx.y, b = blockIdx.z;
   int s, e;
   long_range(lens[b], (starts ? starts : lens)[b], starts != nullptr, p.cap, s, e);
-  const int pos0 = 4 * (int)(blockIdx.x * kLongThreads + threadIdx.x);
+  const int pos0 = 4 * (int)(blockIdx.x * kApplyThreads + threadIdx.x);
   if (pos0 >= e || pos0 + 4 <= s) return;
   f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
   for (int g = 0; g < p.G; ++g) {

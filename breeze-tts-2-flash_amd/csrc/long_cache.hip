@@ -14,6 +14,9 @@ int device_cu_count(int* cus);  // gqa_decode.hip
 
 namespace {
 
+// Threads of a split workgroup. Eight waves measured 6% faster on long rows of 4 bits (4 rows x 4 kv heads of 20001..32768,
+// G 8: 17.9 against 19.0 us) and 2 to 40% slower on everything else.
+constexpr int kLongThreads = 256;
 constexpr int kKv4Tokens = 16;  // most query tokens per row over a 4-bit cache
 
 // Columns (tokens times q heads of a kv head) from which a chunk takes the kernel of window_prefill.cuh.
@@ -57,17 +60,22 @@ int make_plan(int kind, int B, int NH, int NKV, int D, int cap, int T, int windo
 
   // positions a column tile attends, in wave tiles
   int64_t len = max_seq_len > 0 && max_seq_len < cap ? max_seq_len : cap;
-  if (window > 0 && (int64_t)window + pl->tpt + sinks < len) len = (int64_t)window + pl->tpt + sinks;
+  const bool cut = window > 0 && (int64_t)window + pl->tpt + sinks < len;  // the rows reach past the window
+  if (cut) len = (int64_t)window + pl->tpt + sinks;
   const int P = kv4 ? 32 : 16;
   const int n = (int)((len + P - 1) / P) + 1;
-  pl->min_tiles = kLongWaves;
+  pl->min_tiles = kLongThreads / kWave;
   pl->one_split = (kOneSplitBytes / (kv4 ? D + D / 16 : 4 * D)) / P;
   int splits = num_splits;
   if (splits == 0) {
     int cus = 0;
     const int rc = bz::device_cu_count(&cus);
     if (rc != BZ_OK) return rc;
-    splits = (int)(2 * cus / pl->units);
+    // One round of workgroups where a window makes the rows alike (4 rows x 8 kv heads, window 4096: 8 splits 15.2 us, 16
+    // 15.3..16.0; 16 rows: 2 splits 42.6, 4 44.8), two where their lengths differ (track, 4 rows of 9000..16384: 8 splits 49.7,
+    // 16 47.3) and for 4-bit tiles, whose conversion leaves a wave alone on its SIMD half idle (16 kv heads x 32768: 16
+    // splits 19.2, 32 19.0; 1 row x 8 of 8192: 32 splits 8.2, 64 7.6 .. 8.6).
+    splits = (int)((kv4 || !cut ? 2 : 1) * cus / pl->units);
     const int most = (n + pl->min_tiles - 1) / pl->min_tiles;
     if (splits > most) splits = most;
     if (splits > 64) splits = 64;
@@ -167,9 +175,9 @@ template <bool KV4, bool TRACK>
 int launch_split(const bz_gqa_decode_args* a, int D, const LongParams& p, const Plan& pl, int B, hipStream_t stream) {
   const dim3 grid(pl.splits, p.NKV, B * pl.tiles);
   if (D == 128)
-    hipLaunchKernelGGL((long_split_kernel<128, KV4, TRACK>), grid, dim3(kLongThreads), 0, stream, a->seq_lens, a->kv_start, p);
+    hipLaunchKernelGGL((long_split_kernel<128, KV4, TRACK, kLongThreads>), grid, dim3(kLongThreads), 0, stream, a->seq_lens, a->kv_start, p);
   else
-    hipLaunchKernelGGL((long_split_kernel<64, KV4, TRACK>), grid, dim3(kLongThreads), 0, stream, a->seq_lens, a->kv_start, p);
+    hipLaunchKernelGGL((long_split_kernel<64, KV4, TRACK, kLongThreads>), grid, dim3(kLongThreads), 0, stream, a->seq_lens, a->kv_start, p);
   return hipGetLastError() == hipSuccess ? BZ_OK : BZ_ERR_LAUNCH;
 }
 
@@ -254,8 +262,8 @@ BZ_EXPORT int bz_gqa_decode_tracked(const bz_gqa_tracked_args* ta, hipStream_t s
   const LongParams p = long_params(a, pl, 0, 0);
   rc = launch_split<false, true>(a, a->head_dim, p, pl, a->batch, stream);
   if (rc != BZ_OK) return rc;
-  const dim3 grid((a->capacity + 4 * kLongThreads - 1) / (4 * kLongThreads), a->num_kv_heads, a->batch);
-  hipLaunchKernelGGL(track_apply_kernel, grid, dim3(kLongThreads), 0, stream, a->seq_lens, a->kv_start, ta->weights,
+  const dim3 grid((a->capacity + 4 * kApplyThreads - 1) / (4 * kApplyThreads), a->num_kv_heads, a->batch);
+  hipLaunchKernelGGL(track_apply_kernel, grid, dim3(kApplyThreads), 0, stream, a->seq_lens, a->kv_start, ta->weights,
                      ta->weights_out, ta->w_stride_b, ta->w_stride_h, ta->wo_stride_b, ta->wo_stride_h, ta->decay, p);
   return hipGetLastError() == hipSuccess ? BZ_OK : BZ_ERR_LAUNCH;
 }
