@@ -19,9 +19,6 @@ namespace {
 constexpr int kLongThreads = 256;
 constexpr int kKv4Tokens = 16;  // most query tokens per row over a 4-bit cache
 
-// Columns (tokens times q heads of a kv head) from which a chunk takes the kernel of window_prefill.cuh.
-constexpr int64_t kPrefillCols = 64;
-
 bool dim_ok(int D) { return D == 64 || D == 128; }
 bool group_ok(int G) { return G == 1 || G == 2 || G == 4 || G == 8; }
 size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -31,6 +28,7 @@ size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 // written before it is read).
 struct Plan {
   bool prefill;  // gqa_window: the chunk kernel, which needs no workspace
+  int cgroups;   // its column groups
   int G, gshift, tpt, tiles, splits, min_tiles, one_split, score_stride;
   int64_t units;
   size_t ml, acc, head_ml, scores, total;
@@ -49,9 +47,24 @@ int make_plan(int kind, int B, int NH, int NKV, int D, int cap, int T, int windo
   pl->tpt = kLongCols / pl->G < T ? kLongCols / pl->G : T;
   pl->tiles = (T + pl->tpt - 1) / pl->tpt;
   pl->units = (int64_t)B * pl->tiles * NKV;
-  pl->prefill = kind == BZ_LONG_WINDOW && (int64_t)T * pl->G >= kPrefillCols;
+  int cus = 0;
+  if (num_splits == 0 || (kind == BZ_LONG_WINDOW && pl->tiles > 1)) {
+    const int rc = bz::device_cu_count(&cus);
+    if (rc != BZ_OK) return rc;
+  }
+  // A chunk whose 16-column tiles would be more workgroups than CUs takes the kernel of window_prefill.cuh: the split kernel
+  // reads K and V again for each tile of 16 columns, but spreads a few of them over the whole device (us, split / chunk
+  // kernel, head_dim 128: 8 kv heads, 4096 positions, 64 columns 14.0 / 40.3, 256 27.5 / 40.6, 512 43.9 / 40.7; 4 rows x 8,
+  // window 1024: 128 columns 13.1 / 16.7, 256 23.8 / 17.7; 2 x 4 heads, head_dim 64, 4096 positions: 256 17.0 / 22.6, 512
+  // 28.0 / 22.7).
+  pl->prefill = kind == BZ_LONG_WINDOW && pl->tiles > 1 && pl->units >= cus;
   if (pl->prefill) {
-    pl->tiles = (int)(((int64_t)T * pl->G + kPreCols - 1) / kPreCols);
+    auto tiles = [&](int cg) { return ((int64_t)T * pl->G + kPreWaveCols * cg - 1) / (kPreWaveCols * cg); };
+    // The widest column tiles that still give every CU work, three workgroups each for the widest (us for 1 / 2 / 4 groups,
+    // head_dim 128: 2 x 8 kv heads x 2048 tokens 122.8 / 53.1 / 57.5; 8 x 8192, window 4096: 509 / 243 / 223; 8 x 1024: 23.1 /
+    // 18.0 / 23.6; 8 x 512 behind 3584: 40.5 / 49.2 / 71.4).
+    pl->cgroups = tiles(4) * B * NKV >= 3 * cus ? 4 : tiles(2) * B * NKV >= cus ? 2 : 1;
+    pl->tiles = (int)tiles(pl->cgroups);
     pl->splits = 1;
     pl->ml = pl->acc = pl->head_ml = pl->scores = pl->total = 0;
     return pl->tiles <= 65535 && B <= 65535 ? BZ_OK : BZ_ERR_SHAPE;
@@ -68,9 +81,6 @@ int make_plan(int kind, int B, int NH, int NKV, int D, int cap, int T, int windo
   pl->one_split = (kOneSplitBytes / (kv4 ? D + D / 16 : 4 * D)) / P;
   int splits = num_splits;
   if (splits == 0) {
-    int cus = 0;
-    const int rc = bz::device_cu_count(&cus);
-    if (rc != BZ_OK) return rc;
     // One round of workgroups where a window makes the rows alike (4 rows x 8 kv heads, window 4096: 8 splits 15.2 us, 16
     // 15.3..16.0; 16 rows: 2 splits 42.6, 4 44.8), two where their lengths differ (track, 4 rows of 9000..16384: 8 splits 49.7,
     // 16 47.3) and for 4-bit tiles, whose conversion leaves a wave alone on its SIMD half idle (16 kv heads x 32768: 16
@@ -216,10 +226,10 @@ BZ_EXPORT int bz_gqa_window(const bz_gqa_window_args* wa, hipStream_t stream) {
   const LongParams p = long_params(a, pl, wa->window, wa->sinks);
   if (!pl.prefill) return launch_split<false, false>(a, a->head_dim, p, pl, a->batch, stream);
   const dim3 grid(a->num_kv_heads, pl.tiles, a->batch);
-  if (a->head_dim == 128)
-    hipLaunchKernelGGL(window_prefill_kernel<128>, grid, dim3(kPreThreads), 0, stream, a->seq_lens, a->kv_start, p);
-  else
-    hipLaunchKernelGGL(window_prefill_kernel<64>, grid, dim3(kPreThreads), 0, stream, a->seq_lens, a->kv_start, p);
+  using Fn = void (*)(const int32_t*, const int32_t*, const LongParams);
+  const Fn fns[2][3] = {{window_prefill_kernel<64, 1>, window_prefill_kernel<64, 2>, window_prefill_kernel<64, 4>},
+                        {window_prefill_kernel<128, 1>, window_prefill_kernel<128, 2>, window_prefill_kernel<128, 4>}};
+  hipLaunchKernelGGL(fns[a->head_dim == 128][pl.cgroups / 2], grid, dim3(kPreThreads), 0, stream, a->seq_lens, a->kv_start, p);
   return hipGetLastError() == hipSuccess ? BZ_OK : BZ_ERR_LAUNCH;
 }
 

@@ -1,9 +1,13 @@
 // Device code of bz_gqa_window over a chunk of many query tokens (include/bz_long_cache.h).
 //
-// A workgroup of four waves takes 128 columns: (token, q head) pairs of one kv head, 128 / G tokens of a row times its G
-// heads, 32 a wave, so K and V are fetched once for the whole group. It walks the positions any of its tokens attends (the
-// sinks' tiles, then the window's; tile_range) in tiles of 64 staged in LDS, two buffers each of K and V, the next loads in
-// flight while a tile is worked on.
+// The (token, q head) pairs of one kv head are the columns of two products, 32 a wave. The four waves of a workgroup are CG
+// column groups times PG = 4 / CG position groups: 4 x 1 fetches K and V once for 128 columns (128 / G tokens of a row times
+// its G heads); with 2 x 2 and 1 x 4 a small chunk has more workgroups and fewer steps, each position group taking every
+// PG-th tile, and the groups' accumulators are merged through LDS at the end by the log-sum-exp rule.
+//
+// A workgroup walks the positions any of its tokens attends (the sinks' tiles, then the window's; tile_range) in tiles of 64
+// (PG = 1) or 32 positions staged in LDS, two buffers each of K and V per position group, the next loads in flight while a
+// tile is worked on.
 //   S^T = K Q^T   mfma 32x32x16: A = K rows, B = Q^T (registers, loaded once). A lane then holds 32 scores of one column, the
 //                 rows 8 (v / 4) + 4 half + v % 4 of each block of 32 positions, so the softmax is within a lane but for one
 //                 swap with lane ^ 32.
@@ -21,29 +25,30 @@ namespace {
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef short s16x4_lds __attribute__((ext_vector_type(4)));
 
-constexpr int kPreThreads = 256, kPreCols = 128, kPreTile = 64, kPreRows = kPreTile / 4;
+constexpr int kPreThreads = 256, kPreWaveCols = 32;
 
-// LDS of one buffer: K, then V, 64 rows of D bf16 each, in 16-byte chunks. Chunk c of row r lies in slot c ^ swizzle(r), so
-// that the lanes of one read, which take the same chunk of different rows, fall into different banks.
-template <int D>
+// LDS of one tile of K or V: TP rows of D bf16, in 16-byte chunks. Chunk c of row r lies in slot c ^ swizzle(r), so that the
+// lanes of one read, which take the same chunk of different rows, fall into different banks.
+template <int D, int TP>
 struct PreLds {
-  static constexpr int kRow = 2 * D, kBytes = kPreTile * kRow;
+  static constexpr int kRow = 2 * D, kBytes = TP * kRow;
   static __device__ __forceinline__ int k_swz(int r) { return r & (D / 8 - 1); }
   static __device__ __forceinline__ int v_swz(int r) { return D == 128 ? 2 * (r & 7) : 2 * ((r >> 1) & 3); }
 };
 
-// Loads the 64 rows from pos0 on (clamped to `last`: a row past it holds a copy of that one, and no column attends it) into
-// LDS at base: 64 lanes write 1 KB in lane order, so the swizzle is in which chunk each lane fetches.
-template <int D, bool V>
-__device__ __forceinline__ void stage_tile(char* base, const Rsrc& rsrc, int pos0, int last, uint32_t row_bytes, int w, int lane) {
-  using L = PreLds<D>;
+// Loads the TP rows from pos0 on (clamped to `last`: a row past it holds a copy of that one, and no column attends it) into
+// LDS at base, by CG waves (this one is cg): 64 lanes write 1 KB in lane order, so the swizzle is in which chunk each lane
+// fetches.
+template <int D, int TP, int CG, bool V>
+__device__ __forceinline__ void stage_tile(char* base, const Rsrc& rsrc, int pos0, int last, uint32_t row_bytes, int cg, int lane) {
+  using L = PreLds<D, TP>;
   constexpr int RPI = 1024 / L::kRow, CH = D / 8;  // rows an instruction, chunks a row
 #pragma unroll
-  for (int u = 0; u < kPreRows / RPI; ++u) {
-    const int row = kPreRows * w + RPI * u + lane / CH, c = lane % CH;
+  for (int u = 0; u < L::kBytes / 1024 / CG; ++u) {
+    const int row0 = RPI * (cg * (L::kBytes / 1024 / CG) + u), row = row0 + lane / CH, c = lane % CH;
     const uint32_t off = (uint32_t)min(pos0 + row, last) * row_bytes + 16 * (c ^ (V ? L::v_swz(row) : L::k_swz(row)));
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(
-        rsrc, (__attribute__((address_space(3))) void*)(base + (kPreRows * w + RPI * u) * L::kRow), 16, off, 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(base + row0 * L::kRow), 16, off, 0, 0,
+                                             0);
   }
 }
 
@@ -51,13 +56,13 @@ __device__ __forceinline__ void stage_tile(char* base, const Rsrc& rsrc, int pos
 // result is not finite, which is right where the column attends an infinity or NaN and wrong where a tile held one that it
 // does not (0 times it). The lanes score 64 positions, then each accumulates D / 64 dims over them.
 template <int D>
-__device__ __forceinline__ void prefill_careful(const LongParams& p, int b, int h, int s, int e, int t0, int ntok, int w) {
+__device__ __forceinline__ void prefill_careful(const LongParams& p, int b, int h, int s, int e, int t0, int ntok, int cg) {
   constexpr int DV = D / 64;
   const int lane = threadIdx.x % kWave;
   const char* const kb = p.k + (int64_t)b * p.kv_sb + (int64_t)h * p.kv_sh;
   const char* const vb = p.v + (int64_t)b * p.kv_sb + (int64_t)h * p.kv_sh;
-  for (int c = 0; c < 32; ++c) {
-    const int m0 = 32 * w + c, tok = t0 + (m0 >> p.gshift), hq = (h << p.gshift) + (m0 & (p.G - 1));
+  for (int c = 0; c < kPreWaveCols; ++c) {
+    const int m0 = kPreWaveCols * cg + c, tok = t0 + (m0 >> p.gshift), hq = (h << p.gshift) + (m0 & (p.G - 1));
     if (tok >= t0 + ntok) break;
     const int end = max(s, e - (p.T - 1 - tok));
     const Reach r = reach_of(s, end, p.window, p.sinks);
@@ -100,17 +105,18 @@ __device__ __forceinline__ void prefill_careful(const LongParams& p, int b, int 
 
 // grid (kv heads, column tiles, rows): workgroups go to the XCDs in turn, so with a multiple of 8 kv heads each head's K and V
 // pass through one XCD's L2 alone. The last tiles, which attend most, start first.
-template <int D>
+template <int D, int CG>
 __global__ void __launch_bounds__(kPreThreads, 2)
     window_prefill_kernel(const int32_t* lens, const int32_t* starts, const LongParams p) {
-  using L = PreLds<D>;
-  constexpr int NQ = D / 16, ND = D / 32;
+  constexpr int PG = 4 / CG, TP = PG == 1 ? 64 : 32, NB = TP / 32, NQ = D / 16, ND = D / 32, kCols = CG * kPreWaveCols;
+  using L = PreLds<D, TP>;
   const int h = blockIdx.x, tile = gridDim.y - 1 - blockIdx.y, b = blockIdx.z;
   const int e_raw = lens[b], s_raw = (starts ? starts : lens)[b];
   const int lane = threadIdx.x % kWave, w = wave_uniform((int)threadIdx.x / kWave), c = lane % 32, half = lane / 32;
+  const int cg = w % CG, pg = w / CG;
 
-  const int t0 = tile * (kPreCols >> p.gshift), ntok = min(kPreCols >> p.gshift, p.T - t0);
-  const int mine = 32 * w + c, tok = t0 + min(mine >> p.gshift, ntok - 1), hq = (h << p.gshift) + (mine & (p.G - 1));
+  const int t0 = tile * (kCols >> p.gshift), ntok = min(kCols >> p.gshift, p.T - t0);
+  const int mine = kPreWaveCols * cg + c, tok = t0 + min(mine >> p.gshift, ntok - 1), hq = (h << p.gshift) + (mine & (p.G - 1));
 
   const float scale = positive_scale(p.scale_log2);
   bf16x8_t qf[NQ];
@@ -125,28 +131,30 @@ __global__ void __launch_bounds__(kPreThreads, 2)
   auto token_end = [&](int t) { return max(s, e - (p.T - 1 - t)); };
   const Reach me = reach_of(s, token_end(tok), p.window, p.sinks);
   const int e1 = token_end(t0 + ntok - 1);
-  const TileRange tr = tile_range<kPreTile>(s, token_end(t0), e1, p.window, p.sinks);
-  const int n = tr.na + tr.nb;
-  auto pos_of = [&](int j) { return j < tr.na ? tr.fa + kPreTile * j : tr.fb + kPreTile * (j - tr.na); };
-  // of this wave's tokens: the first one's end, and the last one's window start and end
-  const int wt0 = t0 + min((32 * w) >> p.gshift, ntok - 1), wt1 = t0 + min((32 * w + 31) >> p.gshift, ntok - 1);
-  const int we0 = token_end(wt0), we1 = token_end(wt1);
-  const int wlo1 = max(s, we1 - p.window);
+  const TileRange tr = tile_range<TP>(s, token_end(t0), e1, p.window, p.sinks);
+  const int n = (tr.na + tr.nb + PG - 1) / PG;  // steps; position group pg takes tile PG j + pg in step j
+  auto pos_of = [&](int j) {  // (a tile past the last begins at or past e1: nothing there is attended)
+    const int i = PG * j + pg;
+    return i < tr.na ? tr.fa + TP * i : tr.fb + TP * (i - tr.na);
+  };
+  // every column of the wave attends the whole of [whole_lo, whole_end)
+  const int whole_end = token_end(t0 + min((kPreWaveCols * cg) >> p.gshift, ntok - 1));
+  const int whole_lo = max(s, token_end(t0 + min((kPreWaveCols * cg + kPreWaveCols - 1) >> p.gshift, ntok - 1)) - p.window);
 
   // arrays of their own, and the tiles' parity known at compile time: the compiler then sees that the reads of one do not
   // depend on the loads in flight to another (it would wait for all of them)
-  __shared__ __align__(16) char k_even[L::kBytes], k_odd[L::kBytes], v_even[L::kBytes], v_odd[L::kBytes];
+  __shared__ __align__(16) char k_even[PG * L::kBytes], k_odd[PG * L::kBytes], v_even[PG * L::kBytes], v_odd[PG * L::kBytes];
   const int64_t head = (int64_t)b * p.kv_sb + (int64_t)h * p.kv_sh;
   const uint32_t row_bytes = (uint32_t)p.kv_ss;
   const Rsrc rk = span_rsrc(p.k + head, e1 * (int)p.kv_ss), rv = span_rsrc(p.v + head, e1 * (int)p.kv_ss);
 
   // this lane's LDS addresses: K chunk 2 j + half of row c; V, transposed: the four rows and 16 dims of its group of 16 lanes
-  const int k_addr = c * L::kRow, k_sw = L::k_swz(c);
+  const int group = pg * L::kBytes, k_addr = group + c * L::kRow, k_sw = L::k_swz(c);
   const int l16 = lane % 16, v_row = 4 * half + l16 / 4;
   int v_addr[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d)
-    v_addr[d] = v_row * L::kRow + 16 * ((4 * d + 2 * ((lane / 16) % 2) + (l16 % 4) / 2) ^ L::v_swz(v_row)) + 8 * (l16 % 2);
+    v_addr[d] = group + v_row * L::kRow + 16 * ((4 * d + 2 * ((lane / 16) % 2) + (l16 % 4) / 2) ^ L::v_swz(v_row)) + 8 * (l16 % 2);
 
   float m = -INFINITY, l = 0.f;
   f32x16_t acc[ND];
@@ -155,10 +163,10 @@ __global__ void __launch_bounds__(kPreThreads, 2)
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
 
-  // K operand i of the tile in buf: positions 32 (i % 2) .., contraction step i / 2 (the two blocks' products alternate, since
-  // one that adds to the product before it waits for it)
+  // K operand i of the tile in buf: positions 32 (i % NB) .., contraction step i / NB (the two blocks' products alternate,
+  // since one that adds to the product before it waits for it)
   auto k_read = [&](const char* buf, int i) __attribute__((always_inline)) {
-    return *reinterpret_cast<const bf16x8_t*>(buf + k_addr + 32 * (i % 2) * L::kRow + 16 * ((2 * (i / 2) + half) ^ k_sw));
+    return *reinterpret_cast<const bf16x8_t*>(buf + k_addr + 32 * (i % NB) * L::kRow + 16 * ((2 * (i / NB) + half) ^ k_sw));
   };
   // V^T operand d of 16 positions: the lane's 8, in two reads
   auto v_read = [&](const char* buf, int ut, int d) __attribute__((always_inline)) {
@@ -168,34 +176,34 @@ __global__ void __launch_bounds__(kPreThreads, 2)
     const uint2 b = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Tr)(at + 8 * L::kRow)));
     return __builtin_bit_cast(bf16x8_t, make_uint4(a.x, a.y, b.x, b.y));
   };
-  constexpr int NK = 2 * NQ, PG = 16 / NK;  // products of K q, and pairs of terms worked out beside each
+  constexpr int NK = NB * NQ, PT = 8 * NB / NK, KA = NK < 8 ? NK : 8;  // products of K q, pairs of terms beside each, reads ahead
   // Tile j: its scores x into the running maximum, sum and accumulators, and the scores of tile j + 1 (next; unused after the
   // last). A wave has the matrix unit, the vector unit and LDS at work at once only if its instructions alternate, and an
-  // operand read just before its product costs the LDS latency each time: so the first 8 K operands are read before the
-  // maximum is taken, each product of K q is followed by the read 8 products ahead (or of V) and a share of the
+  // operand read just before its product costs the LDS latency each time: so the first KA K operands are read before the
+  // maximum is taken, each product of K q is followed by the read KA products ahead (or of V) and a share of the
   // exponentials, and each product of V p by the read 4 ahead. The scheduling barriers keep that order.
-  auto step = [&](auto odd, int j, f32x16_t (&x)[2], f32x16_t (&next)[2]) __attribute__((always_inline)) {
+  auto step = [&](auto odd, int j, f32x16_t (&x)[NB], f32x16_t (&next)[NB]) __attribute__((always_inline)) {
     constexpr bool kOdd = decltype(odd)::value;
     const char *const kbuf = kOdd ? k_even : k_odd, *const vbuf = kOdd ? v_odd : v_even;
     __builtin_amdgcn_s_waitcnt(0x0f70);  // this wave's loads of K j + 1 and V j are in LDS
     __syncthreads();                     // everyone's are, and nobody reads K j or V j - 1 any more
-    bf16x8_t kf[8], vf[2][ND];
+    bf16x8_t kf[KA], vf[2][ND];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) kf[i] = k_read(kbuf, i);
+    for (int i = 0; i < KA; ++i) kf[i] = k_read(kbuf, i);
     __builtin_amdgcn_sched_barrier(0);
-    if (j + 2 < n) stage_tile<D, false>(kOdd ? k_odd : k_even, rk, pos_of(j + 2), e1 - 1, row_bytes, w, lane);
-    if (j + 1 < n) stage_tile<D, true>(kOdd ? v_even : v_odd, rv, pos_of(j + 1), e1 - 1, row_bytes, w, lane);
+    if (j + 2 < n) stage_tile<D, TP, CG, false>((kOdd ? k_odd : k_even) + group, rk, pos_of(j + 2), e1 - 1, row_bytes, cg, lane);
+    if (j + 1 < n) stage_tile<D, TP, CG, true>((kOdd ? v_even : v_odd) + group, rv, pos_of(j + 1), e1 - 1, row_bytes, cg, lane);
     const int p0 = pos_of(j);
-    if (!(p0 + kPreTile <= we0 && p0 >= wlo1)) {
+    if (!(p0 + TP <= whole_end && p0 >= whole_lo)) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < NB; ++u)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           x[u][i] = attends(me, s, p0 + 32 * u + 8 * (i / 4) + 4 * half + i % 4) ? x[u][i] : -INFINITY;
     }
     float top = x[0][0];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < NB; ++u)
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, x[u][i]);
     float other = top;
@@ -211,16 +219,16 @@ __global__ void __launch_bounds__(kPreThreads, 2)
       for (int d = 0; d < ND; ++d) acc[d] *= alpha;
     }
     const float base = m == -INFINITY ? 0.f : m;
-    uint32_t pk[2][8];
+    uint32_t pk[NB][8];
     const f32x16_t zero = {};
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
-      next[i % 2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i % 8], qf[i / 2], i < 2 ? zero : next[i % 2], 0, 0, 0);
-      if (i + 8 < NK) kf[i % 8] = k_read(kbuf, i + 8);
-      else if (i - (NK - 8) < ND) vf[0][i - (NK - 8)] = v_read(vbuf, 0, i - (NK - 8));
+      next[i % NB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[i % KA], qf[i / NB], i < NB ? zero : next[i % NB], 0, 0, 0);
+      if (i + KA < NK) kf[i % KA] = k_read(kbuf, i + KA);
+      else if (i - (NK - KA) < ND) vf[0][i - (NK - KA)] = v_read(vbuf, 0, i - (NK - KA));
 #pragma unroll
-      for (int g = PG * i; g < PG * (i + 1); ++g) {
+      for (int g = PT * i; g < PT * (i + 1); ++g) {
         const int u = g / 8, v = 2 * (g % 8);
         pk[u][g % 8] = pack_bf16x2(fast_exp2(fmaf(x[u][v], scale, -base)), fast_exp2(fmaf(x[u][v + 1], scale, -base)));
         l = dot2_bf16(pk[u][g % 8], 0x3f803f80u, l);  // the sum of the rounded terms, the ones that meet V
@@ -228,27 +236,27 @@ __global__ void __launch_bounds__(kPreThreads, 2)
       __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
-    for (int ut = 0; ut < 4; ++ut) {
+    for (int ut = 0; ut < 2 * NB; ++ut) {
       const uint32_t* const q = &pk[ut / 2][4 * (ut % 2)];
       const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, make_uint4(q[0], q[1], q[2], q[3]));
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
         acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[ut % 2][d], pf, acc[d], 0, 0, 0);
-        if (ut < 3) vf[(ut + 1) % 2][d] = v_read(vbuf, ut + 1, d);
+        if (ut + 1 < 2 * NB) vf[(ut + 1) % 2][d] = v_read(vbuf, ut + 1, d);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
   };
   if (n > 0) {
-    stage_tile<D, false>(k_even, rk, pos_of(0), e1 - 1, row_bytes, w, lane);
+    stage_tile<D, TP, CG, false>(k_even + group, rk, pos_of(0), e1 - 1, row_bytes, cg, lane);
     __builtin_amdgcn_s_waitcnt(0x0f70);
     __syncthreads();
-    if (n > 1) stage_tile<D, false>(k_odd, rk, pos_of(1), e1 - 1, row_bytes, w, lane);
-    stage_tile<D, true>(v_even, rv, pos_of(0), e1 - 1, row_bytes, w, lane);
-    f32x16_t xa[2], xb[2];
+    if (n > 1) stage_tile<D, TP, CG, false>(k_odd + group, rk, pos_of(1), e1 - 1, row_bytes, cg, lane);
+    stage_tile<D, TP, CG, true>(v_even + group, rv, pos_of(0), e1 - 1, row_bytes, cg, lane);
+    f32x16_t xa[NB], xb[NB];
 #pragma unroll
     for (int i = 0; i < NK; ++i)
-      xa[i % 2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_read(k_even, i), qf[i / 2], i < 2 ? f32x16_t{} : xa[i % 2], 0, 0, 0);
+      xa[i % NB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_read(k_even, i), qf[i / NB], i < NB ? f32x16_t{} : xa[i % NB], 0, 0, 0);
     for (int j = 0; j < n; j += 2) {
       step(std::false_type{}, j, xa, xb);
       if (j + 1 < n) step(std::true_type{}, j + 1, xb, xa);
@@ -258,6 +266,42 @@ __global__ void __launch_bounds__(kPreThreads, 2)
   float other = l;
   swap32(l, other);
   l += other;
+  if constexpr (PG > 1) {
+    // the position groups' accumulators through the tiles' LDS: for PG = 4 groups 2 and 3 to 0 and 1, then (as for PG = 2)
+    // group 1 to 0
+    __shared__ float s_m[4][kPreWaveCols], s_l[4][kPreWaveCols];
+#pragma unroll
+    for (int from = PG / 2; from > 0; from /= 2) {
+      __syncthreads();  // the tiles, or the round before, have been read
+      const bool gives = pg >= from && pg < 2 * from, takes = pg < from;
+      const int giver = gives ? w : w + from * CG;  // its wave
+      char* const at = (giver % 2 ? k_odd : k_even) + 16 * lane;  // 16 ND registers of a wave: 4 KB ND, half an array's least
+      if (gives) {
+        if (half == 0) s_m[w][c] = m, s_l[w][c] = l;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<f32x4_t*>(at + 4096 * d + 256 * i) = f32x4_t{acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]};
+      }
+      __syncthreads();
+      if (takes) {
+        const float mo = s_m[giver][c], mn = fmaxf(m, mo), mu = mn == -INFINITY ? 0.f : mn;
+        const float f0 = fast_exp2(m - mu), f1 = fast_exp2(mo - mu);
+        m = mn;
+        l = l * f0 + s_l[giver][c] * f1;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            const f32x4_t y = *reinterpret_cast<const f32x4_t*>(at + 4096 * d + 256 * i);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[d][i + k] = acc[d][i + k] * f0 + y[k] * f1;
+          }
+      }
+    }
+    if (pg > 0) return;
+  }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   float worst = 0.f;
 #pragma unroll
@@ -265,7 +309,7 @@ __global__ void __launch_bounds__(kPreThreads, 2)
 #pragma unroll
     for (int i = 0; i < 16; ++i) worst += fabsf(acc[d][i]) * 0x1p-8f;
   if (__builtin_expect(__ballot(!(worst < INFINITY) || !(l < INFINITY)) != 0, 0)) {
-    prefill_careful<D>(p, b, h, s, e, t0, ntok, w);
+    prefill_careful<D>(p, b, h, s, e, t0, ntok, cg);
     return;
   }
   if ((mine >> p.gshift) >= ntok) return;

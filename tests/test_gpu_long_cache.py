@@ -62,6 +62,12 @@ WINDOW_CASES = [
     (1, 2, 64, 64, 64, [64], None, 1000, 1000),
     (1, 2, 128, 260, 257, [257, 260], [0, 100], 70, 0),
     (1, 1, 128, 200, 200, [200], None, 129, 3),
+    # as many columns as the chunk kernel takes, by one, two and four column groups of a workgroup
+    (8, 4, 128, 200, 160, [200, 170], [30, 0], 77, 4),
+    (8, 8, 64, 150, 150, [150, 149, 3], [0, 5, 0], 40, 9),
+    (8, 8, 128, 330, 300, [330, 300], None, 100, 0),
+    (8, 8, 64, 515, 515, [515, 400, 90], [0, 3, 0], 0, 0),
+    (8, 8, 128, 390, 390, [390, 389, 200, 1], [0, 30, 0, 0], 64, 1),
 ]
 
 
@@ -122,20 +128,23 @@ def test_window_layouts(device, T):
     assert (full[..., D:] == 7).all()
 
 
-@pytest.mark.parametrize("T", [3, 70])
+# the split kernel, and the chunk kernel by one, two and four column groups
+@pytest.mark.parametrize("T,NKV,G,D", [(3, 1, 2, 128), (70, 1, 2, 128), (70, 8, 8, 128), (70, 8, 8, 64), (130, 32, 8, 128),
+                                       (800, 64, 2, 128), (800, 64, 2, 64)])
 @pytest.mark.parametrize("value", [float("inf"), float("nan")])
-def test_unattended_values_do_not_reach_a_token(device, T, value):
+def test_unattended_values_do_not_reach_a_token(device, T, NKV, G, D, value):
     """A position that some tokens of a chunk attend and others do not: only those that do may see what it holds."""
     rng = np.random.default_rng(T)
-    NKV, G, D, n, window, sinks = 1, 2, 128, 200, 30, 2
+    n, window, sinks = T + 130, 30, 2
     q, k, v = randn(rng, 1, NKV * G, T, D), randn(rng, 1, NKV, n, D), randn(rng, 1, NKV, n, D)
     at = [n - 1, n - T + 1, n - T - window + 2]
     vp = v.clone()
     vp[0, 0, at, 5] = value
     out = pkg.gqa_window(q.to(device), k.to(device), vp.to(device), ints([n], device), D ** -0.5, window, sinks=sinks)
-    out = out.float().cpu()[0]
+    assert torch.isfinite(out[0, :, G:].float()).all()  # the other kv heads
+    out = out.float().cpu()[0, :, :G]
     clean = pkg.gqa_window(q.to(device), k.to(device), v.to(device), ints([n], device), D ** -0.5, window, sinks=sinks)
-    clean = clean.float().cpu()[0]
+    clean = clean.float().cpu()[0, :, :G]
     from oracle.long_cache import attended
     for t, pos in enumerate(attended(0, n, T, window, sinks)):
         hit = any(a in pos for a in at)
@@ -152,7 +161,7 @@ def test_unattended_values_do_not_reach_a_token(device, T, value):
     kp = k.clone()
     kp[0, 0, n - 1] = float("nan")
     out = pkg.gqa_window(q.to(device), kp.to(device), v.to(device), ints([n], device), D ** -0.5, window, sinks=sinks)
-    assert torch.isnan(out[0, T - 1].float()).all() and torch.isfinite(out[0, :T - 1].float()).all()
+    assert torch.isnan(out[0, T - 1, :G].float()).all() and torch.isfinite(out[0, :T - 1].float()).all()
 
 
 @pytest.mark.parametrize("scale", [-0.3, 0.0, 3.0])
