@@ -30,6 +30,7 @@ struct LongParams {
   int out_wide;                 // out and its strides are multiples of 8 bytes
   int NKV, G, gshift, T, cap;   // G = 1 << gshift q heads per kv head
   int tiles, tpt;               // column tiles per row, tokens per column tile (16 / G)
+  float inv_splits;             // 1 / splits
   int splits, min_tiles, one_split;  // a split takes at least min_tiles wave tiles; up to one_split in all are not split
   float* part_acc;              // [row * tile, kv head, split, column, D] unnormalised sums
   float2* part_ml;              // [row * tile, kv head, split, column] (max, sum)
@@ -37,6 +38,11 @@ struct LongParams {
   float* scores;                // tracked: [row, q head, score_stride] scores times log2(e)
   int score_stride;
   float2* head_ml;              // tracked: [row, q head] (max, 1 / sum)
+  const float* weights;         // tracked
+  float* weights_out;
+  int64_t w_sb, w_sh, wo_sb, wo_sh;
+  float decay;
+  int fuse;                     // tracked: the merging workgroup adds the row's weights too (no second launch)
 };
 
 }  // namespace bz
@@ -46,7 +52,7 @@ namespace {
 using bz::LongParams;
 
 constexpr int kApplyThreads = 256;
-constexpr int kLongCols = 16;
+constexpr int kLongCols = 16, kMaxGroup = 8;
 
 __device__ __forceinline__ int clamp_int(int x, int lo, int hi) { return min(max(x, lo), hi); }
 
@@ -315,6 +321,41 @@ __device__ __forceinline__ void merge_columns(const float* part_acc, const float
   }
 }
 
+// weights_out[b, h, pos] = decay * weights[b, h, pos] + sum_g 2^(score - max_g) / sum_g over the row's range [s, e), by threads
+// first, first + step, ..: four consecutive positions a thread and turn (16-byte score loads, coherent with the other
+// workgroups' stores). ml(g): (max, 1 / sum) of the group's q head g.
+template <class Ml>
+__device__ __forceinline__ void add_weights(const LongParams& p, int b, int h, int s, int e, int first, int step, Ml ml) {
+  const float* const wi = p.weights + (int64_t)b * p.w_sb + (int64_t)h * p.w_sh;
+  float* const wo = p.weights_out + (int64_t)b * p.wo_sb + (int64_t)h * p.wo_sh;
+  for (int pos0 = (s & ~3) + 4 * first; pos0 < e; pos0 += 4 * step) {
+    f32x4_t acc = {0.f, 0.f, 0.f, 0.f}, old = acc, x[kMaxGroup];
+    // every load before the first use
+#pragma unroll
+    for (int g = 0; g < kMaxGroup; ++g) {
+      if (g >= p.G) break;
+      const int64_t hq = ((int64_t)b * p.NKV + h) * p.G + g;
+      const Rsrc rs = span_rsrc(wave_uniform(p.scores + hq * p.score_stride), p.score_stride * 4);
+      x[g] = __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, 4 * pos0, 0, kSc1));
+    }
+    if (p.decay != 0.f) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) old[i] = wi[clamp_int(pos0 + i, s, e - 1)];  // outside the range: unused
+    }
+#pragma unroll
+    for (int g = 0; g < kMaxGroup; ++g) {
+      if (g >= p.G) break;
+      const float2 y = ml(g);
+      const float mu = y.x == -INFINITY ? 0.f : y.x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] = fmaf(fast_exp2(x[g][i] - mu), y.y, acc[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (pos0 + i >= s && pos0 + i < e) wo[pos0 + i] = p.decay == 0.f ? acc[i] : fmaf(p.decay, old[i], acc[i]);
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ split kernel
 
 // grid (splits, kv heads, rows * column tiles). KV4: a 4-bit cache. TRACK: also writes the scores (one token per row).
@@ -328,18 +369,17 @@ __global__ void __launch_bounds__(NT, 2)
   const int tid = threadIdx.x, lane = tid % kWave, w = wave_uniform(tid / kWave), r = lane % 16, g = lane / 16;
 
   const int ntok = min(p.tpt, p.T - t0), ncol = ntok << p.gshift;
-  const int col = r % ncol;  // columns past the last repeat earlier ones
+  const int col = p.T == 1 ? r & (p.G - 1) : r % ncol;  // columns past the last repeat earlier ones
   const int tok = t0 + (col >> p.gshift), hq = (h << p.gshift) + (col & (p.G - 1));
 
-  // the B operand of K . q^T: this lane's column, dims as the tile's K has them
-  bf16x8_t qf[NJ];
+  // the B operand of K . q^T: this lane's column, dims as the tile's K has them; loaded now, used after the first tiles' loads
+  // are on their way
+  uint4 qr[NJ];
   {
     const uint16_t* qsrc = p.q + (int64_t)b * p.q_sb + (int64_t)tok * p.q_st + (int64_t)hq * p.q_sh;
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
-      qf[j] = signed_q(*reinterpret_cast<const uint4*>(qsrc + (KV4 ? (D / 4) * g + 8 * j : 32 * j + 8 * g)), p.scale_log2);
+    for (int j = 0; j < NJ; ++j) qr[j] = *reinterpret_cast<const uint4*>(qsrc + (KV4 ? (D / 4) * g + 8 * j : 32 * j + 8 * g));
   }
-  const float scale = positive_scale(p.scale_log2);
 
   int s, e;
   long_range(e_raw, s_raw, starts != nullptr, p.cap, s, e);
@@ -347,10 +387,10 @@ __global__ void __launch_bounds__(NT, 2)
   const Reach mine = reach_of(s, token_end(tok), p.window, p.sinks);
   const TileRange tr = tile_range<P>(s, token_end(t0), token_end(t0 + ntok - 1), p.window, p.sinks);
   const int n = tr.na + tr.nb;
-  int per = n <= p.one_split ? n : max(p.min_tiles, (n + p.splits - 1) / p.splits);
-  per = max(NW, (per + NW - 1) / NW * NW);
-  const int nact = max(1, (n + per - 1) / per);
-  if (split >= nact) return;
+  // tiles per split, a multiple of the waves (no integer division: about 30 dependent instructions before the first load)
+  const int least = n <= p.one_split ? n : max(p.min_tiles, ceil_div_est(n, p.splits, p.inv_splits));
+  const int per = max(NW, (least + NW - 1) & ~(NW - 1));
+  if (split > 0 && split * per >= n) return;  // past the row's last tile (split 0 always stays)
   const int j0 = split * per, j1 = min(n, j0 + per);
   const int e1 = token_end(t0 + ntok - 1);
   // every column attends the whole of [whole_lo, whole_end)
@@ -389,6 +429,15 @@ __global__ void __launch_bounds__(NT, 2)
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) st.acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
+  int j = j0 + w;
+  load(ta, j);
+  load(tb, j + NW);
+  __builtin_amdgcn_sched_barrier(0);  // q's conversion waits for q: not before the tiles' loads
+  const int nact = ceil_div_est(max(n, 1), per, __builtin_amdgcn_rcpf((float)per));  // splits with tiles
+  const float scale = positive_scale(p.scale_log2);
+  bf16x8_t qf[NJ];
+#pragma unroll
+  for (int i = 0; i < NJ; ++i) qf[i] = signed_q(qr[i], p.scale_log2);
   auto consume = [&](auto& t, int j) {
     const int pos0 = pos_of(j);
     auto pos = [&](int i) { return pos0 + 16 * (i / 4) + 4 * g + i % 4; };
@@ -417,7 +466,11 @@ __global__ void __launch_bounds__(NT, 2)
     if constexpr (TRACK) {
       if (r < ncol) {
         float* const row = p.scores + ((int64_t)b * p.NKV * p.G + hq) * p.score_stride;
-        *reinterpret_cast<f32x4_t*>(row + pos0 + 4 * g) = f32x4_t{x[0], x[1], x[2], x[3]} * scale;
+        // as the partials are: another workgroup of this launch may read them
+        const Rsrc rs = span_rsrc(row, p.score_stride * 4);
+        using U4 = decltype(__builtin_amdgcn_raw_buffer_load_b128(rs, 0, 0, 0));
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(U4, f32x4_t{x[0], x[1], x[2], x[3]} * scale), rs,
+                                               4 * (pos0 + 4 * g), 0, kSc1);
       }
     }
     fold_scores<D, N>(st, x, scale);
@@ -442,10 +495,6 @@ __global__ void __launch_bounds__(NT, 2)
     }
   };
 
-  int j = j0 + w;
-  load(ta, j);
-  load(tb, j + NW);
-  __builtin_amdgcn_sched_barrier(0);
   for (; j < j1; j += 2 * NW) {
     consume(ta, j);
     if (j + NW >= j1) break;
@@ -479,13 +528,23 @@ __global__ void __launch_bounds__(NT, 2)
   }
   __syncthreads();
 
+  __shared__ float2 s_head[TRACK ? kLongCols : 1];
   auto write = [&](int c, int d, const f32x4_t& a, float m, float l) {
     const int ot = t0 + (c >> p.gshift), oh = (h << p.gshift) + (c & (p.G - 1));
     const float inv = l == 0.f ? 0.f : 1.f / l;  // a NaN sum stays one
     uint16_t* const o = p.out + (int64_t)b * p.o_sb + (int64_t)ot * p.o_st + (int64_t)oh * p.o_sh + d;
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] = f32_to_bf16(l == 0.f ? 0.f : a[i] * inv);
-    if (TRACK && d == 0) p.head_ml[(int64_t)b * p.NKV * p.G + oh] = make_float2(m, inv);
+    if (TRACK && d == 0) {
+      if (p.fuse) s_head[c] = make_float2(m, inv);
+      else p.head_ml[(int64_t)b * p.NKV * p.G + oh] = make_float2(m, inv);
+    }
+  };
+  auto finish = [&]() {  // tracked: the row's weights, once every score of it is written and its heads' sums are in s_head
+    if (TRACK && p.fuse) {
+      __syncthreads();
+      add_weights(p, b, h, s, e, tid, NT, [&](int q) { return s_head[q]; });
+    }
   };
 
   const int ncols_max = p.tpt << p.gshift;
@@ -519,7 +578,11 @@ __global__ void __launch_bounds__(NT, 2)
       }
     }
   }
-  if (nact == 1) return;
+  if (nact == 1) {
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    finish();
+    return;
+  }
 
   // the last workgroup of this (row, tile, kv head) to count in merges, as in gqa_split_kernel
   __shared__ int s_last;
@@ -535,35 +598,18 @@ __global__ void __launch_bounds__(NT, 2)
   if (!s_last) return;
   merge_columns<D, NT>(p.part_acc + unit * p.splits * ncols_max * D, p.part_ml + unit * p.splits * ncols_max, ncols_max, ncol, nact,
                    write);
+  finish();
 }
 
-// weights_out[b, h, pos] = decay * weights[b, h, pos] + sum_g 2^(score - max_g) / sum_g over the row's range; grid (chunks of
-// kApplyThreads * 4 positions, kv heads, rows), after the split kernel that wrote the scores. Four consecutive positions a
-// thread (16-byte score loads).
+// add_weights in a launch of its own, after the split kernel that wrote the scores: grid (chunks of kApplyThreads * 4
+// positions, kv heads, rows).
 __global__ void __launch_bounds__(kApplyThreads)
-    track_apply_kernel(const int32_t* lens, const int32_t* starts, const float* weights, float* weights_out, int64_t w_sb,
-                       int64_t w_sh, int64_t wo_sb, int64_t wo_sh, float decay, const LongParams p) {
+    track_apply_kernel(const int32_t* lens, const int32_t* starts, const LongParams p) {
   const int h = blockIdx.y, b = blockIdx.z;
   int s, e;
   long_range(lens[b], (starts ? starts : lens)[b], starts != nullptr, p.cap, s, e);
-  const int pos0 = 4 * (int)(blockIdx.x * kApplyThreads + threadIdx.x);
-  if (pos0 >= e || pos0 + 4 <= s) return;
-  f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-  for (int g = 0; g < p.G; ++g) {
-    const int64_t hq = ((int64_t)b * p.NKV + h) * p.G + g;
-    const float2 ml = p.head_ml[hq];
-    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(p.scores + hq * p.score_stride + pos0);
-    const float mu = ml.x == -INFINITY ? 0.f : ml.x;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] = fmaf(fast_exp2(x[i] - mu), ml.y, acc[i]);
-  }
-  const float* const wi = weights + (int64_t)b * w_sb + (int64_t)h * w_sh;
-  float* const wo = weights_out + (int64_t)b * wo_sb + (int64_t)h * wo_sh;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int pos = pos0 + i;
-    if (pos >= s && pos < e) wo[pos] = decay == 0.f ? acc[i] : fmaf(decay, wi[pos], acc[i]);
-  }
+  add_weights(p, b, h, s, e, blockIdx.x * kApplyThreads + threadIdx.x, gridDim.x * kApplyThreads,
+              [&](int g) { return p.head_ml[((int64_t)b * p.NKV + h) * p.G + g]; });
 }
 
 }  // namespace

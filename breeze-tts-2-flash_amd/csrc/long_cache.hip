@@ -17,6 +17,10 @@ namespace {
 // Threads of a split workgroup. Eight waves measured 6% faster on long rows of 4 bits (4 rows x 4 kv heads of 20001..32768,
 // G 8: 17.9 against 19.0 us) and 2 to 40% slower on everything else.
 constexpr int kLongThreads = 256;
+// Rows up to which the merging workgroup of a tracked step adds the weights itself (two turns of its threads), in place of a
+// second launch (us, second launch / itself: 2 x 8 kv heads, G 2: 500 positions 8.97 / 7.30, 1377 10.26 / 9.65, 2048 10.82 /
+// 10.31, 4096 13.79 / 15.49; G 8, 1 x 8 x 1024 10.71 / 8.81).
+constexpr int kFusePositions = 2048;
 constexpr int kKv4Tokens = 16;  // most query tokens per row over a 4-bit cache
 
 bool dim_ok(int D) { return D == 64 || D == 128; }
@@ -81,11 +85,11 @@ int make_plan(int kind, int B, int NH, int NKV, int D, int cap, int T, int windo
   pl->one_split = (kOneSplitBytes / (kv4 ? D + D / 16 : 4 * D)) / P;
   int splits = num_splits;
   if (splits == 0) {
-    // One round of workgroups where a window makes the rows alike (4 rows x 8 kv heads, window 4096: 8 splits 15.2 us, 16
-    // 15.3..16.0; 16 rows: 2 splits 42.6, 4 44.8), two where their lengths differ (track, 4 rows of 9000..16384: 8 splits 49.7,
-    // 16 47.3) and for 4-bit tiles, whose conversion leaves a wave alone on its SIMD half idle (16 kv heads x 32768: 16
-    // splits 19.2, 32 19.0; 1 row x 8 of 8192: 32 splits 8.2, 64 7.6 .. 8.6).
-    splits = (int)((kv4 || !cut ? 2 : 1) * cus / pl->units);
+    // One round of workgroups (us: 1 row x 8 kv heads x 8192 positions of 4 bits: 32 splits 7.5, 64 8.6; 2 rows tracked, 1377:
+    // 16 splits 10.2, 32 11.1; 4 rows, window 4096: 8 splits 14.8, 16 15.3; 16 rows: 2 splits 42.1, 4 44.5), two for a server's
+    // batch (more than three rows) whose lengths differ because no window cuts them (4 rows of 9000..16384 tracked: 8 splits
+    // 49.3, 16 47.1; 16 rows of 128..2048 of 4 bits: 2 splits 11.3, 4 10.8; 32 rows, head_dim 64: 1 split 22.9, 2 18.7).
+    splits = (int)((!cut && B > 3 ? 2 : 1) * cus / pl->units);
     const int most = (n + pl->min_tiles - 1) / pl->min_tiles;
     if (splits > most) splits = most;
     if (splits > 64) splits = 64;
@@ -170,6 +174,7 @@ LongParams long_params(const bz_gqa_decode_args* a, const Plan& pl, int window, 
   p.NKV = a->num_kv_heads, p.G = pl.G, p.gshift = pl.gshift, p.T = a->tokens_per_row > 1 ? a->tokens_per_row : 1;
   p.cap = a->capacity;
   p.tiles = pl.tiles, p.tpt = pl.tpt;
+  p.inv_splits = 1.0f / (float)pl.splits;
   p.splits = pl.splits, p.min_tiles = pl.min_tiles, p.one_split = pl.one_split;
   char* const ws = static_cast<char*>(a->workspace);
   p.counters = reinterpret_cast<int*>(ws);
@@ -269,12 +274,16 @@ BZ_EXPORT int bz_gqa_decode_tracked(const bz_gqa_tracked_args* ta, hipStream_t s
   if (rc == BZ_OK) rc = check_bf16_cache(a);
   if (rc == BZ_OK) rc = check_workspace(a, pl);
   if (rc != BZ_OK) return rc;
-  const LongParams p = long_params(a, pl, 0, 0);
+  LongParams p = long_params(a, pl, 0, 0);
+  p.weights = ta->weights, p.w_sb = ta->w_stride_b, p.w_sh = ta->w_stride_h;
+  p.weights_out = ta->weights_out, p.wo_sb = ta->wo_stride_b, p.wo_sh = ta->wo_stride_h;
+  p.decay = ta->decay;
+  const int longest = a->max_seq_len > 0 && a->max_seq_len < a->capacity ? a->max_seq_len : a->capacity;
+  p.fuse = longest <= kFusePositions;
   rc = launch_split<false, true>(a, a->head_dim, p, pl, a->batch, stream);
-  if (rc != BZ_OK) return rc;
-  const dim3 grid((a->capacity + 4 * kApplyThreads - 1) / (4 * kApplyThreads), a->num_kv_heads, a->batch);
-  hipLaunchKernelGGL(track_apply_kernel, grid, dim3(kApplyThreads), 0, stream, a->seq_lens, a->kv_start, ta->weights,
-                     ta->weights_out, ta->w_stride_b, ta->w_stride_h, ta->wo_stride_b, ta->wo_stride_h, ta->decay, p);
+  if (rc != BZ_OK || p.fuse) return rc;
+  const dim3 grid((longest + 4 * kApplyThreads - 1) / (4 * kApplyThreads), a->num_kv_heads, a->batch);
+  hipLaunchKernelGGL(track_apply_kernel, grid, dim3(kApplyThreads), 0, stream, a->seq_lens, a->kv_start, p);
   return hipGetLastError() == hipSuccess ? BZ_OK : BZ_ERR_LAUNCH;
 }
 
