@@ -466,11 +466,12 @@ __global__ void __launch_bounds__(NT, 2)
     if constexpr (TRACK) {
       if (r < ncol) {
         float* const row = p.scores + ((int64_t)b * p.NKV * p.G + hq) * p.score_stride;
-        // as the partials are: another workgroup of this launch may read them
         const Rsrc rs = span_rsrc(row, p.score_stride * 4);
         using U4 = decltype(__builtin_amdgcn_raw_buffer_load_b128(rs, 0, 0, 0));
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(U4, f32x4_t{x[0], x[1], x[2], x[3]} * scale), rs,
-                                               4 * (pos0 + 4 * g), 0, kSc1);
+        const U4 y = __builtin_bit_cast(U4, f32x4_t{x[0], x[1], x[2], x[3]} * scale);
+        // coherent where another workgroup of this launch may read them (for 4 rows of 9000..16384 such stores cost 3 us)
+        if (p.fuse) __builtin_amdgcn_raw_buffer_store_b128(y, rs, 4 * (pos0 + 4 * g), 0, kSc1);
+        else __builtin_amdgcn_raw_buffer_store_b128(y, rs, 4 * (pos0 + 4 * g), 0, 0);
       }
     }
     fold_scores<D, N>(st, x, scale);
