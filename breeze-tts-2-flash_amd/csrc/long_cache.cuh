@@ -534,8 +534,12 @@ __global__ void __launch_bounds__(NT, 2)
     const int ot = t0 + (c >> p.gshift), oh = (h << p.gshift) + (c & (p.G - 1));
     const float inv = l == 0.f ? 0.f : 1.f / l;  // a NaN sum stays one
     uint16_t* const o = p.out + (int64_t)b * p.o_sb + (int64_t)ot * p.o_st + (int64_t)oh * p.o_sh + d;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = f32_to_bf16(l == 0.f ? 0.f : a[i] * inv);
+    const uint2 y = make_uint2(pack_bf16x2(a[0] * inv, a[1] * inv), pack_bf16x2(a[2] * inv, a[3] * inv));  // l == 0: a is 0
+    if (p.out_wide) {
+      *reinterpret_cast<uint2*>(o) = y;
+    } else {
+      o[0] = (uint16_t)y.x, o[1] = (uint16_t)(y.x >> 16), o[2] = (uint16_t)y.y, o[3] = (uint16_t)(y.y >> 16);
+    }
     if (TRACK && d == 0) {
       if (p.fuse) s_head[c] = make_float2(m, inv);
       else p.head_ml[(int64_t)b * p.NKV * p.G + oh] = make_float2(m, inv);

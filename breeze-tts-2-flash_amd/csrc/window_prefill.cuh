@@ -36,17 +36,19 @@ struct PreLds {
   static __device__ __forceinline__ int v_swz(int r) { return D == 128 ? 2 * (r & 7) : 2 * ((r >> 1) & 3); }
 };
 
-// Loads the TP rows from pos0 on (clamped to `last`: a row past it holds a copy of that one, and no column attends it) into
+// Loads the TP rows from pos0 on (clamped to [first, last]: a row outside holds a copy of the nearest, and no column attends it;
+// what lies there, such as NaN in memory that nothing has written, is not read) into
 // LDS at base, by CG waves (this one is cg): 64 lanes write 1 KB in lane order, so the swizzle is in which chunk each lane
 // fetches.
 template <int D, int TP, int CG, bool V>
-__device__ __forceinline__ void stage_tile(char* base, const Rsrc& rsrc, int pos0, int last, uint32_t row_bytes, int cg, int lane) {
+__device__ __forceinline__ void stage_tile(char* base, const Rsrc& rsrc, int pos0, int first, int last, uint32_t row_bytes, int cg,
+                                           int lane) {
   using L = PreLds<D, TP>;
   constexpr int RPI = 1024 / L::kRow, CH = D / 8;  // rows an instruction, chunks a row
 #pragma unroll
   for (int u = 0; u < L::kBytes / 1024 / CG; ++u) {
     const int row0 = RPI * (cg * (L::kBytes / 1024 / CG) + u), row = row0 + lane / CH, c = lane % CH;
-    const uint32_t off = (uint32_t)min(pos0 + row, last) * row_bytes + 16 * (c ^ (V ? L::v_swz(row) : L::k_swz(row)));
+    const uint32_t off = (uint32_t)clamp_int(pos0 + row, first, last) * row_bytes + 16 * (c ^ (V ? L::v_swz(row) : L::k_swz(row)));
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(base + row0 * L::kRow), 16, off, 0, 0,
                                              0);
   }
@@ -191,8 +193,8 @@ __global__ void __launch_bounds__(kPreThreads, 2)
 #pragma unroll
     for (int i = 0; i < KA; ++i) kf[i] = k_read(kbuf, i);
     __builtin_amdgcn_sched_barrier(0);
-    if (j + 2 < n) stage_tile<D, TP, CG, false>((kOdd ? k_odd : k_even) + group, rk, pos_of(j + 2), e1 - 1, row_bytes, cg, lane);
-    if (j + 1 < n) stage_tile<D, TP, CG, true>((kOdd ? v_even : v_odd) + group, rv, pos_of(j + 1), e1 - 1, row_bytes, cg, lane);
+    if (j + 2 < n) stage_tile<D, TP, CG, false>((kOdd ? k_odd : k_even) + group, rk, pos_of(j + 2), s, e1 - 1, row_bytes, cg, lane);
+    if (j + 1 < n) stage_tile<D, TP, CG, true>((kOdd ? v_even : v_odd) + group, rv, pos_of(j + 1), s, e1 - 1, row_bytes, cg, lane);
     const int p0 = pos_of(j);
     if (!(p0 + TP <= whole_end && p0 >= whole_lo)) {
 #pragma unroll
@@ -248,11 +250,11 @@ __global__ void __launch_bounds__(kPreThreads, 2)
     }
   };
   if (n > 0) {
-    stage_tile<D, TP, CG, false>(k_even + group, rk, pos_of(0), e1 - 1, row_bytes, cg, lane);
+    stage_tile<D, TP, CG, false>(k_even + group, rk, pos_of(0), s, e1 - 1, row_bytes, cg, lane);
     __builtin_amdgcn_s_waitcnt(0x0f70);
     __syncthreads();
-    if (n > 1) stage_tile<D, TP, CG, false>(k_odd + group, rk, pos_of(1), e1 - 1, row_bytes, cg, lane);
-    stage_tile<D, TP, CG, true>(v_even + group, rv, pos_of(0), e1 - 1, row_bytes, cg, lane);
+    if (n > 1) stage_tile<D, TP, CG, false>(k_odd + group, rk, pos_of(1), s, e1 - 1, row_bytes, cg, lane);
+    stage_tile<D, TP, CG, true>(v_even + group, rv, pos_of(0), s, e1 - 1, row_bytes, cg, lane);
     f32x16_t xa[NB], xb[NB];
 #pragma unroll
     for (int i = 0; i < NK; ++i)
