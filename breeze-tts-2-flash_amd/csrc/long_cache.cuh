@@ -53,6 +53,7 @@ using bz::LongParams;
 
 constexpr int kApplyThreads = 256;
 constexpr int kLongCols = 16, kMaxGroup = 8;
+constexpr int kBf16 = 0, kKv4 = 1, kKv4Packed = 2;  // cache formats of the split kernel
 
 __device__ __forceinline__ int clamp_int(int x, int lo, int hi) { return min(max(x, lo), hi); }
 
@@ -96,14 +97,6 @@ __device__ __forceinline__ TileRange tile_range(int s, int e0, int e1, int windo
 // With r = lane % 16 and g = lane / 16, a lane scores the positions pos0 + 16 s + 4 g + i (s < P / 16, i < 4) of column r,
 // and holds V of the same positions, so P goes from K . q^T to V^T . P^T without leaving its lane.
 
-// 16 bf16 positions: WaveTile (gqa_kernels.cuh).
-template <int D>
-struct Bf16Tile {
-  static constexpr int P = 16;
-  WaveTile<D> t;
-  Spans sp;
-};
-
 // 32 positions of 4-bit codes. K: lane (r, g) holds the D / 4 dims from (D / 4) g on of rows r and 16 + r, one load each
 // (64 lanes read 16 whole rows); the products take dims in any order as long as q's operand has the same, so product j
 // of a row takes dims (D / 4) g + 8 j .. + 7, and all of a lane's codes lie in one block of 32: one scale. V: dims (D / 16) r
@@ -122,13 +115,18 @@ struct Kv4Spans {
   uint32_t row_bytes;
 };
 
-template <int D>
+// PACKED: the rows lie one behind the other, so the loads of a tile differ by constants, which the instructions hold: about 30
+// vector instructions a tile fewer (one workgroup over 32768 positions, head_dim 128: 169 us; with the row's stride 177).
+template <int D, bool PACKED>
 __device__ __forceinline__ void load_kv4_tile(Kv4Tile<D>& t, const Kv4Spans& sp, int pos0, int r, int g) {
   constexpr int SB = D / 32;  // scale bytes of a position
+  const uint32_t row_bytes = PACKED ? D / 2 : sp.row_bytes;
+  uint32_t ko = (pos0 + r) * row_bytes + (D / 8) * g, kso = (pos0 + r) * SB + (D == 128 ? g : g / 2);
+  uint32_t vo = (pos0 + 4 * g) * row_bytes + (D / 32) * r, vso = (pos0 + 4 * g) * SB + r / (D == 128 ? 4 : 8);
+  asm("" : "+v"(ko), "+v"(kso), "+v"(vo), "+v"(vso));  // sums as they stand here: not as ors, which no instruction holds
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
-    const uint32_t pos = (uint32_t)(pos0 + 16 * s + r);
-    const uint32_t off = pos * sp.row_bytes + (D / 8) * g;
+    const uint32_t off = ko + 16 * s * row_bytes;
     if constexpr (D == 128) {
       const uint4 w = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(sp.k, off, 0, kStream));
       t.k[s][0] = w.x, t.k[s][1] = w.y, t.k[s][2] = w.z, t.k[s][3] = w.w;
@@ -136,15 +134,15 @@ __device__ __forceinline__ void load_kv4_tile(Kv4Tile<D>& t, const Kv4Spans& sp,
       const uint2 w = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(sp.k, off, 0, kStream));
       t.k[s][0] = w.x, t.k[s][1] = w.y;
     }
-    t.ks[s] = __builtin_amdgcn_raw_buffer_load_b8(sp.ks, pos * SB + (D == 128 ? g : g / 2), 0, 0);
+    t.ks[s] = __builtin_amdgcn_raw_buffer_load_b8(sp.ks, kso + 16 * s * SB, 0, 0);
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const uint32_t pos = (uint32_t)(pos0 + 16 * (i / 4) + 4 * g + i % 4);
-    const uint32_t off = pos * sp.row_bytes + (D / 32) * r;
+    const int step = 16 * (i / 4) + i % 4;
+    const uint32_t off = vo + step * row_bytes;
     if constexpr (D == 128) t.v[i] = __builtin_amdgcn_raw_buffer_load_b32(sp.v, off, 0, kStream);
     else t.v[i] = __builtin_amdgcn_raw_buffer_load_b16(sp.v, off, 0, kStream);
-    t.vs[i] = __builtin_amdgcn_raw_buffer_load_b8(sp.vs, pos * SB + r / (D == 128 ? 4 : 8), 0, 0);
+    t.vs[i] = __builtin_amdgcn_raw_buffer_load_b8(sp.vs, vso + step * SB, 0, 0);
   }
 }
 
@@ -358,10 +356,11 @@ __device__ __forceinline__ void add_weights(const LongParams& p, int b, int h, i
 
 // ------------------------------------------------------------------------------------------------ split kernel
 
-// grid (splits, kv heads, rows * column tiles). KV4: a 4-bit cache. TRACK: also writes the scores (one token per row).
-template <int D, bool KV4, bool TRACK, int NT>
+// FMT: the cache's format. TRACK: also writes the scores (one token per row). grid (splits, kv heads, rows * column tiles).
+template <int D, int FMT, bool TRACK, int NT>
 __global__ void __launch_bounds__(NT, 2)
     long_split_kernel(const int32_t* lens, const int32_t* starts, const LongParams p) {
+  constexpr bool KV4 = FMT != kBf16;
   constexpr int NW = NT / kWave, P = KV4 ? 32 : 16, NS = P / 16, N = 4 * NS, NJ = D / 32;
   const int split = blockIdx.x, h = blockIdx.y, z = blockIdx.z;
   const int b = p.tiles == 1 ? z : z / p.tiles, t0 = (z - b * p.tiles) * p.tpt;
@@ -419,7 +418,7 @@ __global__ void __launch_bounds__(NT, 2)
     }
   }
   auto load = [&](auto& t, int j) {
-    if constexpr (KV4) load_kv4_tile<D>(t, sp4, pos_of(j), r, g);
+    if constexpr (KV4) load_kv4_tile<D, FMT == kKv4Packed>(t, sp4, pos_of(j), r, g);
     else load_wave_tile<D, BZ_MASK_NONE>(t, sp, pos_of(j), r, g);
   };
 

@@ -186,13 +186,13 @@ LongParams long_params(const bz_gqa_decode_args* a, const Plan& pl, int window, 
   return p;
 }
 
-template <bool KV4, bool TRACK>
+template <int FMT, bool TRACK>
 int launch_split(const bz_gqa_decode_args* a, int D, const LongParams& p, const Plan& pl, int B, hipStream_t stream) {
   const dim3 grid(pl.splits, p.NKV, B * pl.tiles);
   if (D == 128)
-    hipLaunchKernelGGL((long_split_kernel<128, KV4, TRACK, kLongThreads>), grid, dim3(kLongThreads), 0, stream, a->seq_lens, a->kv_start, p);
+    hipLaunchKernelGGL((long_split_kernel<128, FMT, TRACK, kLongThreads>), grid, dim3(kLongThreads), 0, stream, a->seq_lens, a->kv_start, p);
   else
-    hipLaunchKernelGGL((long_split_kernel<64, KV4, TRACK, kLongThreads>), grid, dim3(kLongThreads), 0, stream, a->seq_lens, a->kv_start, p);
+    hipLaunchKernelGGL((long_split_kernel<64, FMT, TRACK, kLongThreads>), grid, dim3(kLongThreads), 0, stream, a->seq_lens, a->kv_start, p);
   return hipGetLastError() == hipSuccess ? BZ_OK : BZ_ERR_LAUNCH;
 }
 
@@ -229,7 +229,7 @@ BZ_EXPORT int bz_gqa_window(const bz_gqa_window_args* wa, hipStream_t stream) {
   if (rc == BZ_OK) rc = check_workspace(a, pl);
   if (rc != BZ_OK) return rc;
   const LongParams p = long_params(a, pl, wa->window, wa->sinks);
-  if (!pl.prefill) return launch_split<false, false>(a, a->head_dim, p, pl, a->batch, stream);
+  if (!pl.prefill) return launch_split<kBf16, false>(a, a->head_dim, p, pl, a->batch, stream);
   const dim3 grid(a->num_kv_heads, pl.tiles, a->batch);
   using Fn = void (*)(const int32_t*, const int32_t*, const LongParams);
   const Fn fns[2][3] = {{window_prefill_kernel<64, 1>, window_prefill_kernel<64, 2>, window_prefill_kernel<64, 4>},
@@ -258,7 +258,8 @@ BZ_EXPORT int bz_gqa_decode_kv4(const bz_gqa_kv4_args* ka, hipStream_t stream) {
   p.k_scale = static_cast<const uint8_t*>(c->k_scale);
   p.v_scale = static_cast<const uint8_t*>(c->v_scale);
   p.sc_sb = c->scale_stride_b, p.sc_sh = c->scale_stride_h;
-  return launch_split<true, false>(&a, a.head_dim, p, pl, a.batch, stream);
+  if (c->stride_s == a.head_dim / 2) return launch_split<kKv4Packed, false>(&a, a.head_dim, p, pl, a.batch, stream);
+  return launch_split<kKv4, false>(&a, a.head_dim, p, pl, a.batch, stream);
 }
 
 BZ_EXPORT int bz_gqa_decode_tracked(const bz_gqa_tracked_args* ta, hipStream_t stream) {
@@ -280,7 +281,7 @@ BZ_EXPORT int bz_gqa_decode_tracked(const bz_gqa_tracked_args* ta, hipStream_t s
   p.decay = ta->decay;
   const int longest = a->max_seq_len > 0 && a->max_seq_len < a->capacity ? a->max_seq_len : a->capacity;
   p.fuse = longest <= kFusePositions;
-  rc = launch_split<false, true>(a, a->head_dim, p, pl, a->batch, stream);
+  rc = launch_split<kBf16, true>(a, a->head_dim, p, pl, a->batch, stream);
   if (rc != BZ_OK || p.fuse) return rc;
   const dim3 grid((longest + 4 * kApplyThreads - 1) / (4 * kApplyThreads), a->num_kv_heads, a->batch);
   hipLaunchKernelGGL(track_apply_kernel, grid, dim3(kApplyThreads), 0, stream, a->seq_lens, a->kv_start, p);

@@ -275,6 +275,25 @@ def test_kv4_attention(device, NKV, G, D, cap, T, lens, starts, window, sinks):
                     sinks, starts)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_kv4_strided_cache(device, D):
+    """Codes [B, capacity, NKV, D / 2] with K and V side by side, scales in views: the same cache otherwise."""
+    rng = np.random.default_rng(D)
+    B, NKV, G, cap = 2, 2, 2, 150
+    codes = torch.zeros(B, cap, NKV, 2, D // 2, dtype=torch.uint8, device=device).permute(0, 2, 1, 3, 4)
+    scales = torch.zeros(B, NKV + 1, 2, cap + 6, D // 32, dtype=torch.uint8, device=device)
+    cache = pkg.Kv4Cache(codes[:, :, :, 0], codes[:, :, :, 1], scales[:, 1:, 0, 2:cap + 2], scales[:, 1:, 1, 2:cap + 2])
+    plain = pkg.kv4_cache(B, NKV, cap, D, device)
+    q, k, v = randn(rng, B, NKV * G, D).to(device), randn(rng, B, NKV, cap, D).to(device), randn(rng, B, NKV, cap, D).to(device)
+    zero, lens = ints([0, 0], device), ints([150, 77], device)
+    for c in (cache, plain):
+        pkg.kv4_store(k, v, c, zero)
+    assert all(torch.equal(a, b) for a, b in zip(cache, plain))
+    assert all(torch.equal(a, b) for a, b in zip(pkg.kv4_load(cache, zero, cap), pkg.kv4_load(plain, zero, cap)))
+    a, b = (pkg.gqa_decode_kv4(q, c, lens, D ** -0.5, window=100, sinks=3) for c in (cache, plain))
+    assert torch.equal(a, b)
+
+
 def test_kv4_attention_reads_what_load_returns(device):
     """The attention over the codes is the window attention over kv4_load's values, to the last bf16 step."""
     rng = np.random.default_rng(3)
