@@ -99,7 +99,8 @@ int make_plan(int kind, int B, int NH, int NKV, int D, int cap, int T, int windo
 
   const size_t cols = (size_t)pl->units * splits * pl->tpt * pl->G;
   const bool merged = splits > 1;
-  pl->ml = merged ? (size_t)pl->units * kCounterStride * sizeof(int) : 0;
+  // a tracked call of one split has no use for the counters, but a later call with the same workspace finds them zero
+  pl->ml = merged || kind == BZ_LONG_TRACKED ? (size_t)pl->units * kCounterStride * sizeof(int) : 0;
   pl->acc = up256(pl->ml + (merged ? cols * sizeof(float2) : 0));
   pl->head_ml = up256(pl->acc + (merged ? cols * D * sizeof(float) : 0));
   pl->total = pl->head_ml;

@@ -474,6 +474,21 @@ def test_bounded_generation(device, fmt):
     assert (weights.sum((1, 2)) <= 50 * NKV * G + 1e-2).all()
 
 
+def test_tracked_splits_share_a_workspace(device):
+    """One split writes no partials; a call of several that follows in the same workspace still finds its counters zero."""
+    rng = np.random.default_rng(12)
+    B, NKV, G, D, cap = 2, 2, 2, 64, 700
+    q, k, v = (randn(rng, *s).to(device) for s in ((B, NKV * G, D), (B, NKV, cap, D), (B, NKV, cap, D)))
+    lens, w = ints([700, 300], device), torch.zeros(B, NKV, cap, device=device)
+    ws = pkg.long_workspace("tracked", device, B, NKV * G, NKV, D, cap, num_splits=5)
+    for splits in (5, 1, 5, 1, 3):
+        wo = torch.full_like(w, 7.0)
+        out = pkg.gqa_decode_tracked(q, k, v, lens, D ** -0.5, w, weights_out=wo, num_splits=splits, workspace=ws)
+        check_attention(out, q.float().cpu()[:, :, None], k.float().cpu(), v.float().cpu(), [700, 300], D ** -0.5,
+                        what=f"{splits} splits")
+        assert abs(float(wo[1, :, :300].sum()) - NKV * G) < 1e-3 and (wo[1, :, 300:] == 7).all(), splits
+
+
 def _calls(device, seed):
     """One call of each kind on inputs of its own: (name, run(workspaces), state to vary)."""
     rng = np.random.default_rng(seed)
