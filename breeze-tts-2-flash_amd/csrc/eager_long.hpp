@@ -70,6 +70,13 @@ const int32_t* rows_or_null(PyObject* o, int64_t B, const char* name, const at::
   return o == Py_None ? nullptr : rows_arg(o, B, name, dev);
 }
 
+// Whether no two elements of t share a place because of a broadcast dim.
+bool one_place_each(const at::Tensor& t) {
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.stride(i) == 0 && t.size(i) > 1) return false;
+  return true;
+}
+
 // The query's, ranges' and output's part of a call's arguments. out: the caller's or nullptr (then out_shape is what to
 // allocate).
 void fill_query(const at::Tensor& q, const at::Tensor* out, PyObject* seq_lens, PyObject* kv_start, PyObject* scale,
@@ -106,6 +113,7 @@ void fill_query(const at::Tensor& q, const at::Tensor* out, PyObject* seq_lens, 
       throw Error{"out must be [B, T, NH, D], [B, NH, T, D] or (T = 1) [B, NH, D] with B=" + std::to_string(B) +
                   ", T=" + std::to_string(T) + ", NH=" + std::to_string(NH) + ", D=" + std::to_string(D)};
     }
+    require(one_place_each(o), "out must not be a broadcast view");
     a.out = o.data_ptr();
   }
   a.seq_lens = rows_arg(seq_lens, B, "seq_lens", q.device());
@@ -173,6 +181,9 @@ bool long_workspace(int kind, int idx, hipStream_t stream, int window, int sinks
     it = g_long_bytes.emplace(sizes, n).first;
   }
   if (it->second == 0) return true;
+  if (capturing(stream))
+    throw Error{"a call being captured into a graph needs workspace= (long_workspace(...), made before the capture; " +
+                std::to_string(it->second) + " bytes): graphs that shared the stream's own could not run at the same time"};
   const LongKey key{idx, (int64_t)reinterpret_cast<uintptr_t>(stream), kind, a.batch, a.num_q_heads, a.num_kv_heads,
                     a.tokens_per_row};
   auto ws = g_long_ws.find(key);
@@ -181,9 +192,6 @@ bool long_workspace(int kind, int idx, hipStream_t stream, int window, int sinks
     a.workspace_bytes = (size_t)ws->second.numel();
     return true;
   }
-  if (capturing(stream))
-    throw Error{"no workspace of " + std::to_string(it->second) + " bytes exists for the stream being captured, and nothing is "
-                "allocated during a capture: pass workspace= (long_workspace(...), made before the capture)"};
   *need = Py_BuildValue("(LLLLLLLn)", (long long)key[0], (long long)key[1], (long long)key[2], (long long)key[3],
                         (long long)key[4], (long long)key[5], (long long)key[6], (Py_ssize_t)it->second);
   return false;
@@ -357,6 +365,9 @@ PyObject* kv4_store(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     bz_kv4_cache c{};
     const at::Device dev = fill_kv4(args + 2, c);
     check_kv(k, v, c, dev);
+    for (int i = 2; i < 6; ++i)
+      require(one_place_each(THPVariable_Unpack(args[i])), "a cache that is written must not be a broadcast view");
+    require(c.k != c.v && c.k_scale != c.v_scale, "a cache's K and V must not be the same tensor");
     const int32_t *slots = rows_arg(args[6], c.batch, "slots", dev), *counts = rows_or_null(args[7], c.batch, "counts", dev);
     const int idx = dev.index();
     DeviceScope scope(idx);
@@ -383,6 +394,8 @@ PyObject* kv4_load(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     at::Tensor v = vg ? *vg : at::empty({c.batch, c.num_kv_heads, tokens, c.head_dim}, options);
     check_kv(k, v, c, dev);
     require(k.size(2) == tokens, "the outputs must hold as many tokens as are asked for");
+    require(one_place_each(k) && one_place_each(v), "an output must not be a broadcast view");
+    require(k.data_ptr() != v.data_ptr(), "the outputs must not be the same tensor");
     check_status(g_load(&c, slots, tokens, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
                         c10::hip::getCurrentHIPStream(idx).stream()),
                  "bz_kv4_load");

@@ -17,6 +17,7 @@
 namespace {
 
 constexpr int kStoreThreads = 256;
+constexpr int kMaxTokens = 1 << 30;  // sums of tokens and workgroup sizes stay in 32 bits
 
 struct StoreParams {
   const uint16_t *k, *v;  // bf16 in (store) or out (load)
@@ -104,6 +105,7 @@ int check_store(const void* k, const void* v, int64_t sb, int64_t sh, int64_t st
   if (k == nullptr || v == nullptr || slots == nullptr || c == nullptr) return BZ_ERR_NULL;
   if (c->k == nullptr || c->v == nullptr || c->k_scale == nullptr || c->v_scale == nullptr) return BZ_ERR_NULL;
   if (tokens <= 0 || c->batch <= 0 || c->num_kv_heads <= 0 || c->capacity <= 0) return BZ_ERR_SHAPE;
+  if (tokens > kMaxTokens || c->capacity > kMaxTokens) return BZ_ERR_SHAPE;
   if (c->batch > 32767 || c->num_kv_heads > 65535) return BZ_ERR_SHAPE;  // grid limits
   const int D = c->head_dim;
   if (D != 64 && D != 128) return BZ_ERR_UNSUPPORTED;

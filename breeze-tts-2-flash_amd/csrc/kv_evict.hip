@@ -9,6 +9,8 @@
 
 namespace {
 
+constexpr int kMaxCapacity = 1 << 30;  // sums of positions and strip sizes stay in 32 bits
+
 // ---------------------------------------------------------------------------------------------------- selection
 //
 // One workgroup per (row, kv head). The threshold is the m-th largest key of the middle positions (m = keep - sinks -
@@ -282,7 +284,7 @@ BZ_EXPORT int bz_kv_select(const bz_kv_select_args* a, hipStream_t stream) {
   if (a == nullptr || a->weights == nullptr || a->seq_lens == nullptr || a->index == nullptr || a->lens == nullptr)
     return BZ_ERR_NULL;
   if (a->batch <= 0 || a->num_kv_heads <= 0 || a->capacity <= 0 || a->keep <= 0 || a->keep > a->capacity || a->sinks < 0 ||
-      a->recent < 0 || (int64_t)a->sinks + a->recent > a->keep || a->batch > 65535)
+      a->recent < 0 || (int64_t)a->sinks + a->recent > a->keep || a->batch > 65535 || a->capacity > kMaxCapacity)
     return BZ_ERR_SHAPE;
   const uintptr_t ptrs = reinterpret_cast<uintptr_t>(a->weights) | reinterpret_cast<uintptr_t>(a->weights_out) |
                          reinterpret_cast<uintptr_t>(a->seq_lens) | reinterpret_cast<uintptr_t>(a->kv_start) |
@@ -296,6 +298,8 @@ BZ_EXPORT int bz_kv_select(const bz_kv_select_args* a, hipStream_t stream) {
   p.NKV = a->num_kv_heads, p.cap = a->capacity, p.keep = a->keep, p.sinks = a->sinks, p.recent = a->recent;
   // workgroups of a row read seq_lens and kv_start; lens that lies on either is written by a launch of its own
   auto apart = [&](const int32_t* x) { return x == nullptr || a->lens + a->batch <= x || x + a->batch <= a->lens; };
+  for (const int32_t* x : {a->seq_lens, a->kv_start})  // shifted over it, one row's lens would be another's end
+    if (!apart(x) && a->lens != x) return BZ_ERR_SHAPE;
   p.write_lens = apart(a->seq_lens) && apart(a->kv_start);
   hipLaunchKernelGGL(pick_select(a->capacity), dim3(a->num_kv_heads, a->batch), dim3(kSelThreads), 0, stream, p);
   if (hipGetLastError() != hipSuccess) return BZ_ERR_LAUNCH;
@@ -308,7 +312,7 @@ BZ_EXPORT int bz_kv_compact(const bz_kv_tensor* tensors, int32_t num_tensors, co
                             int32_t batch, int32_t num_kv_heads, int32_t capacity, int32_t keep, hipStream_t stream) {
   if (tensors == nullptr || index == nullptr || lens == nullptr) return BZ_ERR_NULL;
   if (num_tensors <= 0 || num_tensors > BZ_KV_TENSORS || batch <= 0 || num_kv_heads <= 0 || capacity <= 0 || keep <= 0 ||
-      keep > capacity || (int64_t)batch * num_kv_heads > 65535)
+      keep > capacity || capacity > kMaxCapacity || (int64_t)batch * num_kv_heads > 65535)
     return BZ_ERR_SHAPE;
   if ((reinterpret_cast<uintptr_t>(index) | reinterpret_cast<uintptr_t>(lens)) & 3) return BZ_ERR_ALIGNMENT;
   MoveParams p{};

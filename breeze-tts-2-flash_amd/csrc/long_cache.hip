@@ -21,6 +21,7 @@ constexpr int kLongThreads = 256;
 // second launch (us, second launch / itself: 2 x 8 kv heads, G 2: 500 positions 8.97 / 7.30, 1377 10.26 / 9.65, 2048 10.82 /
 // 10.31, 4096 13.79 / 15.49; G 8, 1 x 8 x 1024 10.71 / 8.81).
 constexpr int kFusePositions = 2048;
+constexpr int kMaxTokens = 1 << 30;  // sums of tokens and tile sizes stay in 32 bits
 constexpr int kKv4Tokens = 16;  // most query tokens per row over a 4-bit cache
 
 bool dim_ok(int D) { return D == 64 || D == 128; }
@@ -41,6 +42,7 @@ struct Plan {
 int make_plan(int kind, int B, int NH, int NKV, int D, int cap, int T, int window, int sinks, int num_splits, int max_seq_len,
               Plan* pl) {
   if (B <= 0 || NH <= 0 || NKV <= 0 || cap <= 0 || T <= 0 || NH % NKV != 0 || window < 0 || sinks < 0) return BZ_ERR_SHAPE;
+  if (T > kMaxTokens) return BZ_ERR_SHAPE;
   if (num_splits < 0 || num_splits > kMaxSplits) return BZ_ERR_SHAPE;
   if (!dim_ok(D) || !group_ok(NH / NKV)) return BZ_ERR_UNSUPPORTED;
   if (kind == BZ_LONG_KV4 && T > kKv4Tokens) return BZ_ERR_UNSUPPORTED;

@@ -8,7 +8,8 @@ implementations (shapes only) do nothing, as the outputs are the caller's tensor
 functions: without one, a call takes its stream's cached workspace (allocated, when first needed, outside any graph
 memory pool), except while the stream is being captured, as when torch.compile's CUDA-graph trees record a graph:
 bz::gqa_decode and bz::gqa_decode_masked then run on the library's static scratch (bz_gqa_decode_noalloc) and
-bz::gqa_decode_fused raises unless it is given a workspace made beforehand. So compiled calls on different streams
+bz::gqa_decode_fused, bz::gqa_window, bz::gqa_decode_kv4 and bz::gqa_decode_tracked raise unless they are given a workspace
+made beforehand (or need none). So compiled calls on different streams
 never share a workspace. The package functions (attention.gqa_decode and the rest) call these operators while
 torch.compile traces them and call the C ABI directly otherwise, which keeps the eager per-call host cost of a plain
 function call.

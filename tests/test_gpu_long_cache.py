@@ -544,6 +544,40 @@ def test_capture_without_workspace_raises(device):
     torch.cuda.synchronize()
 
 
+def test_capture_takes_no_stream_workspace(device):
+    """Two graphs captured on a stream that has a workspace of its own: each needs one passed, so that both may run at once."""
+    rng = np.random.default_rng(6)
+    k = randn(rng, 1, 2, 5000, 128).to(device)
+    lens, side = ints([5000], device), torch.cuda.Stream()
+    qs = [randn(rng, 1, 4, 128).to(device) for _ in range(2)]
+    outs, graphs = [torch.empty_like(q) for q in qs], [torch.cuda.CUDAGraph() for _ in qs]
+    ws = [pkg.long_workspace("window", device, 1, 4, 2, 128, 5000) for _ in qs]
+    want = [pkg.gqa_window(q, k, k, lens, 0.1, 0) for q in qs]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        pkg.gqa_window(qs[0], k, k, lens, 0.1, 0)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="workspace"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+            pkg.gqa_window(qs[0], k, k, lens, 0.1, 0)
+    torch.cuda.synchronize()
+    for q, o, g, w in zip(qs, outs, graphs, ws):
+        with torch.cuda.graph(g, stream=side):
+            for _ in range(8):
+                pkg.gqa_window(q, k, k, lens, 0.1, 0, o, workspace=w)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, x) for o, x in zip(outs, want))
+
+
 def test_two_streams(device):
     """Calls in flight on two streams do not share workspaces."""
     a, b = _calls(device, 1), _calls(device, 2)
@@ -608,6 +642,17 @@ def test_refusals(device):
         lambda: pkg.kv_select(w, lens, 65), lambda: pkg.kv_select(w, lens, 0), lambda: pkg.kv_select(w, lens, 8, sinks=5, recent=4),
         lambda: pkg.kv_compact((k, k.clone(), k.clone(), k.clone(), k.clone()), ints([[[0]] * 2] * 2, device), lens),
         lambda: pkg.kv_compact((k,), ints([[[0]] * 2] * 2, device), lens, (k.float(),)),
+    ]
+    codes = lambda n: torch.zeros(2, 1, 64, n, dtype=torch.uint8, device=device).expand(2, 2, 64, n)  # noqa: E731
+    both = torch.empty(3, dtype=torch.int32, device=device)
+    bad += [
+        lambda: pkg.gqa_window(q, k, k, lens, 0.1, 8, torch.empty(2, 1, 128, dtype=BF16, device=device).expand(2, 4, 128)),
+        lambda: pkg.kv4_store(k, k, pkg.Kv4Cache(codes(64), codes(64), cache.k_scale, cache.v_scale), lens),
+        lambda: pkg.kv4_store(k, k, cache._replace(k_scale=codes(4), v_scale=codes(4)), lens),
+        lambda: pkg.kv4_store(k, k, cache._replace(v=cache.k), lens),
+        lambda: pkg.kv4_load(cache, lens, 64, k, k),
+        lambda: pkg.kv4_load(cache, lens, 4, *(k[:, :1, :4].expand(2, 2, 4, 128), k[:, 1:, :4].expand(2, 2, 4, 128))),
+        lambda: pkg.kv_select(w, both[:2], 8, lens=both[1:]),
     ]
     for i, call in enumerate(bad):
         with pytest.raises(RuntimeError):

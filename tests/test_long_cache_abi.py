@@ -166,6 +166,30 @@ def test_compact_refusals(lib, K, over, num, code):
     assert lib.bz_kv_compact(arr, num, 0x80000, 0x90000, 2, 8, 4096, 100, None) == code
 
 
+def test_sizes_past_32_bits(lib, K):
+    """Lengths whose sums with a tile's would pass 32 bits, and lens shifted over what the call reads."""
+    big = 2**31 - 1
+    w = K.GqaWindowArgs()
+    w.base = _base(K, tokens_per_row=big, q_stride_t=0)
+    assert lib.bz_gqa_window(ctypes.byref(w), None) == -2
+    c = _cache(K)
+    assert lib.bz_kv4_store(0x10000, 0x20000, 1024, 128, 1024, big, 0x30000, None, ctypes.byref(c), None) == -2
+    c.capacity = big
+    assert lib.bz_kv4_load(ctypes.byref(c), 0x30000, 1, 0x10000, 0x20000, 1024, 128, 1024, None) == -2
+    a = K.KvSelectArgs()
+    a.weights, a.seq_lens, a.index, a.lens = 0x70000, 0x30000, 0x80000, 0x90000
+    a.batch, a.num_kv_heads, a.capacity, a.keep = 2, 8, big, 100
+    assert lib.bz_kv_select(ctypes.byref(a), None) == -2
+    a.capacity, a.lens = 4096, 0x30004
+    assert lib.bz_kv_select(ctypes.byref(a), None) == -2
+    a.lens, a.kv_start = 0x90000, 0x8fffc
+    assert lib.bz_kv_select(ctypes.byref(a), None) == -2
+    arr = (K.KvTensor * 4)()
+    arr[0].src, arr[0].dst, arr[0].row_bytes = 0x100000, 0x900000, 256
+    arr[0].src_stride_s = arr[0].dst_stride_s = 256
+    assert lib.bz_kv_compact(arr, 1, 0x80000, 0x90000, 2, 8, big, 100, None) == -2
+
+
 def test_workspace_size(lib, K):
     n = ctypes.c_size_t(0)
     size = lambda *a: lib.bz_long_workspace_size(*a, ctypes.byref(n))  # noqa: E731
