@@ -30,10 +30,11 @@ struct LongParams {
   int out_wide;                 // out and its strides are multiples of 8 bytes
   int NKV, G, gshift, T, cap;   // G = 1 << gshift q heads per kv head
   int tiles, tpt;               // column tiles per row, tokens per column tile (16 / G)
-  float inv_splits;             // 1 / splits
+  int rows;                     // rows * column tiles; balanced: at most 64
+  float inv_splits;             // 1 / splits; balanced: 1 / (splits * rows)
   int splits, min_tiles, one_split;  // a split takes at least min_tiles wave tiles; up to one_split in all are not split
-  float* part_acc;              // [row * tile, kv head, split, column, D] unnormalised sums
-  float2* part_ml;              // [row * tile, kv head, split, column] (max, sum)
+  float* part_acc;              // [row * tile, kv head, split, column, D] unnormalised sums; balanced: [kv head, workgroup, ..]
+  float2* part_ml;              // [row * tile, kv head, split, column] (max, sum); the same
   int* counters;                // [row * tile, kv head] x kCounterStride
   float* scores;                // tracked: [row, q head, score_stride] scores times log2(e)
   int score_stride;
@@ -357,7 +358,47 @@ __device__ __forceinline__ void add_weights(const LongParams& p, int b, int h, i
 
 // ------------------------------------------------------------------------------------------------ split kernel
 
-// FMT: the cache's format. TRACK: also writes the scores (one token per row). grid (splits, kv heads, rows * column tiles).
+// What a workgroup takes: (row, column tile) z; balanced, also the first workgroup of z and the wave tiles of a split.
+struct Share {
+  int z, first, per;
+};
+// Balanced: lane i works out how many wave tiles (row, column tile) i has, and the wave the tiles a split takes, the same for all
+// rows (every workgroup streams at about the same rate, so the longest share is what the launch takes), in steps of the
+// waves. First what all rows have together over the grid, which fits where lengths are equal; then the same with as many
+// workgroups set aside as rounding up took; then what fits for certain, sum max(1, ceil(n / c)) <= sum n / c + rows <= grid.
+// At most 64 splits of a row to merge.
+template <int P, int NW, bool BAL>
+__device__ __forceinline__ Share deal_splits(const int32_t* lens, const int32_t* starts, const LongParams& p) {
+  if constexpr (!BAL) return {(int)blockIdx.z, 0, 0};
+  const int lane = threadIdx.x % kWave, zl = min(lane, p.rows - 1);
+  const int b = p.tiles == 1 ? zl : zl / p.tiles, t0 = (zl - b * p.tiles) * p.tpt;
+  const int e_raw = lens[b], s_raw = (starts ? starts : lens)[b];
+  const int e = clamp_int(e_raw, 0, p.cap), s = starts ? clamp_int(s_raw, 0, e) : 0;
+  auto token_end = [&](int t) { return max(s, e - (p.T - 1 - t)); };
+  const TileRange tr = tile_range<P>(s, token_end(t0), token_end(min(t0 + p.tpt, p.T) - 1), p.window, p.sinks);
+  const int n = lane < p.rows ? tr.na + tr.nb : 0;
+  const float all = 1.000001f * (float)__builtin_amdgcn_readlane((int)wave_scan((uint32_t)n), kWave - 1);
+  const int least = max(p.min_tiles, (wave_uniform((int)wave_max((float)n)) + 63) / 64);
+  const int grid = p.splits * p.rows;
+  float share = all * p.inv_splits;
+  int per, k, last;
+  for (int i = 0; i < 3; ++i) {
+    per = (max(least, (int)share + 1) + NW - 1) & ~(NW - 1);
+    const float inv = __builtin_amdgcn_rcpf((float)per);
+    k = lane >= p.rows ? 0 : n <= p.one_split ? 1 : max(1, ceil_div_est(n, per, inv));
+    last = (int)wave_scan((uint32_t)k);
+    const int need = __builtin_amdgcn_readlane(last, kWave - 1);
+    if (need <= grid) break;
+    share = all / (i == 0 ? fmaxf((float)grid - ((float)need - all * inv), (float)(grid - p.rows)) : (float)(grid - p.rows));
+  }
+  const uint64_t mine = __ballot((int)blockIdx.x < last && (int)blockIdx.x >= last - k);
+  if (mine == 0) return {-1, 0, 0};
+  const int z = __builtin_ctzll(mine);
+  return {z, __builtin_amdgcn_readlane(last - k, z), per};
+}
+
+// FMT: the cache's format. TRACK: also writes the scores (one token per row). Grid (splits, kv heads, rows * column tiles), each
+// row cut into as many splits; BAL: (splits * rows * column tiles, kv heads), dealt to the rows by their lengths (deal_splits).
 //
 // Four waves take every fourth wave tile of their split; a tile's loads are issued two tiles ahead, into registers, and the
 // product's columns are complete within a wave, so the waves meet once, at the end (LDS), and the workgroups once (the
@@ -366,12 +407,15 @@ __device__ __forceinline__ void add_weights(const LongParams& p, int b, int h, i
 // merge across workgroups (2 rows, window 1024: 6.3, 8.4 MB); a 4-bit cache the vector instructions, about 160 a tile of
 // 32 positions with one wave a SIMD, 64 of them conversions and 32 the transposition of V's pairs (4 rows of 20001..32768, 4 kv
 // heads of 8 q: 61 MB in 17.7, 3.4 TB/s).
-template <int D, int FMT, bool TRACK, int NT>
+template <int D, int FMT, bool TRACK, bool BAL, int NT>
 __global__ void __launch_bounds__(NT, 2)
     long_split_kernel(const int32_t* lens, const int32_t* starts, const LongParams p) {
   constexpr bool KV4 = FMT != kBf16;
   constexpr int NW = NT / kWave, P = KV4 ? 32 : 16, NS = P / 16, N = 4 * NS, NJ = D / 32;
-  const int split = blockIdx.x, h = blockIdx.y, z = blockIdx.z;
+  const int h = blockIdx.y;
+  const Share share = deal_splits<P, NW, BAL>(lens, starts, p);
+  if (BAL && share.z < 0) return;  // more workgroups than splits
+  const int z = share.z, split = BAL ? (int)blockIdx.x - share.first : (int)blockIdx.x;
   const int b = p.tiles == 1 ? z : z / p.tiles, t0 = (z - b * p.tiles) * p.tpt;
   const int e_raw = lens[b], s_raw = (starts ? starts : lens)[b];
   const int tid = threadIdx.x, lane = tid % kWave, w = wave_uniform(tid / kWave), r = lane % 16, g = lane / 16;
@@ -396,7 +440,7 @@ __global__ void __launch_bounds__(NT, 2)
   const TileRange tr = tile_range<P>(s, token_end(t0), token_end(t0 + ntok - 1), p.window, p.sinks);
   const int n = tr.na + tr.nb;
   // tiles per split, a multiple of the waves (no integer division: about 30 dependent instructions before the first load)
-  const int least = n <= p.one_split ? n : max(p.min_tiles, ceil_div_est(n, p.splits, p.inv_splits));
+  const int least = n <= p.one_split ? n : BAL ? share.per : max(p.min_tiles, ceil_div_est(n, p.splits, p.inv_splits));
   const int per = max(NW, (least + NW - 1) & ~(NW - 1));
   if (split > 0 && split * per >= n) return;  // past the row's last tile (split 0 always stays)
   const int j0 = split * per, j1 = min(n, j0 + per);
@@ -562,6 +606,7 @@ __global__ void __launch_bounds__(NT, 2)
 
   const int ncols_max = p.tpt << p.gshift;
   const int64_t unit = (int64_t)z * p.NKV + h;
+  const int64_t part0 = BAL ? (int64_t)h * gridDim.x + share.first : unit * p.splits;  // its first partials
   for (int o = tid; o < ncol * D / 4; o += NT) {
     const int c = o / (D / 4), d = 4 * (o % (D / 4));
     float M = s_m[0][c];
@@ -581,7 +626,7 @@ __global__ void __launch_bounds__(NT, 2)
     if (nact == 1) {
       write(c, d, A, M, L);
     } else {
-      const int64_t ps = (unit * p.splits + split) * ncols_max;
+      const int64_t ps = (part0 + split) * ncols_max;
       const Rsrc rp = span_rsrc(p.part_acc + ps * D, ncols_max * D * 4);
       using U4 = decltype(__builtin_amdgcn_raw_buffer_load_b128(rp, 0, 0, 0));
       __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(U4, A), rp, 16 * o, 0, kSc1);
@@ -609,8 +654,7 @@ __global__ void __launch_bounds__(NT, 2)
   }
   __syncthreads();
   if (!s_last) return;
-  merge_columns<D, NT>(p.part_acc + unit * p.splits * ncols_max * D, p.part_ml + unit * p.splits * ncols_max, ncols_max, ncol, nact,
-                   write);
+  merge_columns<D, NT>(p.part_acc + part0 * ncols_max * D, p.part_ml + part0 * ncols_max, ncols_max, ncol, nact, write);
   finish();
 }
 

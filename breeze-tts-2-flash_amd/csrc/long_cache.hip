@@ -21,6 +21,9 @@ constexpr int kLongThreads = 256;
 // second launch (us, second launch / itself: 2 x 8 kv heads, G 2: 500 positions 8.97 / 7.30, 1377 10.26 / 9.65, 2048 10.82 /
 // 10.31, 4096 13.79 / 15.49; G 8, 1 x 8 x 1024 10.71 / 8.81).
 constexpr int kFusePositions = 2048;
+// Bytes of the longest row a split takes from which on splits are dealt (4 rows of 20001..32768 of 4 bits, 16 splits, 278 KB:
+// 18.6 us dealt or not; 16 rows of 128..2048, 2 splits, 139 KB: 10.9 dealt, 10.7 not).
+constexpr int64_t kDealBytes = 1 << 18;
 constexpr int kMaxTokens = 1 << 30;  // sums of tokens and tile sizes stay in 32 bits
 constexpr int kKv4Tokens = 16;  // most query tokens per row over a 4-bit cache
 
@@ -34,6 +37,7 @@ size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 struct Plan {
   bool prefill;  // gqa_window: the chunk kernel, which needs no workspace
   int cgroups;   // its column groups
+  bool balanced; // splits are dealt to the rows by their lengths
   int G, gshift, tpt, tiles, splits, min_tiles, one_split, score_stride;
   int64_t units;
   size_t ml, acc, head_ml, scores, total;
@@ -85,19 +89,29 @@ int make_plan(int kind, int B, int NH, int NKV, int D, int cap, int T, int windo
   const int n = (int)((len + P - 1) / P) + 1;
   pl->min_tiles = kLongThreads / kWave;
   pl->one_split = (kOneSplitBytes / (kv4 ? D + D / 16 : 4 * D)) / P;
+  // A server's batch: more than three rows whose lengths differ because no window cuts them. Its splits are dealt to the rows by
+  // their lengths where a split streams long enough for that to show (deal_splits costs about 0.5 us before the first load;
+  // 64 rows: a lane for each).
+  const bool batch = !cut && B > 3;
+  const int64_t row_bytes = kv4 ? D + D / 16 : 4 * D;
+  auto dealt = [&](int64_t s) { return s > 1 && batch && (int64_t)B * pl->tiles <= kWave && len * row_bytes / s >= kDealBytes; };
   int splits = num_splits;
   if (splits == 0) {
     // One round of workgroups (us: 1 row x 8 kv heads x 8192 positions of 4 bits: 32 splits 7.5, 64 8.6; 2 rows tracked, 1377:
-    // 16 splits 10.2, 32 11.1; 4 rows, window 4096: 8 splits 14.8, 16 15.3; 16 rows: 2 splits 42.1, 4 44.5), two for a server's
-    // batch (more than three rows) whose lengths differ because no window cuts them (4 rows of 9000..16384 tracked: 8 splits
-    // 49.3, 16 47.1; 16 rows of 128..2048 of 4 bits: 2 splits 11.3, 4 10.8; 32 rows, head_dim 64: 1 split 22.9, 2 18.7).
-    splits = (int)((!cut && B > 3 ? 2 : 1) * cus / pl->units);
+    // 16 splits 10.2, 32 11.1; 4 rows, window 4096: 8 splits 14.8, 16 15.3; 16 rows: 2 splits 42.1, 4 44.5). For a batch two,
+    // which even its rows out (16 rows of 128..2048 of 4 bits: 2 splits 11.3, 4 10.8; 32 rows, head_dim 64: 1 split 22.9, 2
+    // 18.7), or at least four dealt splits (us, 8 kv heads, head_dim 128, one round dealt / two, each row as many: 8 rows of
+    // 100..8192 27.1 / 31.9; 4 of 9000..16384 tracked 46.8 / 48.8; 6 of 500..8192, 4 tokens, 4 kv heads 16.1 / 20.2; fewer are
+    // too coarse to deal: 16 of 300..4096 tracked, 2 splits dealt 39.3, 4 34.2, 4 each 38.0).
+    const int64_t round = cus / pl->units;
+    splits = (int)(batch && !(round >= 4 && dealt(round)) ? 2 * cus / pl->units : round);
     const int most = (n + pl->min_tiles - 1) / pl->min_tiles;
     if (splits > most) splits = most;
     if (splits > 64) splits = 64;
     if (n <= pl->one_split || splits < 1) splits = 1;
   }
   pl->splits = splits;
+  pl->balanced = dealt(splits);
 
   const size_t cols = (size_t)pl->units * splits * pl->tpt * pl->G;
   const bool merged = splits > 1;
@@ -177,7 +191,8 @@ LongParams long_params(const bz_gqa_decode_args* a, const Plan& pl, int window, 
   p.NKV = a->num_kv_heads, p.G = pl.G, p.gshift = pl.gshift, p.T = a->tokens_per_row > 1 ? a->tokens_per_row : 1;
   p.cap = a->capacity;
   p.tiles = pl.tiles, p.tpt = pl.tpt;
-  p.inv_splits = 1.0f / (float)pl.splits;
+  p.rows = a->batch * pl.tiles;
+  p.inv_splits = 1.0f / (float)(pl.balanced ? pl.splits * p.rows : pl.splits);
   p.splits = pl.splits, p.min_tiles = pl.min_tiles, p.one_split = pl.one_split;
   char* const ws = static_cast<char*>(a->workspace);
   p.counters = reinterpret_cast<int*>(ws);
@@ -190,12 +205,13 @@ LongParams long_params(const bz_gqa_decode_args* a, const Plan& pl, int window, 
 }
 
 template <int FMT, bool TRACK>
-int launch_split(const bz_gqa_decode_args* a, int D, const LongParams& p, const Plan& pl, int B, hipStream_t stream) {
-  const dim3 grid(pl.splits, p.NKV, B * pl.tiles);
-  if (D == 128)
-    hipLaunchKernelGGL((long_split_kernel<128, FMT, TRACK, kLongThreads>), grid, dim3(kLongThreads), 0, stream, a->seq_lens, a->kv_start, p);
-  else
-    hipLaunchKernelGGL((long_split_kernel<64, FMT, TRACK, kLongThreads>), grid, dim3(kLongThreads), 0, stream, a->seq_lens, a->kv_start, p);
+int launch_split(const bz_gqa_decode_args* a, int D, const LongParams& p, const Plan& pl, hipStream_t stream) {
+  const dim3 grid = pl.balanced ? dim3(pl.splits * p.rows, p.NKV) : dim3(pl.splits, p.NKV, p.rows);
+  using Fn = void (*)(const int32_t*, const int32_t*, const LongParams);
+  const Fn fns[2][2] = {
+      {long_split_kernel<64, FMT, TRACK, false, kLongThreads>, long_split_kernel<64, FMT, TRACK, true, kLongThreads>},
+      {long_split_kernel<128, FMT, TRACK, false, kLongThreads>, long_split_kernel<128, FMT, TRACK, true, kLongThreads>}};
+  hipLaunchKernelGGL(fns[D == 128][pl.balanced], grid, dim3(kLongThreads), 0, stream, a->seq_lens, a->kv_start, p);
   return hipGetLastError() == hipSuccess ? BZ_OK : BZ_ERR_LAUNCH;
 }
 
@@ -232,7 +248,7 @@ BZ_EXPORT int bz_gqa_window(const bz_gqa_window_args* wa, hipStream_t stream) {
   if (rc == BZ_OK) rc = check_workspace(a, pl);
   if (rc != BZ_OK) return rc;
   const LongParams p = long_params(a, pl, wa->window, wa->sinks);
-  if (!pl.prefill) return launch_split<kBf16, false>(a, a->head_dim, p, pl, a->batch, stream);
+  if (!pl.prefill) return launch_split<kBf16, false>(a, a->head_dim, p, pl, stream);
   const dim3 grid(a->num_kv_heads, pl.tiles, a->batch);
   using Fn = void (*)(const int32_t*, const int32_t*, const LongParams);
   const Fn fns[2][3] = {{window_prefill_kernel<64, 1>, window_prefill_kernel<64, 2>, window_prefill_kernel<64, 4>},
@@ -261,8 +277,8 @@ BZ_EXPORT int bz_gqa_decode_kv4(const bz_gqa_kv4_args* ka, hipStream_t stream) {
   p.k_scale = static_cast<const uint8_t*>(c->k_scale);
   p.v_scale = static_cast<const uint8_t*>(c->v_scale);
   p.sc_sb = c->scale_stride_b, p.sc_sh = c->scale_stride_h;
-  if (c->stride_s == a.head_dim / 2) return launch_split<kKv4Packed, false>(&a, a.head_dim, p, pl, a.batch, stream);
-  return launch_split<kKv4, false>(&a, a.head_dim, p, pl, a.batch, stream);
+  if (c->stride_s == a.head_dim / 2) return launch_split<kKv4Packed, false>(&a, a.head_dim, p, pl, stream);
+  return launch_split<kKv4, false>(&a, a.head_dim, p, pl, stream);
 }
 
 BZ_EXPORT int bz_gqa_decode_tracked(const bz_gqa_tracked_args* ta, hipStream_t stream) {
@@ -284,7 +300,7 @@ BZ_EXPORT int bz_gqa_decode_tracked(const bz_gqa_tracked_args* ta, hipStream_t s
   p.decay = ta->decay;
   const int longest = a->max_seq_len > 0 && a->max_seq_len < a->capacity ? a->max_seq_len : a->capacity;
   p.fuse = longest <= kFusePositions;
-  rc = launch_split<kBf16, true>(a, a->head_dim, p, pl, a->batch, stream);
+  rc = launch_split<kBf16, true>(a, a->head_dim, p, pl, stream);
   if (rc != BZ_OK || p.fuse) return rc;
   const dim3 grid((longest + 4 * kApplyThreads - 1) / (4 * kApplyThreads), a->num_kv_heads, a->batch);
   hipLaunchKernelGGL(track_apply_kernel, grid, dim3(kApplyThreads), 0, stream, a->seq_lens, a->kv_start, p);

@@ -495,6 +495,38 @@ def test_bounded_generation(device, fmt):
     assert (weights.sum((1, 2)) <= 50 * NKV * G + 1e-2).all()
 
 
+@pytest.mark.parametrize("kind,T,lens,splits", [
+    ("window", 1, [4000, 1, 0, 37, 3999], 0), ("window", 1, [1] * 7 + [6000], 3), ("window", 5, [4000, 2500, 3, 0, 900, 17], 2),
+    ("tracked", 1, [4000, 1200, 0, 64, 2000, 5], 0), ("tracked", 1, [6000] * 4, 7), ("kv4", 3, [9000, 4, 0, 5000, 31], 2),
+    ("kv4", 1, [16000, 15999, 1, 8000], 4), ("window", 9, [3000, 17, 0, 2900], 2),
+])
+def test_splits_dealt_by_length(device, kind, T, lens, splits):
+    """A batch of long rows of very different lengths (also none at all): the splits of a launch go to the rows by length. Every
+    row against the oracle, and what it gets alone."""
+    rng = np.random.default_rng(len(lens) + T)
+    B, NKV, G, D, cap = len(lens), 1, 4, 128, max(lens) + 5
+    q = randn(rng, B, NKV * G, T, D)
+    k, v = randn(rng, B, NKV, cap, D), randn(rng, B, NKV, cap, D)
+    starts = [min(7 * b, n) for b, n in enumerate(lens)]
+    qd, kd, vd, ld, sd = q.to(device), k.to(device), v.to(device), ints(lens, device), ints(starts, device)
+    qd, kw = qd if T > 1 else qd[:, :, 0], dict(kv_start=sd, num_splits=splits)
+    if kind == "window":
+        out = pkg.gqa_window(qd, kd, vd, ld, D ** -0.5, 0, **kw)
+    elif kind == "kv4":
+        cache = pkg.kv4_store(kd, vd, pkg.kv4_cache(B, NKV, cap, D, device), ints([0] * B, device))
+        k, v = (x.cpu() for x in pkg.kv4_load(cache, ints([0] * B, device), cap))
+        out = pkg.gqa_decode_kv4(qd, cache, ld, D ** -0.5, **kw)
+    else:
+        w, wo = torch.rand(B, NKV, cap, device=device), torch.full((B, NKV, cap), -3.0, device=device)
+        out = pkg.gqa_decode_tracked(qd, kd, vd, ld, D ** -0.5, w, weights_out=wo, **kw)
+        for b, n in enumerate(lens):
+            grown = wo[b, 0, starts[b]:n].double() - w[b, 0, starts[b]:n].double()
+            # fp32 sums of a weight below 5 (2^-22 each) and of probabilities (their errors below 2^-16 relative)
+            assert abs(float(grown.sum()) - (G if n > starts[b] else 0)) <= n * 2.0 ** -22 + G * 2.0 ** -16, b
+            assert (wo[b, 0, :starts[b]] == -3).all() and (wo[b, 0, n:] == -3).all(), b
+    check_attention(out, q.float(), k.float(), v.float(), lens, D ** -0.5, starts=starts, what=f"{kind} {lens}")
+
+
 def test_tracked_splits_share_a_workspace(device):
     """One split writes no partials; a call of several that follows in the same workspace still finds its counters zero."""
     rng = np.random.default_rng(12)
