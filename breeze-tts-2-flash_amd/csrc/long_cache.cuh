@@ -404,9 +404,10 @@ __device__ __forceinline__ Share deal_splits(const int32_t* lens, const int32_t*
 // product's columns are complete within a wave, so the waves meet once, at the end (LDS), and the workgroups once (the
 // counters). What bounds it (us): a bf16 cache over long rows the stream (16 rows of 500..16384 behind a window of 4096, 8 kv
 // heads, head_dim 128: 269 MB in 38.4, 7.0 TB/s, a plain read's rate); few rows the launch, two round trips of loads and the
-// merge across workgroups (2 rows, window 1024: 6.3, 8.4 MB); a 4-bit cache the vector instructions, about 160 a tile of
-// 32 positions with one wave a SIMD, 64 of them conversions and 32 the transposition of V's pairs (4 rows of 20001..32768, 4 kv
-// heads of 8 q: 61 MB in 17.7, 3.4 TB/s).
+// merge across workgroups (2 rows, window 1024: 6.3, 8.4 MB); a 4-bit cache both its stream and the vector instructions, about
+// 160 a tile of 32 positions, 64 of them conversions and 32 the transposition of V's pairs (4 rows of 20001..32768, 4 kv
+// heads of 8 q: 61 MB in 17.7; a copy of the kernel with the loads alone 17.4 where this took 18.9, with tiles from the L2 17.1).
+// V's scales as two 16-byte loads and a bit field each, in place of eight byte loads: no faster.
 template <int D, int FMT, bool TRACK, bool BAL, int NT>
 __global__ void __launch_bounds__(NT, 2)
     long_split_kernel(const int32_t* lens, const int32_t* starts, const LongParams p) {

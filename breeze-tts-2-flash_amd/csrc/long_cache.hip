@@ -100,11 +100,12 @@ int make_plan(int kind, int B, int NH, int NKV, int D, int cap, int T, int windo
     // One round of workgroups (us: 1 row x 8 kv heads x 8192 positions of 4 bits: 32 splits 7.5, 64 8.6; 2 rows tracked, 1377:
     // 16 splits 10.2, 32 11.1; 4 rows, window 4096: 8 splits 14.8, 16 15.3; 16 rows: 2 splits 42.1, 4 44.5). For a batch two,
     // which even its rows out (16 rows of 128..2048 of 4 bits: 2 splits 11.3, 4 10.8; 32 rows, head_dim 64: 1 split 22.9, 2
-    // 18.7), or at least four dealt splits (us, 8 kv heads, head_dim 128, one round dealt / two, each row as many: 8 rows of
-    // 100..8192 27.1 / 31.9; 4 of 9000..16384 tracked 46.8 / 48.8; 6 of 500..8192, 4 tokens, 4 kv heads 16.1 / 20.2; fewer are
-    // too coarse to deal: 16 of 300..4096 tracked, 2 splits dealt 39.3, 4 34.2, 4 each 38.0).
+    // 18.7; dealt, 8 rows of 100..32768 of 4 bits: 4 splits 39.4, 8 33.1); over bf16 one, if that is at least four dealt splits
+    // (us, 8 kv heads, head_dim 128, one round dealt / two, each row as many: 8 rows of 100..8192 27.1 / 31.9; 4 of 9000..16384
+    // tracked 46.8 / 48.8; 6 of 500..8192, 4 tokens, 4 kv heads 16.1 / 20.2; fewer are too coarse to deal: 16 of 300..4096
+    // tracked, 2 splits dealt 39.3, 4 34.2, 4 each 38.0).
     const int64_t round = cus / pl->units;
-    splits = (int)(batch && !(round >= 4 && dealt(round)) ? 2 * cus / pl->units : round);
+    splits = (int)(batch && (kv4 || round < 4 || !dealt(round)) ? 2 * cus / pl->units : round);
     const int most = (n + pl->min_tiles - 1) / pl->min_tiles;
     if (splits > most) splits = most;
     if (splits > 64) splits = 64;
