@@ -320,40 +320,46 @@ __device__ __forceinline__ void merge_columns(const float* part_acc, const float
   }
 }
 
-// (Memory bound: 4 rows x 8 kv heads of 9000..16384, groups of 4: 5.0 us for 9.4 MB of scores and weights, most of them in L2.)
-// weights_out[b, h, pos] = decay * weights[b, h, pos] + sum_g 2^(score - max_g) / sum_g over the row's range [s, e), by threads
-// first, first + step, ..: four consecutive positions a thread and turn (16-byte score loads, coherent with the other
-// workgroups' stores). ml(g): (max, 1 / sum) of the group's q head g.
-template <class Ml>
-__device__ __forceinline__ void add_weights(const LongParams& p, int b, int h, int s, int e, int first, int step, Ml ml) {
-  const float* const wi = p.weights + (int64_t)b * p.w_sb + (int64_t)h * p.w_sh;
-  float* const wo = p.weights_out + (int64_t)b * p.wo_sb + (int64_t)h * p.wo_sh;
-  for (int pos0 = (s & ~3) + 4 * first; pos0 < e; pos0 += 4 * step) {
-    f32x4_t acc = {0.f, 0.f, 0.f, 0.f}, old = acc, x[kMaxGroup];
-    // every load before the first use
+// weights_out[b, h, pos] = decay * weights[b, h, pos] + sum_g 2^(score - max_g) / sum_g over the row's range [s, e): four consecutive
+// positions a thread and turn, their scores (16-byte loads, coherent with the other workgroups' stores) and old weights loaded by
+// load_turn and added by add_turn. ml(g): (max, 1 / sum) of the group's q head g.
+struct WeightTurn {
+  f32x4_t x[kMaxGroup], old;
+};
+__device__ __forceinline__ WeightTurn load_turn(const LongParams& p, int b, int h, int s, int e, int pos0) {
+  WeightTurn t;
+  t.old = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  if (pos0 >= e) return t;
+  const int row = p.score_stride * 4;  // bytes; below 2^27 (host), so those of a group below 2^30
+  const Rsrc rs = span_rsrc(wave_uniform(p.scores + ((int64_t)b * p.NKV + h) * p.G * p.score_stride), p.G * row);
 #pragma unroll
-    for (int g = 0; g < kMaxGroup; ++g) {
-      if (g >= p.G) break;
-      const int64_t hq = ((int64_t)b * p.NKV + h) * p.G + g;
-      const Rsrc rs = span_rsrc(wave_uniform(p.scores + hq * p.score_stride), p.score_stride * 4);
-      x[g] = __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, 4 * pos0, 0, kSc1));
-    }
-    if (p.decay != 0.f) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) old[i] = wi[clamp_int(pos0 + i, s, e - 1)];  // outside the range: unused
-    }
-#pragma unroll
-    for (int g = 0; g < kMaxGroup; ++g) {
-      if (g >= p.G) break;
-      const float2 y = ml(g);
-      const float mu = y.x == -INFINITY ? 0.f : y.x;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] = fmaf(fast_exp2(x[g][i] - mu), y.y, acc[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (pos0 + i >= s && pos0 + i < e) wo[pos0 + i] = p.decay == 0.f ? acc[i] : fmaf(p.decay, old[i], acc[i]);
+  for (int g = 0; g < kMaxGroup; ++g) {
+    if (g >= p.G) break;
+    t.x[g] = __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, 4 * pos0, g * row, kSc1));
   }
+  if (p.decay != 0.f) {
+    const float* const wi = p.weights + (int64_t)b * p.w_sb + (int64_t)h * p.w_sh;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t.old[i] = wi[clamp_int(pos0 + i, s, e - 1)];  // outside the range: unused
+  }
+  return t;
+}
+template <class Ml>
+__device__ __forceinline__ void add_turn(const LongParams& p, int b, int h, int s, int e, int pos0, const WeightTurn& t, Ml ml) {
+  float* const wo = p.weights_out + (int64_t)b * p.wo_sb + (int64_t)h * p.wo_sh;
+  if (pos0 >= e) return;
+  f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int g = 0; g < kMaxGroup; ++g) {
+    if (g >= p.G) break;
+    const float2 y = ml(g);
+    const float mu = y.x == -INFINITY ? 0.f : y.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = fmaf(fast_exp2(t.x[g][i] - mu), y.y, acc[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (pos0 + i >= s && pos0 + i < e) wo[pos0 + i] = p.decay == 0.f ? acc[i] : fmaf(p.decay, t.old[i], acc[i]);
 }
 
 // ------------------------------------------------------------------------------------------------ split kernel
@@ -598,11 +604,12 @@ __global__ void __launch_bounds__(NT, 2)
       else p.head_ml[(int64_t)b * p.NKV * p.G + oh] = make_float2(m, inv);
     }
   };
-  auto finish = [&]() {  // tracked: the row's weights, once every score of it is written and its heads' sums are in s_head
-    if (TRACK && p.fuse) {
-      __syncthreads();
-      add_weights(p, b, h, s, e, tid, NT, [&](int q) { return s_head[q]; });
-    }
+  // tracked: the row's weights, once every score of it is written and its heads' sums are in s_head. The first two turns (all
+  // there are up to 2048 positions) may have been loaded before.
+  const int turn0 = (s & ~3) + 4 * tid;
+  auto turn = [&](int u) { return load_turn(p, b, h, s, e, turn0 + 4 * NT * u); };
+  auto add = [&](int u, const WeightTurn& t) {
+    add_turn(p, b, h, s, e, turn0 + 4 * NT * u, t, [&](int q) { return s_head[q]; });
   };
 
   const int ncols_max = p.tpt << p.gshift;
@@ -638,8 +645,11 @@ __global__ void __launch_bounds__(NT, 2)
     }
   }
   if (nact == 1) {
-    __builtin_amdgcn_s_waitcnt(0x0f70);
-    finish();
+    if (TRACK && p.fuse) {
+      __builtin_amdgcn_s_waitcnt(0x0f70);
+      __syncthreads();
+      for (int u = 0; turn0 + 4 * NT * u < e; ++u) add(u, turn(u));
+    }
     return;
   }
 
@@ -655,19 +665,32 @@ __global__ void __launch_bounds__(NT, 2)
   }
   __syncthreads();
   if (!s_last) return;
-  merge_columns<D, NT>(p.part_acc + part0 * ncols_max * D, p.part_ml + part0 * ncols_max, ncols_max, ncol, nact, write);
-  finish();
+  const auto merge = [&]() {
+    merge_columns<D, NT>(p.part_acc + part0 * ncols_max * D, p.part_ml + part0 * ncols_max, ncols_max, ncol, nact, write);
+  };
+  if (TRACK && p.fuse) {
+    const WeightTurn a = turn(0), c = turn(1);  // with the partials, not after them
+    merge();
+    __syncthreads();
+    add(0, a);
+    add(1, c);
+    for (int u = 2; turn0 + 4 * NT * u < e; ++u) add(u, turn(u));
+  } else {
+    merge();
+  }
 }
 
-// add_weights in a launch of its own, after the split kernel that wrote the scores: grid (chunks of kApplyThreads * 4
-// positions, kv heads, rows).
+// The weights in a launch of their own, after the split kernel that wrote the scores: grid (chunks of kApplyThreads * 4 positions,
+// kv heads, rows). Memory bound: 4 rows x 8 kv heads of 9000..16384, groups of 4: 5.0 us for 15 MB of scores and weights, most
+// of them in the L2.
 __global__ void __launch_bounds__(kApplyThreads)
     track_apply_kernel(const int32_t* lens, const int32_t* starts, const LongParams p) {
   const int h = blockIdx.y, b = blockIdx.z;
   int s, e;
   long_range(lens[b], (starts ? starts : lens)[b], starts != nullptr, p.cap, s, e);
-  add_weights(p, b, h, s, e, blockIdx.x * kApplyThreads + threadIdx.x, gridDim.x * kApplyThreads,
-              [&](int g) { return p.head_ml[((int64_t)b * p.NKV + h) * p.G + g]; });
+  for (int pos0 = (s & ~3) + 4 * (blockIdx.x * kApplyThreads + threadIdx.x); pos0 < e; pos0 += 4 * gridDim.x * kApplyThreads)
+    add_turn(p, b, h, s, e, pos0, load_turn(p, b, h, s, e, pos0),
+             [&](int g) { return p.head_ml[((int64_t)b * p.NKV + h) * p.G + g]; });
 }
 
 }  // namespace
