@@ -21,8 +21,9 @@ constexpr int kMaxCapacity = 1 << 30;  // sums of positions and strip sizes stay
 //
 // A row's bytes are few (4 a position) and one workgroup reads them all, so its latencies are the bound: a row of up to
 // 1024 IPT positions is loaded once, all loads at a time, and everything after works from registers. A longer one goes
-// through in chunks of that many, loaded again for each pass. 32 (row, head) pairs of 7000..8192, keep 4096: 10.7 us (three
-// passes of about 2 us between barriers, launch and first loads 3).
+// through in chunks of that many, loaded again for each pass. 32 (row, head) pairs of 7000..8192, keep 4096: 10.0 us (three
+// passes of about 2 us between barriers, launch and first loads 3; with keys held beside the weights, not worked out anew in
+// each pass, from 10.7).
 
 constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / kWave;
@@ -56,6 +57,11 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* s) {
   return (w > 0 ? (uint32_t)__builtin_amdgcn_readlane((int)sums, w - 1) : 0u) + v - x;
 }
 
+// How many lanes below this one a ballot holds.
+__device__ __forceinline__ uint32_t lanes_below(uint64_t m) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
+}
+
 template <int IPT>
 __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const SelectParams p) {
   constexpr int kCounts = IPT * kSelWaves, kChunk = IPT * kSelThreads;
@@ -73,13 +79,29 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const SelectPara
   int32_t* const index = p.index + ((int64_t)b * p.NKV + h) * p.keep;
 
   // a chunk's weights: strip i holds the positions c0 + 1024 i .. + 1023, one a thread
+  const int lo = s + p.sinks, hi = e - p.recent;  // the middle, of which positions stay by weight
   float x[IPT];
+  constexpr bool kHold = IPT <= 16;    // the keys as well (with 32 strips there are no registers for both)
+  uint32_t key[kHold ? IPT : 1], middle = 0;  // bit i: strip i's position lies in the middle (held as well)
+  auto key_of = [&](int i) { return kHold ? key[i] : weight_key(x[i]); };
+  auto in_middle = [&](int i, int c0) {
+    const int pos = c0 + i * kSelThreads + tid;
+    return kHold ? (middle >> i & 1) != 0 : pos >= lo && pos < hi;
+  };
   auto load = [&](int c0) {
 #pragma unroll
     for (int i = 0; i < IPT; ++i) x[i] = w[max(min(c0 + i * kSelThreads + tid, e - 1), 0)];  // past the row: unused
+    if constexpr (kHold) {
+      middle = 0;
+#pragma unroll
+      for (int i = 0; i < IPT; ++i) {
+        const int pos = c0 + i * kSelThreads + tid;
+        key[i] = weight_key(x[i]);
+        middle |= pos >= lo && pos < hi ? 1u << i : 0u;
+      }
+    }
   };
   load(s);
-  const int lo = s + p.sinks, hi = e - p.recent;  // the middle, of which m positions stay
   const uint32_t m = n > p.keep ? (uint32_t)(p.keep - p.sinks - p.recent) : 0u;
   uint32_t prefix = 0, left = m;  // the threshold's top bits; how many of the keys with those bits stay
   if (m > 0) {                    // then hi - lo > m
@@ -93,10 +115,13 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const SelectPara
         if (n > kChunk && (pass > 0 || c0 > s)) load(c0);
 #pragma unroll
         for (int i = 0; i < IPT; ++i) {
-          const int pos = c0 + i * kSelThreads + tid;
-          const uint32_t k = weight_key(x[i]);
-          if (pos >= lo && pos < hi && (pass == 0 || k >> (32 - known) == prefix))
-            atomicAdd(&s_hist[(k >> shift) & ((1u << bits) - 1)], 1u);
+          if (in_middle(i, c0) && (pass == 0 || key_of(i) >> (32 - known) == prefix)) {
+            // lanes that all have one digit count at once (rows of 8192 equal weights: 27.7 us without this)
+            const uint32_t digit = (key_of(i) >> shift) & ((1u << bits) - 1), one = __builtin_amdgcn_readfirstlane(digit);
+            const uint64_t lanes = __ballot(true);
+            if (__ballot(digit != one) != 0) atomicAdd(&s_hist[digit], 1u);
+            else if (lanes_below(lanes) == 0) atomicAdd(&s_hist[digit], (uint32_t)__popcll(lanes));
+          }
         }
       }
       __syncthreads();
@@ -122,8 +147,8 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const SelectPara
 #pragma unroll
     for (int i = 0; i < IPT; ++i) {
       const int pos = c0 + i * kSelThreads + tid;
-      const uint32_t k = weight_key(x[i]);
-      const bool ends = n <= p.keep || pos < lo || pos >= hi;
+      const uint32_t k = key_of(i);
+      const bool ends = n <= p.keep || !in_middle(i, c0);
       const bool stays = pos < e && (ends || (m > 0 && k > prefix)), ties = pos < e && !ends && m > 0 && k == prefix;
       above |= stays ? 1u << i : 0u;
       equal |= ties ? 1u << i : 0u;
@@ -146,10 +171,9 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const SelectPara
 #pragma unroll
     for (int i = 0; i < IPT; ++i) {
       const bool stays = (above >> i) & 1, ties = (equal >> i) & 1;
-      const uint64_t bs = __ballot(stays), bt = __ballot(ties), below = (1ull << lane) - 1;
       const uint32_t c = s_count[i * kSelWaves + wv];
-      const uint32_t at = before + (c & 0xffffu) + (uint32_t)__popcll(bs & below);
-      const uint32_t tie = ties_before + (c >> 16) + (uint32_t)__popcll(bt & below);
+      const uint32_t at = before + (c & 0xffffu) + lanes_below(__ballot(stays));
+      const uint32_t tie = ties_before + (c >> 16) + lanes_below(__ballot(ties));
       if (stays || (ties && tie < left)) {
         const int d = (int)(at + min(tie, left));
         index[d] = c0 + i * kSelThreads + tid;

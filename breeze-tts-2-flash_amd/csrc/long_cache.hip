@@ -17,9 +17,9 @@ namespace {
 // Threads of a split workgroup. Eight waves measured 6% faster on long rows of 4 bits (4 rows x 4 kv heads of 20001..32768,
 // G 8: 17.9 against 19.0 us) and 2 to 40% slower on everything else.
 constexpr int kLongThreads = 256;
-// Rows up to which the merging workgroup of a tracked step adds the weights itself (two turns of its threads), in place of a
-// second launch (us, second launch / itself: 2 x 8 kv heads, G 2: 500 positions 8.97 / 7.30, 1377 10.26 / 9.65, 2048 10.82 /
-// 10.31, 4096 13.79 / 15.49; G 8, 1 x 8 x 1024 10.71 / 8.81).
+// Rows up to which the merging workgroup of a tracked step adds the weights itself (the two turns of its threads whose scores it
+// loads with the partials), in place of a second launch (us, second launch / itself, 2 x 8 kv heads, G 2: 500 positions 8.5 /
+// 6.5, 1377 10.4 / 8.6, 2048 10.7 / 9.3, 2600 12.2 / 12.0, 4096 13.3 / 14.8; G 8, 1 x 8 x 1024 10.3 / 8.2, 2048 12.4 / 11.0).
 constexpr int kFusePositions = 2048;
 // Bytes of the longest row a split takes from which on splits are dealt (4 rows of 20001..32768 of 4 bits, 16 splits, 278 KB:
 // 18.6 us dealt or not; 16 rows of 128..2048, 2 splits, 139 KB: 10.9 dealt, 10.7 not).
