@@ -194,7 +194,8 @@ __global__ void __launch_bounds__(kPreThreads, 2)
     constexpr bool kOdd = decltype(odd)::value;
     const char *const kbuf = kOdd ? k_even : k_odd, *const vbuf = kOdd ? v_odd : v_even;
     __builtin_amdgcn_s_waitcnt(0x0f70);  // this wave's loads of K j + 1 and V j are in LDS
-    __syncthreads();                     // everyone's are, and nobody reads K j or V j - 1 any more
+    // everyone's are, and nobody reads K j or V j - 1 any more (a wave with tiles of its own has just used what it read of them)
+    if constexpr (CG > 1) __syncthreads();
     bf16x8_t kf[KA], vf[2][ND];
 #pragma unroll
     for (int i = 0; i < KA; ++i) kf[i] = k_read(kbuf, i);
@@ -258,7 +259,7 @@ __global__ void __launch_bounds__(kPreThreads, 2)
   if (n > 0) {
     stage_tile<D, TP, CG, false>(k_even + group, rk, pos_of(0), s, e1 - 1, row_bytes, cg, lane);
     __builtin_amdgcn_s_waitcnt(0x0f70);
-    __syncthreads();
+    if constexpr (CG > 1) __syncthreads();
     if (n > 1) stage_tile<D, TP, CG, false>(k_odd + group, rk, pos_of(1), s, e1 - 1, row_bytes, cg, lane);
     stage_tile<D, TP, CG, true>(v_even + group, rv, pos_of(0), s, e1 - 1, row_bytes, cg, lane);
     f32x16_t xa[NB], xb[NB];
