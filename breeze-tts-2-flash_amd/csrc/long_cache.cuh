@@ -30,7 +30,7 @@ struct LongParams {
   int out_wide;                 // out and its strides are multiples of 8 bytes
   int NKV, G, gshift, T, cap;   // G = 1 << gshift q heads per kv head
   int tiles, tpt;               // column tiles per row, tokens per column tile (16 / G)
-  int rows;                     // rows * column tiles; balanced: at most 64
+  int rows;                     // balanced: rows * column tiles, at most 64
   float inv_splits;             // 1 / splits; balanced: 1 / (splits * rows)
   int splits, min_tiles, one_split;  // a split takes at least min_tiles wave tiles; up to one_split in all are not split
   float* part_acc;              // [row * tile, kv head, split, column, D] unnormalised sums; balanced: [kv head, workgroup, ..]

@@ -4,6 +4,8 @@
 
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "bz_long_cache.h"
 #include "long_cache.cuh"
 #include "window_prefill.cuh"
@@ -35,7 +37,7 @@ size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 // counters first, one 256-byte line per (row, column tile, kv head); they are zero between calls, everything else is
 // written before it is read).
 struct Plan {
-  bool prefill;  // gqa_window: the chunk kernel, which needs no workspace
+  bool prefill;  // gqa_window: the chunk kernel; unsplit, it needs no workspace
   int cgroups;   // its column groups
   bool balanced; // splits are dealt to the rows by their lengths
   int G, gshift, tpt, tiles, splits, min_tiles, one_split, score_stride;
@@ -62,29 +64,63 @@ int make_plan(int kind, int B, int NH, int NKV, int D, int cap, int T, int windo
     const int rc = bz::device_cu_count(&cus);
     if (rc != BZ_OK) return rc;
   }
-  // A chunk whose 16-column tiles would be more workgroups than CUs takes the kernel of window_prefill.cuh: the split kernel
-  // reads K and V again for each tile of 16 columns, but spreads a few of them over the whole device (us, split / chunk
-  // kernel, head_dim 128: 8 kv heads, 4096 positions, 64 columns 14.0 / 40.3, 256 27.5 / 40.6, 512 43.9 / 40.7; 4 rows x 8,
-  // window 1024: 128 columns 13.1 / 16.7, 256 23.8 / 17.7; 2 x 4 heads, head_dim 64, 4096 positions: 256 17.0 / 22.6, 512
-  // 28.0 / 22.7).
-  pl->prefill = kind == BZ_LONG_WINDOW && pl->tiles > 1 && pl->units >= cus;
-  if (pl->prefill) {
+  // positions a row holds, and those a column tile attends
+  const int64_t longest = max_seq_len > 0 && max_seq_len < cap ? max_seq_len : cap;
+  auto attended = [&](int64_t tokens) { return window > 0 ? std::min(longest, (int64_t)window + tokens + sinks) : longest; };
+
+  pl->prefill = pl->balanced = false;
+  if (kind == BZ_LONG_WINDOW && pl->tiles > 1) {
     auto tiles = [&](int cg) { return ((int64_t)T * pl->G + kPreWaveCols * cg - 1) / (kPreWaveCols * cg); };
-    // The widest column tiles that still give every CU work, three workgroups each for the widest (us for 1 / 2 / 4 groups,
-    // head_dim 128: 2 x 8 kv heads x 2048 tokens 122.8 / 53.1 / 57.5; 8 x 8192, window 4096: 509 / 243 / 223; 8 x 1024: 23.1 /
-    // 18.0 / 23.6; 8 x 512 behind 3584: 40.5 / 49.2 / 71.4).
-    pl->cgroups = tiles(4) * B * NKV >= 3 * cus ? 4 : tiles(2) * B * NKV >= cus ? 2 : 1;
-    pl->tiles = (int)tiles(pl->cgroups);
-    pl->splits = 1;
-    pl->ml = pl->acc = pl->head_ml = pl->scores = pl->total = 0;
-    return pl->tiles <= 65535 && B <= 65535 ? BZ_OK : BZ_ERR_SHAPE;
+    const int64_t rows = (int64_t)B * NKV, wide = tiles(4) * rows, steps = attended(4 * kPreWaveCols / pl->G) / 64 + 1;
+    // splits of a 128-column tile's positions that give `workgroups`, each of at least `least` steps of 64
+    auto shares = [&](int64_t workgroups, int64_t least) { return std::max<int64_t>(std::min(workgroups / wide, steps / least), 1); };
+    int64_t splits = std::max(num_splits, 1);
+    if (pl->units < cus) {
+      // Few columns: the split kernel, which reads K and V again for each tile of 16 but spreads a few of them over the whole
+      // device, unless the splits of whole 128-column tiles half fill it (us, split kernel / chunk kernel split, 8 kv heads,
+      // head_dim 128: 256 columns, 8192 positions 45.3 / 26.5, 2048 positions 16.4 / 20.4; 128, 8192 27.1 / 24.3; 4 q heads, 64
+      // tokens, 16384 82.6 / 36.0; 2 kv heads, 512 columns, 4096 16.3 / 20.4).
+      const int64_t s = shares(cus, kPreMinSteps);
+      pl->prefill = num_splits == 0 && (int64_t)T * pl->G >= 4 * kPreWaveCols && wide * s >= cus / 2;
+      if (pl->prefill) splits = s;
+    } else {
+      // Otherwise the chunk kernel (us, split / chunk kernel, head_dim 128: 8 kv heads, 4096 positions, 512 columns 43.9 / 40.4;
+      // 4 rows x 8, window 1024: 256 columns 23.8 / 17.1), by the widest column tiles that still give every CU work, three
+      // workgroups each for the widest (us for 1 / 2 / 4 groups, head_dim 128: 2 x 8 kv heads x 2048 tokens 122.8 / 53.1 / 57.5; 8
+      // x 8192, window 4096: 509 / 243 / 223; 8 x 1024: 23.1 / 18.0 / 23.6). A chunk behind a long context is split over its
+      // positions as well: to two rounds where a split still has 32 steps (8 kv heads, head_dim 128, whole / split: 512
+      // tokens over 16384 132 / 80, 1024 over 8192 98 / 81, 2048 over 16384 283 / 253), else to one where the column tiles fill
+      // none (512 over 4096 40.6 / 34.2, 256 over 8192 70 / 33, 1024 over 1024 17.9 / 27.2). At head_dim 64, where one column group
+      // leaves room for two workgroups a CU, that is only worth it for long splits if those fill it (256 over 8192 43 / 25, 512
+      // over 4096 23 / 27, over 16384 78 / 61).
+      pl->prefill = true;
+      const bool few = D == 128 || tiles(1) * rows < cus;
+      if (num_splits == 0) {
+        if (wide <= cus && shares(2 * cus, 32) == 2 * cus / wide) splits = 2 * cus / wide;
+        else if (tiles(2) * rows < cus) splits = shares(cus, few ? 14 : 64);
+      }
+    }
+    if (pl->prefill) {
+      const size_t counters = (size_t)pl->units * kCounterStride * sizeof(int);
+      pl->cgroups = splits > 1 || wide >= 3 * cus ? 4 : tiles(2) * rows >= cus ? 2 : 1;
+      if (tiles(pl->cgroups) * splits > 65535 || B > 65535 || NKV > 65535) return BZ_ERR_SHAPE;  // grid limits
+      pl->tiles = (int)tiles(pl->cgroups);
+      pl->splits = (int)splits;
+      pl->ml = pl->acc = pl->head_ml = pl->scores = pl->total = 0;
+      if (splits > 1) {
+        const size_t cols = (size_t)(rows * pl->tiles * splits) * 4 * kPreWaveCols;
+        pl->ml = counters;  // other calls' with this workspace
+        pl->acc = up256(pl->ml + cols * sizeof(float2));
+        pl->total = pl->acc + cols * D * sizeof(float);
+      }
+      return BZ_OK;
+    }
   }
   if ((int64_t)B * pl->tiles > 65535 || NKV > 65535) return BZ_ERR_SHAPE;  // grid limits
 
-  // positions a column tile attends, in wave tiles
-  int64_t len = max_seq_len > 0 && max_seq_len < cap ? max_seq_len : cap;
-  const bool cut = window > 0 && (int64_t)window + pl->tpt + sinks < len;  // the rows reach past the window
-  if (cut) len = (int64_t)window + pl->tpt + sinks;
+  // in wave tiles
+  const int64_t len = attended(pl->tpt);
+  const bool cut = len < longest;  // the rows reach past the window
   const int P = kv4 ? 32 : 16;
   const int n = (int)((len + P - 1) / P) + 1;
   pl->min_tiles = kLongThreads / kWave;
@@ -124,8 +160,7 @@ int make_plan(int kind, int B, int NH, int NKV, int D, int cap, int T, int windo
   pl->scores = 0;
   pl->score_stride = 0;
   if (kind == BZ_LONG_TRACKED) {
-    const int64_t longest = cap;  // rows may be longer than max_seq_len, which only steers the tiling
-    pl->score_stride = (int)((longest + 31) & ~(int64_t)31);
+    pl->score_stride = (int)(((int64_t)cap + 31) & ~(int64_t)31);  // rows may be longer than max_seq_len, which steers the tiling
     pl->scores = up256(pl->head_ml + (size_t)B * NH * sizeof(float2));
     pl->total = up256(pl->scores + (size_t)B * NH * pl->score_stride * sizeof(float));
   }
@@ -192,7 +227,7 @@ LongParams long_params(const bz_gqa_decode_args* a, const Plan& pl, int window, 
   p.NKV = a->num_kv_heads, p.G = pl.G, p.gshift = pl.gshift, p.T = a->tokens_per_row > 1 ? a->tokens_per_row : 1;
   p.cap = a->capacity;
   p.tiles = pl.tiles, p.tpt = pl.tpt;
-  p.rows = a->batch * pl.tiles;
+  p.rows = pl.balanced ? a->batch * pl.tiles : 0;
   p.inv_splits = 1.0f / (float)(pl.balanced ? pl.splits * p.rows : pl.splits);
   p.splits = pl.splits, p.min_tiles = pl.min_tiles, p.one_split = pl.one_split;
   char* const ws = static_cast<char*>(a->workspace);
@@ -207,7 +242,7 @@ LongParams long_params(const bz_gqa_decode_args* a, const Plan& pl, int window, 
 
 template <int FMT, bool TRACK>
 int launch_split(const bz_gqa_decode_args* a, int D, const LongParams& p, const Plan& pl, hipStream_t stream) {
-  const dim3 grid = pl.balanced ? dim3(pl.splits * p.rows, p.NKV) : dim3(pl.splits, p.NKV, p.rows);
+  const dim3 grid = pl.balanced ? dim3(pl.splits * p.rows, p.NKV) : dim3(pl.splits, p.NKV, a->batch * pl.tiles);
   using Fn = void (*)(const int32_t*, const int32_t*, const LongParams);
   const Fn fns[2][2] = {
       {long_split_kernel<64, FMT, TRACK, false, kLongThreads>, long_split_kernel<64, FMT, TRACK, true, kLongThreads>},
@@ -250,11 +285,19 @@ BZ_EXPORT int bz_gqa_window(const bz_gqa_window_args* wa, hipStream_t stream) {
   if (rc != BZ_OK) return rc;
   const LongParams p = long_params(a, pl, wa->window, wa->sinks);
   if (!pl.prefill) return launch_split<kBf16, false>(a, a->head_dim, p, pl, stream);
-  const dim3 grid(a->num_kv_heads, pl.tiles, a->batch);
+  const dim3 grid(a->num_kv_heads, pl.tiles * pl.splits, a->batch);
   using Fn = void (*)(const int32_t*, const int32_t*, const LongParams);
-  const Fn fns[2][3] = {{window_prefill_kernel<64, 1>, window_prefill_kernel<64, 2>, window_prefill_kernel<64, 4>},
-                        {window_prefill_kernel<128, 1>, window_prefill_kernel<128, 2>, window_prefill_kernel<128, 4>}};
-  hipLaunchKernelGGL(fns[a->head_dim == 128][pl.cgroups / 2], grid, dim3(kPreThreads), 0, stream, a->seq_lens, a->kv_start, p);
+  const Fn fns[2][4] = {{window_prefill_kernel<64, 1, false>, window_prefill_kernel<64, 2, false>,
+                         window_prefill_kernel<64, 4, false>, window_prefill_kernel<64, 4, true>},
+                        {window_prefill_kernel<128, 1, false>, window_prefill_kernel<128, 2, false>,
+                         window_prefill_kernel<128, 4, false>, window_prefill_kernel<128, 4, true>}};
+  const int wide = a->head_dim == 128;
+  hipLaunchKernelGGL(fns[wide][pl.splits > 1 ? 3 : pl.cgroups / 2], grid, dim3(kPreThreads), 0, stream, a->seq_lens, a->kv_start, p);
+  if (hipGetLastError() != hipSuccess) return BZ_ERR_LAUNCH;
+  if (pl.splits == 1) return BZ_OK;
+  const dim3 columns((unsigned)(((int64_t)p.T * p.G + 3) / 4), a->num_kv_heads, a->batch);
+  const Fn merge = wide ? window_merge_kernel<128> : window_merge_kernel<64>;
+  hipLaunchKernelGGL(merge, columns, dim3(kPreThreads), 0, stream, a->seq_lens, a->kv_start, p);
   return hipGetLastError() == hipSuccess ? BZ_OK : BZ_ERR_LAUNCH;
 }
 

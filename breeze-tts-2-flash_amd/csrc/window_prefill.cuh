@@ -32,6 +32,7 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef short s16x4_lds __attribute__((ext_vector_type(4)));
 
 constexpr int kPreThreads = 256, kPreWaveCols = 32;
+constexpr int kPreMinSteps = 8;  // of a split: below, its sums' way through memory costs more than the steps
 
 // LDS of one tile of K or V: TP rows of D bf16, in 16-byte chunks. Chunk c of row r lies in slot c ^ swizzle(r), so that the
 // lanes of one read, which take the same chunk of different rows, fall into different banks.
@@ -60,65 +61,84 @@ __device__ __forceinline__ void stage_tile(char* base, const Rsrc& rsrc, int pos
   }
 }
 
-// One column at a time, in fp32 and without any product of a position that the column does not attend: for a wave whose
-// result is not finite, which is right where the column attends an infinity or NaN and wrong where a tile held one that it
-// does not (0 times it). The lanes score 64 positions, then each accumulates D / 64 dims over them.
+// One column, by one wave, in fp32 and without any product of a position that the column does not attend: where a result is
+// not finite, which is right where the column attends an infinity or NaN and wrong where a tile held one that it does not (0
+// times it). The lanes score 64 positions, then each accumulates D / 64 dims over them.
 template <int D>
-__device__ __forceinline__ void prefill_careful(const LongParams& p, int b, int h, int s, int e, int t0, int ntok, int cg) {
+__device__ __forceinline__ void careful_column(const LongParams& p, int b, int h, int s, int e, int tok, int hq) {
   constexpr int DV = D / 64;
   const int lane = threadIdx.x % kWave;
   const char* const kb = p.k + (int64_t)b * p.kv_sb + (int64_t)h * p.kv_sh;
   const char* const vb = p.v + (int64_t)b * p.kv_sb + (int64_t)h * p.kv_sh;
-  for (int c = 0; c < kPreWaveCols; ++c) {
-    const int m0 = kPreWaveCols * cg + c, tok = t0 + (m0 >> p.gshift), hq = (h << p.gshift) + (m0 & (p.G - 1));
-    if (tok >= t0 + ntok) break;
-    const int end = max(s, e - (p.T - 1 - tok));
-    const Reach r = reach_of(s, end, p.window, p.sinks);
-    const uint16_t* const q = p.q + (int64_t)b * p.q_sb + (int64_t)tok * p.q_st + (int64_t)hq * p.q_sh;
-    float m = -INFINITY, l = 0.f, acc[DV];
+  const int end = max(s, e - (p.T - 1 - tok));
+  const Reach r = reach_of(s, end, p.window, p.sinks);
+  const uint16_t* const q = p.q + (int64_t)b * p.q_sb + (int64_t)tok * p.q_st + (int64_t)hq * p.q_sh;
+  float m = -INFINITY, l = 0.f, acc[DV];
 #pragma unroll
-    for (int i = 0; i < DV; ++i) acc[i] = 0.f;
-    for (int p0 = s; p0 < end; p0 += kWave) {
-      if (p0 >= s + r.sink && p0 + kWave <= r.lo) {  // between the sinks and the window
-        p0 += (r.lo - p0) / kWave * kWave - kWave;
-        continue;
-      }
-      const int pos = p0 + lane;
-      float x = -INFINITY;
-      if (pos < end && attends(r, s, pos)) {
-        const uint16_t* const kr = reinterpret_cast<const uint16_t*>(kb + (int64_t)pos * p.kv_ss);
-        float d = 0.f;
-        for (int i = 0; i < D; ++i) d = fmaf(bf16_to_f32(q[i]), bf16_to_f32(kr[i]), d);
-        x = d * p.scale_log2;
-      }
-      const float mn = fmaxf(m, wave_max(x)), mu = mn == -INFINITY ? 0.f : mn, alpha = fast_exp2(m - mu);
-      m = mn;
-      const float t = fast_exp2(x - mu);
-      l = l * alpha + wave_sum(t);
-#pragma unroll
-      for (int i = 0; i < DV; ++i) acc[i] *= alpha;
-      for (int j = 0; j < min(kWave, end - p0); ++j) {
-        if (!attends(r, s, p0 + j)) continue;
-        const float tj = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(t), j));
-        const uint16_t* const vr = reinterpret_cast<const uint16_t*>(vb + (int64_t)(p0 + j) * p.kv_ss);
-#pragma unroll
-        for (int i = 0; i < DV; ++i) acc[i] = fmaf(tj, bf16_to_f32(vr[DV * lane + i]), acc[i]);
-      }
+  for (int i = 0; i < DV; ++i) acc[i] = 0.f;
+  for (int p0 = s; p0 < end; p0 += kWave) {
+    if (p0 >= s + r.sink && p0 + kWave <= r.lo) {  // between the sinks and the window
+      p0 += (r.lo - p0) / kWave * kWave - kWave;
+      continue;
     }
-    uint16_t* const o = p.out + (int64_t)b * p.o_sb + (int64_t)tok * p.o_st + (int64_t)hq * p.o_sh;
+    const int pos = p0 + lane;
+    float x = -INFINITY;
+    if (pos < end && attends(r, s, pos)) {
+      const uint16_t* const kr = reinterpret_cast<const uint16_t*>(kb + (int64_t)pos * p.kv_ss);
+      float d = 0.f;
+      for (int i = 0; i < D; ++i) d = fmaf(bf16_to_f32(q[i]), bf16_to_f32(kr[i]), d);
+      x = d * p.scale_log2;
+    }
+    const float mn = fmaxf(m, wave_max(x)), mu = mn == -INFINITY ? 0.f : mn, alpha = fast_exp2(m - mu);
+    m = mn;
+    const float t = fast_exp2(x - mu);
+    l = l * alpha + wave_sum(t);
 #pragma unroll
-    for (int i = 0; i < DV; ++i) o[DV * lane + i] = f32_to_bf16(l == 0.f ? 0.f : acc[i] / l);
+    for (int i = 0; i < DV; ++i) acc[i] *= alpha;
+    for (int j = 0; j < min(kWave, end - p0); ++j) {
+      if (!attends(r, s, p0 + j)) continue;
+      const float tj = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(t), j));
+      const uint16_t* const vr = reinterpret_cast<const uint16_t*>(vb + (int64_t)(p0 + j) * p.kv_ss);
+#pragma unroll
+      for (int i = 0; i < DV; ++i) acc[i] = fmaf(tj, bf16_to_f32(vr[DV * lane + i]), acc[i]);
+    }
   }
+  uint16_t* const o = p.out + (int64_t)b * p.o_sb + (int64_t)tok * p.o_st + (int64_t)hq * p.o_sh;
+#pragma unroll
+  for (int i = 0; i < DV; ++i) o[DV * lane + i] = f32_to_bf16(l == 0.f ? 0.f : acc[i] / l);
+}
+
+// The columns of a wave.
+template <int D>
+__device__ __forceinline__ void prefill_careful(const LongParams& p, int b, int h, int s, int e, int t0, int ntok, int cg) {
+  for (int c = 0; c < kPreWaveCols; ++c) {
+    const int m0 = kPreWaveCols * cg + c, tok = t0 + (m0 >> p.gshift);
+    if (tok >= t0 + ntok) break;
+    careful_column<D>(p, b, h, s, e, tok, (h << p.gshift) + (m0 & (p.G - 1)));
+  }
+}
+
+// The positions a column tile attends, in steps, and how they are cut: splits of `per` steps, nact of them.
+struct PreCut {
+  int n, per, nact;
+};
+template <int TP, int PG>
+__device__ __forceinline__ PreCut cut_steps(const TileRange& tr, int splits) {
+  const int n = (tr.na + tr.nb + PG - 1) / PG, per = splits == 1 ? max(n, 1) : max((n + splits - 1) / splits, kPreMinSteps);
+  return {n, per, max((n + per - 1) / per, 1)};
 }
 
 // grid (kv heads, column tiles, rows): workgroups go to the XCDs in turn, so with a multiple of 8 kv heads each head's K and V
 // pass through one XCD's L2 alone. The last tiles, which attend most, start first.
-template <int D, int CG>
+// SPLIT: grid (kv heads, column tiles * splits, rows), each workgroup a share of the positions; its sums go to the workspace,
+// and window_merge_kernel adds them up.
+template <int D, int CG, bool SPLIT>
 __global__ void __launch_bounds__(kPreThreads, 2)
     window_prefill_kernel(const int32_t* lens, const int32_t* starts, const LongParams p) {
   constexpr int PG = 4 / CG, TP = PG == 1 ? 64 : 32, NB = TP / 32, NQ = D / 16, ND = D / 32, kCols = CG * kPreWaveCols;
   using L = PreLds<D, TP>;
-  const int h = blockIdx.x, tile = gridDim.y - 1 - blockIdx.y, b = blockIdx.z;
+  const int y = gridDim.y - 1 - blockIdx.y, tile = SPLIT ? y / p.splits : y, split = SPLIT ? y - tile * p.splits : 0;
+  const int h = blockIdx.x, b = blockIdx.z;
   const int e_raw = lens[b], s_raw = (starts ? starts : lens)[b];
   const int lane = threadIdx.x % kWave, w = wave_uniform((int)threadIdx.x / kWave), c = lane % 32, half = lane / 32;
   const int cg = w % CG, pg = w / CG;
@@ -140,9 +160,12 @@ __global__ void __launch_bounds__(kPreThreads, 2)
   const Reach me = reach_of(s, token_end(tok), p.window, p.sinks);
   const int e1 = token_end(t0 + ntok - 1);
   const TileRange tr = tile_range<TP>(s, token_end(t0), e1, p.window, p.sinks);
-  const int n = (tr.na + tr.nb + PG - 1) / PG;  // steps; position group pg takes tile PG j + pg in step j
+  const PreCut cut = cut_steps<TP, PG>(tr, SPLIT ? p.splits : 1);
+  const int j0 = SPLIT ? split * cut.per : 0;
+  if (SPLIT && split > 0 && j0 >= cut.n) return;
+  const int n = SPLIT ? min(cut.per, cut.n - j0) : cut.n;  // steps; position group pg takes tile PG (j0 + j) + pg in step j
   auto pos_of = [&](int j) {  // (a tile past the last begins at or past e1: nothing there is attended)
-    const int i = PG * j + pg;
+    const int i = PG * (j0 + j) + pg;
     return i < tr.na ? tr.fa + TP * i : tr.fb + TP * (i - tr.na);
   };
   // every column of the wave attends the whole of [whole_lo, whole_end)
@@ -311,6 +334,17 @@ __global__ void __launch_bounds__(kPreThreads, 2)
     }
     if (pg > 0) return;
   }
+  if (SPLIT && cut.nact > 1) {
+    const int64_t part = ((((int64_t)b * p.tiles + tile) * p.NKV + h) * p.splits + split) * kCols + mine;
+    if (half == 0) p.part_ml[part] = make_float2(m, l);
+    float* const at = p.part_acc + part * D + 4 * half;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4)
+        *reinterpret_cast<f32x4_t*>(at + 32 * d + 2 * i) = f32x4_t{acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]};
+    return;
+  }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   float worst = 0.f;
 #pragma unroll
@@ -335,6 +369,63 @@ __global__ void __launch_bounds__(kPreThreads, 2)
         at[0] = (uint16_t)y.x, at[1] = (uint16_t)(y.x >> 16), at[2] = (uint16_t)y.y, at[3] = (uint16_t)(y.y >> 16);
       }
     }
+}
+
+// Adds up the splits of window_prefill_kernel<D, 4, true> and writes the outputs: a wave a column, grid (columns / 4, kv heads,
+// rows).
+template <int D>
+__global__ void __launch_bounds__(kPreThreads) window_merge_kernel(const int32_t* lens, const int32_t* starts, const LongParams p) {
+  constexpr int DV = D / 64, kCols = 4 * kPreWaveCols, TP = 64;
+  const int h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x % kWave;
+  const int col = wave_uniform((int)(blockIdx.x * (kPreThreads / kWave) + threadIdx.x / kWave));
+  const int tok = col >> p.gshift, hq = (h << p.gshift) + (col & (p.G - 1));
+  if (tok >= p.T) return;
+  int s, e;
+  long_range(lens[b], (starts ? starts : lens)[b], starts != nullptr, p.cap, s, e);
+  auto token_end = [&](int t) { return max(s, e - (p.T - 1 - t)); };
+  const int tile = col / kCols, t0 = tile * (kCols >> p.gshift), last = min(t0 + (kCols >> p.gshift), p.T) - 1;
+  const PreCut cut = cut_steps<TP, 1>(tile_range<TP>(s, token_end(t0), token_end(last), p.window, p.sinks), p.splits);
+  if (cut.nact == 1) return;  // its one split has written them
+  const int64_t part = (((int64_t)b * p.tiles + tile) * p.NKV + h) * p.splits * kCols + col % kCols;
+  float m = -INFINITY, l = 0.f, acc[DV] = {};
+  for (int k0 = 0; k0 < cut.nact; k0 += 8) {
+    float2 ml[8];
+    float x[8][DV];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {  // past the last: the last again, with no weight
+      const int64_t at = part + (int64_t)min(k0 + k, cut.nact - 1) * kCols;
+      ml[k] = p.part_ml[at];
+#pragma unroll
+      for (int i = 0; i < DV; ++i) x[k][i] = p.part_acc[at * D + DV * lane + i];
+    }
+    float mn = m;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) mn = fmaxf(mn, ml[k].x);
+    const float mu = mn == -INFINITY ? 0.f : mn, alpha = fast_exp2(m - mu);
+    m = mn;
+    l *= alpha;
+#pragma unroll
+    for (int i = 0; i < DV; ++i) acc[i] *= alpha;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (k0 + k >= cut.nact) break;
+      const float f = fast_exp2(ml[k].x - mu);
+      l = fmaf(f, ml[k].y, l);
+#pragma unroll
+      for (int i = 0; i < DV; ++i) acc[i] = fmaf(f, x[k][i], acc[i]);
+    }
+  }
+  float worst = fabsf(l) * 0x1p-8f;
+#pragma unroll
+  for (int i = 0; i < DV; ++i) worst += fabsf(acc[i]) * 0x1p-8f;
+  if (__builtin_expect(__ballot(!(worst < INFINITY)) != 0, 0)) {
+    careful_column<D>(p, b, h, s, e, tok, hq);
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint16_t* const o = p.out + (int64_t)b * p.o_sb + (int64_t)tok * p.o_st + (int64_t)hq * p.o_sh + DV * lane;
+#pragma unroll
+  for (int i = 0; i < DV; ++i) o[i] = f32_to_bf16(acc[i] * inv);
 }
 
 }  // namespace

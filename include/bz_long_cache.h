@@ -21,8 +21,7 @@ extern "C" {
 #endif
 
 /* Arguments of bz_gqa_window. base: as for bz_gqa_decode, with mask NULL and mask_dtype 0; tokens_per_row T may be one or
-   a whole prompt (at most 2^30); num_splits 0 picks the default (only calls that go by splits look at it: those of few
-   tokens); combine is ignored; workspace of at least bz_long_workspace_size(..) bytes where that is not 0. Softmax terms
+   a whole prompt (at most 2^30); num_splits 0 picks the default; combine is ignored; workspace of at least bz_long_workspace_size(..) bytes where that is not 0. Softmax terms
    enter the product with V as two bf16 terms (an error of 2^-17 each), over many tokens as one (2^-9). */
 typedef struct bz_gqa_window_args {
   bz_gqa_decode_args base;

@@ -128,11 +128,48 @@ def test_window_layouts(device, T):
     assert (full[..., D:] == 7).all()
 
 
-# the split kernel, and the chunk kernel by one, two and four column groups
+@pytest.mark.parametrize("splits", [2, 3, 7, 40])
+@pytest.mark.parametrize("NKV,G,D,cap,T,lens,starts,window,sinks", [
+    (8, 4, 128, 1300, 160, [1300, 700], [30, 0], 0, 0), (8, 8, 64, 900, 150, [900, 149, 3], [0, 5, 0], 300, 70),
+    (8, 2, 128, 2000, 333, [2000, 333, 0], None, 700, 4), (16, 1, 64, 1500, 260, [1500], [99], 0, 3),
+])
+def test_chunk_splits(device, NKV, G, D, cap, T, lens, starts, window, sinks, splits):
+    """A chunk whose positions are shared out to workgroups; rows that are shorter than the chunk, or empty."""
+    rng = np.random.default_rng(T + splits)
+    B = len(lens)
+    q, k, v = randn(rng, B, NKV * G, T, D), randn(rng, B, NKV, cap, D), randn(rng, B, NKV, cap, D)
+    k[:, :, :: 17] *= 4
+    kp, vp = poison(k, v, lens, starts, T, window, sinks)
+    out = pkg.gqa_window(q.to(device), kp.to(device), vp.to(device), ints(lens, device), D ** -0.5, window, sinks=sinks,
+                         kv_start=None if starts is None else ints(starts, device), num_splits=splits)
+    ref = check_attention(out, q.float(), k.float(), v.float(), lens, D ** -0.5, window, sinks, starts)
+    assert (out.float().cpu().numpy().reshape(ref.shape)[ref == 0] == 0).all()  # rows that attend nothing
+
+
+@pytest.mark.parametrize("T,G,D,n,window", [(128, 2, 128, 5000, 0), (200, 2, 64, 4500, 0), (70, 4, 128, 4200, 4000)])
+def test_chunk_behind_a_long_context(device, T, G, D, n, window):
+    """Few tokens over many positions, whose splits the library chooses; the same with a workspace of the caller's."""
+    rng = np.random.default_rng(T)
+    NKV = 8
+    q, k, v = randn(rng, 1, NKV * G, T, D), randn(rng, 1, NKV, n + 9, D), randn(rng, 1, NKV, n + 9, D)
+    k[:, :, n:], v[:, :, n:] = float("nan"), float("nan")
+    args = (q.to(device), k.to(device), v.to(device), ints([n], device), D ** -0.5, window)
+    out = pkg.gqa_window(*args, sinks=2)
+    check_attention(out, q.float(), k[:, :, :n].float(), v[:, :, :n].float(), [n], D ** -0.5, window, 2)
+    ws = pkg.long_workspace("window", torch.device("cuda", 0), 1, NKV * G, NKV, D, n + 9, T, window=window, sinks=2)
+    assert ws.numel() > 0
+    for _ in range(2):
+        assert torch.equal(pkg.gqa_window(*args, sinks=2, workspace=ws), out)
+    with pytest.raises(RuntimeError):
+        pkg.gqa_window(*args, sinks=2, workspace=ws[:-256])
+
+
+# the split kernel, and the chunk kernel by one, two and four column groups, and split
 @pytest.mark.parametrize("T,NKV,G,D", [(3, 1, 2, 128), (70, 1, 2, 128), (70, 8, 8, 128), (70, 8, 8, 64), (130, 32, 8, 128),
                                        (800, 64, 2, 128), (800, 64, 2, 64)])
 @pytest.mark.parametrize("value", [float("inf"), float("nan")])
-def test_unattended_values_do_not_reach_a_token(device, T, NKV, G, D, value):
+@pytest.mark.parametrize("splits", [0, 3])
+def test_unattended_values_do_not_reach_a_token(device, T, NKV, G, D, value, splits):
     """A position that some tokens of a chunk attend and others do not: only those that do may see what it holds."""
     rng = np.random.default_rng(T)
     n, window, sinks = T + 130, 30, 2
@@ -140,10 +177,10 @@ def test_unattended_values_do_not_reach_a_token(device, T, NKV, G, D, value):
     at = [n - 1, n - T + 1, n - T - window + 2]
     vp = v.clone()
     vp[0, 0, at, 5] = value
-    out = pkg.gqa_window(q.to(device), k.to(device), vp.to(device), ints([n], device), D ** -0.5, window, sinks=sinks)
+    out = pkg.gqa_window(q.to(device), k.to(device), vp.to(device), ints([n], device), D ** -0.5, window, sinks=sinks, num_splits=splits)
     assert torch.isfinite(out[0, :, G:].float()).all()  # the other kv heads
     out = out.float().cpu()[0, :, :G]
-    clean = pkg.gqa_window(q.to(device), k.to(device), v.to(device), ints([n], device), D ** -0.5, window, sinks=sinks)
+    clean = pkg.gqa_window(q.to(device), k.to(device), v.to(device), ints([n], device), D ** -0.5, window, sinks=sinks, num_splits=splits)
     clean = clean.float().cpu()[0, :, :G]
     from oracle.long_cache import attended
     for t, pos in enumerate(attended(0, n, T, window, sinks)):
@@ -160,7 +197,7 @@ def test_unattended_values_do_not_reach_a_token(device, T, NKV, G, D, value):
     # keys: a NaN key poisons exactly the tokens that attend it
     kp = k.clone()
     kp[0, 0, n - 1] = float("nan")
-    out = pkg.gqa_window(q.to(device), kp.to(device), v.to(device), ints([n], device), D ** -0.5, window, sinks=sinks)
+    out = pkg.gqa_window(q.to(device), kp.to(device), v.to(device), ints([n], device), D ** -0.5, window, sinks=sinks, num_splits=splits)
     assert torch.isnan(out[0, T - 1, :G].float()).all() and torch.isfinite(out[0, :T - 1].float()).all()
 
 
