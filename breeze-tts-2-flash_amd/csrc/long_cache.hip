@@ -74,7 +74,8 @@ int make_plan(int kind, int B, int NH, int NKV, int D, int cap, int T, int windo
     const int64_t rows = (int64_t)B * NKV, wide = tiles(4) * rows, steps = attended(4 * kPreWaveCols / pl->G) / 64 + 1;
     // splits of a 128-column tile's positions that give `workgroups`, each of at least `least` steps of 64
     auto shares = [&](int64_t workgroups, int64_t least) { return std::max<int64_t>(std::min(workgroups / wide, steps / least), 1); };
-    int64_t splits = std::max(num_splits, 1);
+    // a caller's: as many as find kPreMinSteps steps each (the kernel gives none fewer)
+    int64_t splits = std::max<int64_t>(std::min<int64_t>(num_splits, (steps + kPreMinSteps - 1) / kPreMinSteps), 1);
     if (pl->units < cus) {
       // Few columns: the split kernel, which reads K and V again for each tile of 16 but spreads a few of them over the whole
       // device, unless the splits of whole 128-column tiles half fill it (us, split kernel / chunk kernel split, 8 kv heads,
