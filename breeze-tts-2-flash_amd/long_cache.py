@@ -70,13 +70,16 @@ def _make_workspace(need) -> None:
         kernels.eager().register_long_workspace(*key, ws)
 
 
-def _attend(entry, *args):
-    """entry(*args) of the native binding, with the workspace it may ask for."""
+def _again(need, entry, *args):
+    """entry(*args) of the native binding once more, with the workspace it asked for (need, the tuple it returned)."""
+    _make_workspace(need)
+    return entry(*args)
+
+
+def _call(entry, *args):
+    """entry(*args) of the native binding, with the workspace it may ask for (for the torch operators)."""
     r = entry(*args)
-    if type(r) is tuple:
-        _make_workspace(r)
-        r = entry(*args)
-    return r
+    return r if type(r) is not tuple else _again(r, entry, *args)
 
 
 def long_workspace(kind: str, device: torch.device, batch: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
@@ -109,12 +112,11 @@ def gqa_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, se
         torch.ops.bz.gqa_window(q, k_cache, v_cache, seq_lens, float(scale), int(window), out, int(sinks), kv_start,
                                 int(num_splits), int(max_seq_len), workspace)
         return out
-    return _gqa_window(q, k_cache, v_cache, seq_lens, scale, window, out, sinks, kv_start, num_splits, max_seq_len, workspace)
-
-
-def _gqa_window(q, k_cache, v_cache, seq_lens, scale, window, out, sinks, kv_start, num_splits, max_seq_len, workspace):
-    return _attend(kernels.eager().window, q, k_cache, v_cache, seq_lens, scale, window, out, sinks, kv_start, num_splits,
-                   max_seq_len, workspace)
+    # (the binding called here, not through another function: 0.3 us of a 4.8 us call)
+    entry = kernels.eager().window
+    r = entry(q, k_cache, v_cache, seq_lens, scale, window, out, sinks, kv_start, num_splits, max_seq_len, workspace)
+    return r if type(r) is not tuple else _again(r, entry, q, k_cache, v_cache, seq_lens, scale, window, out, sinks, kv_start,
+                                                 num_splits, max_seq_len, workspace)
 
 
 # --------------------------------------------------------------------------------------------- 4-bit cache
@@ -127,10 +129,6 @@ def kv4_store(k: torch.Tensor, v: torch.Tensor, cache: Kv4Cache, slots: torch.Te
     if torch.compiler.is_compiling():
         torch.ops.bz.kv4_store(k, v, *cache, slots, counts)
         return cache
-    return _kv4_store(k, v, cache, slots, counts)
-
-
-def _kv4_store(k, v, cache, slots, counts):
     kernels.eager().kv4_store(k, v, *cache, slots, counts)
     return cache
 
@@ -160,12 +158,11 @@ def gqa_decode_kv4(q: torch.Tensor, cache: Kv4Cache, seq_lens: torch.Tensor, sca
         torch.ops.bz.gqa_decode_kv4(q, *cache, seq_lens, float(scale), out, kv_start, int(window), int(sinks), int(num_splits),
                                     int(max_seq_len), workspace)
         return out
-    return _gqa_decode_kv4(q, cache, seq_lens, scale, out, kv_start, window, sinks, num_splits, max_seq_len, workspace)
-
-
-def _gqa_decode_kv4(q, cache, seq_lens, scale, out, kv_start, window, sinks, num_splits, max_seq_len, workspace):
-    return _attend(kernels.eager().kv4, q, *cache, seq_lens, scale, out, kv_start, window, sinks, num_splits, max_seq_len,
-                   workspace)
+    entry = kernels.eager().kv4
+    ck, cv, ks, vs = cache
+    r = entry(q, ck, cv, ks, vs, seq_lens, scale, out, kv_start, window, sinks, num_splits, max_seq_len, workspace)
+    return r if type(r) is not tuple else _again(r, entry, q, ck, cv, ks, vs, seq_lens, scale, out, kv_start, window, sinks,
+                                                 num_splits, max_seq_len, workspace)
 
 
 # ------------------------------------------------------------------------------------------------ eviction
@@ -184,14 +181,10 @@ def gqa_decode_tracked(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
         torch.ops.bz.gqa_decode_tracked(q, k_cache, v_cache, seq_lens, float(scale), weights, out, float(decay),
                                         weights_out, kv_start, int(num_splits), int(max_seq_len), workspace)
         return out
-    return _gqa_decode_tracked(q, k_cache, v_cache, seq_lens, scale, weights, out, decay, weights_out, kv_start, num_splits,
-                               max_seq_len, workspace)
-
-
-def _gqa_decode_tracked(q, k_cache, v_cache, seq_lens, scale, weights, out, decay, weights_out, kv_start, num_splits,
-                        max_seq_len, workspace):
-    return _attend(kernels.eager().tracked, q, k_cache, v_cache, seq_lens, scale, weights, out, decay, weights_out, kv_start,
-                   num_splits, max_seq_len, workspace)
+    entry = kernels.eager().tracked
+    r = entry(q, k_cache, v_cache, seq_lens, scale, weights, out, decay, weights_out, kv_start, num_splits, max_seq_len, workspace)
+    return r if type(r) is not tuple else _again(r, entry, q, k_cache, v_cache, seq_lens, scale, weights, out, decay, weights_out,
+                                                 kv_start, num_splits, max_seq_len, workspace)
 
 
 def kv_select(weights: torch.Tensor, seq_lens: torch.Tensor, keep: int, *, sinks: int = 0, recent: int = 0,

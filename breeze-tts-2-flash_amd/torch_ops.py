@@ -105,12 +105,12 @@ def _rmsnorm(x, w, eps, y):
 
 
 def _gqa_window(q, k_cache, v_cache, seq_lens, scale, window, out, sinks, kv_start, num_splits, max_seq_len, workspace):
-    long_cache._gqa_window(q, k_cache, v_cache, seq_lens, scale, window, out, sinks, kv_start, num_splits, max_seq_len,
-                           workspace)
+    long_cache._call(kernels.eager().window, q, k_cache, v_cache, seq_lens, scale, window, out, sinks, kv_start, num_splits,
+                     max_seq_len, workspace)
 
 
 def _kv4_store(k, v, ck, cv, k_scale, v_scale, slots, counts):
-    long_cache._kv4_store(k, v, long_cache.Kv4Cache(ck, cv, k_scale, v_scale), slots, counts)
+    kernels.eager().kv4_store(k, v, ck, cv, k_scale, v_scale, slots, counts)
 
 
 def _kv4_load(ck, cv, k_scale, v_scale, slots, tokens, k, v):
@@ -119,14 +119,14 @@ def _kv4_load(ck, cv, k_scale, v_scale, slots, tokens, k, v):
 
 def _gqa_decode_kv4(q, ck, cv, k_scale, v_scale, seq_lens, scale, out, kv_start, window, sinks, num_splits, max_seq_len,
                     workspace):
-    long_cache._gqa_decode_kv4(q, long_cache.Kv4Cache(ck, cv, k_scale, v_scale), seq_lens, scale, out, kv_start, window, sinks,
-                               num_splits, max_seq_len, workspace)
+    long_cache._call(kernels.eager().kv4, q, ck, cv, k_scale, v_scale, seq_lens, scale, out, kv_start, window, sinks, num_splits,
+                     max_seq_len, workspace)
 
 
 def _gqa_decode_tracked(q, k_cache, v_cache, seq_lens, scale, weights, out, decay, weights_out, kv_start, num_splits,
                         max_seq_len, workspace):
-    long_cache._gqa_decode_tracked(q, k_cache, v_cache, seq_lens, scale, weights, out, decay, weights_out, kv_start,
-                                   num_splits, max_seq_len, workspace)
+    long_cache._call(kernels.eager().tracked, q, k_cache, v_cache, seq_lens, scale, weights, out, decay, weights_out, kv_start,
+                     num_splits, max_seq_len, workspace)
 
 
 def _kv_select(weights, seq_lens, keep, sinks, recent, kv_start, index, lens, weights_out):
