@@ -371,7 +371,8 @@ struct Share {
 // Balanced: lane i works out how many wave tiles (row, column tile) i has, and the wave the tiles a split takes, the same for all
 // rows (every workgroup streams at about the same rate, so the longest share is what the launch takes), in steps of the
 // waves. First what all rows have together over the grid, which fits where lengths are equal; then the same with as many
-// workgroups set aside as rounding up took; then what fits for certain, sum max(1, ceil(n / c)) <= sum n / c + rows <= grid.
+// workgroups set aside as rounding up took; then what fits for certain: sum max(1, ceil(n / c)) <= sum n / c + rows <= grid, or
+// the longest row in as many splits as each has on average.
 // At most 64 splits of a row to merge.
 template <int P, int NW, bool BAL>
 __device__ __forceinline__ Share deal_splits(const int32_t* lens, const int32_t* starts, const LongParams& p) {
@@ -384,8 +385,9 @@ __device__ __forceinline__ Share deal_splits(const int32_t* lens, const int32_t*
   const TileRange tr = tile_range<P>(s, token_end(t0), token_end(min(t0 + p.tpt, p.T) - 1), p.window, p.sinks);
   const int n = lane < p.rows ? tr.na + tr.nb : 0;
   const float all = 1.000001f * (float)__builtin_amdgcn_readlane((int)wave_scan((uint32_t)n), kWave - 1);
-  const int least = max(p.min_tiles, (wave_uniform((int)wave_max((float)n)) + 63) / 64);
+  const int most = wave_uniform((int)wave_max((float)n)), least = max(p.min_tiles, (most + 63) / 64);
   const int grid = p.splits * p.rows;
+  const float certain = fminf(all / (float)(grid - p.rows), 1.000001f * (float)most / (float)p.splits);
   float share = all * p.inv_splits;
   int per, k, last;
   for (int i = 0; i < 3; ++i) {
@@ -395,7 +397,7 @@ __device__ __forceinline__ Share deal_splits(const int32_t* lens, const int32_t*
     last = (int)wave_scan((uint32_t)k);
     const int need = __builtin_amdgcn_readlane(last, kWave - 1);
     if (need <= grid) break;
-    share = all / (i == 0 ? fmaxf((float)grid - ((float)need - all * inv), (float)(grid - p.rows)) : (float)(grid - p.rows));
+    share = i == 0 ? fminf(all / fmaxf((float)grid - ((float)need - all * inv), 1.f), certain) : certain;
   }
   const uint64_t mine = __ballot((int)blockIdx.x < last && (int)blockIdx.x >= last - k);
   if (mine == 0) return {-1, 0, 0};

@@ -140,7 +140,7 @@ int make_plan(int kind, int B, int NH, int NKV, int D, int cap, int T, int windo
     // 18.7; dealt, 8 rows of 100..32768 of 4 bits: 4 splits 39.4, 8 33.1); over bf16 one, if that is at least four dealt splits
     // (us, 8 kv heads, head_dim 128, one round dealt / two, each row as many: 8 rows of 100..8192 27.1 / 31.9; 4 of 9000..16384
     // tracked 46.8 / 48.8; 6 of 500..8192, 4 tokens, 4 kv heads 16.1 / 20.2; fewer are too coarse to deal: 16 of 300..4096
-    // tracked, 2 splits dealt 39.3, 4 34.2, 4 each 38.0).
+    // tracked, 2 splits dealt 38.6, 4 34.1, 4 each 38.0).
     const int64_t round = cus / pl->units;
     splits = (int)(batch && (kv4 || round < 4 || !dealt(round)) ? 2 * cus / pl->units : round);
     const int most = (n + pl->min_tiles - 1) / pl->min_tiles;
