@@ -21,8 +21,9 @@ extern "C" {
 #endif
 
 /* Arguments of bz_gqa_window. base: as for bz_gqa_decode, with mask NULL and mask_dtype 0; tokens_per_row T may be one or
-   a whole prompt (at most 2^30); num_splits 0 picks the default; combine is ignored; workspace of at least bz_long_workspace_size(..) bytes where that is not 0. Softmax terms
-   enter the product with V as two bf16 terms (an error of 2^-17 each), over many tokens as one (2^-9). */
+   a whole prompt (at most 2^30); num_splits 0 picks the default; combine is ignored; workspace of at least
+   bz_long_workspace_size(..) bytes where that is not 0. Softmax terms enter the product with V as two bf16 terms (an error
+   of 2^-17 each), over many tokens as one (2^-9). */
 typedef struct bz_gqa_window_args {
   bz_gqa_decode_args base;
   int32_t window;             /* >= 0; 0: no window (plain causal attention) */
@@ -49,8 +50,9 @@ typedef struct bz_kv4_cache {
 /* Rounds k and v (bf16 [batch, num_kv_heads, tokens, head_dim], 16-byte aligned with strides of multiples of 8 elements)
    into the slots slots[b] .. slots[b] + tokens - 1 of row b. The scale of a block is the smallest power of two (from
    2^-126) with max |x| / scale <= 7, codes are x / scale rounded to nearest even and saturated at 6; a block that holds NaN
-   or an infinity gets scale byte 255. (Values from 1.75 * 2^127 on become 4 * 2^126, which bf16 reads as infinity.) counts, optional int32 [batch]: only the first counts[b] tokens of row b are
-   stored. Slots outside [0, capacity) are skipped. k and v share strides. */
+   or an infinity gets scale byte 255. (Values from 1.75 * 2^127 on become 4 * 2^126, which bf16 reads as infinity.) counts,
+   optional int32 [batch]: only the first counts[b] tokens of row b are stored. Slots outside [0, capacity) are skipped. k and
+   v share strides. */
 int bz_kv4_store(const void* k, const void* v, int64_t x_stride_b, int64_t x_stride_h, int64_t x_stride_t, int32_t tokens,
                  const int32_t* slots, const int32_t* counts, const bz_kv4_cache* cache, hipStream_t stream);
 
