@@ -48,7 +48,7 @@ struct Plan {
 int make_plan(int kind, int B, int NH, int NKV, int D, int cap, int T, int window, int sinks, int num_splits, int max_seq_len,
               Plan* pl) {
   if (B <= 0 || NH <= 0 || NKV <= 0 || cap <= 0 || T <= 0 || NH % NKV != 0 || window < 0 || sinks < 0) return BZ_ERR_SHAPE;
-  if (T > kMaxTokens) return BZ_ERR_SHAPE;
+  if (T > kMaxTokens || cap > kMaxTokens) return BZ_ERR_SHAPE;
   if (num_splits < 0 || num_splits > kMaxSplits) return BZ_ERR_SHAPE;
   if (!dim_ok(D) || !group_ok(NH / NKV)) return BZ_ERR_UNSUPPORTED;
   if (kind == BZ_LONG_KV4 && T > kKv4Tokens) return BZ_ERR_UNSUPPORTED;

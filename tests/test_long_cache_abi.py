@@ -198,6 +198,7 @@ def test_workspace_size(lib, K):
     assert size(2, 2, 16, 8, 128, 4096, 1, 0, 0, 1, 0) == 0 and n.value >= 2 * 16 * 4096 * 4  # the scores
     assert size(3, 2, 16, 8, 128, 4096, 1, 0, 0, 1, 0) == -2
     assert size(0, 2, 16, 8, 96, 4096, 1, 0, 0, 1, 0) == -3
+    assert size(2, 2, 16, 8, 128, 2**31 - 1, 1, 0, 0, 1, 0) == -2
     assert size(0, 2, 16, 8, 128, 4096, 1, -1, 0, 1, 0) == -2
     assert lib.bz_long_workspace_size(0, 2, 16, 8, 128, 4096, 1, 0, 0, 1, 0, None) == -1
 
