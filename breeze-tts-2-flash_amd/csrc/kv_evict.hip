@@ -4,6 +4,8 @@
 
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "bz_long_cache.h"
 #include "device_common.cuh"
 
@@ -211,11 +213,15 @@ SelectFn pick_select(int cap) {
 //
 // Row d of dst is row index[d] of src. In place (index ascends, index[d] >= d) a step of rows is read whole before it is
 // written, and no later step reads what it writes; the steps of one (row, head) follow each other, so the parallelism comes
-// from the columns: a workgroup takes `lanes` vectors of every row. Otherwise the steps are independent and spread over
-// workgroups too. Bound by memory: K and V of 4 rows x 8 heads x 4096 kept positions of 256 bytes, 134 MB read and written in
-// 25.5 us, 5.2 TB/s (a large copy: 5.0).
+// from the columns: a workgroup takes `lanes` vectors of every row, 128 bytes, one line (us, K and V of 4 rows x 8 heads, 4096
+// kept of 256 bytes: 64 bytes 43.6, 128 30.3, 256 43.3; 32 bytes 122), with 1024 threads, whose wide steps are few (256
+// threads at 64 bytes 39.7; 1 row x 8 heads 28.0, now 21.2). Otherwise the steps are independent and spread over workgroups
+// too. Bound by memory: the first of these, 134 MB read and written, to other tensors 23.5 to 25.5 us, 5.2 to 5.7 TB/s (a large
+// copy: 5.0); in place by the steps' round trips where rows are few.
 
-constexpr int kMoveThreads = 256, kMoveU = 8;
+constexpr int kMaxRowBytes = 1 << 28, kMaxKeep = 65535 * 128;  // one vector of a byte a slice, 128 rows a workgroup at least
+constexpr int kMoveU = 8;  // rows of a thread in flight
+constexpr int move_threads(bool in_place) { return in_place ? 1024 : 256; }
 typedef uint32_t vec8 __attribute__((ext_vector_type(2)));
 typedef uint32_t vec16 __attribute__((ext_vector_type(4)));
 
@@ -225,48 +231,47 @@ struct MoveParams {
   int first[BZ_KV_TENSORS];    // its first slice in grid.x
   int lanes[BZ_KV_TENSORS];    // vectors of a slice
   int vec[BZ_KV_TENSORS];      // bytes of a vector
-  int in_place[BZ_KV_TENSORS];
   int num, cap, keep, NKV;
   const int32_t *index, *lens;
 };
 
-template <class V>
+template <class V, bool IN>
 __device__ __forceinline__ void move_rows(const bz_kv_tensor& t, const char* src, char* dst, const int32_t* index, int cap,
-                                          int len, int slice, int lanes, bool in_place) {
-  const int rows = kMoveThreads / lanes, r = threadIdx.x / lanes, c = slice * lanes + (int)threadIdx.x % lanes;
+                                          int len, int slice, int lanes) {
+  constexpr int U = kMoveU;
+  const int rows = move_threads(IN) / lanes, r = threadIdx.x / lanes, c = slice * lanes + (int)threadIdx.x % lanes;
   const int64_t col = (int64_t)c * (int)sizeof(V);
   const bool mine = col < t.row_bytes;
-  const int step = rows * kMoveU;
-  const int d_begin = in_place ? 0 : (int)blockIdx.y * step, d_end = in_place ? len : min(len, d_begin + step);
+  const int step = rows * U;
+  const int d_begin = IN ? 0 : (int)blockIdx.y * step, d_end = IN ? len : min(len, d_begin + step);
   for (int d0 = d_begin; d0 < d_end; d0 += step) {
-    V x[kMoveU];
-    int from[kMoveU];
+    V x[U];
+    int from[U];
 #pragma unroll
-    for (int u = 0; u < kMoveU; ++u) from[u] = index[min(d0 + u * rows + r, len - 1)];
+    for (int u = 0; u < U; ++u) from[u] = index[min(d0 + u * rows + r, len - 1)];
 #pragma unroll
-    for (int u = 0; u < kMoveU; ++u) {  // every load without a condition; an index that is none reads row 0, unused
+    for (int u = 0; u < U; ++u) {  // every load without a condition; an index that is none reads row 0, unused
       const int64_t i = from[u] >= 0 && from[u] < cap ? from[u] : 0;
       x[u] = __builtin_nontemporal_load(reinterpret_cast<const V*>(src + i * t.src_stride_s + (mine ? col : 0)));
     }
-    if (in_place) {
+    if constexpr (IN) {
       __builtin_amdgcn_s_waitcnt(0x0f70);
       __syncthreads();
     }
 #pragma unroll
-    for (int u = 0; u < kMoveU; ++u) {
+    for (int u = 0; u < U; ++u) {
       const int d = d0 + u * rows + r;
-      if (mine && d < len && from[u] >= 0 && from[u] < cap && !(in_place && from[u] == d))
+      if (mine && d < len && from[u] >= 0 && from[u] < cap && !(IN && from[u] == d))
         __builtin_nontemporal_store(x[u], reinterpret_cast<V*>(dst + d * t.dst_stride_s + col));
     }
   }
 }
 
-__global__ void __launch_bounds__(kMoveThreads) kv_compact_kernel(const MoveParams p) {
+template <bool IN>
+__global__ void __launch_bounds__(move_threads(IN)) kv_compact_kernel(const MoveParams p) {
   int k = 0;
   while (k + 1 < p.num && (int)blockIdx.x >= p.first[k + 1]) ++k;
   const bz_kv_tensor& t = p.t[k];
-  const bool in_place = p.in_place[k];
-  if (in_place && blockIdx.y > 0) return;
   const int h = blockIdx.z % p.NKV, b = blockIdx.z / p.NKV;
   const int len = min(p.lens[b], p.keep);
   const char* const src = static_cast<const char*>(t.src) + b * t.src_stride_b + h * t.src_stride_h;
@@ -274,12 +279,47 @@ __global__ void __launch_bounds__(kMoveThreads) kv_compact_kernel(const MovePara
   const int32_t* const index = p.index + ((int64_t)b * p.NKV + h) * p.keep;
   const int slice = blockIdx.x - p.first[k], lanes = p.lanes[k];
   switch (p.vec[k]) {
-    case 16: move_rows<vec16>(t, src, dst, index, p.cap, len, slice, lanes, in_place); break;
-    case 8: move_rows<vec8>(t, src, dst, index, p.cap, len, slice, lanes, in_place); break;
-    case 4: move_rows<uint32_t>(t, src, dst, index, p.cap, len, slice, lanes, in_place); break;
-    case 2: move_rows<uint16_t>(t, src, dst, index, p.cap, len, slice, lanes, in_place); break;
-    default: move_rows<uint8_t>(t, src, dst, index, p.cap, len, slice, lanes, in_place); break;
+    case 16: move_rows<vec16, IN>(t, src, dst, index, p.cap, len, slice, lanes); break;
+    case 8: move_rows<vec8, IN>(t, src, dst, index, p.cap, len, slice, lanes); break;
+    case 4: move_rows<uint32_t, IN>(t, src, dst, index, p.cap, len, slice, lanes); break;
+    case 2: move_rows<uint16_t, IN>(t, src, dst, index, p.cap, len, slice, lanes); break;
+    default: move_rows<uint8_t, IN>(t, src, dst, index, p.cap, len, slice, lanes); break;
   }
+}
+
+// The tensors that move in place, or the others, in one launch.
+template <bool IN>
+int launch_moves(const bz_kv_tensor* tensors, int num, MoveParams& p, int batch, hipStream_t stream) {
+  int64_t grid_x = 0, grid_y = 1;
+  p.num = 0;
+  for (int i = 0; i < num; ++i) {
+    const bz_kv_tensor& t = tensors[i];
+    if ((t.src == t.dst) != IN) continue;
+    const int k = p.num++;
+    p.t[k] = t;
+    // the widest vector that divides every row's address and length
+    const uint64_t all = reinterpret_cast<uintptr_t>(t.src) | reinterpret_cast<uintptr_t>(t.dst) | (uint64_t)t.src_stride_b |
+                         (uint64_t)t.src_stride_h | (uint64_t)t.src_stride_s | (uint64_t)t.dst_stride_b |
+                         (uint64_t)t.dst_stride_h | (uint64_t)t.dst_stride_s | (uint64_t)t.row_bytes;
+    int vec = 16;
+    while (all % vec) vec /= 2;
+    const int vectors = t.row_bytes / vec, most = IN ? 8 : 16;
+    int lanes = 1;
+    while (lanes < vectors && lanes < most) lanes *= 2;
+    p.vec[k] = vec;
+    p.lanes[k] = lanes;
+    p.slices[k] = (vectors + lanes - 1) / lanes;
+    p.first[k] = (int)grid_x;
+    grid_x += p.slices[k];
+    if (!IN) {
+      const int step = move_threads(IN) / lanes * kMoveU;
+      grid_y = std::max<int64_t>(grid_y, (p.keep + step - 1) / step);
+    }
+  }
+  if (p.num == 0) return BZ_OK;
+  hipLaunchKernelGGL(kv_compact_kernel<IN>, dim3((unsigned)grid_x, (unsigned)grid_y, batch * p.NKV), dim3(move_threads(IN)), 0, stream,
+                     p);
+  return hipGetLastError() == hipSuccess ? BZ_OK : BZ_ERR_LAUNCH;
 }
 
 }  // namespace
@@ -323,40 +363,20 @@ BZ_EXPORT int bz_kv_compact(const bz_kv_tensor* tensors, int32_t num_tensors, co
       keep > capacity || capacity > kMaxCapacity || (int64_t)batch * num_kv_heads > 65535)
     return BZ_ERR_SHAPE;
   if ((reinterpret_cast<uintptr_t>(index) | reinterpret_cast<uintptr_t>(lens)) & 3) return BZ_ERR_ALIGNMENT;
-  MoveParams p{};
-  int grid_x = 0, grid_y = 1;
   for (int k = 0; k < num_tensors; ++k) {
     const bz_kv_tensor& t = tensors[k];
     if (t.src == nullptr || t.dst == nullptr) return BZ_ERR_NULL;
     if (t.row_bytes <= 0 || t.src_stride_s < t.row_bytes || t.dst_stride_s < t.row_bytes) return BZ_ERR_SHAPE;
-    p.t[k] = t;
-    p.in_place[k] = t.src == t.dst;
-    if (p.in_place[k] && (t.src_stride_b != t.dst_stride_b || t.src_stride_h != t.dst_stride_h || t.src_stride_s != t.dst_stride_s))
+    if (t.row_bytes > kMaxRowBytes) return BZ_ERR_SHAPE;  // grid limits
+    if (t.src == t.dst &&
+        (t.src_stride_b != t.dst_stride_b || t.src_stride_h != t.dst_stride_h || t.src_stride_s != t.dst_stride_s))
       return BZ_ERR_SHAPE;
-    // the widest vector that divides every row's address and length
-    const uint64_t all = reinterpret_cast<uintptr_t>(t.src) | reinterpret_cast<uintptr_t>(t.dst) | (uint64_t)t.src_stride_b |
-                         (uint64_t)t.src_stride_h | (uint64_t)t.src_stride_s | (uint64_t)t.dst_stride_b |
-                         (uint64_t)t.dst_stride_h | (uint64_t)t.dst_stride_s | (uint64_t)t.row_bytes;
-    int vec = 16;
-    while (all % vec) vec /= 2;
-    const int vectors = t.row_bytes / vec;
-    int lanes = 1;
-    const int most = p.in_place[k] ? 4 : 16;
-    while (lanes < vectors && lanes < most) lanes *= 2;
-    p.vec[k] = vec;
-    p.lanes[k] = lanes;
-    p.slices[k] = (vectors + lanes - 1) / lanes;
-    p.first[k] = grid_x;
-    grid_x += p.slices[k];
-    if (!p.in_place[k]) {
-      const int step = kMoveThreads / lanes * kMoveU, chunks = (keep + step - 1) / step;
-      if (chunks > grid_y) grid_y = chunks;
-    }
   }
-  if (grid_y > 65535) return BZ_ERR_SHAPE;
-  p.num = num_tensors, p.cap = capacity, p.keep = keep, p.NKV = num_kv_heads, p.index = index, p.lens = lens;
-  hipLaunchKernelGGL(kv_compact_kernel, dim3(grid_x, grid_y, batch * num_kv_heads), dim3(kMoveThreads), 0, stream, p);
-  return hipGetLastError() == hipSuccess ? BZ_OK : BZ_ERR_LAUNCH;
+  if (keep > kMaxKeep) return BZ_ERR_SHAPE;
+  MoveParams p{};
+  p.cap = capacity, p.keep = keep, p.NKV = num_kv_heads, p.index = index, p.lens = lens;
+  const int rc = launch_moves<false>(tensors, num_tensors, p, batch, stream);
+  return rc == BZ_OK ? launch_moves<true>(tensors, num_tensors, p, batch, stream) : rc;
 }
 
 }  // extern "C"

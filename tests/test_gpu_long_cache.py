@@ -463,6 +463,20 @@ def test_compact(device, in_place, cap, lens, keep):
             assert torch.equal(t.cpu(), old)
 
 
+def test_compact_some_in_place(device):
+    """Some tensors of a call move in place and some do not; more rows than a step of either holds."""
+    rng = np.random.default_rng(8)
+    cap, keep = 9000, 4000
+    index, kept, _ = select(heavy(rng, (1, 2, cap)), [cap], keep, 2, 3)
+    a, b, c = (torch.randint(0, 255, (1, 2, cap, w), dtype=torch.uint8, device=device) for w in (256, 96, 4))
+    old, out = [t.clone() for t in (a, b, c)], torch.zeros_like(b)
+    pkg.kv_compact((a, b, c), torch.from_numpy(index).to(device), ints(kept.tolist(), device), (a, out, c))
+    at = torch.from_numpy(index.astype(np.int64)).to(device)[..., None]
+    for got, t in ((a, old[0]), (out, old[1]), (c, old[2])):
+        assert torch.equal(got[:, :, :keep], t.gather(2, at.expand(-1, -1, -1, t.size(3))))
+    assert torch.equal(a[:, :, keep:], old[0][:, :, keep:]) and torch.equal(b, old[1]) and (out[:, :, keep:] == 0).all()
+
+
 def test_compact_leaves_bad_indices_alone(device):
     t = torch.arange(8, device=device, dtype=torch.int64).view(1, 1, 8, 1)
     out = torch.full_like(t, -1)
