@@ -31,8 +31,9 @@ LoadFn g_load = nullptr;
 SelectFn g_select = nullptr;
 CompactFn g_compact = nullptr;
 
-// (device, raw stream, kind, batch, q heads, kv heads, tokens) -> workspace
-using LongKey = std::array<int64_t, 7>;
+// (device, raw stream, kind, sharing) -> workspace. Sharing: calls that find the counters of a workspace where others leave them
+// zero (sharing_of).
+using LongKey = std::array<int64_t, 4>;
 std::map<LongKey, at::Tensor> g_long_ws;
 std::map<std::array<int64_t, 12>, size_t> g_long_bytes;
 
@@ -159,6 +160,15 @@ at::Device fill_kv4(PyObject* const* t, bz_kv4_cache& c) {
   return dev;
 }
 
+// 0 for calls of few units, whose counters have one room for all; 1 for the chunks of bz_gqa_window beyond (more units than the
+// device has CUs: the chunk kernel, which has no counters and writes what it reads); else the units.
+int64_t sharing_of(int kind, const bz_gqa_decode_args& a) {
+  const int64_t group = a.num_q_heads / std::max(a.num_kv_heads, 1), T = a.tokens_per_row;
+  const int64_t tpt = std::min<int64_t>(T, 16 / std::max<int64_t>(std::min<int64_t>(group, 16), 1)), tiles = (T + tpt - 1) / tpt;
+  const int64_t units = a.batch * tiles * a.num_kv_heads;
+  return units <= BZ_LONG_SHARED_UNITS ? 0 : kind == BZ_LONG_WINDOW && tiles > 1 ? 1 : units;
+}
+
 // The workspace of an attention call into a; true if there is one or none is needed. Otherwise `need` is the tuple the
 // Python side makes one from (a call under capture raises instead: nothing is allocated then).
 bool long_workspace(int kind, int idx, hipStream_t stream, int window, int sinks, const at::Tensor* given, const at::Device& dev,
@@ -184,29 +194,28 @@ bool long_workspace(int kind, int idx, hipStream_t stream, int window, int sinks
   if (capturing(stream))
     throw Error{"a call being captured into a graph needs workspace= (long_workspace(...), made before the capture; " +
                 std::to_string(it->second) + " bytes): graphs that shared the stream's own could not run at the same time"};
-  const LongKey key{idx, (int64_t)reinterpret_cast<uintptr_t>(stream), kind, a.batch, a.num_q_heads, a.num_kv_heads,
-                    a.tokens_per_row};
+  const LongKey key{idx, (int64_t)reinterpret_cast<uintptr_t>(stream), kind, sharing_of(kind, a)};
   auto ws = g_long_ws.find(key);
   if (ws != g_long_ws.end() && (size_t)ws->second.numel() >= it->second) {
     a.workspace = ws->second.data_ptr();
     a.workspace_bytes = (size_t)ws->second.numel();
     return true;
   }
-  *need = Py_BuildValue("(LLLLLLLn)", (long long)key[0], (long long)key[1], (long long)key[2], (long long)key[3],
-                        (long long)key[4], (long long)key[5], (long long)key[6], (Py_ssize_t)it->second);
+  *need = Py_BuildValue("(LLLLn)", (long long)key[0], (long long)key[1], (long long)key[2], (long long)key[3],
+                        (Py_ssize_t)it->second);
   return false;
 }
 
-// register_long_workspace(device, stream, kind, batch, q heads, kv heads, tokens, workspace)
+// register_long_workspace(device, stream, kind, sharing, workspace)
 PyObject* register_long_workspace(PyObject*, PyObject* args) {
-  long long k[7];
+  long long k[4];
   PyObject* o;
-  if (!PyArg_ParseTuple(args, "LLLLLLLO", &k[0], &k[1], &k[2], &k[3], &k[4], &k[5], &k[6], &o)) return nullptr;
+  if (!PyArg_ParseTuple(args, "LLLLO", &k[0], &k[1], &k[2], &k[3], &o)) return nullptr;
   if (!THPVariable_Check(o)) {
     PyErr_SetString(PyExc_TypeError, "register_long_workspace: a tensor expected");
     return nullptr;
   }
-  g_long_ws[LongKey{k[0], k[1], k[2], k[3], k[4], k[5], k[6]}] = THPVariable_Unpack(o);
+  g_long_ws[LongKey{k[0], k[1], k[2], k[3]}] = THPVariable_Unpack(o);
   Py_RETURN_NONE;
 }
 

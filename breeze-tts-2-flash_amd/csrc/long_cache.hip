@@ -26,6 +26,7 @@ constexpr int kFusePositions = 2048;
 // Bytes of the longest row a split takes from which on splits are dealt (4 rows of 20001..32768 of 4 bits, 16 splits, 278 KB:
 // 18.6 us dealt or not; 16 rows of 128..2048, 2 splits, 139 KB: 10.9 dealt, 10.7 not).
 constexpr int64_t kDealBytes = 1 << 18;
+constexpr int kCounterLines = BZ_LONG_SHARED_UNITS;
 constexpr int kMaxTokens = 1 << 30;  // sums of tokens and tile sizes stay in 32 bits
 constexpr int kKv4Tokens = 16;  // most query tokens per row over a 4-bit cache
 
@@ -68,6 +69,8 @@ int make_plan(int kind, int B, int NH, int NKV, int D, int cap, int T, int windo
   const int64_t longest = max_seq_len > 0 && max_seq_len < cap ? max_seq_len : cap;
   auto attended = [&](int64_t tokens) { return window > 0 ? std::min(longest, (int64_t)window + tokens + sinks) : longest; };
 
+  // the counters' room, the same for all calls of at most kCounterLines units, so that they can share a workspace
+  const size_t counters = (size_t)std::max<int64_t>(pl->units, kCounterLines) * kCounterStride * sizeof(int);
   pl->prefill = pl->balanced = false;
   if (kind == BZ_LONG_WINDOW && pl->tiles > 1) {
     auto tiles = [&](int cg) { return ((int64_t)T * pl->G + kPreWaveCols * cg - 1) / (kPreWaveCols * cg); };
@@ -102,7 +105,6 @@ int make_plan(int kind, int B, int NH, int NKV, int D, int cap, int T, int windo
       }
     }
     if (pl->prefill) {
-      const size_t counters = (size_t)pl->units * kCounterStride * sizeof(int);
       pl->cgroups = splits > 1 || wide >= 3 * cus ? 4 : tiles(2) * rows >= cus ? 2 : 1;
       if (tiles(pl->cgroups) * splits > 65535 || B > 65535 || NKV > 65535) return BZ_ERR_SHAPE;  // grid limits
       pl->tiles = (int)tiles(pl->cgroups);
@@ -110,7 +112,7 @@ int make_plan(int kind, int B, int NH, int NKV, int D, int cap, int T, int windo
       pl->ml = pl->acc = pl->head_ml = pl->scores = pl->total = 0;
       if (splits > 1) {
         const size_t cols = (size_t)(rows * pl->tiles * splits) * 4 * kPreWaveCols;
-        pl->ml = counters;  // other calls' with this workspace
+        pl->ml = counters;  // room for those of other calls with this workspace
         pl->acc = up256(pl->ml + cols * sizeof(float2));
         pl->total = pl->acc + cols * D * sizeof(float);
       }
@@ -154,7 +156,7 @@ int make_plan(int kind, int B, int NH, int NKV, int D, int cap, int T, int windo
   const size_t cols = (size_t)pl->units * splits * pl->tpt * pl->G;
   const bool merged = splits > 1;
   // a tracked call of one split has no use for the counters, but a later call with the same workspace finds them zero
-  pl->ml = merged || kind == BZ_LONG_TRACKED ? (size_t)pl->units * kCounterStride * sizeof(int) : 0;
+  pl->ml = merged || kind == BZ_LONG_TRACKED ? counters : 0;
   pl->acc = up256(pl->ml + (merged ? cols * sizeof(float2) : 0));
   pl->head_ml = up256(pl->acc + (merged ? cols * D * sizeof(float) : 0));
   pl->total = pl->head_ml;

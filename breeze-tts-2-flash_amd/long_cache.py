@@ -21,7 +21,7 @@ import torch
 from . import attention, kernels
 from .attention import _check
 
-_WS: dict = {}  # (device index, raw stream handle, kind, batch, NH, NKV, T) -> workspace
+_WS: dict = {}  # (device index, raw stream handle, kind, sharing) -> workspace (csrc/eager_long.hpp: sharing_of)
 _KINDS = {"window": kernels.LONG_WINDOW, "kv4": kernels.LONG_KV4, "tracked": kernels.LONG_TRACKED}
 
 
@@ -56,9 +56,9 @@ def _bytes(idx: int, kind: int, B: int, NH: int, NKV: int, D: int, cap: int, T: 
 
 def _make_workspace(need) -> None:
     """Makes and registers the workspace that the native binding asked for: need = (device index, raw stream handle, kind,
-    batch, NH, NKV, T, bytes). Grown, never shrunk; replaced ones are kept for graphs that may hold them, as
+    sharing, bytes). One serves calls of all sizes (but for batches of more than 512 units). Grown, never shrunk; replaced ones are kept for graphs that may hold them, as
     attention.get_workspace keeps its own."""
-    key, n = need[:7], need[7]
+    key, n = need[:4], need[4]
     with attention._WS_LOCK:
         ws = _WS.get(key)
         if ws is None or ws.numel() < n:

@@ -593,6 +593,24 @@ def test_tracked_splits_share_a_workspace(device):
         assert abs(float(wo[1, :, :300].sum()) - NKV * G) < 1e-3 and (wo[1, :, 300:] == 7).all(), splits
 
 
+def test_calls_of_all_sizes_share_the_streams_workspace(device):
+    """Batches, heads, chunk lengths and splits in turn on one stream, which keeps one workspace a kind for them."""
+    from breeze_tts_2_flash_amd import long_cache
+    rng = np.random.default_rng(21)
+    cases = [(1, 1, 2, 64, 1, 900, 0), (3, 2, 4, 128, 2, 700, 5), (1, 8, 2, 128, 200, 1200, 3), (1, 2, 1, 64, 40, 800, 2),
+             (2, 1, 8, 128, 5, 600, 7), (1, 8, 8, 64, 600, 1500, 2), (4, 2, 2, 64, 1, 2000, 0)]
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for again in range(2):
+            for B, NKV, G, D, T, n, splits in cases + cases[::-1]:
+                q, k, v = randn(rng, B, NKV * G, T, D), randn(rng, B, NKV, n, D), randn(rng, B, NKV, n, D)
+                lens = [n - 100 * b for b in range(B)]
+                out = pkg.gqa_window(q.to(device), k.to(device), v.to(device), ints(lens, device), D ** -0.5, 0, num_splits=splits)
+                check_attention(out, q.float(), k.float(), v.float(), lens, D ** -0.5, what=f"{again} {B} {NKV} {G} {D} {T}")
+    side.synchronize()
+    assert len([key for key in long_cache._WS if key[1] == side.cuda_stream]) <= 2  # few units, and chunks of more
+
+
 def _calls(device, seed):
     """One call of each kind on inputs of its own: (name, run(workspaces), state to vary)."""
     rng = np.random.default_rng(seed)
