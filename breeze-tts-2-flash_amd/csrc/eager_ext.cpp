@@ -667,6 +667,8 @@ PyMethodDef kMethods[] = {
      "kv_compact through the C ABI"},
     {"evict", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(evict)), METH_FASTCALL,
      "kv_evict through the C ABI"},
+    {"apart", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(apart_py)), METH_FASTCALL,
+     "whether two tensors share no memory, as the long-cache calls check it"},
     {"bind", bind, METH_VARARGS, "the C ABI functions' addresses"},
     {"bind_long", bind_long, METH_VARARGS, "the long-cache functions' addresses"},
     {"register_long_workspace", register_long_workspace, METH_VARARGS, "a workspace made for a long-cache call's key"},

@@ -308,13 +308,66 @@ std::pair<uintptr_t, uintptr_t> span_of(const at::Tensor& t) {
   return {p, p + (uintptr_t)((last + 1) * (int64_t)t.element_size())};
 }
 
+// One dim of two tensors whose steps in it are alike: the step in bytes and the sizes.
+struct SharedDim {
+  int64_t step, nx, ny;
+};
+// Whether a block of x and one of y meet, for some indices of the dims from `d` on: y's lies diff + sum (j_y - j_x) step bytes
+// behind x's, and they hold ex and ey bytes.
+bool blocks_meet(const SharedDim* d, int dims, int64_t diff, int64_t ex, int64_t ey) {
+  if (dims == 0) return diff < ex && diff > -ey;
+  if (d->step == 0) return blocks_meet(d + 1, dims - 1, diff, ex, ey);
+  int64_t below = ey, above = ex;  // what the inner dims can still move the blocks by
+  for (int i = 1; i < dims; ++i) below += (d[i].ny - 1) * d[i].step, above += (d[i].nx - 1) * d[i].step;
+  const auto floor_div = [](int64_t a, int64_t b) { return a / b - (a % b < 0); };
+  const int64_t lo = std::max(1 - d->nx, floor_div(-below - diff, d->step) + 1);
+  const int64_t hi = std::min(d->ny - 1, -floor_div(diff - above, d->step) - 1);
+  if (hi - lo > 8) return true;  // steps that do not nest: taken to meet
+  for (int64_t j = lo; j <= hi; ++j)
+    if (blocks_meet(d + 1, dims - 1, diff + j * d->step, ex, ey)) return true;
+  return false;
+}
+
+// Whether two tensors share no memory: their spans lie apart, or they are views of one tensor side by side in one of its dims (a
+// cache that holds K and V in turns by batch row, head or position). Their largest steps, as far as both have the same ones, run
+// over blocks that the smaller ones fill; no two of those may meet. Where that cannot be shown they are taken to share some.
+bool apart(const at::Tensor& x, const at::Tensor& y) {
+  const auto a = span_of(x), b = span_of(y);
+  if (a.second <= b.first || b.second <= a.first) return true;
+  if (x.dim() != y.dim() || x.dim() > 8) return false;
+  const int64_t sx = x.element_size(), sy = y.element_size();
+  int order[8], dims = 0;
+  for (int i = 0; i < x.dim(); ++i)
+    if (x.size(i) > 1 || y.size(i) > 1) order[dims++] = i;
+  std::stable_sort(order, order + dims, [&](int i, int j) { return x.stride(i) * sx > x.stride(j) * sx; });
+  SharedDim outer[8];
+  for (int n = 0; n < dims; ++n) {
+    const int i = order[n];
+    if (x.stride(i) * sx != y.stride(i) * sy) return false;
+    outer[n] = {x.stride(i) * sx, x.size(i), y.size(i)};
+    int64_t ex = sx, ey = sy;
+    for (int m = n + 1; m < dims; ++m) {
+      ex += (x.size(order[m]) - 1) * x.stride(order[m]) * sx;
+      ey += (y.size(order[m]) - 1) * y.stride(order[m]) * sy;
+    }
+    if (!blocks_meet(outer, n + 1, (int64_t)(b.first - a.first), ex, ey)) return true;
+  }
+  return false;
+}
+
+// apart(x, y) for tests, on tensors of any device
+PyObject* apart_py(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  return guarded("apart", nargs, 2, [&]() -> PyObject* {
+    return PyBool_FromLong(apart(tensor(args[0], "x"), tensor(args[1], "y")));
+  });
+}
+
 // dst is src itself (the same elements), or shares none of its memory; every element has a place of its own.
 void check_destination(const at::Tensor& src, const at::Tensor& dst, const char* name) {
   for (int64_t i = 0; i < dst.dim(); ++i)
     if (dst.stride(i) <= 0 && dst.size(i) != 1) throw Error{std::string(name) + " must not be a broadcast view"};
   if (dst.data_ptr() == src.data_ptr() && dst.strides() == src.strides()) return;
-  const auto a = span_of(src), b = span_of(dst);
-  if (a.second > b.first && b.second > a.first) throw Error{std::string(name) + " must be its source itself or not overlap it"};
+  if (!apart(src, dst)) throw Error{std::string(name) + " must be its source itself or not overlap it"};
 }
 
 void weights_view(const at::Tensor& t, int64_t B, int64_t NKV, int64_t cap, const char* name, const at::Device& dev) {
@@ -446,25 +499,6 @@ void fill_select(PyObject* const* args, bz_kv_select_args& a, at::Tensor& index,
     a.weights_out = wo->data_ptr<float>(), a.wo_stride_b = wo->stride(0), a.wo_stride_h = wo->stride(1);
   }
   a.batch = (int32_t)B, a.num_kv_heads = (int32_t)NKV, a.capacity = (int32_t)cap;
-}
-
-// Whether two tensors [B, NKV, capacity, X] share no memory: their spans lie apart, or they interleave row by row (views of
-// one tensor, such as a cache that holds K and V side by side).
-bool apart(const at::Tensor& x, const at::Tensor& y) {
-  const auto a = span_of(x), b = span_of(y);
-  if (a.second <= b.first || b.second <= a.first) return true;
-  const int64_t nx = x.element_size(), ny = y.element_size();
-  int64_t step = INT64_MAX;
-  for (int i = 0; i < 3; ++i) {
-    if (x.size(i) == 1 && y.size(i) == 1) continue;
-    if (x.stride(i) * nx != y.stride(i) * ny || x.stride(i) <= 0) return false;
-    step = std::min(step, x.stride(i) * nx);
-  }
-  if (step == INT64_MAX) return false;
-  for (int i = 0; i < 3; ++i)
-    if ((x.size(i) > 1 || y.size(i) > 1) && (x.stride(i) * nx) % step) return false;
-  const int64_t diff = (int64_t)(b.first - a.first), gap = ((diff % step) + step) % step;
-  return x.size(3) * nx <= gap && gap + y.size(3) * ny <= step;
 }
 
 struct Tensors {

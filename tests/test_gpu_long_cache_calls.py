@@ -1,0 +1,45 @@
+"""GPU: calls of the long-cache operators (include/bz_long_cache.h) that their documentation allows, or that they refuse, beyond
+those of test_gpu_long_cache.py."""
+import numpy as np
+import pytest
+import torch
+
+import breeze_tts_2_flash_amd as pkg
+from oracle.long_cache import attention_bound, window_attention
+
+pytestmark = pytest.mark.gpu
+
+BF16 = torch.bfloat16
+
+
+def ints(v, device):
+    return torch.tensor(v, dtype=torch.int32, device=device)
+
+
+def randn(rng, *shape):
+    return torch.from_numpy(rng.standard_normal(shape).astype(np.float32)).to(BF16)
+
+
+# ------------------------------------------------------------------------------------------------- eviction
+
+@pytest.mark.parametrize("shape", ["2bhs", "b2hs", "bh2s", "bsh2"])
+@pytest.mark.parametrize("in_place", [True, False])
+def test_evict_views_of_one_tensor(device, shape, in_place):
+    """K and V side by side in one tensor, by any of its dims."""
+    rng = np.random.default_rng(3)
+    B, NKV, cap, D, keep = 2, 3, 90, 64, 40
+    if shape == "bsh2":
+        kv = randn(rng, B, cap, NKV, 2, D).to(device).permute(3, 0, 2, 1, 4)
+    else:
+        sizes = dict(b=B, h=NKV, s=cap)
+        kv = randn(rng, *(2 if c == "2" else sizes[c] for c in shape), D).to(device).movedim(shape.index("2"), 0)
+    k, v = kv[0], kv[1]
+    assert k.shape == (B, NKV, cap, D)
+    old, weights = kv.clone(), torch.rand(B, NKV, cap, device=device)
+    outs = None if in_place else torch.zeros_like(kv).unbind(0)
+    index, lens = pkg.kv_evict((k, v), weights, ints([cap, cap - 7], device), keep, sinks=2, recent=5, outs=outs)
+    at = index.long()[..., None].expand(-1, -1, -1, D)
+    for i, got in enumerate((k, v) if in_place else outs):
+        assert torch.equal(got[:, :, :keep], old[i].gather(2, at))
+        assert torch.equal(got[:, :, keep:], old[i][:, :, keep:] if in_place else torch.zeros_like(got[:, :, keep:]))
+    assert lens.tolist() == [keep, keep]
