@@ -606,6 +606,10 @@ PyObject* evict(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     fill_select(args, a, index, lens);
     Tensors m;
     fill_compact(args[9], args[10], a.batch, a.num_kv_heads, a.capacity, index.device(), m);
+    if (const at::Tensor* wo = tensor_or_none(args[8], "weights_out"))  // written by the selection, before the tensors move
+      for (int i = 0; i < m.num; ++i)
+        require(apart(m.src[i], wo->unsqueeze(-1)) && apart(m.dst[i], wo->unsqueeze(-1)),
+                "weights_out is compacted with the tensors and must not overlap one of them");
     const int idx = index.device().index();
     DeviceScope scope(idx);
     hipStream_t stream = c10::hip::getCurrentHIPStream(idx).stream();

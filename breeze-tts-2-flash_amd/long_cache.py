@@ -220,7 +220,8 @@ def kv_compact(tensors, index: torch.Tensor, lens: torch.Tensor, outs=None):
 def kv_evict(tensors, weights: torch.Tensor, seq_lens: torch.Tensor, keep: int, *, sinks: int = 0, recent: int = 0,
              kv_start: torch.Tensor | None = None, outs=None,
              weights_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
-    """kv_select, and the cache's tensors and weights compacted to what stays (in place unless outs / weights_out are given).
+    """kv_select, and the cache's tensors and weights compacted to what stays (in place unless outs / weights_out are given;
+    the weights move with the selection, so weights_out shares no memory with the tensors).
     The kept positions of row b are then the slots [0, lens[b]) of every kv head, in their old order, so later calls take
     lens for seq_lens and no kv_start. Returns (index, lens)."""
     weights_out = weights if weights_out is None else weights_out

@@ -43,3 +43,19 @@ def test_evict_views_of_one_tensor(device, shape, in_place):
         assert torch.equal(got[:, :, :keep], old[i].gather(2, at))
         assert torch.equal(got[:, :, keep:], old[i][:, :, keep:] if in_place else torch.zeros_like(got[:, :, keep:]))
     assert lens.tolist() == [keep, keep]
+
+
+def test_evict_refuses_weights_among_the_tensors(device):
+    """The weights move with the selection; as one of the tensors they would move twice."""
+    rng = np.random.default_rng(4)
+    k, w, lens = randn(rng, 1, 2, 64, 64).to(device), torch.rand(1, 2, 64, device=device), ints([64], device)
+    held, other = w.clone(), torch.zeros_like(w)
+    for call in (lambda: pkg.kv_evict((k, w[..., None]), w, lens, 16),
+                 lambda: pkg.kv_evict((other[..., None],), w, lens, 16, outs=(held[..., None],), weights_out=other),
+                 lambda: pkg.kv_evict((k, w[..., None]), w, lens, 16, outs=(torch.zeros_like(k), other[..., None]))):
+        with pytest.raises(RuntimeError):
+            call()
+    assert torch.equal(w, held)
+    # read by the selection and moved to another place, it is a tensor like any other
+    index, _ = pkg.kv_evict((w[..., None],), w, lens, 16, outs=(other[..., None],), weights_out=torch.zeros_like(w))
+    assert torch.equal(other[..., :16], held.gather(2, index.long())) and torch.equal(w, held)
