@@ -167,11 +167,13 @@ __device__ __forceinline__ uint32_t finite_pair(uint32_t w) {
 }
 
 // Scores are taken times a positive scale, which a maximum may be taken before; the query carries the sign. (1e-30 stands for
-// a scale of 0, whose product with an excluded position's -inf would be NaN.)
+// a scale of 0, whose product with an excluded position's -inf would be NaN; for a scale that is NaN as well, and the query is
+// NaN then: so are the scores of the positions a token attends, and no others.)
 __device__ __forceinline__ float positive_scale(float scale_log2) { return fmaxf(fabsf(scale_log2), 1e-30f); }
 __device__ __forceinline__ bf16x8_t signed_q(uint4 q, float scale_log2) {
   const uint32_t flip = scale_log2 < 0.f ? 0x80008000u : 0u;
   q.x ^= flip, q.y ^= flip, q.z ^= flip, q.w ^= flip;
+  if (scale_log2 != scale_log2) q.x = q.y = q.z = q.w = 0x7fff7fffu;
   return __builtin_bit_cast(bf16x8_t, q);
 }
 

@@ -93,6 +93,7 @@ __device__ __forceinline__ void careful_column(const LongParams& p, int b, int h
     m = mn;
     const float t = fast_exp2(x - mu);
     l = l * alpha + wave_sum(t);
+    if (l != l) break;  // a score that is NaN or +inf: all of the output is NaN
 #pragma unroll
     for (int i = 0; i < DV; ++i) acc[i] *= alpha;
     for (int j = 0; j < min(kWave, end - p0); ++j) {

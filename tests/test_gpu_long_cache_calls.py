@@ -20,6 +20,30 @@ def randn(rng, *shape):
     return torch.from_numpy(rng.standard_normal(shape).astype(np.float32)).to(BF16)
 
 
+# ------------------------------------------------------------------------------------------------- attention
+
+@pytest.mark.parametrize("T,NKV,G", [(1, 2, 2), (5, 1, 4), (70, 8, 8), (300, 8, 2)])
+@pytest.mark.parametrize("splits", [0, 3])
+def test_scale_that_is_nan(device, T, NKV, G, splits):
+    """It makes NaN of every token that attends a position; one that attends none still gets zeros."""
+    rng = np.random.default_rng(T)
+    D, cap = 128, T + 400
+    q, k, v = (randn(rng, *s).to(device) for s in ((3, NKV * G, T, D), (3, NKV, cap, D), (3, NKV, cap, D)))
+    lens, nan = ints([cap, T // 2, 0], device), float("nan")
+    outs = [pkg.gqa_window(q, k, v, lens, nan, 100, sinks=3, num_splits=splits)]
+    if T <= 16:
+        cache = pkg.kv4_store(k, v, pkg.kv4_cache(3, NKV, cap, D, device), ints([0] * 3, device))
+        outs.append(pkg.gqa_decode_kv4(q, cache, lens, nan, window=100, sinks=3, num_splits=splits))
+    if T == 1:
+        w = torch.zeros(3, NKV, cap, device=device)
+        outs.append(pkg.gqa_decode_tracked(q, k, v, lens, nan, w, num_splits=splits))
+        assert torch.isnan(w[0]).all() and (w[1:] == 0).all()
+    for out in outs:
+        out = out.view(3, T, -1)
+        assert torch.isnan(out[0]).all() and (out[2] == 0).all()
+        assert (out[1, :T - T // 2] == 0).all() and torch.isnan(out[1, T - T // 2:]).all()
+
+
 # ------------------------------------------------------------------------------------------------- eviction
 
 @pytest.mark.parametrize("shape", ["2bhs", "b2hs", "bh2s", "bsh2"])
