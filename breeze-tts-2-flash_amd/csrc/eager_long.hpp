@@ -429,7 +429,10 @@ PyObject* kv4_store(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     check_kv(k, v, c, dev);
     for (int i = 2; i < 6; ++i)
       require(one_place_each(THPVariable_Unpack(args[i])), "a cache that is written must not be a broadcast view");
-    require(c.k != c.v && c.k_scale != c.v_scale, "a cache's K and V must not be the same tensor");
+    for (int i = 2; i < 6; ++i)
+      for (int j = i + 1; j < 6; ++j)
+        require(apart(THPVariable_Unpack(args[i]), THPVariable_Unpack(args[j])),
+                "the tensors of a cache that is written must not overlap one another");
     const int32_t *slots = rows_arg(args[6], c.batch, "slots", dev), *counts = rows_or_null(args[7], c.batch, "counts", dev);
     const int idx = dev.index();
     DeviceScope scope(idx);
@@ -457,7 +460,7 @@ PyObject* kv4_load(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     check_kv(k, v, c, dev);
     require(k.size(2) == tokens, "the outputs must hold as many tokens as are asked for");
     require(one_place_each(k) && one_place_each(v), "an output must not be a broadcast view");
-    require(k.data_ptr() != v.data_ptr(), "the outputs must not be the same tensor");
+    require(apart(k, v), "the outputs must not overlap one another");
     check_status(g_load(&c, slots, tokens, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
                         c10::hip::getCurrentHIPStream(idx).stream()),
                  "bz_kv4_load");

@@ -44,6 +44,42 @@ def test_scale_that_is_nan(device, T, NKV, G, splits):
         assert (out[1, :T - T // 2] == 0).all() and torch.isnan(out[1, T - T // 2:]).all()
 
 
+# --------------------------------------------------------------------------------------------------- 4 bits
+
+def test_kv4_refuses_overlaps(device):
+    """Outputs, and the tensors of a cache that is written, which share memory with one another."""
+    rng = np.random.default_rng(5)
+    x, slot = randn(rng, 1, 2, 3, 128).to(device), ints([0], device)
+    cache = pkg.kv4_cache(1, 2, 64, 128, device)
+    rows = torch.zeros(1, 2, 80, 128, dtype=BF16, device=device)
+    with pytest.raises(RuntimeError):
+        pkg.kv4_load(cache, slot, 30, rows[:, :, :30], rows[:, :, 10:40])
+    codes, scales = (torch.zeros(1, 2, 80, n, dtype=torch.uint8, device=device) for n in (64, 4))
+    for bad in (cache._replace(k=codes[:, :, :64], v=codes[:, :, 16:]), cache._replace(k_scale=scales[:, :, :64], v_scale=scales[:, :, 16:]),
+                cache._replace(k_scale=cache.k.view(1, 2, 1024, 4)[:, :, :64], v_scale=cache.v.view(1, 2, 1024, 4)[:, :, :64])):
+        with pytest.raises(RuntimeError):
+            pkg.kv4_store(x, x, bad, slot)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_kv4_cache_in_one_tensor(device, D):
+    """A head's codes of K and V and their scales one behind the other in one tensor; outputs side by side."""
+    rng = np.random.default_rng(D)
+    B, NKV, cap, T = 2, 3, 40, 7
+    at, room = [0, cap * D // 2, cap * D, cap * D + cap * D // 32], cap * (D + D // 16)
+    one = torch.zeros(B, NKV, room, dtype=torch.uint8, device=device)
+    cache = pkg.Kv4Cache(*(one.as_strided((B, NKV, cap, n), (NKV * room, room, n, 1), p)
+                           for p, n in zip(at, (D // 2, D // 2, D // 32, D // 32))))
+    plain = pkg.kv4_cache(B, NKV, cap, D, device)
+    k, v, slots = randn(rng, B, NKV, T, D).to(device), randn(rng, B, NKV, T, D).to(device), ints([3, cap - T], device)
+    for c in (cache, plain):
+        pkg.kv4_store(k, v, c, slots)
+    assert all(torch.equal(a, b) for a, b in zip(cache, plain))
+    both = torch.zeros(B, NKV, 2, T, D, dtype=BF16, device=device)
+    pkg.kv4_load(cache, slots, T, both[:, :, 0], both[:, :, 1])
+    assert all(torch.equal(a, b) for a, b in zip(both.unbind(2), pkg.kv4_load(plain, slots, T)))
+
+
 # ------------------------------------------------------------------------------------------------- eviction
 
 @pytest.mark.parametrize("shape", ["2bhs", "b2hs", "bh2s", "bsh2"])
