@@ -71,6 +71,15 @@ const int32_t* rows_or_null(PyObject* o, int64_t B, const char* name, const at::
   return o == Py_None ? nullptr : rows_arg(o, B, name, dev);
 }
 
+// Whether K and V have one shape and the same steps in every dim of more than one element (a single token's keys, rotated, and
+// values, as the projection left them, differ in the step between tokens, which no access uses).
+bool alike(const at::Tensor& k, const at::Tensor& v) {
+  if (v.sizes() != k.sizes()) return false;
+  for (int64_t i = 0; i < k.dim(); ++i)
+    if (k.size(i) > 1 && k.stride(i) != v.stride(i)) return false;
+  return true;
+}
+
 // Whether no two elements of t share a place because of a broadcast dim.
 bool one_place_each(const at::Tensor& t) {
   for (int64_t i = 0; i < t.dim(); ++i)
@@ -127,7 +136,7 @@ void fill_query(const at::Tensor& q, const at::Tensor* out, PyObject* seq_lens, 
 void fill_bf16_cache(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, bz_gqa_decode_args& a) {
   require(k.scalar_type() == at::kBFloat16 && v.scalar_type() == at::kBFloat16, "k_cache and v_cache must be bf16");
   require(k.device() == q.device() && v.device() == q.device(), "all tensors must be on one device");
-  require(k.dim() == 4 && v.sizes() == k.sizes() && v.strides() == k.strides(),
+  require(k.dim() == 4 && alike(k, v),
           "k_cache and v_cache must be [B, NKV, capacity, D] with equal shapes and strides");
   const auto sz = k.sizes(), st = k.strides();
   if (sz[0] != a.batch || sz[3] != a.head_dim || st[3] != 1)
@@ -147,9 +156,9 @@ at::Device fill_kv4(PyObject* const* t, bz_kv4_cache& c) {
             "a 4-bit cache is four uint8 device tensors [B, NKV, capacity, ..] on one device");
   const auto sz = k.sizes(), st = k.strides(), zs = ks.sizes(), ts = ks.strides();
   const int64_t D = 2 * sz[3];
-  require(v.sizes() == sz && v.strides() == st && st[3] == 1,
+  require(alike(k, v) && st[3] == 1,
           "codes k and v must have equal shapes and strides and a contiguous last dim");
-  require(zs[0] == sz[0] && zs[1] == sz[1] && zs[2] == sz[2] && zs[3] == D / 32 && vs.sizes() == zs && vs.strides() == ts,
+  require(zs[0] == sz[0] && zs[1] == sz[1] && zs[2] == sz[2] && zs[3] == D / 32 && alike(ks, vs),
           "scales must be [B, NKV, capacity, D / 32] with equal strides");
   require(ts[3] == 1 && ts[2] == D / 32, "the last two dims of the scales must be contiguous");
   for (int i = 0; i < 4; ++i) require(sz[i] <= INT32_MAX / 2, "the 4-bit cache is too large");
@@ -412,7 +421,7 @@ PyObject* tracked(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 void check_kv(const at::Tensor& k, const at::Tensor& v, const bz_kv4_cache& c, const at::Device& dev) {
   require(k.scalar_type() == at::kBFloat16 && v.scalar_type() == at::kBFloat16 && k.device() == dev && v.device() == dev,
           "k and v must be bf16 on the cache's device");
-  require(k.dim() == 4 && v.sizes() == k.sizes() && v.strides() == k.strides() && k.stride(3) == 1,
+  require(k.dim() == 4 && alike(k, v) && k.stride(3) == 1,
           "k and v must be [B, NKV, T, D] with equal shapes and strides and a contiguous last dim");
   if (k.size(0) != c.batch || k.size(1) != c.num_kv_heads || k.size(3) != c.head_dim)
     throw Error{"k " + shape_str(k) + " does not match a cache of batch " + std::to_string(c.batch) + ", " +

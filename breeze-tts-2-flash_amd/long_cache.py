@@ -123,8 +123,8 @@ def gqa_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, se
 
 def kv4_store(k: torch.Tensor, v: torch.Tensor, cache: Kv4Cache, slots: torch.Tensor, *,
               counts: torch.Tensor | None = None) -> Kv4Cache:
-    """Rounds new keys and values into a 4-bit cache (bz_kv4_store). k, v: [B, NKV, T, D] bf16; row b's tokens go to the
-    slots slots[b] .. slots[b] + T - 1 (slots: int32 [B]); with counts (int32 [B]) only the first counts[b] tokens of row b,
+    """Rounds new keys and values into a 4-bit cache (bz_kv4_store). k, v: [B, NKV, T, D] bf16 with equal strides; row b's tokens go to
+    the slots slots[b] .. slots[b] + T - 1 (slots: int32 [B]); with counts (int32 [B]) only the first counts[b] tokens of row b,
     the rest being a batch's padding. Slots outside the cache are skipped. Returns cache."""
     if torch.compiler.is_compiling():
         torch.ops.bz.kv4_store(k, v, *cache, slots, counts)

@@ -80,6 +80,30 @@ def test_kv4_cache_in_one_tensor(device, D):
     assert all(torch.equal(a, b) for a, b in zip(both.unbind(2), pkg.kv4_load(plain, slots, T)))
 
 
+def test_kv4_store_of_one_token(device):
+    """Keys [B, NKV, 1, D] beside values that are a view of [B, 1, NKV, D], as a rotated key and a projection's value are: the
+    step between tokens differs and is not used. Of two tokens it is, and K and V share it."""
+    rng = np.random.default_rng(6)
+    B, NKV, D, cap = 2, 4, 128, 30
+    k, v, slots = randn(rng, B, NKV, 1, D).to(device), randn(rng, B, 1, NKV, D).to(device).transpose(1, 2), ints([3, 29], device)
+    k = torch.as_strided(k, k.shape, (NKV * D, D, D, 1))
+    v = torch.as_strided(v, v.shape, (NKV * D, D, NKV * D, 1))
+    a, b = (pkg.kv4_store(k, x, pkg.kv4_cache(B, NKV, cap, D, device), slots) for x in (v, v.contiguous()))
+    assert all(torch.equal(x, y) for x, y in zip(a, b)) and b.v.any()
+    two = randn(rng, B, 2, NKV, D).to(device).transpose(1, 2)
+    with pytest.raises(RuntimeError):
+        pkg.kv4_store(two.contiguous(), two, a, slots)
+
+
+def test_window_of_one_row(device):
+    """One row's caches, whose steps between rows differ."""
+    rng = np.random.default_rng(7)
+    q, k, v = (randn(rng, *s).to(device) for s in ((1, 4, 128), (1, 2, 50, 128), (1, 2, 50, 128)))
+    lens = ints([50], device)
+    want = pkg.gqa_window(q, k, v, lens, 0.1, 20)
+    assert torch.equal(pkg.gqa_window(q, k, torch.as_strided(v, v.shape, (8, 50 * 128, 128, 1)), lens, 0.1, 20), want)
+
+
 # ------------------------------------------------------------------------------------------------- eviction
 
 @pytest.mark.parametrize("shape", ["2bhs", "b2hs", "bh2s", "bsh2"])
