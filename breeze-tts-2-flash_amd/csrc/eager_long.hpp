@@ -170,12 +170,16 @@ at::Device fill_kv4(PyObject* const* t, bz_kv4_cache& c) {
 }
 
 // 0 for calls of few units, whose counters have one room for all; 1 for the chunks of bz_gqa_window beyond (more units than the
-// device has CUs: the chunk kernel, which has no counters and writes what it reads); else the units.
+// device has CUs: the chunk kernel, which has no counters and writes what it reads); else the room, a power of two of units.
 int64_t sharing_of(int kind, const bz_gqa_decode_args& a) {
   const int64_t group = a.num_q_heads / std::max(a.num_kv_heads, 1), T = a.tokens_per_row;
   const int64_t tpt = std::min<int64_t>(T, 16 / std::max<int64_t>(std::min<int64_t>(group, 16), 1)), tiles = (T + tpt - 1) / tpt;
   const int64_t units = a.batch * tiles * a.num_kv_heads;
-  return units <= BZ_LONG_SHARED_UNITS ? 0 : kind == BZ_LONG_WINDOW && tiles > 1 ? 1 : units;
+  if (units <= BZ_LONG_SHARED_UNITS) return 0;
+  if (kind == BZ_LONG_WINDOW && tiles > 1) return 1;
+  int64_t room = BZ_LONG_SHARED_UNITS;
+  while (room < units) room *= 2;
+  return room;
 }
 
 // The workspace of an attention call into a; true if there is one or none is needed. Otherwise `need` is the tuple the

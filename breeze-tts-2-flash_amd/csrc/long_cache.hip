@@ -69,8 +69,11 @@ int make_plan(int kind, int B, int NH, int NKV, int D, int cap, int T, int windo
   const int64_t longest = max_seq_len > 0 && max_seq_len < cap ? max_seq_len : cap;
   auto attended = [&](int64_t tokens) { return window > 0 ? std::min(longest, (int64_t)window + tokens + sinks) : longest; };
 
-  // the counters' room, the same for all calls of at most kCounterLines units, so that they can share a workspace
-  const size_t counters = (size_t)std::max<int64_t>(pl->units, kCounterLines) * kCounterStride * sizeof(int);
+  // the counters' room: a power of two of lines, at least kCounterLines, so that all calls of one room can share a workspace and a
+  // server's batches, whatever their sizes, need a few (exact, every batch of more than 64 rows of 8 kv heads had its own)
+  int64_t lines = kCounterLines;
+  while (lines < pl->units) lines *= 2;
+  const size_t counters = (size_t)lines * kCounterStride * sizeof(int);
   pl->prefill = pl->balanced = false;
   if (kind == BZ_LONG_WINDOW && pl->tiles > 1) {
     auto tiles = [&](int cg) { return ((int64_t)T * pl->G + kPreWaveCols * cg - 1) / (kPreWaveCols * cg); };

@@ -56,8 +56,9 @@ def _bytes(idx: int, kind: int, B: int, NH: int, NKV: int, D: int, cap: int, T: 
 
 def _make_workspace(need) -> None:
     """Makes and registers the workspace that the native binding asked for: need = (device index, raw stream handle, kind,
-    sharing, bytes). One serves calls of all sizes (but for batches of more than 512 units). Grown, never shrunk; replaced ones are kept for graphs that may hold them, as
-    attention.get_workspace keeps its own."""
+    sharing, bytes). One serves calls of all sizes of up to 512 units, another those of up to 1024, and so on (bz_long_cache.h).
+    Grown, never shrunk. A replaced one is kept: it was allocated on a stream of its own, and calls on this one may still be at
+    work in it."""
     key, n = need[:4], need[4]
     with attention._WS_LOCK:
         ws = _WS.get(key)
@@ -123,9 +124,9 @@ def gqa_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, se
 
 def kv4_store(k: torch.Tensor, v: torch.Tensor, cache: Kv4Cache, slots: torch.Tensor, *,
               counts: torch.Tensor | None = None) -> Kv4Cache:
-    """Rounds new keys and values into a 4-bit cache (bz_kv4_store). k, v: [B, NKV, T, D] bf16 with equal strides; row b's tokens go to
-    the slots slots[b] .. slots[b] + T - 1 (slots: int32 [B]); with counts (int32 [B]) only the first counts[b] tokens of row b,
-    the rest being a batch's padding. Slots outside the cache are skipped. Returns cache."""
+    """Rounds new keys and values into a 4-bit cache (bz_kv4_store). k, v: [B, NKV, T, D] bf16 with equal strides; row b's
+    tokens go to the slots slots[b] .. slots[b] + T - 1 (slots: int32 [B]); with counts (int32 [B]) only the first counts[b]
+    tokens of row b, the rest being a batch's padding. Slots outside the cache are skipped. Returns cache."""
     if torch.compiler.is_compiling():
         torch.ops.bz.kv4_store(k, v, *cache, slots, counts)
         return cache

@@ -88,10 +88,10 @@ typedef struct bz_gqa_tracked_args {
 int bz_gqa_decode_tracked(const bz_gqa_tracked_args* args, hipStream_t stream);
 
 /* Workspace bytes of the three attention entry points above (0 where none is needed); a workspace is zero-filled once,
-   256-byte aligned, and serves every later call of any of them that it is large enough for, with the same batch, heads and
-   tokens per row or if both have at most BZ_LONG_SHARED_UNITS units: batch * num_kv_heads * the column tiles of a row
-   (tokens_per_row over 16 / group, at most tokens_per_row, rounded up). Two calls that share one must be ordered on one
-   stream. */
+   256-byte aligned, and serves every later call of any of them that it is large enough for and that has as many units once
+   those are rounded up to a power of two, at least BZ_LONG_SHARED_UNITS (units: batch * num_kv_heads * the column tiles of
+   a row, tokens_per_row over 16 / group, at most tokens_per_row, rounded up). Two calls that share one must be ordered on
+   one stream. */
 #define BZ_LONG_SHARED_UNITS 512
 typedef enum bz_long_kind { BZ_LONG_WINDOW = 0, BZ_LONG_KV4 = 1, BZ_LONG_TRACKED = 2 } bz_long_kind;
 int bz_long_workspace_size(int32_t kind, int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,

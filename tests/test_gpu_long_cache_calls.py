@@ -143,3 +143,37 @@ def test_evict_refuses_weights_among_the_tensors(device):
     # read by the selection and moved to another place, it is a tensor like any other
     index, _ = pkg.kv_evict((w[..., None],), w, lens, 16, outs=(other[..., None],), weights_out=torch.zeros_like(w))
     assert torch.equal(other[..., :16], held.gather(2, index.long())) and torch.equal(w, held)
+
+
+# ---------------------------------------------------------------------------------------------- workspaces
+
+def test_batches_of_many_sizes_keep_few_workspaces(device):
+    """A stream whose batch moves, with more than 512 units: one workspace a kind up to 1024, every result the row's own."""
+    from breeze_tts_2_flash_amd import long_cache
+    rng = np.random.default_rng(8)
+    NKV, G, D, cap, most = 8, 1, 64, 200, 130
+    q, k, v = (randn(rng, *s).to(device) for s in ((most, NKV * G, D), (most, NKV, cap, D), (most, NKV, cap, D)))
+    w = torch.rand(most, NKV, cap, device=device)
+    lens = ints([cap - b % 50 for b in range(most)], device)
+    cache = pkg.kv4_store(k, v, pkg.kv4_cache(most, NKV, cap, D, device), ints([0] * most, device))
+
+    def step(B, splits):
+        wo = torch.zeros_like(w[:B])
+        c = pkg.Kv4Cache(*(t[:B] for t in cache))
+        return (pkg.gqa_window(q[:B], k[:B], v[:B], lens[:B], 0.1, 0, num_splits=splits),
+                pkg.gqa_decode_kv4(q[:B], c, lens[:B], 0.1, num_splits=splits),
+                pkg.gqa_decode_tracked(q[:B], k[:B], v[:B], lens[:B], 0.1, w[:B], weights_out=wo, num_splits=splits), wo)
+
+    want = step(64, 3)  # 512 units
+    ref, spread, reach = window_attention(q[:64].float().cpu()[:, :, None], k[:64].float().cpu(), v[:64].float().cpu(),
+                                          lens[:64].tolist(), 0.1)
+    assert (np.abs(want[0].float().cpu().numpy() - ref[:, 0]) <= attention_bound(ref, spread, reach, 0.1, D)[:, 0]).all()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for B in (65, 100, 128, 66, 127, 64, 130, 90):
+            for got, x in zip(step(B, 3), want):
+                assert torch.equal(got[:64], x), B
+    side.synchronize()
+    keys = [key for key in long_cache._WS if key[1] == side.cuda_stream]
+    assert len(keys) == 9, keys  # up to 512, 1024 and 2048 units of each kind

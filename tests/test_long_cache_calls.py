@@ -1,4 +1,5 @@
 """The long-cache calls' host checks on the CPU, where they need no device tensors."""
+import ctypes
 import random
 
 import pytest
@@ -63,3 +64,29 @@ def test_apart_against_brute_force(eager):
             assert apart != meet, (views[0].shape, views[1].shape)
         shared += meet
     assert 100 < shared < 1400
+
+
+@pytest.mark.parametrize("kind,T", [(0, 1), (1, 1), (1, 16), (2, 1)])
+def test_workspaces_of_large_batches_have_one_layout(pkg, kind, T):
+    """The counters take a power of two of lines, so that batches of many sizes can use one workspace."""
+    lib, n = pkg.load(), ctypes.c_size_t(0)
+
+    def size(B, splits):
+        assert lib.bz_long_workspace_size(kind, B, 16, 8, 128, 4096, T, 0, 0, splits, 0, ctypes.byref(n)) == 0
+        return n.value
+
+    up = lambda x: (x + 255) // 256 * 256  # noqa: E731
+    columns = 2 * T  # of a (row, kv head), by two q heads
+    tiles = -(-T // 8)
+    for units in (8, 64, 512, 520, 528, 1016, 1024, 1032, 2048, 4000):
+        B = units // 8 // tiles
+        if B == 0:
+            continue
+        lines = 512
+        while lines < B * 8 * tiles:
+            lines *= 2
+        cols = B * 8 * columns * 2
+        want = up(up(lines * 256 + cols * 8) + cols * 128 * 4)
+        if kind == 2:
+            want = up(want + B * 16 * 8) + B * 16 * 4096 * 4
+        assert size(B, 2) == want, units
