@@ -5,7 +5,7 @@
 // its G heads); with 2 x 2 and 1 x 4 a small chunk has more workgroups and fewer steps, each position group taking every
 // PG-th tile, and the groups' accumulators are merged through LDS at the end by the log-sum-exp rule.
 //
-// A workgroup walks the positions any of its tokens attends (the sinks' tiles, then the window's; tile_range) in tiles of 64
+// A workgroup walks the positions any of its tokens attends (the sinks' tiles, then the window's; pre_range) in tiles of 64
 // (PG = 1) or 32 positions staged in LDS, two buffers each of K and V per position group, the next loads in flight while a
 // tile is worked on.
 //   S^T = K Q^T   mfma 32x32x16: A = K rows, B = Q^T (registers, loaded once). A lane then holds 32 scores of one column, the
@@ -43,19 +43,36 @@ struct PreLds {
   static __device__ __forceinline__ int v_swz(int r) { return D == 128 ? 2 * (r & 7) : 2 * ((r >> 1) & 3); }
 };
 
-// Loads the TP rows from pos0 on (clamped to [first, last]: a row outside holds a copy of the nearest, and no column attends it;
-// what lies there, such as NaN in memory that nothing has written, is not read) into
+// The tiles of TP positions that hold every position some column of a workgroup attends: na from position fa on, of the sinks,
+// [fa, a1), and nb from fb on, of the window, up to e1; where sinks and window touch, nb of both. They begin with what is attended,
+// aligned to nothing, and their rows past a1 or e1 are not read (stage_tile): what no column attends, such as NaN or infinities
+// in memory that nothing has written or that was given up between the sinks and the window, would as a factor of 0 send every
+// column to careful_column (1024 tokens, 8 kv heads, G 2, window 1000 behind 5 sinks with NaN between them: 5749 us, 41
+// without). e0 and e1: the ends of the workgroup's first and last token.
+struct PreRange {
+  int fa, a1, na, fb, nb;
+};
+template <int TP>
+__device__ __forceinline__ PreRange pre_range(int s, int e0, int e1, int window, int sinks) {
+  if (e1 <= s) return {s, s, 0, s, 0};
+  PreRange t{s, s + min(sinks, e1 - s), 0, max(s, e0 - window), 0};
+  if (t.a1 >= t.fb) t.fb = s;
+  else t.na = (t.a1 - s + TP - 1) / TP;
+  t.nb = (e1 - t.fb + TP - 1) / TP;
+  return t;
+}
+
+// Loads the TP rows from pos0 on (a row past `last` holds a copy of that one, and no column attends it) into
 // LDS at base, by CG waves (this one is cg): 64 lanes write 1 KB in lane order, so the swizzle is in which chunk each lane
 // fetches.
 template <int D, int TP, int CG, bool V>
-__device__ __forceinline__ void stage_tile(char* base, const Rsrc& rsrc, int pos0, int first, int last, uint32_t row_bytes, int cg,
-                                           int lane) {
+__device__ __forceinline__ void stage_tile(char* base, const Rsrc& rsrc, int pos0, int last, uint32_t row_bytes, int cg, int lane) {
   using L = PreLds<D, TP>;
   constexpr int RPI = 1024 / L::kRow, CH = D / 8;  // rows an instruction, chunks a row
 #pragma unroll
   for (int u = 0; u < L::kBytes / 1024 / CG; ++u) {
     const int row0 = RPI * (cg * (L::kBytes / 1024 / CG) + u), row = row0 + lane / CH, c = lane % CH;
-    const uint32_t off = (uint32_t)clamp_int(pos0 + row, first, last) * row_bytes + 16 * (c ^ (V ? L::v_swz(row) : L::k_swz(row)));
+    const uint32_t off = (uint32_t)min(pos0 + row, last) * row_bytes + 16 * (c ^ (V ? L::v_swz(row) : L::k_swz(row)));
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(base + row0 * L::kRow), 16, off, 0, 0,
                                              0);
   }
@@ -124,7 +141,7 @@ struct PreCut {
   int n, per, nact;
 };
 template <int TP, int PG>
-__device__ __forceinline__ PreCut cut_steps(const TileRange& tr, int splits) {
+__device__ __forceinline__ PreCut cut_steps(const PreRange& tr, int splits) {
   const int n = (tr.na + tr.nb + PG - 1) / PG, per = splits == 1 ? max(n, 1) : max((n + splits - 1) / splits, kPreMinSteps);
   return {n, per, max((n + per - 1) / per, 1)};
 }
@@ -160,15 +177,17 @@ __global__ void __launch_bounds__(kPreThreads, 2)
   auto token_end = [&](int t) { return max(s, e - (p.T - 1 - t)); };
   const Reach me = reach_of(s, token_end(tok), p.window, p.sinks);
   const int e1 = token_end(t0 + ntok - 1);
-  const TileRange tr = tile_range<TP>(s, token_end(t0), e1, p.window, p.sinks);
+  const PreRange tr = pre_range<TP>(s, token_end(t0), e1, p.window, p.sinks);
   const PreCut cut = cut_steps<TP, PG>(tr, SPLIT ? p.splits : 1);
   const int j0 = SPLIT ? split * cut.per : 0;
   if (SPLIT && split > 0 && j0 >= cut.n) return;
   const int n = SPLIT ? min(cut.per, cut.n - j0) : cut.n;  // steps; position group pg takes tile PG (j0 + j) + pg in step j
+  auto of_sinks = [&](int j) { return PG * (j0 + j) + pg < tr.na; };
   auto pos_of = [&](int j) {  // (a tile past the last begins at or past e1: nothing there is attended)
     const int i = PG * (j0 + j) + pg;
     return i < tr.na ? tr.fa + TP * i : tr.fb + TP * (i - tr.na);
   };
+  auto last_of = [&](int j) { return (of_sinks(j) ? tr.a1 : e1) - 1; };
   // every column of the wave attends the whole of [whole_lo, whole_end)
   const int whole_end = token_end(t0 + min((kPreWaveCols * cg) >> p.gshift, ntok - 1));
   const int whole_lo = max(s, token_end(t0 + min((kPreWaveCols * cg + kPreWaveCols - 1) >> p.gshift, ntok - 1)) - p.window);
@@ -224,15 +243,16 @@ __global__ void __launch_bounds__(kPreThreads, 2)
 #pragma unroll
     for (int i = 0; i < KA; ++i) kf[i] = k_read(kbuf, i);
     __builtin_amdgcn_sched_barrier(0);
-    if (j + 2 < n) stage_tile<D, TP, CG, false>((kOdd ? k_odd : k_even) + group, rk, pos_of(j + 2), s, e1 - 1, row_bytes, cg, lane);
-    if (j + 1 < n) stage_tile<D, TP, CG, true>((kOdd ? v_even : v_odd) + group, rv, pos_of(j + 1), s, e1 - 1, row_bytes, cg, lane);
+    if (j + 2 < n) stage_tile<D, TP, CG, false>((kOdd ? k_odd : k_even) + group, rk, pos_of(j + 2), last_of(j + 2), row_bytes, cg, lane);
+    if (j + 1 < n) stage_tile<D, TP, CG, true>((kOdd ? v_even : v_odd) + group, rv, pos_of(j + 1), last_of(j + 1), row_bytes, cg, lane);
     const int p0 = pos_of(j);
     if (!(p0 + TP <= whole_end && p0 >= whole_lo)) {
+      const Reach part{me.lo, of_sinks(j) ? 0 : me.len, me.sink};  // a sinks' tile may end in the window, whose tiles have that
 #pragma unroll
       for (int u = 0; u < NB; ++u)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          x[u][i] = attends(me, s, p0 + 32 * u + 8 * (i / 4) + 4 * half + i % 4) ? x[u][i] : -INFINITY;
+          x[u][i] = attends(part, s, p0 + 32 * u + 8 * (i / 4) + 4 * half + i % 4) ? x[u][i] : -INFINITY;
     }
     float top = x[0][0];
 #pragma unroll
@@ -281,11 +301,11 @@ __global__ void __launch_bounds__(kPreThreads, 2)
     }
   };
   if (n > 0) {
-    stage_tile<D, TP, CG, false>(k_even + group, rk, pos_of(0), s, e1 - 1, row_bytes, cg, lane);
+    stage_tile<D, TP, CG, false>(k_even + group, rk, pos_of(0), last_of(0), row_bytes, cg, lane);
     __builtin_amdgcn_s_waitcnt(0x0f70);
     if constexpr (CG > 1) __syncthreads();
-    if (n > 1) stage_tile<D, TP, CG, false>(k_odd + group, rk, pos_of(1), s, e1 - 1, row_bytes, cg, lane);
-    stage_tile<D, TP, CG, true>(v_even + group, rv, pos_of(0), s, e1 - 1, row_bytes, cg, lane);
+    if (n > 1) stage_tile<D, TP, CG, false>(k_odd + group, rk, pos_of(1), last_of(1), row_bytes, cg, lane);
+    stage_tile<D, TP, CG, true>(v_even + group, rv, pos_of(0), last_of(0), row_bytes, cg, lane);
     f32x16_t xa[NB], xb[NB];
 #pragma unroll
     for (int i = 0; i < NK; ++i)
@@ -385,7 +405,7 @@ __global__ void __launch_bounds__(kPreThreads) window_merge_kernel(const int32_t
   long_range(lens[b], (starts ? starts : lens)[b], starts != nullptr, p.cap, s, e);
   auto token_end = [&](int t) { return max(s, e - (p.T - 1 - t)); };
   const int tile = col / kCols, t0 = tile * (kCols >> p.gshift), last = min(t0 + (kCols >> p.gshift), p.T) - 1;
-  const PreCut cut = cut_steps<TP, 1>(tile_range<TP>(s, token_end(t0), token_end(last), p.window, p.sinks), p.splits);
+  const PreCut cut = cut_steps<TP, 1>(pre_range<TP>(s, token_end(t0), token_end(last), p.window, p.sinks), p.splits);
   if (cut.nact == 1) return;  // its one split has written them
   const int64_t part = (((int64_t)b * p.tiles + tile) * p.NKV + h) * p.splits * kCols + col % kCols;
   float m = -INFINITY, l = 0.f, acc[DV] = {};

@@ -44,6 +44,28 @@ def test_scale_that_is_nan(device, T, NKV, G, splits):
         assert (out[1, :T - T // 2] == 0).all() and torch.isnan(out[1, T - T // 2:]).all()
 
 
+@pytest.mark.parametrize("T,NKV,G,D,n,start,window,sinks", [
+    (333, 4, 4, 64, 1501, 7, 777, 5), (200, 8, 4, 128, 300, 0, 90, 5), (200, 8, 4, 64, 300, 3, 60, 37), (250, 8, 2, 128, 900, 0, 500, 0),
+    (130, 32, 8, 128, 500, 2, 100, 66), (200, 16, 8, 64, 700, 0, 33, 130), (800, 64, 2, 128, 1300, 1, 200, 4),
+    (800, 64, 2, 64, 1100, 0, 222, 64),
+])
+@pytest.mark.parametrize("splits", [0, 3])
+@pytest.mark.parametrize("value", [float("nan"), float("-inf")])
+def test_positions_given_up_cost_a_chunk_nothing(device, T, NKV, G, D, n, start, window, sinks, splits, value):
+    """What lies where no token looks (between the sinks and the window too) changes no bit of a chunk's output: it enters no
+    product, and no column is worked out anew because of it."""
+    from oracle.long_cache import attended
+    rng = np.random.default_rng(T + n)
+    q, k, v = (randn(rng, *s).to(device) for s in ((1, NKV * G, T, D), (1, NKV, n + 30, D), (1, NKV, n + 30, D)))
+    args = dict(sinks=sinks, kv_start=ints([start], device), num_splits=splits)
+    want = pkg.gqa_window(q, k, v, ints([n], device), D ** -0.5, window, **args)
+    seen = set().union(*map(set, attended(start, n, T, window, sinks)))
+    out = [p for p in range(n + 30) if p not in seen]
+    assert any(start + sinks <= p < n for p in out)
+    k[:, :, out], v[:, :, out] = value, value
+    assert torch.equal(pkg.gqa_window(q, k, v, ints([n], device), D ** -0.5, window, **args), want)
+
+
 # --------------------------------------------------------------------------------------------------- 4 bits
 
 def test_kv4_refuses_overlaps(device):
