@@ -8,8 +8,10 @@
  * Range rule. Row b holds positions [kv_start[b], seq_lens[b]) (clamped as in bz_gqa_decode). With T query tokens per
  * row, token t is the row's position seq_lens[b] - T + t and ends at e_t = max(kv_start[b], seq_lens[b] - (T - 1 - t)).
  * It attends the positions p of [kv_start[b], e_t) with window == 0, p >= e_t - window, or p < kv_start[b] + sinks: the
- * last `window` positions up to its own, and the row's first `sinks`. A token that attends nothing yields zeros. What is
- * stored at positions a token does not attend (NaN and infinities among it) does not reach its output.
+ * last `window` positions up to its own, and the row's first `sinks`. A token that attends nothing, or whose scores are all
+ * -inf, yields zeros, as in bz_gqa_decode. What is stored at positions a token does not attend (NaN and infinities among it)
+ * does not reach its output. Outputs are sums in fp32 of terms of up to 2^8 times V, divided by the terms' sum at the end: the sum
+ * of |V| over the positions a token attends must stay below 2^119.
  */
 #ifndef BZ_LONG_CACHE_H
 #define BZ_LONG_CACHE_H

@@ -44,6 +44,38 @@ def test_scale_that_is_nan(device, T, NKV, G, splits):
         assert (out[1, :T - T // 2] == 0).all() and torch.isnan(out[1, T - T // 2:]).all()
 
 
+@pytest.mark.parametrize("T,NKV,G,D", [(1, 2, 2, 128), (6, 1, 4, 64), (70, 8, 8, 64), (300, 8, 2, 128)])
+@pytest.mark.parametrize("splits", [0, 4])
+def test_scores_of_minus_infinity(device, T, NKV, G, D, splits):
+    """Zeros where all a token attends scores -inf, and nothing of such a position where others score more."""
+    rng = np.random.default_rng(T)
+    n, window = T + 300, 90
+    q, k, v = randn(rng, 1, NKV * G, T, D), randn(rng, 1, NKV, n, D), randn(rng, 1, NKV, n, D)
+    q[..., 0], k[..., 0] = 1, 0
+    clean = k.clone()
+    half = n - T // 2 - 1  # the first tokens attend only positions before it
+    k[:, :, :half, 0] = float("-inf")
+    args = (ints([n], device), D ** -0.5, window)
+    out = pkg.gqa_window(q.to(device), k.to(device), v.to(device), *args, num_splits=splits).view(T, NKV * G, D)
+    end = n - T + 1 + torch.arange(T)
+    none = end <= half
+    assert none.any() or T == 1
+    assert (out[none.to(device)] == 0).all() and (out[~none.to(device)] != 0).any(-1).all()
+    # the others: as if the row began at `half`
+    ref, spread, reach = window_attention(q.float(), clean.float(), v.float(), [n], D ** -0.5, window, 0, [half])
+    late = (~none).numpy()
+    excess = np.abs(out.float().cpu().numpy() - ref[0]) - attention_bound(ref, spread, reach, D ** -0.5, D, T > 16)[0]
+    assert excess[late].max() <= 0
+    if T == 1:
+        k[..., 0] = float("-inf")
+        kd, w = k.to(device), torch.rand(1, NKV, n, device=device)
+        held = w.clone()
+        for out in (pkg.gqa_window(q.to(device), kd, v.to(device), *args), pkg.gqa_decode(q[:, :, 0].to(device), kd, v.to(device), *args[:2]),
+                    pkg.gqa_decode_tracked(q[:, :, 0].to(device), kd, v.to(device), *args[:2], w, num_splits=splits)):
+            assert (out == 0).all()
+        assert torch.equal(w, held)
+
+
 @pytest.mark.parametrize("T,NKV,G,D,n,start,window,sinks", [
     (333, 4, 4, 64, 1501, 7, 777, 5), (200, 8, 4, 128, 300, 0, 90, 5), (200, 8, 4, 64, 300, 3, 60, 37), (250, 8, 2, 128, 900, 0, 500, 0),
     (130, 32, 8, 128, 500, 2, 100, 66), (200, 16, 8, 64, 700, 0, 33, 130), (800, 64, 2, 128, 1300, 1, 200, 4),
