@@ -231,3 +231,32 @@ def test_batches_of_many_sizes_keep_few_workspaces(device):
     side.synchronize()
     keys = [key for key in long_cache._WS if key[1] == side.cuda_stream]
     assert len(keys) == 9, keys  # up to 512, 1024 and 2048 units of each kind
+
+
+# ---------------------------------------------------------------------------------------- torch.compile
+
+@pytest.mark.parametrize("fmt", ["bf16", "kv4"])
+def test_compiled_in_place(device, fmt):
+    """The default forms, which write what they read, under torch.compile: outputs and the tensors left as in eager."""
+    rng = np.random.default_rng(10)
+    B, NKV, cap, D, keep = 2, 2, 300, 128, 90
+    q, k, v = (randn(rng, *s).to(device) for s in ((B, 2 * NKV, D), (B, NKV, cap, D), (B, NKV, cap, D)))
+    state = [k, v, torch.rand(B, NKV, cap, device=device), ints([300, 222], device)]
+    if fmt == "kv4":
+        state += pkg.kv4_store(k, v, pkg.kv4_cache(B, NKV, cap, D, device), ints([0, 0], device))
+
+    def step(q, k, v, w, lens, *cache):
+        out = pkg.gqa_decode_tracked(q, k, v, lens, 0.1, w, decay=0.5)
+        index, n = pkg.kv_evict(pkg.Kv4Cache(*cache) if cache else (k, v), w, lens, keep, sinks=3, recent=7)
+        more = pkg.gqa_decode_kv4(q, pkg.Kv4Cache(*cache), n, 0.1) if cache else pkg.gqa_window(q, k, v, n, 0.1, 50)
+        return out, index, n, more
+
+    def chosen(w, lens):
+        return pkg.kv_select(w, lens, keep, sinks=3, weights_out=w, lens=lens)
+
+    for call, first, mutated in ((step, (q,), True), (chosen, (), False)):
+        args = state if mutated else state[2:4]
+        a, b = [t.clone() for t in args], [t.clone() for t in args]
+        want, got = call(*first, *a), torch.compile(call, fullgraph=True)(*first, *b)
+        assert all(torch.equal(x, y) for x, y in zip(want, got)) and all(torch.equal(x, y) for x, y in zip(a, b))
+        assert not torch.equal(a[0], args[0]) or fmt == "kv4"
