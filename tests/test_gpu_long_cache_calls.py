@@ -260,3 +260,39 @@ def test_compiled_in_place(device, fmt):
         want, got = call(*first, *a), torch.compile(call, fullgraph=True)(*first, *b)
         assert all(torch.equal(x, y) for x, y in zip(want, got)) and all(torch.equal(x, y) for x, y in zip(a, b))
         assert not torch.equal(a[0], args[0]) or fmt == "kv4"
+
+
+# ------------------------------------------------------------------------------------- terms, and workspaces shared
+
+@pytest.mark.parametrize("T,NKV,G,D,n,splits", [(64, 2, 2, 128, 150, 0), (37, 1, 4, 128, 700, 0), (50, 2, 1, 64, 900, 3), (130, 1, 2, 128, 400, 0),
+                                                (100, 1, 2, 64, 2000, 5), (16, 8, 2, 128, 3000, 0), (16, 8, 8, 64, 500, 4)])
+def test_split_kernel_holds_two_terms(device, T, NKV, G, D, n, splits):
+    """Chunks of fewer column tiles than CUs, which the split kernel takes: softmax terms to 2^-17, not to a bf16's 2^-8."""
+    rng = np.random.default_rng(T)
+    q, k, v = randn(rng, 1, NKV * G, T, D), randn(rng, 1, NKV, n, D), randn(rng, 1, NKV, n, D)
+    out = pkg.gqa_window(q.to(device), k.to(device), v.to(device), ints([n], device), D ** -0.5, 90, sinks=3, num_splits=splits)
+    ref, spread, reach = window_attention(q.float(), k.float(), v.float(), [n], D ** -0.5, 90, 3)
+    assert (np.abs(out.float().cpu().numpy() - ref) <= attention_bound(ref, spread, reach, D ** -0.5, D)).all()
+
+
+def test_chunk_splits_share_a_workspace_with_counters(device):
+    """A chunk's splits and decode steps in turn in one workspace: the chunk's sums leave the counters at zero."""
+    rng = np.random.default_rng(11)
+    NKV, G, D, n, T = 8, 2, 128, 5000, 128
+    q, k, v = (randn(rng, *s).to(device) for s in ((1, NKV * G, T, D), (1, NKV, n, D), (1, NKV, n, D)))
+    lens, row = ints([n], device), q[:, :, -1].contiguous()
+    chunk = pkg.long_workspace("window", torch.device("cuda", 0), 1, NKV * G, NKV, D, n, T)
+    step = pkg.long_workspace("window", torch.device("cuda", 0), 1, NKV * G, NKV, D, n, 1, num_splits=9)
+    assert chunk.numel() > step.numel() > 0
+    w = torch.zeros(1, NKV, n, device=device)
+    calls = [lambda ws: pkg.gqa_window(q, k, v, lens, D ** -0.5, 0, workspace=ws),
+             lambda ws: pkg.gqa_window(row, k, v, lens, D ** -0.5, 0, num_splits=9, workspace=ws),
+             lambda ws: pkg.gqa_decode_tracked(row, k, v, lens, D ** -0.5, w, weights_out=torch.zeros_like(w), workspace=ws)]
+    want = [f(None) for f in calls]
+    for i in (0, 1, 0, 2, 1, 0, 2, 0, 1):
+        assert torch.equal(calls[i](chunk), want[i]), i
+    last = window_attention(q[:, :, -1:].float().cpu(), k.float().cpu(), v.float().cpu(), [n], D ** -0.5)
+    excess = np.abs(want[1].float().cpu().numpy() - last[0][:, 0]) - attention_bound(*last, D ** -0.5, D)[:, 0]
+    assert excess.max() <= 0
+    excess = np.abs(want[0][:, -1].float().cpu().numpy() - last[0][:, 0]) - attention_bound(*last, D ** -0.5, D, True)[:, 0]
+    assert excess.max() <= 0
