@@ -211,8 +211,8 @@ __device__ __forceinline__ void fold_scores(LongState<D>& st, float (&x)[N], flo
   }
 }
 
-// The softmax terms as two bf16 terms each, hi + lo (16 bits of each p: an error of 2^-17, below the 2^-9 that the output's
-// own rounding to bf16 costs; one term alone would add as much error again as that rounding).
+// The softmax terms as two bf16 terms each, hi + lo (16 bits of each p: an error of 2^-17 at most, below the 2^-8 that the
+// output's own rounding to bf16 costs at most; one term alone would add as much error again as that rounding).
 template <int N>
 __device__ __forceinline__ void split_terms(const float (&p)[N], uint32_t (&hi)[N / 2], uint32_t (&lo)[N / 2]) {
 #pragma unroll

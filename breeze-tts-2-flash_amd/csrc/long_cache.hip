@@ -131,9 +131,12 @@ int make_plan(int kind, int B, int NH, int NKV, int D, int cap, int T, int windo
   const int n = (int)((len + P - 1) / P) + 1;
   pl->min_tiles = kLongThreads / kWave;
   pl->one_split = (kOneSplitBytes / (kv4 ? D + D / 16 : 4 * D)) / P;
-  // A server's batch: more than three rows whose lengths differ because no window cuts them. Its splits are dealt to the rows by
+  // A server's batch: more than three rows, whose lengths differ because no window cuts them. Its splits are dealt to the rows by
   // their lengths where a split streams long enough for that to show (deal_splits costs about 0.5 us before the first load;
-  // 64 rows: a lane for each).
+  // 64 rows: a lane for each). Two and three rows are taken to be alike, as those of a guidance pair are: dealt they cost a little,
+  // and win where they are not (us, not dealt / dealt, 8 kv heads: 2 rows of 8192 14.5 / 14.7, of 16384 tracked 28.2 / 29.5, of
+  // 20000..32768 of 4 bits, 4 kv heads of 8 q 12.6 / 15.0, of 500..8192 11.5 / 10.6, of 2000..32768 of 4 bits 16.5 / 12.5; 3 rows
+  // of 8192 18.7 / 19.1, of 500..8192 15.3 / 12.9).
   const bool batch = !cut && B > 3;
   const int64_t row_bytes = kv4 ? D + D / 16 : 4 * D;
   auto dealt = [&](int64_t s) { return s > 1 && batch && (int64_t)B * pl->tiles <= kWave && len * row_bytes / s >= kDealBytes; };

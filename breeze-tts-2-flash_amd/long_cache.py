@@ -6,9 +6,10 @@ of the native binding (csrc/eager_long.hpp), which checks the tensors, picks the
 The reference keeps every position of its static cache (third_party/breeze-tts/models/cudagraph/backbone_graph.py:73-75)
 in bf16 and attends all of them (flash/csrc/bb_attn.cu:416-429); these operators bound what a decode step reads instead.
 
-Workspaces: one per device, stream and kind of call, made on first use. A call made while its stream is being captured into
-a HIP graph takes none of those, which graphs would then share: it needs workspace=, made beforehand by long_workspace (one
-serves every call of a graph; the calls that need none are captured without). Errors raise RuntimeError.
+Workspaces: made on first use, for each device, stream and kind of call one for calls of up to 512 units (bz_long_cache.h),
+one up to 1024, and so on. A call made while its stream is being captured into a HIP graph takes none of those, which graphs
+would then share: it needs workspace=, made beforehand by long_workspace (one serves every call of a graph with as many units,
+rounded up so; the calls that need none are captured without). Errors raise RuntimeError.
 """
 from __future__ import annotations
 

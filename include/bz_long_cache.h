@@ -23,9 +23,14 @@ extern "C" {
 #endif
 
 /* Arguments of bz_gqa_window. base: as for bz_gqa_decode, with mask NULL and mask_dtype 0; tokens_per_row T may be one or
-   a whole prompt (at most 2^30); num_splits 0 picks the default; combine is ignored; workspace of at least
-   bz_long_workspace_size(..) bytes where that is not 0. Softmax terms enter the product with V as two bf16 terms (an error
-   of 2^-17 each), over many tokens as one (2^-9). */
+   a whole prompt; num_splits 0 picks the default; combine is ignored; workspace of at least bz_long_workspace_size(..)
+   bytes where that is not 0.
+   Two kernels, by the units of the call (batch * num_kv_heads * the tiles of 16 (token, q head) columns a row has, at most 16
+   / group tokens each). With one tile a row, or fewer units than the device has CUs, the split kernel, unless num_splits is 0,
+   a row has at least 128 columns and the positions are long enough to half fill the device with shares of 128 columns; else the
+   chunk kernel. Softmax terms meet V as two bf16 terms in the split kernel (each off by at most 2^-17 of itself), as
+   one in the chunk kernel (at most 2^-8, as the output's own rounding), where the products are the bound. The chunk kernel
+   takes at most 65535 tiles of 128 columns, times splits, a row (BZ_ERR_SHAPE beyond): about a million tokens with a group of 8. */
 typedef struct bz_gqa_window_args {
   bz_gqa_decode_args base;
   int32_t window;             /* >= 0; 0: no window (plain causal attention) */

@@ -296,3 +296,15 @@ def test_chunk_splits_share_a_workspace_with_counters(device):
     assert excess.max() <= 0
     excess = np.abs(want[0][:, -1].float().cpu().numpy() - last[0][:, 0]) - attention_bound(*last, D ** -0.5, D, True)[:, 0]
     assert excess.max() <= 0
+
+
+def test_longest_chunk(device):
+    """The chunk kernel's grid holds 65535 column tiles: 65535 * 16 tokens of 8 q heads; longer ones are refused, not launched."""
+    dev, size = torch.device("cuda", 0), (1, 8, 1, 64, 1 << 22)
+    assert pkg.long_workspace("window", dev, *size, 65535 * 16, num_splits=1).numel() == 0
+    with pytest.raises(RuntimeError):
+        pkg.long_workspace("window", dev, *size, 65535 * 16 + 1, num_splits=1)
+    q = torch.zeros(1, 8, 1, 64, dtype=BF16, device=device).expand(1, 8, 1 << 20, 64)
+    k = torch.zeros(1, 1, 64, 64, dtype=BF16, device=device)
+    with pytest.raises(RuntimeError):
+        pkg.gqa_window(q, k, k, ints([64], device), 0.1, 0, torch.empty(1, 1 << 20, 8, 64, dtype=BF16, device=device), num_splits=1)
