@@ -59,12 +59,12 @@ typedef struct bz_kv4_cache {
    2^-126) with max |x| / scale <= 7, codes are x / scale rounded to nearest even and saturated at 6; a block that holds NaN
    or an infinity gets scale byte 255. (Values from 1.75 * 2^127 on become 4 * 2^126, which bf16 reads as infinity.) counts,
    optional int32 [batch]: only the first counts[b] tokens of row b are stored. Slots outside [0, capacity) are skipped. k and
-   v share strides. */
+   v share strides; the cache's four tensors share no memory. */
 int bz_kv4_store(const void* k, const void* v, int64_t x_stride_b, int64_t x_stride_h, int64_t x_stride_t, int32_t tokens,
                  const int32_t* slots, const int32_t* counts, const bz_kv4_cache* cache, hipStream_t stream);
 
-/* The bf16 values of slots slots[b] .. slots[b] + tokens - 1 of row b, into k and v (layout as in bz_kv4_store); zeros for
-   slots outside [0, capacity). */
+/* The bf16 values of slots slots[b] .. slots[b] + tokens - 1 of row b, into k and v (layout as in bz_kv4_store; they
+   share no memory); zeros for slots outside [0, capacity). */
 int bz_kv4_load(const bz_kv4_cache* cache, const int32_t* slots, int32_t tokens, void* k, void* v, int64_t x_stride_b,
                 int64_t x_stride_h, int64_t x_stride_t, hipStream_t stream);
 

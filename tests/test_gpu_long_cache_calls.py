@@ -308,3 +308,36 @@ def test_longest_chunk(device):
     k = torch.zeros(1, 1, 64, 64, dtype=BF16, device=device)
     with pytest.raises(RuntimeError):
         pkg.gqa_window(q, k, k, ints([64], device), 0.1, 0, torch.empty(1, 1 << 20, 8, 64, dtype=BF16, device=device), num_splits=1)
+
+
+def test_chunks_captured_and_replayed(device):
+    """A chunk in splits, one whole, a window's and the 4-bit calls in one graph, on lengths and inputs that change between the
+    replays, with eager work between them; every replay as in eager."""
+    rng = np.random.default_rng(12)
+    dev, NKV, G, D, n = torch.device("cuda", 0), 8, 2, 128, 4000
+    q, k, v = (randn(rng, *s).to(device) for s in ((1, NKV * G, 400, D), (1, NKV, n, D), (1, NKV, n, D)))
+    few = q[:, :, :128].contiguous()
+    lens, slot, cache = ints([n], device), ints([0], device), pkg.kv4_cache(1, NKV, 64, D, device)
+    ws = pkg.long_workspace("window", dev, 1, NKV * G, NKV, D, n, 128)
+    assert ws.numel() > 0 and pkg.long_workspace("window", dev, 1, NKV * G, NKV, D, n, 400, window=90).numel() == 0
+
+    def run(ws):
+        pkg.kv4_store(k[:, :, :64], v[:, :, :64], cache, slot)
+        return [pkg.gqa_window(few, k, v, lens, D ** -0.5, 0, workspace=ws), pkg.gqa_window(q, k, v, lens, D ** -0.5, 90, sinks=3),
+                *pkg.kv4_load(cache, slot, 50)]
+
+    run(ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run(ws)
+    for i in range(4):
+        lens.fill_(n - 777 * i)
+        slot.fill_(i)
+        q.copy_(randn(rng, *q.shape))
+        few.copy_(q[:, :, 100:228])
+        graph.replay()
+        torch.cuda.synchronize()
+        held = [t.clone() for t in got]
+        for a, b in zip(held, run(None)):
+            assert torch.equal(a, b), i
