@@ -7,7 +7,8 @@
 // registers it here and launches. Every attention check and error message is the Python path's, so both raise the
 // same RuntimeError for the same arguments. The GEMVs need no workspace and go through this module alone.
 //
-// The long-cache operators (eager_long.hpp) go through it alone as well; Python only makes their workspaces.
+// The long-cache and paged-cache operators (eager_long.hpp, eager_paged.hpp) go through it alone as well; Python only makes their
+// workspaces.
 //
 // The C ABI functions come as addresses (bind), taken from the library the package has already loaded and checked,
 // so this module never loads a second copy of it. Host code only: compiled with g++ against torch's headers.
@@ -634,6 +635,7 @@ PyObject* register_workspace(PyObject*, PyObject* args) {
 }  // namespace
 
 #include "eager_long.hpp"
+#include "eager_paged.hpp"
 
 namespace {
 
@@ -669,15 +671,26 @@ PyMethodDef kMethods[] = {
      "kv_evict through the C ABI"},
     {"apart", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(apart_py)), METH_FASTCALL,
      "whether two tensors share no memory, as the long-cache calls check it"},
+    {"rope", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(rope)), METH_FASTCALL,
+     "rope through the C ABI"},
+    {"paged_store", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(paged_store)), METH_FASTCALL,
+     "paged_store through the C ABI"},
+    {"rope_store", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(rope_store)), METH_FASTCALL,
+     "rope_store through the C ABI"},
+    {"paged_load", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(paged_load)), METH_FASTCALL,
+     "paged_load through the C ABI"},
+    {"paged", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(paged)), METH_FASTCALL,
+     "gqa_paged through the C ABI, or what its missing workspace needs"},
     {"bind", bind, METH_VARARGS, "the C ABI functions' addresses"},
     {"bind_long", bind_long, METH_VARARGS, "the long-cache functions' addresses"},
-    {"register_long_workspace", register_long_workspace, METH_VARARGS, "a workspace made for a long-cache call's key"},
+    {"bind_paged", bind_paged, METH_VARARGS, "the paged-cache functions' addresses"},
+    {"register_long_workspace", register_long_workspace, METH_VARARGS, "a workspace made for a long-cache or paged-cache call's key"},
     {"register_workspace", register_workspace, METH_VARARGS, "a workspace made for (device, stream, groups)"},
     {"build_id", build_id, METH_NOARGS, "hash of the sources this module was built from"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_bz_eager",
-                       "native eager binding of the decode-attention and long-cache entries and the backbone GEMVs", -1, kMethods};
+                       "native eager binding of the decode-attention, long-cache and paged-cache entries and the backbone GEMVs", -1, kMethods};
 
 }  // namespace
 

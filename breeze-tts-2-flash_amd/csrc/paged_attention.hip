@@ -1,0 +1,162 @@
+// Host side of bz_gqa_paged (include/bz_paged_cache.h): argument checks, workspace layout, how the work is dealt, launches. The
+// device code is in paged_split.cuh and paged_chunk.cuh.
+#include <hip/hip_runtime.h>
+
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "bz_paged_cache.h"
+#include "paged_chunk.cuh"
+#include "paged_split.cuh"
+
+namespace bz {
+int device_cu_count(int* cus);  // gqa_decode.hip
+}
+
+namespace {
+
+constexpr int kFewThreads = 256;
+// Workspace: the arrival counters, then (max, sum) pairs and sums of 2 * kSlotsPerCu slots a CU, at places that depend on nothing else, so
+// that calls of all sizes can share one. A kernel's splits of all kv heads number at most kSlotsPerCu a CU, and those of rows that
+// are split at most twice that (deal_paged).
+constexpr int kSlotsPerCu = 2;
+
+size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+struct Layout {
+  int64_t slots;
+  size_t ml, acc, total;
+};
+Layout layout(int cus, int D, int cols) {
+  Layout y;
+  y.slots = (int64_t)2 * kSlotsPerCu * cus;
+  y.ml = (size_t)y.slots * kCounterStride * sizeof(int);
+  y.acc = up256(y.ml + (size_t)y.slots * cols * sizeof(float2));
+  y.total = up256(y.acc + (size_t)y.slots * cols * D * sizeof(float));
+  return y;
+}
+
+bool group_ok(int G) { return G == 1 || G == 2 || G == 4 || G == 8; }
+
+// Rows of more new tokens than this are the chunk kernel's, where there can be any.
+int few_tokens(int G) { return kLongCols / G; }
+
+}  // namespace
+
+#define BZ_EXPORT __attribute__((visibility("default")))
+
+extern "C" {
+
+BZ_EXPORT int bz_paged_workspace_size(int32_t head_dim, int32_t group, int32_t max_tokens, size_t* bytes) {
+  if (bytes == nullptr) return BZ_ERR_NULL;
+  if (max_tokens < 0) return BZ_ERR_SHAPE;
+  if ((head_dim != 64 && head_dim != 128) || !group_ok(group)) return BZ_ERR_UNSUPPORTED;
+  int cus = 0;
+  const int rc = bz::device_cu_count(&cus);
+  if (rc != BZ_OK) return rc;
+  const bool few = max_tokens > 0 && max_tokens <= few_tokens(group);
+  *bytes = layout(cus, head_dim, few ? kLongCols : kChunkCols).total;
+  return BZ_OK;
+}
+
+BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
+  if (a == nullptr || a->q == nullptr || a->out == nullptr) return BZ_ERR_NULL;
+  const bz_paged_cache* c = &a->cache;
+  int rc = bz::check_paged(c, true);
+  if (rc != BZ_OK) return rc;
+  const int NH = a->num_q_heads, NKV = c->num_kv_heads, D = c->head_dim;
+  if (NH <= 0 || NH % NKV != 0 || a->max_tokens < 0 || a->max_seq_len < 0) return BZ_ERR_SHAPE;
+  const int G = NH / NKV;
+  if (!group_ok(G)) return BZ_ERR_UNSUPPORTED;
+  if ((reinterpret_cast<uintptr_t>(a->q) & 15) || ((a->q_stride_t | a->q_stride_h) & 7)) return BZ_ERR_ALIGNMENT;
+  if (reinterpret_cast<uintptr_t>(a->out) & 1) return BZ_ERR_ALIGNMENT;
+  int cus = 0;
+  rc = bz::device_cu_count(&cus);
+  if (rc != BZ_OK) return rc;
+
+  const int64_t N = c->tokens, B = c->batch;
+  const int few = few_tokens(G);
+  // Whether a row can have more tokens than the split kernel takes at once; where the caller says that none has, that kernel takes
+  // whatever comes, several column tiles a row.
+  const bool chunks = c->q_start != nullptr && N > few && !(a->max_tokens > 0 && a->max_tokens <= few);
+  const bool small = !chunks || B > 1 || N <= few;  // (one row of unknown tokens may have few, but then the chunk kernel takes it)
+  const Layout ws = layout(cus, D, chunks ? kChunkCols : kLongCols);
+  if (a->workspace == nullptr || a->workspace_bytes < ws.total) return BZ_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(a->workspace) & 255) return BZ_ERR_ALIGNMENT;
+
+  PagedParams p{};
+  p.rows = bz::paged_rows(c);
+  p.q = static_cast<const uint16_t*>(a->q);
+  p.q_st = a->q_stride_t, p.q_sh = a->q_stride_h;
+  p.out = static_cast<uint16_t*>(a->out);
+  p.o_st = a->out_stride_t, p.o_sh = a->out_stride_h;
+  p.out_wide = !((reinterpret_cast<uintptr_t>(a->out) & 7) || ((p.o_st | p.o_sh) & 3));
+  p.k = static_cast<const char*>(c->k), p.v = static_cast<const char*>(c->v);
+  p.kv_sp = c->stride_page, p.kv_sh = c->stride_h, p.kv_ss = (int)c->stride_s;
+  p.page_bytes = (int)(c->stride_s * (c->page_size - 1)) + (c->bits == 8 ? D : 2 * D);
+  p.ks = static_cast<const uint8_t*>(c->k_scale), p.vs = static_cast<const uint8_t*>(c->v_scale);
+  p.sc_sp = c->scale_stride_page, p.sc_sh = c->scale_stride_h;
+  p.NKV = NKV, p.G = G, p.gshift = __builtin_ctz(G);
+  p.scale_log2 = a->scale * kLog2e;
+  p.part_slots = (int)(ws.slots / NKV);
+  char* const base = static_cast<char*>(a->workspace);
+  p.counters = reinterpret_cast<int*>(base);
+  p.part_ml = reinterpret_cast<float2*>(base + ws.ml);
+  p.part_acc = reinterpret_cast<float*>(base + ws.acc);
+  const bool f8 = c->bits == 8;
+  const int64_t cap = (int64_t)c->max_pages * c->page_size;
+  const int64_t longest = a->max_seq_len > 0 && a->max_seq_len < cap ? a->max_seq_len : cap;
+  using Fn = void (*)(const PagedParams);
+
+  if (chunks) {
+    const int tpt = kChunkCols / G;
+    const int64_t units = N / tpt + B;
+    p.few = small ? few : 0;
+    p.splits = (N / tpt + 1) * NKV < kSlotsPerCu * cus ? kSlotsPerCu * cus / NKV : 0;
+    p.least = kPreMinSteps, p.one_split = kPreMinSteps;
+    const int64_t grid = (units * 2 <= p.splits ? p.splits : p.splits + units) * NKV;
+    const int64_t merge_grid = units * NKV * (kChunkCols / kMergeCols);
+    if (grid > kMaxGrid || merge_grid > kMaxGrid) return BZ_ERR_SHAPE;
+    const Fn fns[2][2] = {{paged_chunk_kernel<64, false>, paged_chunk_kernel<64, true>},
+                          {paged_chunk_kernel<128, false>, paged_chunk_kernel<128, true>}};
+    const Fn merges[2][2] = {{paged_merge_kernel<64, false>, paged_merge_kernel<64, true>},
+                             {paged_merge_kernel<128, false>, paged_merge_kernel<128, true>}};
+    hipLaunchKernelGGL(fns[D == 128][f8], dim3((unsigned)grid), dim3(kPreThreads), 0, stream, p);
+    if (hipGetLastError() != hipSuccess) return BZ_ERR_LAUNCH;
+    if (p.splits > 0) {
+      hipLaunchKernelGGL(merges[D == 128][f8], dim3((unsigned)merge_grid), dim3(kPreThreads), 0, stream, p);
+      if (hipGetLastError() != hipSuccess) return BZ_ERR_LAUNCH;
+    }
+    if (!small) return BZ_OK;
+  }
+
+  // rows of few tokens (all of them, if there are no others)
+  const int P = f8 ? 32 : 16, row_bytes = f8 ? 2 * D + 2 : 4 * D;
+  const int64_t n = (longest + P - 1) / P;
+  p.few = chunks ? few : INT32_MAX;
+  p.least = kFewThreads / kWave;
+  p.one_split = kOneSplitBytes / row_bytes / P;
+  const int64_t round = std::max<int64_t>(cus / NKV, 1);
+  const bool alike = c->q_start == nullptr && B <= 3;
+  int64_t grid;
+  if (alike) {
+    const int64_t most = (n + p.least - 1) / p.least;
+    p.splits = n <= p.one_split ? 1 : (int)std::max<int64_t>(std::min({round / B, most, (int64_t)64}), 1);
+    grid = B * p.splits * NKV;
+  } else {
+    const int tpt = kLongCols / G;
+    const int64_t units = N / tpt + B;
+    p.splits = n <= p.one_split ? 0 : (int)std::max<int64_t>(kSlotsPerCu * cus / NKV, 1);
+    grid = (units * 2 <= p.splits ? p.splits : p.splits + units) * NKV;
+  }
+  if (grid > kMaxGrid) return BZ_ERR_SHAPE;
+  const Fn fns[2][2][2] = {{{paged_split_kernel<64, false, false, kFewThreads>, paged_split_kernel<64, false, true, kFewThreads>},
+                            {paged_split_kernel<64, true, false, kFewThreads>, paged_split_kernel<64, true, true, kFewThreads>}},
+                           {{paged_split_kernel<128, false, false, kFewThreads>, paged_split_kernel<128, false, true, kFewThreads>},
+                            {paged_split_kernel<128, true, false, kFewThreads>, paged_split_kernel<128, true, true, kFewThreads>}}};
+  hipLaunchKernelGGL(fns[D == 128][f8][!alike], dim3((unsigned)grid), dim3(kFewThreads), 0, stream, p);
+  return hipGetLastError() == hipSuccess ? BZ_OK : BZ_ERR_LAUNCH;
+}
+
+}  // extern "C"

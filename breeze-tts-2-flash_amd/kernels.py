@@ -24,8 +24,9 @@ INCLUDE = REPO_DIR / "include"
 LIB_NAME = "libbz_gqa_decode.so"
 LIB_PATH = PKG_DIR / LIB_NAME
 SOURCES = ["gqa_decode.hip", "gqa_fused.hip", "gemv.hip", "long_cache.hip", "kv4_store.hip",
-           "kv_evict.hip"]  # translation units, compiled in parallel
-HEADERS = ["gqa_kernels.cuh", "gqa_wave.cuh", "device_common.cuh", "long_cache.cuh", "window_prefill.cuh"]
+           "kv_evict.hip", "paged_store.hip", "paged_attention.hip"]  # translation units, compiled in parallel
+HEADERS = ["gqa_kernels.cuh", "gqa_wave.cuh", "device_common.cuh", "long_cache.cuh", "window_prefill.cuh", "paged_common.cuh",
+           "paged_split.cuh", "paged_chunk.cuh"]
 ARCH = "gfx950"
 # -packed-fp32-ops: keep hipcc from emitting packed fp32 VALU ops (v_pk_*_f32)
 # -falign-loops=64: loop heads on 64-byte boundaries (instruction fetch); the split kernels measured 1-4% faster with
@@ -39,7 +40,7 @@ HIPCC_FLAGS = [
     "-mllvm", "-amdgpu-kernarg-preload-count=14",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 # exported symbols and their ctypes signatures (include/*.h)
 EXPORTS = (
@@ -47,7 +48,8 @@ EXPORTS = (
     "bz_gqa_decode_default_splits", "bz_status_string", "bz_gqa_decode_abi_version", "bz_gemv", "bz_rmsnorm",
     "bz_mask_interval", "bz_gqa_decode_wave", "bz_gqa_decode_build_id", "bz_gqa_decode_noalloc",
     "bz_gqa_decode_probs", "bz_gqa_decode_fused_probs", "bz_gqa_window", "bz_gqa_decode_kv4", "bz_gqa_decode_tracked",
-    "bz_long_workspace_size", "bz_kv4_store", "bz_kv4_load", "bz_kv_select", "bz_kv_compact",
+    "bz_long_workspace_size", "bz_kv4_store", "bz_kv4_load", "bz_kv_select", "bz_kv_compact", "bz_rope_apply", "bz_paged_store",
+    "bz_paged_load", "bz_gqa_paged", "bz_paged_workspace_size",
 )
 
 
@@ -171,6 +173,66 @@ KV_TENSORS = 4  # BZ_KV_TENSORS
 LONG_WINDOW, LONG_KV4, LONG_TRACKED = 0, 1, 2
 
 
+class PagedCacheArgs(ctypes.Structure):
+    """Mirror of struct bz_paged_cache (include/bz_paged_cache.h)."""
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("stride_page", ctypes.c_int64), ("stride_h", ctypes.c_int64), ("stride_s", ctypes.c_int64),
+        ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+        ("scale_stride_page", ctypes.c_int64), ("scale_stride_h", ctypes.c_int64),
+        ("pages", ctypes.c_int32), ("num_kv_heads", ctypes.c_int32), ("page_size", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("bits", ctypes.c_int32),
+        ("page_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+        ("batch", ctypes.c_int32), ("max_pages", ctypes.c_int32),
+        ("seq_lens", ctypes.c_void_p), ("q_start", ctypes.c_void_p), ("tokens", ctypes.c_int32),
+    ]
+
+
+class RopeSpec(ctypes.Structure):
+    """Mirror of struct bz_rope."""
+    _fields_ = [("inv_freq", ctypes.c_void_p), ("rotary_dim", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+                ("factor", ctypes.c_float)]
+
+
+class RopeArgs(ctypes.Structure):
+    """Mirror of struct bz_rope_args."""
+    _fields_ = [
+        ("rope", RopeSpec),
+        ("x", ctypes.c_void_p), ("x_stride_t", ctypes.c_int64), ("x_stride_h", ctypes.c_int64),
+        ("out", ctypes.c_void_p), ("out_stride_t", ctypes.c_int64), ("out_stride_h", ctypes.c_int64),
+        ("positions", ctypes.c_void_p), ("positions_64", ctypes.c_int32), ("inverse", ctypes.c_int32),
+        ("tokens", ctypes.c_int32), ("heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+    ]
+
+
+class PagedStoreArgs(ctypes.Structure):
+    """Mirror of struct bz_paged_store_args."""
+    _fields_ = [
+        ("cache", PagedCacheArgs),
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("k_stride_t", ctypes.c_int64), ("k_stride_h", ctypes.c_int64),
+        ("v_stride_t", ctypes.c_int64), ("v_stride_h", ctypes.c_int64),
+        ("rope", RopeSpec),
+        ("q", ctypes.c_void_p), ("q_stride_t", ctypes.c_int64), ("q_stride_h", ctypes.c_int64),
+        ("q_out", ctypes.c_void_p), ("q_out_stride_t", ctypes.c_int64), ("q_out_stride_h", ctypes.c_int64),
+        ("num_q_heads", ctypes.c_int32),
+        ("q_norm_weight", ctypes.c_void_p), ("k_norm_weight", ctypes.c_void_p), ("eps", ctypes.c_float),
+        ("positions", ctypes.c_void_p), ("positions_64", ctypes.c_int32),
+    ]
+
+
+class GqaPagedArgs(ctypes.Structure):
+    """Mirror of struct bz_gqa_paged_args."""
+    _fields_ = [
+        ("cache", PagedCacheArgs),
+        ("q", ctypes.c_void_p), ("q_stride_t", ctypes.c_int64), ("q_stride_h", ctypes.c_int64),
+        ("out", ctypes.c_void_p), ("out_stride_t", ctypes.c_int64), ("out_stride_h", ctypes.c_int64),
+        ("scale", ctypes.c_float), ("num_q_heads", ctypes.c_int32), ("max_tokens", ctypes.c_int32),
+        ("max_seq_len", ctypes.c_int32),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 _LOCK = threading.Lock()
 _LIB = None
 
@@ -199,7 +261,7 @@ STAMP_PATH = PKG_DIR / "libbz_bench_stamp.so"  # bench.py's GPU timestamp kernel
 
 # The native eager binding (csrc/eager_ext.cpp): a CPython extension module built with g++ against torch's headers,
 # host code only, which calls the C ABI functions of the loaded library (eager()).
-EAGER_SOURCE, EAGER_HEADER = "eager_ext.cpp", "eager_long.hpp"
+EAGER_SOURCE, EAGER_HEADERS = "eager_ext.cpp", ("eager_long.hpp", "eager_paged.hpp")
 EAGER_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM"]
 
 
@@ -212,7 +274,7 @@ def eager_path() -> Path:
 def eager_id() -> str:
     """Hash of what the eager module is built from: its sources, the C ABI headers and its flags."""
     h = hashlib.sha256()
-    for f in [CSRC / EAGER_SOURCE, CSRC / EAGER_HEADER] + sorted(INCLUDE.glob("*.h")):
+    for f in [CSRC / n for n in (EAGER_SOURCE, *EAGER_HEADERS)] + sorted(INCLUDE.glob("*.h")):
         h.update(f.name.encode() + b"\0" + f.read_bytes() + b"\0")
     h.update(" ".join(EAGER_FLAGS).encode())
     return h.hexdigest()[:16]
@@ -310,6 +372,14 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.bz_kv_select.argtypes = [P(KvSelectArgs), ctypes.c_void_p]
     lib.bz_kv_compact.argtypes = [P(KvTensor), ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p] + [
         ctypes.c_int32] * 4 + [ctypes.c_void_p]
+    lib.bz_rope_apply.argtypes = [P(RopeArgs), ctypes.c_void_p]
+    lib.bz_paged_store.argtypes = [P(PagedStoreArgs), ctypes.c_void_p]
+    lib.bz_paged_load.argtypes = [P(PagedCacheArgs), ctypes.c_void_p, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p] + [
+        ctypes.c_int64] * 3 + [ctypes.c_void_p]
+    lib.bz_gqa_paged.argtypes = [P(GqaPagedArgs), ctypes.c_void_p]
+    lib.bz_paged_workspace_size.argtypes = [ctypes.c_int32] * 3 + [P(ctypes.c_size_t)]
+    for name in ("bz_rope_apply", "bz_paged_store", "bz_paged_load", "bz_gqa_paged", "bz_paged_workspace_size"):
+        getattr(lib, name).restype = ctypes.c_int
     for name in ("bz_gqa_window", "bz_gqa_decode_kv4", "bz_gqa_decode_tracked", "bz_long_workspace_size", "bz_kv4_store",
                  "bz_kv4_load", "bz_kv_select", "bz_kv_compact"):
         getattr(lib, name).restype = ctypes.c_int
@@ -376,6 +446,8 @@ def eager():
     mod.bind_long(addr(lib.bz_gqa_window), addr(lib.bz_gqa_decode_kv4), addr(lib.bz_gqa_decode_tracked),
                   addr(lib.bz_long_workspace_size), addr(lib.bz_kv4_store), addr(lib.bz_kv4_load), addr(lib.bz_kv_select),
                   addr(lib.bz_kv_compact))
+    mod.bind_paged(addr(lib.bz_rope_apply), addr(lib.bz_paged_store), addr(lib.bz_paged_load), addr(lib.bz_gqa_paged),
+                   addr(lib.bz_paged_workspace_size))
     with _LOCK:
         if _EAGER is None:
             _EAGER = mod

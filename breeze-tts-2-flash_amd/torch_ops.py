@@ -8,7 +8,7 @@ implementations (shapes only) do nothing, as the outputs are the caller's tensor
 functions: without one, a call takes its stream's cached workspace (allocated, when first needed, outside any graph
 memory pool), except while the stream is being captured, as when torch.compile's CUDA-graph trees record a graph:
 bz::gqa_decode and bz::gqa_decode_masked then run on the library's static scratch (bz_gqa_decode_noalloc) and
-bz::gqa_decode_fused, bz::gqa_window, bz::gqa_decode_kv4 and bz::gqa_decode_tracked raise unless they are given a workspace
+bz::gqa_decode_fused, bz::gqa_window, bz::gqa_decode_kv4, bz::gqa_decode_tracked and bz::gqa_paged raise unless they are given a workspace
 made beforehand (or need none). So compiled calls on different streams
 never share a workspace. The package functions (attention.gqa_decode and the rest) call these operators while
 torch.compile traces them and call the C ABI directly otherwise, which keeps the eager per-call host cost of a plain
@@ -60,6 +60,17 @@ _SCHEMAS = {
     "kv_select": "(Tensor weights, Tensor seq_lens, SymInt keep, SymInt sinks, SymInt recent, Tensor? kv_start, "
                  "Tensor(a!) index, Tensor(b!) lens, Tensor(c!)? weights_out) -> ()",
     "kv_compact": "(Tensor[] tensors, Tensor index, Tensor lens, Tensor(a!)[] outs) -> ()",
+    "rope": "(Tensor x, Tensor positions, Tensor inv_freq, float factor, bool interleaved, bool inverse, Tensor(a!) out) -> ()",
+    "paged_store": "(Tensor k, Tensor v, Tensor(a!) ck, Tensor(b!) cv, Tensor(c!)? k_scale, Tensor(d!)? v_scale, "
+                   "Tensor page_table, Tensor seq_lens, Tensor? q_start) -> ()",
+    "rope_store": "(Tensor q, Tensor k, Tensor v, Tensor(a!) ck, Tensor(b!) cv, Tensor(c!)? k_scale, Tensor(d!)? v_scale, "
+                  "Tensor page_table, Tensor seq_lens, Tensor inv_freq, float factor, bool interleaved, Tensor? q_start, "
+                  "Tensor(e!) out, Tensor? positions, Tensor? q_norm_weight, Tensor? k_norm_weight, float eps) -> ()",
+    "paged_load": "(Tensor ck, Tensor cv, Tensor? k_scale, Tensor? v_scale, Tensor page_table, Tensor starts, SymInt tokens, "
+                  "Tensor(a!) k, Tensor(b!) v) -> ()",
+    "gqa_paged": "(Tensor q, Tensor ck, Tensor cv, Tensor? k_scale, Tensor? v_scale, Tensor page_table, Tensor seq_lens, "
+                 "float scale, Tensor? q_start, Tensor(a!) out, SymInt max_tokens, SymInt max_seq_len, "
+                 "Tensor(b!)? workspace) -> ()",
 }
 
 
@@ -137,6 +148,29 @@ def _kv_compact(tensors, index, lens, outs):
     kernels.eager().compact(tensors, index, lens, outs)
 
 
+def _rope(x, positions, inv_freq, factor, interleaved, inverse, out):
+    kernels.eager().rope(x, positions, inv_freq, factor, interleaved, inverse, out)
+
+
+def _paged_store(k, v, ck, cv, k_scale, v_scale, page_table, seq_lens, q_start):
+    kernels.eager().paged_store(k, v, ck, cv, k_scale, v_scale, page_table, seq_lens, q_start)
+
+
+def _rope_store(q, k, v, ck, cv, k_scale, v_scale, page_table, seq_lens, inv_freq, factor, interleaved, q_start, out, positions,
+                q_norm_weight, k_norm_weight, eps):
+    kernels.eager().rope_store(q, k, v, ck, cv, k_scale, v_scale, page_table, seq_lens, inv_freq, factor, interleaved, q_start, out,
+                               positions, q_norm_weight, k_norm_weight, eps)
+
+
+def _paged_load(ck, cv, k_scale, v_scale, page_table, starts, tokens, k, v):
+    kernels.eager().paged_load(ck, cv, k_scale, v_scale, page_table, starts, tokens, k, v)
+
+
+def _gqa_paged(q, ck, cv, k_scale, v_scale, page_table, seq_lens, scale, q_start, out, max_tokens, max_seq_len, workspace):
+    long_cache._call(kernels.eager().paged, q, ck, cv, k_scale, v_scale, page_table, seq_lens, scale, q_start, out, max_tokens,
+                     max_seq_len, workspace)
+
+
 _KERNELS = {
     "gqa_decode": _gqa_decode,
     "gqa_decode_wave": _gqa_decode_wave,
@@ -154,6 +188,11 @@ _KERNELS = {
     "gqa_decode_tracked": _gqa_decode_tracked,
     "kv_select": _kv_select,
     "kv_compact": _kv_compact,
+    "rope": _rope,
+    "paged_store": _paged_store,
+    "rope_store": _rope_store,
+    "paged_load": _paged_load,
+    "gqa_paged": _gqa_paged,
 }
 
 
