@@ -39,8 +39,15 @@ Layout layout(int cus, int D, int cols) {
 
 bool group_ok(int G) { return G == 1 || G == 2 || G == 4 || G == 8; }
 
-// Rows of more new tokens than this are the chunk kernel's, where there can be any.
+// Columns of a workgroup, by the most tokens of a row as far as the host knows: 16 or 32 of the split kernel up to 64 columns a row, else
+// 128 of the chunk kernel, with the split kernel for the batch's rows of at most 16 (us, 8 rows of 700 .. 8192, 8 kv heads,
+// head_dim 128, bf16 / 8 bits: 20 columns 32.9 / 30.6 by two sets of 16, 42.4 / 33.1 by 16 a workgroup, 56.1 / 58.7 by the chunk kernel;
+// 64 columns 48.1 / 41.6, 76.0 / 58.5, 57.1 / 61.0).
+constexpr int kWideCols = 2 * kLongCols, kSplitCols = 64;
 int few_tokens(int G) { return kLongCols / G; }
+int columns_of(int G, int64_t max_tokens) {
+  return max_tokens <= few_tokens(G) ? kLongCols : max_tokens <= kSplitCols / G ? kWideCols : kChunkCols;
+}
 
 }  // namespace
 
@@ -55,8 +62,7 @@ BZ_EXPORT int bz_paged_workspace_size(int32_t head_dim, int32_t group, int32_t m
   int cus = 0;
   const int rc = bz::device_cu_count(&cus);
   if (rc != BZ_OK) return rc;
-  const bool few = max_tokens > 0 && max_tokens <= few_tokens(group);
-  *bytes = layout(cus, head_dim, few ? kLongCols : kChunkCols).total;
+  *bytes = layout(cus, head_dim, max_tokens > 0 ? columns_of(group, max_tokens) : kChunkCols).total;
   return BZ_OK;
 }
 
@@ -77,11 +83,12 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
 
   const int64_t N = c->tokens, B = c->batch;
   const int few = few_tokens(G);
-  // Whether a row can have more tokens than the split kernel takes at once; where the caller says that none has, that kernel takes
-  // whatever comes, several column tiles a row.
-  const bool chunks = c->q_start != nullptr && N > few && !(a->max_tokens > 0 && a->max_tokens <= few);
-  const bool small = !chunks || B > 1 || N <= few;  // (one row of unknown tokens may have few, but then the chunk kernel takes it)
-  const Layout ws = layout(cus, D, chunks ? kChunkCols : kLongCols);
+  // The most tokens of a row, as far as the host knows; where the caller says that none has many, the split kernel takes whatever comes,
+  // several column tiles a row.
+  const int cols = columns_of(G, c->q_start == nullptr ? 1 : a->max_tokens > 0 ? std::min<int64_t>(a->max_tokens, N) : N);
+  const bool chunks = cols == kChunkCols;
+  const bool small = !chunks || B > 1;  // (one row of unknown tokens may have few, but then the chunk kernel takes it)
+  const Layout ws = layout(cus, D, cols);
   if (a->workspace == nullptr || a->workspace_bytes < ws.total) return BZ_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(a->workspace) & 255) return BZ_ERR_ALIGNMENT;
 
@@ -145,17 +152,23 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
     p.splits = n <= p.one_split ? 1 : (int)std::max<int64_t>(std::min({round / B, most, (int64_t)64}), 1);
     grid = B * p.splits * NKV;
   } else {
-    const int tpt = kLongCols / G;
+    const int tpt = (chunks ? kLongCols : cols) / G;
     const int64_t units = N / tpt + B;
-    p.splits = n <= p.one_split ? 0 : (int)std::max<int64_t>(kSlotsPerCu * cus / NKV, 1);
+    p.splits = n <= p.one_split ? 0 : (int)(units * 2 > round ? 2 * round : round);
+    p.lanes = units * 2 > round ? (int)round : 0;
     grid = (units * 2 <= p.splits ? p.splits : p.splits + units) * NKV;
   }
   if (grid > kMaxGrid) return BZ_ERR_SHAPE;
-  const Fn fns[2][2][2] = {{{paged_split_kernel<64, false, false, kFewThreads>, paged_split_kernel<64, false, true, kFewThreads>},
-                            {paged_split_kernel<64, true, false, kFewThreads>, paged_split_kernel<64, true, true, kFewThreads>}},
-                           {{paged_split_kernel<128, false, false, kFewThreads>, paged_split_kernel<128, false, true, kFewThreads>},
-                            {paged_split_kernel<128, true, false, kFewThreads>, paged_split_kernel<128, true, true, kFewThreads>}}};
-  hipLaunchKernelGGL(fns[D == 128][f8][!alike], dim3((unsigned)grid), dim3(kFewThreads), 0, stream, p);
+  const Fn fns[2][2][3] = {
+      {{paged_split_kernel<64, false, false, 1, kFewThreads>, paged_split_kernel<64, false, true, 1, kFewThreads>,
+        paged_split_kernel<64, false, true, 2, kFewThreads>},
+       {paged_split_kernel<64, true, false, 1, kFewThreads>, paged_split_kernel<64, true, true, 1, kFewThreads>,
+        paged_split_kernel<64, true, true, 2, kFewThreads>}},
+      {{paged_split_kernel<128, false, false, 1, kFewThreads>, paged_split_kernel<128, false, true, 1, kFewThreads>,
+        paged_split_kernel<128, false, true, 2, kFewThreads>},
+       {paged_split_kernel<128, true, false, 1, kFewThreads>, paged_split_kernel<128, true, true, 1, kFewThreads>,
+        paged_split_kernel<128, true, true, 2, kFewThreads>}}};
+  hipLaunchKernelGGL(fns[D == 128][f8][alike ? 0 : cols == kWideCols ? 2 : 1], dim3((unsigned)grid), dim3(kFewThreads), 0, stream, p);
   return hipGetLastError() == hipSuccess ? BZ_OK : BZ_ERR_LAUNCH;
 }
 

@@ -88,8 +88,8 @@ __global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const Paged
   using L = PreLds<D, TP>;
   const int at = (int)(blockIdx.x / (uint32_t)p.NKV), h = (int)blockIdx.x - at * p.NKV;
   const PagedShare share = deal_paged<true, false, TP, 1>(p, kChunkCols, at);
-  if (share.row < 0) return;
-  const PagedRow row = paged_row(p.rows, share.row);
+  if (share.b < 0) return;
+  const PagedRow& row = share.row;
   const int lane = threadIdx.x % kWave, w = wave_uniform((int)threadIdx.x / kWave), c = lane % 32, half = lane / 32;
   const int tpt = kChunkCols >> p.gshift, tiles = (row.T + tpt - 1) / tpt, tile = tiles - 1 - share.tile;  // the longest first
   const int t0 = tile * tpt, ntok = min(tpt, row.T - t0);
@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const Paged
   __shared__ __align__(16) char k_even[L::kBytes], k_odd[L::kBytes], v_even[L::kBytes], v_odd[L::kBytes];
   const int64_t khead = (int64_t)h * p.kv_sh, shead = (int64_t)h * p.sc_sh;
   const int pshift = p.rows.pshift, pmask = (1 << pshift) - 1;
-  const Rsrc table = span_rsrc(p.rows.table + share.row * p.rows.table_st, p.rows.max_pages * 4);
+  const Rsrc table = span_rsrc(p.rows.table + share.b * p.rows.table_st, p.rows.max_pages * 4);
 
   // Lane i holds the page of block i of 16 positions, of the 64 blocks (16 steps) at hand: that of the block's first position, or of
   // the last attended one where the block lies behind it. odd: the blocks without one; they are read from page 0 (any memory
@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const Paged
     for (int i = 0; i < kPreWaveCols; ++i) {
       const int col = kPreWaveCols * w + i, t = t0 + (col >> p.gshift);
       if (t >= t0 + ntok) break;
-      paged_careful<D, F8>(p, h, share.row, row.q0 + t, (h << p.gshift) + (col & (p.G - 1)), wave_uniform(token_end(t)));
+      paged_careful<D, F8>(p, h, share.b, row.q0 + t, (h << p.gshift) + (col & (p.G - 1)), wave_uniform(token_end(t)));
     }
     return;
   }
@@ -389,8 +389,8 @@ __global__ void __launch_bounds__(kPreThreads) paged_merge_kernel(const PagedPar
   const int u = (int)(blockIdx.x / (uint32_t)(p.NKV * kGroups)), rest = (int)blockIdx.x - u * p.NKV * kGroups;
   const int h = rest / kGroups, c0 = kMergeCols * (rest - h * kGroups);
   const PagedShare share = deal_paged<true, true, kChunkStep, 1>(p, kChunkCols, u);
-  if (share.row < 0 || share.k <= 1) return;
-  const PagedRow row = paged_row(p.rows, share.row);
+  if (share.b < 0 || share.k <= 1) return;
+  const PagedRow& row = share.row;
   const int lane = threadIdx.x % kWave, w = wave_uniform((int)threadIdx.x / kWave);
   const int tpt = kChunkCols >> p.gshift, tiles = (row.T + tpt - 1) / tpt, tile = tiles - 1 - share.tile;
   const int t0 = tile * tpt, ntok = min(tpt, row.T - t0);
@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(kPreThreads) paged_merge_kernel(const PagedPar
       for (int i = 0; i < CPW; ++i) {
         const int cc = c1 + i, t = t0 + (cc >> p.gshift);
         if (!(off >> (LPC * i) & (LPC == 64 ? ~0ull : (1ull << LPC) - 1))) continue;
-        paged_careful<D, F8>(p, h, share.row, row.q0 + t, (h << p.gshift) + (cc & (p.G - 1)), wave_uniform(paged_end(p.rows, row, t)));
+        paged_careful<D, F8>(p, h, share.b, row.q0 + t, (h << p.gshift) + (cc & (p.G - 1)), wave_uniform(paged_end(p.rows, row, t)));
       }
     }
     if (!mine || (off >> (lane / LPC * LPC) & ((1ull << LPC) - 1))) continue;

@@ -29,6 +29,7 @@ struct PagedParams {
   float scale_log2;             // scale * log2(e)
   int few;                      // the split kernel takes the rows of at most `few` new tokens, the chunk kernel the others
   int splits;                   // not dealt: splits of a row; dealt: splits of all rows together (0: rows are not split)
+  int lanes;                    // workgroups of a kv head that run at once, where rows may better stay whole (0: they may not)
   int least, one_split;         // tiles of a split at least; up to one_split a row is not split
   int part_slots;               // splits of a kv head that the workspace has room for
   float* part_acc;              // [kv head, slot, column, D] unnormalised sums
@@ -62,9 +63,10 @@ __device__ __forceinline__ int paged_end(const bz::PagedRows& r, const PagedRow&
   return (int)(e < 0 ? 0 : e > cap ? cap : e);
 }
 
-// A workgroup's share: column tile `tile` of row `row`, split `split` of `k`; first: the tile's first slot in the workspace.
+// A workgroup's share: column tile `tile` of row b, split `split` of `k`; first: the tile's first slot in the workspace.
 struct PagedShare {
-  int row, tile, split, k, first;
+  int b, tile, split, k, first;
+  PagedRow row;
 };
 
 // Every wave works out the same: each row's tiles of columns and positions, how many splits it is cut into so that all are about
@@ -78,45 +80,60 @@ template <bool CHUNK, bool PER_TILE, int P, int STEP>
 __device__ __forceinline__ PagedShare deal_paged(const PagedParams& p, int cols, int at) {
   const int lane = threadIdx.x % kWave, B = p.rows.B, tshift = __builtin_ctz(cols) - p.gshift;
   struct Row {
-    int nt, n;
+    PagedRow r;
+    int nt, n;  // its column tiles, and the position tiles of the longest
   };
   auto row_at = [&](int b) {
-    Row x{0, 0};
+    Row x{{0, 0, 0}, 0, 0};
     if (b < B) {
-      const PagedRow r = paged_row(p.rows, b);
-      if (r.T > 0 && (r.T > p.few) == CHUNK) {
-        x.nt = (r.T + (1 << tshift) - 1) >> tshift;
-        x.n = (paged_end(p.rows, r, r.T - 1) + P - 1) / P;
+      x.r = paged_row(p.rows, b);
+      if (x.r.T > 0 && (x.r.T > p.few) == CHUNK) {
+        x.nt = (x.r.T + (1 << tshift) - 1) >> tshift;
+        x.n = (paged_end(p.rows, x.r, x.r.T - 1) + P - 1) / P;
       }
     }
     return x;
   };
   const Row first = row_at(lane);
-  float per = 0.f, inv = 0.f;
+  float per, inv = 0.f;
   auto splits_of = [&](const Row& x) {
     return inv == 0.f || x.n <= p.one_split ? 1 : max(1, (int)__builtin_ceilf((float)x.n * inv));
   };
   if (p.splits > 0) {
-    float total = 0.f, units = 0.f;
+    float total = 0.f, units = 0.f, most = 0.f;
     for (int b0 = 0; b0 < B; b0 += kWave) {
       const Row x = b0 == 0 ? first : row_at(b0 + lane);
       total += wave_sum((float)x.nt * (float)x.n);
       units += wave_sum((float)x.nt);
+      most = fmaxf(most, wave_max((float)x.n));
     }
-    const float want = (float)p.splits;
-    for (int turn = 0; turn < 3; ++turn) {
-      const float over = units < want ? 0.5f * (float)turn * units : 0.f;
-      per = fmaxf((float)p.least, 1.00001f * total / (want - over));
-      per = (float)STEP * __builtin_ceilf(per * (1.f / STEP));
-      inv = 0.99999f / per;  // (never more splits than the exact quotient has)
-      if (over == 0.f && turn > 0) break;
-      float need = 0.f;
-      for (int b0 = 0; b0 < B; b0 += kWave) {
-        const Row x = b0 == 0 ? first : row_at(b0 + lane);
-        need += wave_sum((float)x.nt * (float)splits_of(x));
+    const float want = (float)p.splits, even = 1.00001f * total;
+    // Whole column tiles where those keep the device as busy: `lanes` workgroups of a head at a time, each the longest's time.
+    const bool whole = p.lanes > 0 && most * (float)p.lanes * __builtin_ceilf(units / (float)p.lanes) <= 1.35f * total;
+    // else the shortest of a few `per` that keeps within p.splits, by how many of them are set aside for rounding up: none to U (all
+    // tried at once: a turn for each cost 0.2 us)
+    constexpr int TRIES = 9;
+    constexpr float kAside[TRIES] = {0.f, 0.25f, 0.375f, 0.4375f, 0.5f, 0.5625f, 0.625f, 0.75f, 1.f};
+    float pers[TRIES], need[TRIES];
+    const float aside = units < want ? units : 0.f;
+#pragma unroll
+    for (int i = 0; i < TRIES; ++i) {
+      pers[i] = fmaxf((float)p.least, even * __builtin_amdgcn_rcpf(want - kAside[i] * aside));
+      pers[i] = (float)STEP * __builtin_ceilf(pers[i] * (1.f / STEP));
+      need[i] = 0.f;
+    }
+    for (int b0 = 0; b0 < B && aside > 0.f; b0 += kWave) {
+      const Row x = b0 == 0 ? first : row_at(b0 + lane);
+#pragma unroll
+      for (int i = 0; i < TRIES; ++i) {
+        inv = 0.99999f * __builtin_amdgcn_rcpf(pers[i]);  // (never more splits than the exact quotient has)
+        need[i] += wave_sum((float)x.nt * (float)splits_of(x));
       }
-      if (need <= want) break;
     }
+    per = pers[TRIES - 1];
+#pragma unroll
+    for (int i = TRIES - 2; i >= 0; --i) per = need[i] <= want ? pers[i] : per;
+    inv = whole ? 0.f : 0.99999f * __builtin_amdgcn_rcpf(per);
   }
   int seen = 0, parts = 0;
   for (int b0 = 0; b0 < B; b0 += kWave) {
@@ -128,12 +145,13 @@ __device__ __forceinline__ PagedShare deal_paged(const PagedParams& p, int cols,
       const int l = __builtin_ctzll(hit);
       const int kk = __builtin_amdgcn_readlane(k, l), u = at - __builtin_amdgcn_readlane(last - mine, l);
       const int tile = PER_TILE ? u : u / kk;
-      return {b0 + l, tile, PER_TILE ? 0 : u - tile * kk, kk, __builtin_amdgcn_readlane(pl - part, l) + tile * kk};
+      const PagedRow r{__builtin_amdgcn_readlane(x.r.q0, l), __builtin_amdgcn_readlane(x.r.T, l), __builtin_amdgcn_readlane(x.r.len, l)};
+      return {b0 + l, tile, PER_TILE ? 0 : u - tile * kk, kk, __builtin_amdgcn_readlane(pl - part, l) + tile * kk, r};
     }
     seen = __builtin_amdgcn_readlane(last, kWave - 1);
     parts = __builtin_amdgcn_readlane(pl, kWave - 1);
   }
-  return {-1, 0, 0, 1, 0};
+  return {-1, 0, 0, 1, 0, {0, 0, 0}};
 }
 
 // The pages of a wave's tiles: lane i holds that of its i-th tile (of the 64 at hand), -1 past the table.
@@ -174,36 +192,67 @@ __device__ __forceinline__ void load_f8_half(F8Tile<D>& t, int s, const Rsrc& k,
   t.vs[s] = __builtin_amdgcn_raw_buffer_load_b32(vs, at + 4 * g, 0, 0);
 }
 
+// st.acc += what the non-finite values of V add to the columns that attend their positions (accumulate's product of its own for each
+// column; ncol columns, one a lane r).
+template <int D, int N, class Pos>
+__device__ __forceinline__ void odd_columns(LongState<D>& st, const uint32_t (&v)[N][D / 32], const uint32_t (&hi)[N / 2], int r, int ncol,
+                                            const Reach& mine, Pos pos) {
+  for (int c = 0; c < ncol; ++c) {
+    const Reach rc{0, __builtin_amdgcn_readlane(mine.len, c), 0};
+    uint32_t keep[N / 2];  // the halves of each operand word whose positions the column attends
+#pragma unroll
+    for (int a = 0; a < N / 2; ++a)
+      keep[a] = (attends(rc, 0, pos(2 * a)) ? 0xffffu : 0u) | (attends(rc, 0, pos(2 * a + 1)) ? 0xffff0000u : 0u);
+#pragma unroll
+    for (int n = 0; n < D / 16; ++n) {
+      uint32_t vt[N / 2];
+#pragma unroll
+      for (int a = 0; a < N / 2; ++a) {
+        vt[a] = n % 2 ? pair_hi(v[2 * a][n / 2], v[2 * a + 1][n / 2]) : pair_lo(v[2 * a][n / 2], v[2 * a + 1][n / 2]);
+        vt[a] = odd_pair(vt[a]) & keep[a];
+        asm volatile("" : "+v"(vt[a]));  // worked out here, not for all columns before the loop (registers)
+      }
+      const f32x4_t t = mfma_pv<N>(vt, hi, f32x4_t{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+      for (int i = 0; i < 4; ++i) st.acc[n][i] += r == c ? t[i] : 0.f;
+    }
+  }
+}
+
 // Grid slots * kv heads, a slot's heads side by side; not dealt (DEAL false, rows taken to be alike): slot = row * splits + split,
-// one token a row.
-template <int D, bool F8, bool DEAL, int NT>
+// one token a row. C sets of 16 columns a workgroup: two where rows have more than 16, so that K and V are read and converted once for
+// both.
+template <int D, bool F8, bool DEAL, int C, int NT>
 __global__ void __launch_bounds__(NT, 2) paged_split_kernel(const PagedParams p) {
-  constexpr int NW = NT / kWave, P = F8 ? 32 : 16, NS = P / 16, N = 4 * NS, NJ = D / 32;
+  constexpr int NW = NT / kWave, P = F8 ? 32 : 16, NS = P / 16, N = 4 * NS, NJ = D / 32, COLS = C * kLongCols;
   const int at = (int)(blockIdx.x / (uint32_t)p.NKV), h = (int)blockIdx.x - at * p.NKV;
   const int tid = threadIdx.x, lane = tid % kWave, w = wave_uniform(tid / kWave), r = lane % 16, g = lane / 16;
   PagedShare share;
   if constexpr (DEAL) {
-    share = deal_paged<false, false, P, NW>(p, kLongCols, at);
-    if (share.row < 0) return;
+    share = deal_paged<false, false, P, NW>(p, COLS, at);
+    if (share.b < 0) return;
   } else {
-    const int row = at / p.splits;
-    share = {row, 0, at - row * p.splits, p.splits, row * p.splits};
+    const int b = at / p.splits;
+    share = {b, 0, at - b * p.splits, p.splits, b * p.splits, paged_row(p.rows, b)};
   }
-  const PagedRow row = paged_row(p.rows, share.row);
-  const int tpt = kLongCols >> p.gshift, t0 = share.tile * tpt, ntok = min(tpt, row.T - t0), ncol = ntok << p.gshift;
-  const int col = r % ncol;  // columns past the last repeat earlier ones
-  const int tok = t0 + (col >> p.gshift), hq = (h << p.gshift) + (col & (p.G - 1));
-
-  // the B operand of K . q^T: this lane's column, dims as the tile's K has them
-  uint4 qr[NJ];
-  {
-    const uint16_t* qsrc = p.q + (int64_t)(row.q0 + tok) * p.q_st + (int64_t)hq * p.q_sh;
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) qr[j] = *reinterpret_cast<const uint4*>(qsrc + (F8 ? (D / 4) * g + 8 * j : 32 * j + 8 * g));
-  }
+  const PagedRow& row = share.row;
+  const int tpt = COLS >> p.gshift, t0 = share.tile * tpt, ntok = min(tpt, row.T - t0), ncol = ntok << p.gshift;
   auto token_end = [&](int t) { return paged_end(p.rows, row, t); };
   const int e1 = wave_uniform(token_end(t0 + ntok - 1)), whole_end = wave_uniform(token_end(t0));  // every column attends [0, whole_end)
-  const Reach mine{0, token_end(tok), 0};
+
+  // the B operands of K . q^T: this lane's columns, dims as the tile's K has them
+  int col[C];
+  Reach mine[C];
+  uint4 qr[C][NJ];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    col[c] = (kLongCols * c + r) % ncol;  // columns past the last repeat earlier ones
+    const int tok = t0 + (col[c] >> p.gshift), hq = (h << p.gshift) + (col[c] & (p.G - 1));
+    const uint16_t* qsrc = p.q + (int64_t)(row.q0 + tok) * p.q_st + (int64_t)hq * p.q_sh;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) qr[c][j] = *reinterpret_cast<const uint4*>(qsrc + (F8 ? (D / 4) * g + 8 * j : 32 * j + 8 * g));
+    mine[c] = {0, token_end(tok), 0};
+  }
   const int n = (e1 + P - 1) / P;
   int k = share.k;
   if constexpr (!DEAL) k = n <= p.one_split ? 1 : min(k, max(1, (n + p.least - 1) / p.least));
@@ -211,7 +260,7 @@ __global__ void __launch_bounds__(NT, 2) paged_split_kernel(const PagedParams p)
   if (share.split >= nact) return;
   const int j0 = share.split * NW + w, stride = nact * NW, count = j0 < n ? (n - j0 + stride - 1) / stride : 0;
 
-  const Rsrc table = span_rsrc(p.rows.table + share.row * p.rows.table_st, p.rows.max_pages * 4);
+  const Rsrc table = span_rsrc(p.rows.table + share.b * p.rows.table_st, p.rows.max_pages * 4);
   constexpr bool TWO = NS == 2;
   int ids[NS];
   auto fetch = [&](int i0) {
@@ -223,6 +272,7 @@ __global__ void __launch_bounds__(NT, 2) paged_split_kernel(const PagedParams p)
     std::conditional_t<F8, F8Tile<D>, WaveTile<D>> t;
     int page[NS];  // -1: none, nothing of it is read
   };
+  constexpr bool ONE = F8 && D == 128 && C == 2;  // one tile at a time: two would not fit the registers
   Tile ta, tb;
   const int64_t khead = (int64_t)h * p.kv_sh, shead = (int64_t)h * p.sc_sh;
   const int pmask = (1 << p.rows.pshift) - 1;
@@ -249,52 +299,58 @@ __global__ void __launch_bounds__(NT, 2) paged_split_kernel(const PagedParams p)
     }
   };
 
-  LongState<D> st;
-  st.m = -INFINITY;
-  st.l = 0.f;
+  LongState<D> st[C];
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i) st.acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int c = 0; c < C; ++c) {
+    st[c].m = -INFINITY;
+    st[c].l = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) st[c].acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
 
   fetch(0);
   load(ta, 0);
-  load(tb, 1);
+  if constexpr (!ONE) load(tb, 1);
   __builtin_amdgcn_sched_barrier(0);  // q's conversion waits for q: not before the tiles' loads
   const float scale = positive_scale(p.scale_log2);
-  bf16x8_t qf[NJ];
+  bf16x8_t qf[C][NJ];
 #pragma unroll
-  for (int i = 0; i < NJ; ++i) qf[i] = signed_q(qr[i], p.scale_log2);
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int i = 0; i < NJ; ++i) qf[c][i] = signed_q(qr[c][i], p.scale_log2);
 
   auto consume = [&](Tile& y, int i) {
     auto& t = y.t;
     const int pos0 = P * (j0 + i * stride);
     auto pos = [&](int u) { return pos0 + 16 * (u / 4) + 4 * g + u % 4; };
-    float x[N];
+    float x[C][N];
 #pragma unroll
     for (int u = 0; u < NS; ++u) {
-      f32x4_t d = {0.f, 0.f, 0.f, 0.f};
+      f32x4_t d[C];
+#pragma unroll
+      for (int c = 0; c < C; ++c) d[c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
         bf16x8_t kf;
         if constexpr (F8) kf = __builtin_bit_cast(bf16x8_t, bz::f8_values(make_uint2(t.k[u][2 * j], t.k[u][2 * j + 1]), t.ks[u]));
         else kf = k_operand<D>(t, j);
-        d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[j], d, 0, 0, 0);
+#pragma unroll
+        for (int c = 0; c < C; ++c) d[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[c][j], d[c], 0, 0, 0);
       }
 #pragma unroll
-      for (int c = 0; c < 4; ++c) x[4 * u + c] = d[c];
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[c][4 * u + i] = d[c][i];
     }
-    uint32_t v[N][NJ];
-#pragma unroll
-    for (int c = 0; c < N; ++c)
-#pragma unroll
-      for (int m = 0; m < NJ; ++m) {
-        if constexpr (F8) {
-          const uint32_t e = (t.vs[c / 4] >> (8 * (c % 4))) & 255u;
-          v[c][m] = m % 2 ? bz::f8_pair<true>(t.v[c][m / 2], e) : bz::f8_pair<false>(t.v[c][m / 2], e);
-        } else {
-          v[c][m] = t.v[c][m];
-        }
+    auto value = [&](int i, int m) __attribute__((always_inline)) {  // dims 2 m and 2 m + 1 of this lane's at its i-th position
+      if constexpr (F8) {
+        const uint32_t e = (t.vs[i / 4] >> (8 * (i % 4))) & 255u;
+        return m % 2 ? bz::f8_pair<true>(t.v[i][m / 2], e) : bz::f8_pair<false>(t.v[i][m / 2], e);
+      } else {
+        return t.v[i][m];
       }
-    // An infinity takes one product alone (accumulate). Of 8 bits it can only be under the largest scale, and a NaN matters only where
+    };
+    // An infinity takes one product alone (odd_columns). Of 8 bits it can only be under the largest scale, and a NaN matters only where
     // not every column attends it.
     bool bad = false;
     if constexpr (F8) {
@@ -304,60 +360,140 @@ __global__ void __launch_bounds__(NT, 2) paged_split_kernel(const PagedParams p)
     } else {
       uint32_t top = 0;
 #pragma unroll
-      for (int c = 0; c < N; ++c)
+      for (int i = 0; i < N; ++i)
 #pragma unroll
-        for (int m = 0; m < NJ; ++m) top = max_u16x2(top, v[c][m] & 0x7fff7fffu);
+        for (int m = 0; m < NJ; ++m) top = max_u16x2(top, t.v[i][m] & 0x7fff7fffu);
       bad = pair_not_finite(top);
     }
-    // Where not every column attends the whole tile. V of positions that none attends (behind the row's end, where a page may hold
-    // anything) becomes 0.
-    if (pos0 + P > whole_end || (y.page[0] | y.page[NS - 1]) < 0) {
-      uint32_t top = 0;
+    const bool part = pos0 + P > whole_end || (y.page[0] | y.page[NS - 1]) < 0;  // not every column attends the whole tile
+    uint32_t hi[C][N / 2], lo[C][N / 2];
+    // st.acc += V^T P, v(m, x): dims 2 m and 2 m + 1 of the lane's positions
+    auto products = [&](auto v) __attribute__((always_inline)) {
 #pragma unroll
-      for (int c = 0; c < N; ++c) {
-        const bool some = pos(c) < e1 && y.page[c / 4] >= 0;
-        x[c] = some && pos(c) < mine.len ? x[c] : -INFINITY;
+      for (int m = 0; m < NJ; ++m) {
+        uint32_t vm[N];
+        v(m, vm);
 #pragma unroll
-        for (int m = 0; m < NJ; ++m) {
-          v[c][m] = some ? v[c][m] : 0u;
-          top = max_u16x2(top, v[c][m] & 0x7fff7fffu);
+        for (int n = 2 * m; n < 2 * m + 2; ++n) {
+          uint32_t vt[N / 2];
+#pragma unroll
+          for (int a = 0; a < N / 2; ++a) vt[a] = n % 2 ? pair_hi(vm[2 * a], vm[2 * a + 1]) : pair_lo(vm[2 * a], vm[2 * a + 1]);
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            st[c].acc[n] = mfma_pv<N>(vt, hi[c], st[c].acc[n]);
+            st[c].acc[n] = mfma_pv<N>(vt, lo[c], st[c].acc[n]);
+          }
         }
       }
-      bad = pair_not_finite(top);
+    };
+    if constexpr (C == 1 && !F8) {  // (one path: with two, 206 registers in place of 151, and 64 rows of 128 .. 2048 take 56.7 us, not 52.3)
+      uint32_t v[N][NJ];
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int m = 0; m < NJ; ++m) v[i][m] = t.v[i][m];
+      if (part) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const bool some = pos(i) < e1 && y.page[i / 4] >= 0;
+          x[0][i] = some && pos(i) < mine[0].len ? x[0][i] : -INFINITY;
+#pragma unroll
+          for (int m = 0; m < NJ; ++m) {
+            v[i][m] = some ? v[i][m] : 0u;
+            top = max_u16x2(top, v[i][m] & 0x7fff7fffu);
+          }
+        }
+        bad = pair_not_finite(top);
+      }
+      fold_scores<D, N>(st[0], x[0], scale);
+      accumulate<D, N>(st[0], v, x[0], bad, col[0], ncol, mine[0], 0, pos);
+      return;
     }
-    fold_scores<D, N>(st, x, scale);
-    accumulate<D, N>(st, v, x, bad, col, ncol, mine, 0, pos);
+    if (part || __ballot(bad) != 0) {
+      // V of positions that none attends (behind the row's end, where a page may hold anything) becomes 0
+      uint32_t v[N][NJ], top = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const bool some = pos(i) < e1 && y.page[i / 4] >= 0;
+#pragma unroll
+        for (int c = 0; c < C; ++c) x[c][i] = some && pos(i) < mine[c].len ? x[c][i] : -INFINITY;
+#pragma unroll
+        for (int m = 0; m < NJ; ++m) {
+          v[i][m] = some ? value(i, m) : 0u;
+          top = max_u16x2(top, v[i][m] & 0x7fff7fffu);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        fold_scores<D, N>(st[c], x[c], scale);
+        split_terms(x[c], hi[c], lo[c]);
+      }
+      if (__builtin_expect(__ballot(pair_not_finite(top)) != 0, 0)) {
+#pragma unroll
+        for (int c = 0; c < C; ++c)  // (a set's columns are its lanes r up to their number)
+          odd_columns<D, N>(st[c], v, hi[c], r, min(kLongCols, ncol - kLongCols * c), mine[c], pos);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+          for (int m = 0; m < NJ; ++m) v[i][m] = finite_pair(v[i][m]);
+      }
+      products([&](int m, uint32_t (&vm)[N]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) vm[i] = v[i][m];
+      });
+      return;
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      fold_scores<D, N>(st[c], x[c], scale);
+      split_terms(x[c], hi[c], lo[c]);
+    }
+    products([&](int m, uint32_t (&vm)[N]) __attribute__((always_inline)) {  // (a few values of 8 bits as bf16 at a time: registers)
+#pragma unroll
+      for (int i = 0; i < N; ++i) vm[i] = value(i, m);
+    });
   };
 
-  for (int i = 0; i < count; i += 2) {
-    consume(ta, i);
-    if (i + 1 >= count) break;
-    load(ta, i + 2);
-    consume(tb, i + 1);
-    load(tb, i + 3);
+  if constexpr (ONE) {
+    for (int i = 0; i < count; ++i) {
+      consume(ta, i);
+      load(ta, i + 1);
+    }
+  } else {
+    for (int i = 0; i < count; i += 2) {
+      consume(ta, i);
+      if (i + 1 >= count) break;
+      load(ta, i + 2);
+      consume(tb, i + 1);
+      load(tb, i + 3);
+    }
   }
 
-  // the columns are complete over the wave's positions; only the sums are still one per lane group
-  float y = st.l;
-  swap16(st.l, y);
-  st.l += y;
-  y = st.l;
-  swap32(st.l, y);
-  st.l += y;
-
   constexpr int PD = D + 4;  // keeps the 16-byte stores free of bank conflicts
-  __shared__ __align__(16) float s_acc[NW][kLongCols][PD];
-  __shared__ float s_m[NW][kLongCols], s_l[NW][kLongCols];
-  if (r < ncol) {
+  __shared__ __align__(16) float s_acc[NW][COLS][PD];
+  __shared__ float s_m[NW][COLS], s_l[NW][COLS];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+  for (int c = 0; c < C; ++c) {
+    // the columns are complete over the wave's positions; only the sums are still one per lane group
+    float z = st[c].l;
+    swap16(st[c].l, z);
+    st[c].l += z;
+    z = st[c].l;
+    swap32(st[c].l, z);
+    st[c].l += z;
+    const int to = kLongCols * c + r;
+    if (to < ncol) {
 #pragma unroll
-      for (int q = 0; q < D / 16; q += 4)
-        *reinterpret_cast<f32x4_t*>(&s_acc[w][r][D / 16 * (4 * g + i) + q]) =
-            f32x4_t{st.acc[q][i], st.acc[q + 1][i], st.acc[q + 2][i], st.acc[q + 3][i]};
-    if (g == 0) {
-      s_m[w][r] = st.m;
-      s_l[w][r] = st.l;
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int q = 0; q < D / 16; q += 4)
+          *reinterpret_cast<f32x4_t*>(&s_acc[w][to][D / 16 * (4 * g + i) + q]) =
+              f32x4_t{st[c].acc[q][i], st[c].acc[q + 1][i], st[c].acc[q + 2][i], st[c].acc[q + 3][i]};
+      if (g == 0) {
+        s_m[w][to] = st[c].m;
+        s_l[w][to] = st[c].l;
+      }
     }
   }
   __syncthreads();
@@ -393,8 +529,8 @@ __global__ void __launch_bounds__(NT, 2) paged_split_kernel(const PagedParams p)
     if (nact == 1) {
       write(c, d, A, M, L);
     } else {
-      const int64_t ps = (slot + share.split) * kLongCols;
-      const Rsrc rp = span_rsrc(p.part_acc + ps * D, kLongCols * D * 4);
+      const int64_t ps = (slot + share.split) * COLS;
+      const Rsrc rp = span_rsrc(p.part_acc + ps * D, COLS * D * 4);
       using U4 = decltype(__builtin_amdgcn_raw_buffer_load_b128(rp, 0, 0, 0));
       __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(U4, A), rp, 16 * o, 0, kSc1);
       if (d == 0) {
@@ -417,7 +553,7 @@ __global__ void __launch_bounds__(NT, 2) paged_split_kernel(const PagedParams p)
   }
   __syncthreads();
   if (!s_last) return;
-  merge_columns<D, NT>(p.part_acc + slot * kLongCols * D, p.part_ml + slot * kLongCols, kLongCols, ncol, nact, write);
+  merge_columns<D, NT>(p.part_acc + slot * COLS * D, p.part_ml + slot * COLS, COLS, ncol, nact, write);
 }
 
 }  // namespace

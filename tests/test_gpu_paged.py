@@ -272,6 +272,10 @@ FEW_CASES = [
     ([60, 1, 500, 77], [1, 1, 1, 1], 32, 1, 8, 64), ([5000, 100, 17], [1, 1, 1], 64, 1, 4, 128), ([100, 33, 0, 2], [3, 0, 5, 1], 16, 2, 2, 64),
     ([2000, 511, 9], [2, 1, 4], 256, 4, 4, 128), ([300] * 70, [1, 2] * 35, 16, 1, 1, 64), ([31, 200] * 3, [8, 8] * 3, 32, 2, 2, 128),
     ([3000], [16], 128, 1, 1, 128), ([900, 40], [2, 2], 1024, 2, 8, 64),
+    # 17 to 64 columns: two sets a workgroup
+    ([100, 700, 5], [9, 3, 16], 16, 2, 2, 128), ([2000, 31], [8, 5], 64, 1, 8, 64), ([500], [20], 32, 1, 1, 128), ([1], [17], 16, 1, 1, 64),
+    ([40, 900, 0], [5, 5, 2], 16, 2, 4, 64), ([1000, 3, 70], [16, 1, 0], 16, 1, 4, 128), ([5000, 64], [33, 64], 256, 2, 1, 64),
+    ([300] * 70, [3, 8] * 35, 16, 1, 4, 64),
 ]
 
 
@@ -358,10 +362,10 @@ def test_rows_without_positions(device, bits):
         assert (out[:b.q_start[2]] == 0).all() and (ref[:b.q_start[2]] == 0).all()
 
 
-@pytest.mark.parametrize("T,G", [(1, 2), (5, 2), (60, 2), (33, 4)])
+@pytest.mark.parametrize("T,G,hint", [(1, 2, 0), (5, 2, 0), (60, 2, 0), (33, 4, 0), (5, 2, 5), (10, 2, 10), (13, 4, 13), (60, 2, 1)])
 @pytest.mark.parametrize("bits", [8, 16])
 @pytest.mark.parametrize("value", [float("nan"), float("inf")])
-def test_later_tokens_values_stay_out(device, T, G, bits, value):
+def test_later_tokens_values_stay_out(device, T, G, hint, bits, value):
     """A non-finite value at a token's own position reaches that token and those behind it, and no other."""
     rng = np.random.default_rng(T + G)
     b = Batch(rng, [130, 70], [T, T], 16, 2, 128, device, bits)
@@ -375,13 +379,13 @@ def test_later_tokens_values_stay_out(device, T, G, bits, value):
         cache.v[pg, 1, pl, 3:5] = value
     q = randn(rng, b.N, 2 * G, 128)
     table, lens = b.args()
-    out = pkg.gqa_paged(q.to(device), cache, table, lens, 128 ** -0.5, b.starts())
+    out = pkg.gqa_paged(q.to(device), cache, table, lens, 128 ** -0.5, b.starts(), max_tokens=hint)
     torch.cuda.synchronize()
     ref, spread, reach = paged_attention(f64(q), k, v, b.table, b.lens, b.q_start, 128 ** -0.5)
     got = f64(out)
     clean = np.ones((b.N, 2 * G), bool)
     clean[at:T, G:] = False
-    excess = np.abs(got - ref) - attention_bound(ref, spread, reach, 128 ** -0.5, 128, T > 16 // G)
+    excess = np.abs(got - ref) - attention_bound(ref, spread, reach, 128 ** -0.5, 128, T > 16 // G and hint == 0)
     assert np.isfinite(got[clean]).all() and excess[clean].max() <= 0
     hit = got[at:T, G:]
     if bits == 8 or np.isnan(value):
