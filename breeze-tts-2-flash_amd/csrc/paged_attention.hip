@@ -83,9 +83,22 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
 
   const int64_t N = c->tokens, B = c->batch;
   const int few = few_tokens(G);
-  // The most tokens of a row, as far as the host knows; where the caller says that none has many, the split kernel takes whatever comes,
-  // several column tiles a row.
-  const int cols = columns_of(G, c->q_start == nullptr ? 1 : a->max_tokens > 0 ? std::min<int64_t>(a->max_tokens, N) : N);
+  // Columns of a workgroup by the most tokens of a row, as far as the host knows; where the caller says that none has many, the split
+  // kernel takes whatever comes, several column tiles a row.
+  int cols = columns_of(G, c->q_start == nullptr ? 1 : a->max_tokens > 0 ? std::min<int64_t>(a->max_tokens, N) : N);
+  const int64_t cap = (int64_t)c->max_pages * c->page_size;
+  const int64_t longest = a->max_seq_len > 0 && a->max_seq_len < cap ? a->max_seq_len : cap;
+  if (cols == kChunkCols) {
+    // Short chunks of few heads: the split kernel for all rows. It reads K and V again for each 16 columns, but in one launch (us, split
+    // kernel / chunk kernels, 100 tokens alone 6.1 / 8.6, behind 1000 10 .. 14 / 17; 4 kv heads of 2 q, head_dim 128: 300 behind 1000 18.0 /
+    // 19.5, 100 behind 6000 22.8 / 26.0, 300 behind 6000 50.9 / 29.8; 2 of 2: 1000 alone 14.9 / 16.0; head_dim 64, 4 of 2: 100 behind 1000
+    // 8.8 / 10.6, 300 12.0 / 11.8). Where the batch may have rows of few tokens as well the chunk kernels take a launch more, about 6 us, in which
+    // the split kernel does 10000 tiles of 16 columns and 16 positions (2 kv heads, head_dim 64, 1151 tokens and four rows of one:
+    // 11.4 / 17.7).
+    const int64_t columns = N * NH, length = std::max<int64_t>(longest - std::min(longest, N / B) / 2, 1);
+    const int64_t most = D == 128 ? 512 + (1 << 21) / length : 1280;
+    if (columns <= (B > 1 ? most + (5 << 19) / length : most)) cols = kLongCols;
+  }
   const bool chunks = cols == kChunkCols;
   const bool small = !chunks || B > 1;  // (one row of unknown tokens may have few, but then the chunk kernel takes it)
   const Layout ws = layout(cus, D, cols);
@@ -112,24 +125,36 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
   p.part_ml = reinterpret_cast<float2*>(base + ws.ml);
   p.part_acc = reinterpret_cast<float*>(base + ws.acc);
   const bool f8 = c->bits == 8;
-  const int64_t cap = (int64_t)c->max_pages * c->page_size;
-  const int64_t longest = a->max_seq_len > 0 && a->max_seq_len < cap ? a->max_seq_len : cap;
   using Fn = void (*)(const PagedParams);
 
   if (chunks) {
-    const int tpt = kChunkCols / G;
-    const int64_t units = N / tpt + B;
+    // Workgroups of a chunk kernel with cg column groups (of all kv heads; without the tiles that rows' ends leave part empty), and
+    // its grid.
+    auto tiles = [&](int cg) { return (N * G + kPreWaveCols * cg - 1) / (kPreWaveCols * cg) * NKV; };
+    auto units = [&](int cg) { return N / (kPreWaveCols * cg / G) + B; };
+    const int64_t steps = longest / kChunkStep + 1;
+    // Few column tiles of 128 over many positions are split over those as well (us, 8 kv heads of 2 q, head_dim 128, whole / split: 1024
+    // tokens over 8192 105 / 82, 2048 over 16384 301 / 263, 256 over 8192 70 / 36); at head_dim 64, where one column group leaves
+    // room for two workgroups a CU, only over very many unless even that leaves CUs idle. Else the widest column tiles that give every
+    // CU work (1024 tokens alone: 26.6 by four groups, split, 18.7 by one; 4096 97 by four, 92 by two).
+    const bool idle = D == 128 || tiles(1) < cus;
+    const bool split = (tiles(4) <= cus && steps >= 32 * (2 * cus / tiles(4))) ||
+                       (tiles(2) < cus && std::min(cus / tiles(4), steps / (idle ? 14 : 64)) > 1);
+    const int cg = split || tiles(4) >= 3 * cus ? 4 : tiles(2) >= cus ? 2 : 1;
     p.few = small ? few : 0;
-    p.splits = (N / tpt + 1) * NKV < kSlotsPerCu * cus ? kSlotsPerCu * cus / NKV : 0;
+    p.splits = split ? kSlotsPerCu * cus / NKV : 0;
     p.least = kPreMinSteps, p.one_split = kPreMinSteps;
-    const int64_t grid = (units * 2 <= p.splits ? p.splits : p.splits + units) * NKV;
-    const int64_t merge_grid = units * NKV * (kChunkCols / kMergeCols);
+    p.merge_cols = units(4) * NKV * (kChunkCols / 16) <= 2 * cus ? 8 : 16;
+    const int64_t grid = (units(cg) * 2 <= p.splits ? p.splits : p.splits + units(cg)) * NKV;
+    const int64_t merge_grid = units(4) * NKV * (kChunkCols / p.merge_cols);
     if (grid > kMaxGrid || merge_grid > kMaxGrid) return BZ_ERR_SHAPE;
-    const Fn fns[2][2] = {{paged_chunk_kernel<64, false>, paged_chunk_kernel<64, true>},
-                          {paged_chunk_kernel<128, false>, paged_chunk_kernel<128, true>}};
+    const Fn fns[2][2][3] = {{{paged_chunk_kernel<64, false, 1>, paged_chunk_kernel<64, false, 2>, paged_chunk_kernel<64, false, 4>},
+                              {paged_chunk_kernel<64, true, 1>, paged_chunk_kernel<64, true, 2>, paged_chunk_kernel<64, true, 4>}},
+                             {{paged_chunk_kernel<128, false, 1>, paged_chunk_kernel<128, false, 2>, paged_chunk_kernel<128, false, 4>},
+                              {paged_chunk_kernel<128, true, 1>, paged_chunk_kernel<128, true, 2>, paged_chunk_kernel<128, true, 4>}}};
     const Fn merges[2][2] = {{paged_merge_kernel<64, false>, paged_merge_kernel<64, true>},
                              {paged_merge_kernel<128, false>, paged_merge_kernel<128, true>}};
-    hipLaunchKernelGGL(fns[D == 128][f8], dim3((unsigned)grid), dim3(kPreThreads), 0, stream, p);
+    hipLaunchKernelGGL(fns[D == 128][f8][cg / 2], dim3((unsigned)grid), dim3(kPreThreads), 0, stream, p);
     if (hipGetLastError() != hipSuccess) return BZ_ERR_LAUNCH;
     if (p.splits > 0) {
       hipLaunchKernelGGL(merges[D == 128][f8], dim3((unsigned)merge_grid), dim3(kPreThreads), 0, stream, p);

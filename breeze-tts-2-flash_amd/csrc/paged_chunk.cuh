@@ -82,18 +82,24 @@ struct F8Rows {
 
 // Grid slots * kv heads, a slot's heads side by side (workgroups go to the XCDs in turn, so with a multiple of 8 kv heads each head's
 // K and V pass through one XCD's L2 alone).
-template <int D, bool F8>
+// CG column groups, one a wave, times PG = 4 / CG position groups: 4 x 1 in steps of 64; with 2 x 2 and 1 x 4 a small chunk has
+// more workgroups and fewer steps, each position group taking every PG-th tile of 32, and the groups' accumulators meet in LDS. Only
+// 4 x 1 is split.
+template <int D, bool F8, int CG>
 __global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const PagedParams p) {
-  constexpr int TP = kChunkStep, NB = TP / 32, NQ = D / 16, ND = D / 32;
+  constexpr int PG = 4 / CG, TP = PG == 1 ? kChunkStep : 32, NB = TP / 32, NQ = D / 16, ND = D / 32, COLS = CG * kPreWaveCols;
+  constexpr int BL = TP / 16, UB = BL / CG;         // blocks of 16 positions of a tile, and those that a wave stages
+  constexpr int WS = kWave / BL;                    // steps whose pages a wave holds
   using L = PreLds<D, TP>;
   const int at = (int)(blockIdx.x / (uint32_t)p.NKV), h = (int)blockIdx.x - at * p.NKV;
-  const PagedShare share = deal_paged<true, false, TP, 1>(p, kChunkCols, at);
+  const PagedShare share = deal_paged<true, false, kChunkStep, 1>(p, COLS, at);
   if (share.b < 0) return;
   const PagedRow& row = share.row;
   const int lane = threadIdx.x % kWave, w = wave_uniform((int)threadIdx.x / kWave), c = lane % 32, half = lane / 32;
-  const int tpt = kChunkCols >> p.gshift, tiles = (row.T + tpt - 1) / tpt, tile = tiles - 1 - share.tile;  // the longest first
+  const int cg = PG == 1 ? w : w % CG, pg = PG == 1 ? 0 : w / CG;
+  const int tpt = COLS >> p.gshift, tiles = (row.T + tpt - 1) / tpt, tile = tiles - 1 - share.tile;  // the longest first
   const int t0 = tile * tpt, ntok = min(tpt, row.T - t0);
-  const int mine = kPreWaveCols * w + c, tok = t0 + min(mine >> p.gshift, ntok - 1), hq = (h << p.gshift) + (mine & (p.G - 1));
+  const int mine = kPreWaveCols * cg + c, tok = t0 + min(mine >> p.gshift, ntok - 1), hq = (h << p.gshift) + (mine & (p.G - 1));
 
   const float scale = positive_scale(p.scale_log2);
   bf16x8_t qf[NQ];
@@ -105,84 +111,104 @@ __global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const Paged
 
   auto token_end = [&](int t) { return paged_end(p.rows, row, t); };
   const int my_end = token_end(tok), e1 = wave_uniform(token_end(t0 + ntok - 1)), last = e1 - 1;
-  const int whole_end = wave_uniform(token_end(t0 + min((kPreWaveCols * w) >> p.gshift, ntok - 1)));  // of the wave's columns
-  const int steps = (e1 + TP - 1) / TP;
-  const ChunkCut cut = cut_chunk(steps, share.k);
-  const int j0 = share.split * cut.per;
-  if (share.split > 0 && j0 >= steps) return;
+  const int whole_end = wave_uniform(token_end(t0 + min((kPreWaveCols * cg) >> p.gshift, ntok - 1)));  // of the wave's columns
+  const int steps = (e1 + TP * PG - 1) / (TP * PG);
+  const ChunkCut cut = cut_chunk(steps, PG == 1 ? share.k : 1);
+  const int j0 = PG == 1 ? share.split * cut.per : 0;
+  if (PG == 1 && share.split > 0 && j0 >= steps) return;
   const int n = min(cut.per, steps - j0);  // steps of this split
-  auto pos_of = [&](int j) { return TP * (j0 + j); };
+  auto pos_of = [&](int j) { return TP * (PG * (j0 + j) + pg); };
 
   // arrays of their own, and the steps' parity known at compile time: the compiler then sees that the reads of one do not
   // depend on the loads in flight to another (it would wait for all of them)
-  __shared__ __align__(16) char k_even[L::kBytes], k_odd[L::kBytes], v_even[L::kBytes], v_odd[L::kBytes];
+  __shared__ __align__(16) char k_even[PG * L::kBytes], k_odd[PG * L::kBytes], v_even[PG * L::kBytes], v_odd[PG * L::kBytes];
   const int64_t khead = (int64_t)h * p.kv_sh, shead = (int64_t)h * p.sc_sh;
   const int pshift = p.rows.pshift, pmask = (1 << pshift) - 1;
   const Rsrc table = span_rsrc(p.rows.table + share.b * p.rows.table_st, p.rows.max_pages * 4);
 
-  // Lane i holds the page of block i of 16 positions, of the 64 blocks (16 steps) at hand: that of the block's first position, or of
-  // the last attended one where the block lies behind it. odd: the blocks without one; they are read from page 0 (any memory
-  // that is there) and attended by nobody.
+  // Lane i holds the page of block i of 16 positions, of the 64 blocks (WS steps) of this wave's tiles at hand: that of the block's
+  // first position, or of the last attended one where the block lies behind it. odd: the blocks without one; they are read from
+  // page 0 (any memory that is there) and attended by nobody.
   int ids = 0;
   uint64_t odd = 0;
   auto fetch = [&](int j) __attribute__((always_inline)) {
-    ids = page_ids(table, p.rows.max_pages, min(pos_of(j) + 16 * lane, max(last, 0)) >> pshift);
+    ids = page_ids(table, p.rows.max_pages, min(pos_of(j + lane / BL) + 16 * (lane % BL), max(last, 0)) >> pshift);
   };
   auto settle = [&]() __attribute__((always_inline)) {
     const bool there = (uint32_t)ids < (uint32_t)p.rows.pages;
     odd = __ballot(!there);
     ids = there ? ids : 0;
   };
-  auto page_at = [&](int j) __attribute__((always_inline)) { return (int64_t)__builtin_amdgcn_readlane(ids, (4 * j + w) & 63); };
-  auto odd_at = [&](int j) __attribute__((always_inline)) { return (uint32_t)(odd >> (4 * (j & 15))) & 15u; };
+  struct Pages {
+    int id[UB];  // of the blocks that this wave stages
+  };
+  auto page_at = [&](int j) __attribute__((always_inline)) {
+    Pages x;
+#pragma unroll
+    for (int u = 0; u < UB; ++u) x.id[u] = __builtin_amdgcn_readlane(ids, BL * (j & (WS - 1)) + cg * UB + u);
+    return x;
+  };
+  auto odd_at = [&](int j) __attribute__((always_inline)) { return (uint32_t)(odd >> (BL * (j & (WS - 1)))) & ((1u << BL) - 1); };
   // the place in its page of position x, behind the last attended one that one's
   auto place = [&](int x) __attribute__((always_inline)) { return min(x, last) & pmask; };
 
-  // Rows 16 w .. of step j of K or V into LDS. 64 lanes write 1 KB in lane order, so the swizzle is in which chunk each fetches.
-  auto stage = [&](auto isv, char* buf, int j, int64_t page) __attribute__((always_inline)) {
+  // This wave's rows of step j of K or V into LDS. 64 lanes write 1 KB in lane order, so the swizzle is in which chunk each fetches.
+  const int group = pg * L::kBytes;
+  auto stage = [&](auto isv, char* buf, int j, const Pages& pages) __attribute__((always_inline)) {
     constexpr bool V = decltype(isv)::value;
     constexpr int RPI = 1024 / L::kRow, CH = D / 8;  // rows an instruction, chunks a row
-    const Rsrc rsrc = span_rsrc((V ? p.v : p.k) + page * p.kv_sp + khead, p.page_bytes);
     const int p0 = pos_of(j);
 #pragma unroll
-    for (int u = 0; u < 16 / RPI; ++u) {
-      const int row0 = 16 * w + RPI * u, rw = row0 + lane / CH, ch = lane % CH;
-      const uint32_t off = (uint32_t)place(p0 + rw) * p.kv_ss + 16 * (ch ^ (V ? L::v_swz(rw) : L::k_swz(rw)));
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(buf + row0 * L::kRow), 16, off, 0, 0, 0);
+    for (int b = 0; b < UB; ++b) {
+      const Rsrc rsrc = span_rsrc((V ? p.v : p.k) + pages.id[b] * p.kv_sp + khead, p.page_bytes);
+#pragma unroll
+      for (int u = 0; u < 16 / RPI; ++u) {
+        const int row0 = 16 * (cg * UB + b) + RPI * u, rw = row0 + lane / CH, ch = lane % CH;
+        const uint32_t off = (uint32_t)place(p0 + rw) * p.kv_ss + 16 * (ch ^ (V ? L::v_swz(rw) : L::k_swz(rw)));
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(buf + group + row0 * L::kRow), 16, off,
+                                                 0, 0, 0);
+      }
     }
   };
-  auto load8 = [&](auto isv, F8Rows<D>& x, int j, int64_t page) __attribute__((always_inline)) {
+  auto load8 = [&](auto isv, F8Rows<D> (&x)[UB], int j, const Pages& pages) __attribute__((always_inline)) {
     constexpr bool V = decltype(isv)::value;
-    const Rsrc rsrc = span_rsrc((V ? p.v : p.k) + page * p.kv_sp + khead, p.page_bytes);
-    const Rsrc rs = span_rsrc((V ? p.vs : p.ks) + page * p.sc_sp + shead, pmask + 1);
-    const int at = place(pos_of(j) + 16 * w + lane / 4);
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i)
-      x.c[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(
-                                             rsrc, (uint32_t)at * p.kv_ss + (D / 4) * (lane % 4) + 16 * i, 0, 0));
-    x.e = __builtin_amdgcn_raw_buffer_load_b8(rs, at, 0, 0);
+    for (int b = 0; b < UB; ++b) {
+      const int64_t page = pages.id[b];
+      const Rsrc rsrc = span_rsrc((V ? p.v : p.k) + page * p.kv_sp + khead, p.page_bytes);
+      const Rsrc rs = span_rsrc((V ? p.vs : p.ks) + page * p.sc_sp + shead, pmask + 1);
+      const int at = place(pos_of(j) + 16 * (cg * UB + b) + lane / 4);
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i)
+        x[b].c[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                  rsrc, (uint32_t)at * p.kv_ss + (D / 4) * (lane % 4) + 16 * i, 0, 0));
+      x[b].e = __builtin_amdgcn_raw_buffer_load_b8(rs, at, 0, 0);
+    }
   };
-  auto put8 = [&](auto isv, char* buf, const F8Rows<D>& x) __attribute__((always_inline)) {
+  auto put8 = [&](auto isv, char* buf, const F8Rows<D> (&x)[UB]) __attribute__((always_inline)) {
     constexpr bool V = decltype(isv)::value;
-    const int rw = 16 * w + lane / 4, swz = V ? L::v_swz(rw) : L::k_swz(rw);
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i)
+    for (int b = 0; b < UB; ++b) {
+      const int rw = 16 * (cg * UB + b) + lane / 4, swz = V ? L::v_swz(rw) : L::k_swz(rw);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint2 code = u ? make_uint2(x.c[i].z, x.c[i].w) : make_uint2(x.c[i].x, x.c[i].y);
-        const int ch = (D / 32) * (lane % 4) + 2 * i + u;
-        *reinterpret_cast<uint4*>(buf + rw * L::kRow + 16 * (ch ^ swz)) = bz::f8_values(code, x.e);
-      }
+      for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const uint2 code = u ? make_uint2(x[b].c[i].z, x[b].c[i].w) : make_uint2(x[b].c[i].x, x[b].c[i].y);
+          const int ch = (D / 32) * (lane % 4) + 2 * i + u;
+          *reinterpret_cast<uint4*>(buf + group + rw * L::kRow + 16 * (ch ^ swz)) = bz::f8_values(code, x[b].e);
+        }
+    }
   };
   constexpr std::false_type isk{};
   constexpr std::true_type isv{};
 
   // this lane's LDS addresses: K chunk 2 j + half of row c; V, transposed: the four rows and 16 dims of its group of 16 lanes
-  const int k_addr = c * L::kRow, k_sw = L::k_swz(c), l16 = lane % 16, v_row = 4 * half + l16 / 4;
+  const int k_addr = group + c * L::kRow, k_sw = L::k_swz(c), l16 = lane % 16, v_row = 4 * half + l16 / 4;
   int v_addr[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d)
-    v_addr[d] = v_row * L::kRow + 16 * ((4 * d + 2 * ((lane / 16) % 2) + (l16 % 4) / 2) ^ L::v_swz(v_row)) + 8 * (l16 % 2);
+    v_addr[d] = group + v_row * L::kRow + 16 * ((4 * d + 2 * ((lane / 16) % 2) + (l16 % 4) / 2) ^ L::v_swz(v_row)) + 8 * (l16 % 2);
 
   float m = -INFINITY, l = 0.f;
   f32x16_t acc[ND];
@@ -204,12 +230,13 @@ __global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const Paged
 
   // In step j K of step j + AHEAD is asked for and V of the step before that: bf16 straight into LDS, where the next steps read
   // them; 8 bits into kr and vr, which go to LDS one step later. vpage: the page of that V. holes: the blocks without a page of
-  // the steps from j on, four bits each.
+  // the steps from j on, BL bits each.
   constexpr int AHEAD = F8 ? 3 : 2;
-  int64_t vpage = 0;
+  Pages vpage{};
   uint32_t holes = 0;
-  F8Rows<D> kr, vr;
-  constexpr int NK = NB * NQ, PT = 8 * NB / NK, KA = NK < 8 ? NK : 8;  // products of K q, pairs of terms beside each, reads ahead
+  F8Rows<D> kr[UB], vr[UB];
+  // products of K q, pairs of terms beside each, reads ahead (8 bits, D 128: fewer, for the registers)
+  constexpr int NK = NB * NQ, PT = 8 * NB / NK, AH = F8 && D == 128 && CG == 4 ? 4 : 8, KA = NK < AH ? NK : AH;
 
   // Step j: its scores x into the running maximum, sum and accumulators, and the scores of step j + 1 (next; unused after the
   // last), in window_prefill_kernel's order.
@@ -218,23 +245,25 @@ __global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const Paged
     const char *const kbuf = kOdd ? k_even : k_odd, *const vbuf = kOdd ? v_odd : v_even;
     char *const knew = kOdd ? k_odd : k_even, *const vnew = kOdd ? v_even : v_odd;
     __builtin_amdgcn_s_waitcnt(0x0f70);  // this wave's loads have arrived: of K j + 1 and V j, or (8 bits) of K j + 2 and V j + 1
-    __syncthreads();                     // K j + 1 and V j are in LDS, and nobody reads K j or V j - 1 any more
+    // K j + 1 and V j are in LDS, and nobody reads K j or V j - 1 any more (a wave with tiles of its own has just used what it read)
+    if constexpr (CG > 1) __syncthreads();
+    else asm volatile("" ::: "memory");
     bf16x8_t kf[KA], vf[2][ND];
 #pragma unroll
     for (int i = 0; i < KA; ++i) kf[i] = k_read(kbuf, i);
     __builtin_amdgcn_sched_barrier(0);
-    const uint32_t hole = holes & 15u;
-    holes >>= 4;
+    const uint32_t hole = holes & ((1u << BL) - 1);
+    holes >>= BL;
     const int jk = j + AHEAD;
-    if ((jk & 15) == 0 && jk < n) settle();
+    if ((jk & (WS - 1)) == 0 && jk < n) settle();
     if constexpr (F8) {
       if (j + 2 < n) put8(isk, knew, kr);
       if (j + 1 < n) put8(isv, vnew, vr);
     }
-    int64_t kpage = 0;
+    Pages kpage{};
     if (jk < n) {
       kpage = page_at(jk);
-      holes |= odd_at(jk) << (4 * (AHEAD - 1));
+      holes |= odd_at(jk) << (BL * (AHEAD - 1));
       if constexpr (F8) load8(isk, kr, jk, kpage);
       else stage(isk, knew, jk, kpage);
     }
@@ -243,7 +272,7 @@ __global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const Paged
       else stage(isv, vnew, jk - 1, vpage);
     }
     vpage = kpage;
-    if ((jk & 15) == 15 && jk + 1 < n) fetch(jk + 1);  // (there with the next step's wait)
+    if ((jk & (WS - 1)) == WS - 1 && jk + 1 < n) fetch(jk + 1);  // (there with the next step's wait)
     const int p0 = pos_of(j);
     if (p0 + TP > whole_end || hole != 0) {
 #pragma unroll
@@ -301,11 +330,11 @@ __global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const Paged
   if (n > 0) {
     fetch(0);
     settle();
-    const int64_t page0 = page_at(0), page1 = page_at(1);  // (behind the last step: any page, unused)
-    holes = odd_at(0) | odd_at(1) << 4;
+    const Pages page0 = page_at(0), page1 = page_at(1);  // (behind the last step: any page, unused)
+    holes = odd_at(0) | odd_at(1) << BL;
     f32x16_t xa[NB], xb[NB];
     if constexpr (F8) {
-      F8Rows<D> k0;
+      F8Rows<D> k0[UB];
       load8(isk, k0, 0, page0);
       if (n > 1) load8(isk, kr, 1, page1);
       load8(isv, vr, 0, page0);
@@ -313,7 +342,7 @@ __global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const Paged
       if (n > 1) put8(isk, k_odd, kr);
       put8(isv, v_even, vr);
       vpage = page_at(2);
-      holes |= odd_at(2) << 8;
+      holes |= odd_at(2) << (2 * BL);
       if (n > 2) load8(isk, kr, 2, vpage);
       if (n > 1) load8(isv, vr, 1, page1);
     } else {
@@ -321,7 +350,8 @@ __global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const Paged
       vpage = page1;
     }
     if constexpr (!F8) __builtin_amdgcn_s_waitcnt(0x0f70);
-    __syncthreads();
+    if constexpr (CG > 1) __syncthreads();
+    else asm volatile("" ::: "memory");
     if constexpr (!F8) {
       if (n > 1) stage(isk, k_odd, 1, page1);
       stage(isv, v_even, 0, page0);
@@ -338,7 +368,43 @@ __global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const Paged
   float other = l;
   swap32(l, other);
   l += other;
-  if (cut.nact > 1) {
+  if constexpr (PG > 1) {
+    // the position groups' accumulators through the tiles' LDS: for PG = 4 groups 2 and 3 to 0 and 1, then (as for PG = 2)
+    // group 1 to 0
+    __shared__ float s_m[4][kPreWaveCols], s_l[4][kPreWaveCols];
+#pragma unroll
+    for (int from = PG / 2; from > 0; from /= 2) {
+      __syncthreads();  // the tiles, or the round before, have been read
+      const bool gives = pg >= from && pg < 2 * from, takes = pg < from;
+      const int giver = gives ? w : w + from * CG;  // its wave
+      char* const to = (giver % 2 ? k_odd : k_even) + 16 * lane;  // 16 ND registers of a wave: 4 KB ND, half an array's least
+      if (gives) {
+        if (half == 0) s_m[w][c] = m, s_l[w][c] = l;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<f32x4_t*>(to + 4096 * d + 256 * i) = f32x4_t{acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]};
+      }
+      __syncthreads();
+      if (takes) {
+        const float mo = s_m[giver][c], mn = fmaxf(m, mo), mu = mn == -INFINITY ? 0.f : mn;
+        const float f0 = fast_exp2(m - mu), f1 = fast_exp2(mo - mu);
+        m = mn;
+        l = l * f0 + s_l[giver][c] * f1;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            const f32x4_t y = *reinterpret_cast<const f32x4_t*>(to + 4096 * d + 256 * i);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) acc[d][i + q] = acc[d][i + q] * f0 + y[q] * f1;
+          }
+      }
+    }
+    if (pg > 0) return;
+  }
+  if (PG == 1 && cut.nact > 1) {
     const int64_t part = ((int64_t)h * p.part_slots + share.first + share.split) * kChunkCols + mine;
     if (half == 0) p.part_ml[part] = make_float2(m, l);
     float* const to = p.part_acc + part * D + 4 * half;
@@ -357,7 +423,7 @@ __global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const Paged
     for (int i = 0; i < 16; ++i) worst += fabsf(acc[d][i]) * 0x1p-8f;
   if (__builtin_expect(__ballot(!(worst < INFINITY) || !(l < INFINITY)) != 0, 0)) {
     for (int i = 0; i < kPreWaveCols; ++i) {
-      const int col = kPreWaveCols * w + i, t = t0 + (col >> p.gshift);
+      const int col = kPreWaveCols * cg + i, t = t0 + (col >> p.gshift);
       if (t >= t0 + ntok) break;
       paged_careful<D, F8>(p, h, share.b, row.q0 + t, (h << p.gshift) + (col & (p.G - 1)), wave_uniform(token_end(t)));
     }
@@ -379,15 +445,14 @@ __global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const Paged
     }
 }
 
-constexpr int kMergeCols = 16;  // columns of a workgroup
-
 // Adds up the splits of paged_chunk_kernel's tiles and writes their outputs, four dims a lane. Grid column tiles * kv heads * (128 /
-// kMergeCols), a tile's heads side by side.
+// p.merge_cols), a tile's heads side by side.
 template <int D, bool F8>
 __global__ void __launch_bounds__(kPreThreads) paged_merge_kernel(const PagedParams p) {
-  constexpr int LPC = D / 4, CPW = kWave / LPC, kGroups = kChunkCols / kMergeCols;  // lanes a column, columns a wave at a time
-  const int u = (int)(blockIdx.x / (uint32_t)(p.NKV * kGroups)), rest = (int)blockIdx.x - u * p.NKV * kGroups;
-  const int h = rest / kGroups, c0 = kMergeCols * (rest - h * kGroups);
+  constexpr int LPC = D / 4, CPW = kWave / LPC;  // lanes a column, columns a wave at a time
+  const int groups = kChunkCols / p.merge_cols;
+  const int u = (int)(blockIdx.x / (uint32_t)(p.NKV * groups)), rest = (int)blockIdx.x - u * p.NKV * groups;
+  const int h = rest / groups, c0 = p.merge_cols * (rest - h * groups);
   const PagedShare share = deal_paged<true, true, kChunkStep, 1>(p, kChunkCols, u);
   if (share.b < 0 || share.k <= 1) return;
   const PagedRow& row = share.row;
@@ -397,7 +462,7 @@ __global__ void __launch_bounds__(kPreThreads) paged_merge_kernel(const PagedPar
   const ChunkCut cut = cut_chunk((paged_end(p.rows, row, t0 + ntok - 1) + kChunkStep - 1) / kChunkStep, share.k);
   if (cut.nact == 1) return;  // its one split has written them
   const int64_t slot = (int64_t)h * p.part_slots + share.first;
-  for (int c1 = c0 + CPW * w; c1 < c0 + kMergeCols; c1 += CPW * (kPreThreads / kWave)) {
+  for (int c1 = c0 + CPW * w; c1 < c0 + p.merge_cols; c1 += CPW * (kPreThreads / kWave)) {
     const int col = c1 + lane / LPC, d = 4 * (lane % LPC);
     if ((c1 >> p.gshift) >= ntok) return;  // (uniform: a wave's columns lie side by side)
     float m = -INFINITY, l = 0.f;

@@ -31,6 +31,7 @@ struct PagedParams {
   int splits;                   // not dealt: splits of a row; dealt: splits of all rows together (0: rows are not split)
   int lanes;                    // workgroups of a kv head that run at once, where rows may better stay whole (0: they may not)
   int least, one_split;         // tiles of a split at least; up to one_split a row is not split
+  int merge_cols;               // columns of a workgroup of the merge kernel
   int part_slots;               // splits of a kv head that the workspace has room for
   float* part_acc;              // [kv head, slot, column, D] unnormalised sums
   float2* part_ml;              // [kv head, slot, column] (max, sum)
@@ -107,7 +108,8 @@ __device__ __forceinline__ PagedShare deal_paged(const PagedParams& p, int cols,
       units += wave_sum((float)x.nt);
       most = fmaxf(most, wave_max((float)x.n));
     }
-    const float want = (float)p.splits, even = 1.00001f * total;
+    // (a chunk's splits: two rounds of workgroups where each still has 12 steps, else one: their sums' way through memory costs more)
+    const float want = CHUNK && total < 12.f * (float)p.splits ? fmaxf(0.5f * (float)p.splits, 1.f) : (float)p.splits, even = 1.00001f * total;
     // Whole column tiles where those keep the device as busy: `lanes` workgroups of a head at a time, each the longest's time.
     const bool whole = p.lanes > 0 && most * (float)p.lanes * __builtin_ceilf(units / (float)p.lanes) <= 1.35f * total;
     // else the shortest of a few `per` that keeps within p.splits, by how many of them are set aside for rounding up: none to U (all
