@@ -88,16 +88,18 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
   int cols = columns_of(G, c->q_start == nullptr ? 1 : a->max_tokens > 0 ? std::min<int64_t>(a->max_tokens, N) : N);
   const int64_t cap = (int64_t)c->max_pages * c->page_size;
   const int64_t longest = a->max_seq_len > 0 && a->max_seq_len < cap ? a->max_seq_len : cap;
+  const int64_t columns = N * NH, length = std::max<int64_t>(longest - std::min(longest, N / B) / 2, 1);  // of all heads; about a token's
   if (cols == kChunkCols) {
     // Short chunks of few heads: the split kernel for all rows. It reads K and V again for each 16 columns, but in one launch (us, split
     // kernel / chunk kernels, 100 tokens alone 6.1 / 8.6, behind 1000 10 .. 14 / 17; 4 kv heads of 2 q, head_dim 128: 300 behind 1000 18.0 /
     // 19.5, 100 behind 6000 22.8 / 26.0, 300 behind 6000 50.9 / 29.8; 2 of 2: 1000 alone 14.9 / 16.0; head_dim 64, 4 of 2: 100 behind 1000
-    // 8.8 / 10.6, 300 12.0 / 11.8). Where the batch may have rows of few tokens as well the chunk kernels take a launch more, about 6 us, in which
-    // the split kernel does 10000 tiles of 16 columns and 16 positions (2 kv heads, head_dim 64, 1151 tokens and four rows of one:
-    // 11.4 / 17.7).
-    const int64_t columns = N * NH, length = std::max<int64_t>(longest - std::min(longest, N / B) / 2, 1);
+    // 8.8 / 10.6, 300 12.0 / 11.8). Where the batch may have rows of few tokens as well the chunk kernels take a launch more, about 6 us,
+    // in which the split kernel does 10000 tiles of 16 columns and 16 positions (2 kv heads, head_dim 64, 1151 tokens and four rows of
+    // one: 11.4 / 17.7).
     const int64_t most = D == 128 ? 512 + (1 << 21) / length : 1280;
     if (columns <= (B > 1 ? most + (5 << 19) / length : most)) cols = kLongCols;
+  } else if (cols == kWideCols && columns * length <= 5 << 19) {
+    cols = kLongCols;  // (as few tiles: two sets of columns only make a workgroup slower, 2 rows of 20 tokens behind 500 9.0 / 12.0)
   }
   const bool chunks = cols == kChunkCols;
   const bool small = !chunks || B > 1;  // (one row of unknown tokens may have few, but then the chunk kernel takes it)
@@ -125,13 +127,15 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
   p.part_ml = reinterpret_cast<float2*>(base + ws.ml);
   p.part_acc = reinterpret_cast<float*>(base + ws.acc);
   const bool f8 = c->bits == 8;
-  using Fn = void (*)(const PagedParams);
-
+  // The chunk kernel's part: its parameters, grid and merge.
+  PagedParams pc = p;
+  int cg = 0;
+  int64_t chunk_grid = 0, merge_grid = 0;
   if (chunks) {
-    // Workgroups of a chunk kernel with cg column groups (of all kv heads; without the tiles that rows' ends leave part empty), and
-    // its grid.
-    auto tiles = [&](int cg) { return (N * G + kPreWaveCols * cg - 1) / (kPreWaveCols * cg) * NKV; };
-    auto units = [&](int cg) { return N / (kPreWaveCols * cg / G) + B; };
+    // Workgroups of a chunk kernel with g column groups (of all kv heads; without the tiles that rows' ends leave part empty), and
+    // its column tiles at most.
+    auto tiles = [&](int g) { return (N * G + kPreWaveCols * g - 1) / (kPreWaveCols * g) * NKV; };
+    auto units = [&](int g) { return N / (kPreWaveCols * g / G) + B; };
     const int64_t steps = longest / kChunkStep + 1;
     // Few column tiles of 128 over many positions are split over those as well (us, 8 kv heads of 2 q, head_dim 128, whole / split: 1024
     // tokens over 8192 105 / 82, 2048 over 16384 301 / 263, 256 over 8192 70 / 36); at head_dim 64, where one column group leaves
@@ -140,50 +144,61 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
     const bool idle = D == 128 || tiles(1) < cus;
     const bool split = (tiles(4) <= cus && steps >= 32 * (2 * cus / tiles(4))) ||
                        (tiles(2) < cus && std::min(cus / tiles(4), steps / (idle ? 14 : 64)) > 1);
-    const int cg = split || tiles(4) >= 3 * cus ? 4 : tiles(2) >= cus ? 2 : 1;
-    p.few = small ? few : 0;
-    p.splits = split ? kSlotsPerCu * cus / NKV : 0;
-    p.least = kPreMinSteps, p.one_split = kPreMinSteps;
-    p.merge_cols = units(4) * NKV * (kChunkCols / 16) <= 2 * cus ? 8 : 16;
-    const int64_t grid = (units(cg) * 2 <= p.splits ? p.splits : p.splits + units(cg)) * NKV;
-    const int64_t merge_grid = units(4) * NKV * (kChunkCols / p.merge_cols);
-    if (grid > kMaxGrid || merge_grid > kMaxGrid) return BZ_ERR_SHAPE;
+    cg = split || tiles(4) >= 3 * cus ? 4 : tiles(2) >= cus ? 2 : 1;
+    pc.few = small ? few : 0;
+    pc.splits = split ? kSlotsPerCu * cus / NKV : 0;
+    pc.least = kPreMinSteps, pc.one_split = kPreMinSteps;
+    pc.merge_cols = units(4) * NKV * (kChunkCols / 16) <= 2 * cus ? 8 : 16;
+    chunk_grid = (units(cg) * 2 <= pc.splits ? pc.splits : pc.splits + units(cg)) * NKV;
+    merge_grid = pc.splits > 0 ? units(4) * NKV * (kChunkCols / pc.merge_cols) : 0;
+  }
+
+  // The split kernel's, for rows of few tokens (all of them, if there are no others).
+  const bool alike = c->q_start == nullptr && B <= 3;
+  int64_t split_grid = 0;
+  if (small) {
+    const int P = f8 ? 32 : 16, row_bytes = f8 ? 2 * D + 2 : 4 * D;
+    const int64_t n = (longest + P - 1) / P;
+    p.few = chunks ? few : INT32_MAX;
+    p.least = kFewThreads / kWave;
+    p.one_split = kOneSplitBytes / row_bytes / P;
+    const int64_t round = std::max<int64_t>(cus / NKV, 1);
+    if (alike) {
+      const int64_t most = (n + p.least - 1) / p.least;
+      p.splits = n <= p.one_split ? 1 : (int)std::max<int64_t>(std::min({round / B, most, (int64_t)64}), 1);
+      split_grid = B * p.splits * NKV;
+    } else {
+      // One round of workgroups, and two for a batch of many rows, whose splits are coarser (us, 8 kv heads of 2 q, head_dim 128, one round /
+      // two: 32 rows of 512 .. 8192 of 8 bits 78 / 67, 64 of 128 .. 2048 56 / 52; 8 of 512 .. 8192 30.1 / 29.8; 4 of 1024 .. 16384 of 8 bits 18.7
+      // / 21.0; three and four rounds take as long or longer).
+      const int64_t units = N / ((chunks ? kLongCols : cols) / G) + B;
+      p.splits = n <= p.one_split ? 0 : (int)(units * 2 > round ? 2 * round : round);
+      p.lanes = units * 2 > round ? (int)round : 0;
+      split_grid = (units * 2 <= p.splits ? p.splits : p.splits + units) * NKV;
+    }
+  }
+  if (std::max({chunk_grid, merge_grid, split_grid}) > kMaxGrid) return BZ_ERR_SHAPE;
+
+  using Fn = void (*)(const PagedParams);
+  static_assert(kPreThreads == kFewThreads, "all by one launch()");
+  auto launch = [&](Fn fn, int64_t grid, const PagedParams& params) {
+    hipLaunchKernelGGL(fn, dim3((unsigned)grid), dim3(kFewThreads), 0, stream, params);
+    return hipGetLastError() == hipSuccess ? BZ_OK : BZ_ERR_LAUNCH;
+  };
+  if (chunks) {
     const Fn fns[2][2][3] = {{{paged_chunk_kernel<64, false, 1>, paged_chunk_kernel<64, false, 2>, paged_chunk_kernel<64, false, 4>},
                               {paged_chunk_kernel<64, true, 1>, paged_chunk_kernel<64, true, 2>, paged_chunk_kernel<64, true, 4>}},
                              {{paged_chunk_kernel<128, false, 1>, paged_chunk_kernel<128, false, 2>, paged_chunk_kernel<128, false, 4>},
                               {paged_chunk_kernel<128, true, 1>, paged_chunk_kernel<128, true, 2>, paged_chunk_kernel<128, true, 4>}}};
-    const Fn merges[2][2] = {{paged_merge_kernel<64, false>, paged_merge_kernel<64, true>},
-                             {paged_merge_kernel<128, false>, paged_merge_kernel<128, true>}};
-    hipLaunchKernelGGL(fns[D == 128][f8][cg / 2], dim3((unsigned)grid), dim3(kPreThreads), 0, stream, p);
-    if (hipGetLastError() != hipSuccess) return BZ_ERR_LAUNCH;
-    if (p.splits > 0) {
-      hipLaunchKernelGGL(merges[D == 128][f8], dim3((unsigned)merge_grid), dim3(kPreThreads), 0, stream, p);
-      if (hipGetLastError() != hipSuccess) return BZ_ERR_LAUNCH;
+    rc = launch(fns[D == 128][f8][cg / 2], chunk_grid, pc);
+    if (rc != BZ_OK) return rc;
+    if (merge_grid > 0) {
+      const Fn merges[2][2] = {{paged_merge_kernel<64, false>, paged_merge_kernel<64, true>},
+                               {paged_merge_kernel<128, false>, paged_merge_kernel<128, true>}};
+      rc = launch(merges[D == 128][f8], merge_grid, pc);
     }
-    if (!small) return BZ_OK;
+    if (rc != BZ_OK || !small) return rc;
   }
-
-  // rows of few tokens (all of them, if there are no others)
-  const int P = f8 ? 32 : 16, row_bytes = f8 ? 2 * D + 2 : 4 * D;
-  const int64_t n = (longest + P - 1) / P;
-  p.few = chunks ? few : INT32_MAX;
-  p.least = kFewThreads / kWave;
-  p.one_split = kOneSplitBytes / row_bytes / P;
-  const int64_t round = std::max<int64_t>(cus / NKV, 1);
-  const bool alike = c->q_start == nullptr && B <= 3;
-  int64_t grid;
-  if (alike) {
-    const int64_t most = (n + p.least - 1) / p.least;
-    p.splits = n <= p.one_split ? 1 : (int)std::max<int64_t>(std::min({round / B, most, (int64_t)64}), 1);
-    grid = B * p.splits * NKV;
-  } else {
-    const int tpt = (chunks ? kLongCols : cols) / G;
-    const int64_t units = N / tpt + B;
-    p.splits = n <= p.one_split ? 0 : (int)(units * 2 > round ? 2 * round : round);
-    p.lanes = units * 2 > round ? (int)round : 0;
-    grid = (units * 2 <= p.splits ? p.splits : p.splits + units) * NKV;
-  }
-  if (grid > kMaxGrid) return BZ_ERR_SHAPE;
   const Fn fns[2][2][3] = {
       {{paged_split_kernel<64, false, false, 1, kFewThreads>, paged_split_kernel<64, false, true, 1, kFewThreads>,
         paged_split_kernel<64, false, true, 2, kFewThreads>},
@@ -193,8 +208,7 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
         paged_split_kernel<128, false, true, 2, kFewThreads>},
        {paged_split_kernel<128, true, false, 1, kFewThreads>, paged_split_kernel<128, true, true, 1, kFewThreads>,
         paged_split_kernel<128, true, true, 2, kFewThreads>}}};
-  hipLaunchKernelGGL(fns[D == 128][f8][alike ? 0 : cols == kWideCols ? 2 : 1], dim3((unsigned)grid), dim3(kFewThreads), 0, stream, p);
-  return hipGetLastError() == hipSuccess ? BZ_OK : BZ_ERR_LAUNCH;
+  return launch(fns[D == 128][f8][alike ? 0 : cols == kWideCols ? 2 : 1], split_grid, p);
 }
 
 }  // extern "C"

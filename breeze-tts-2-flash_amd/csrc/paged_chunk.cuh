@@ -64,6 +64,17 @@ __device__ __forceinline__ void paged_careful(const PagedParams& p, int h, int r
   for (int i = 0; i < DV; ++i) o[DV * lane + i] = f32_to_bf16(l == 0.f ? 0.f : acc[i] / l);
 }
 
+// LDS of one tile of K or V: TP rows of D bf16, in 16-byte chunks. Chunk c of row r lies in slot c ^ swizzle(r): the 16 lanes of a cycle of
+// a K read take the same chunk of 16 rows, the 32 of a transposing V read four chunks each of four rows, and either way they fall
+// into all 64 banks, as do the 16 lanes that write rows of 8 bits, four rows of the same chunks in each quarter (with V swizzled for
+// reads of 16 lanes, as window_prefill.cuh does, a third of the LDS cycles were conflicts).
+template <int D, int TP>
+struct ChunkLds {
+  static constexpr int kRow = 2 * D, kBytes = TP * kRow;
+  static __device__ __forceinline__ int k_swz(int r) { return r & (D / 8 - 1); }
+  static __device__ __forceinline__ int v_swz(int r) { return D == 128 ? 5 * (r & 3) : 5 * ((r >> 1) & 1); }
+};
+
 // How a column tile of n steps is cut: `per` steps a split, nact of them.
 struct ChunkCut {
   int per, nact;
@@ -76,7 +87,7 @@ __device__ __forceinline__ ChunkCut cut_chunk(int n, int k) {
 // 16 rows of 8-bit codes on their way to LDS: lane l holds the D / 4 dims from (D / 4) (l % 4) on of row l / 4, and its scale.
 template <int D>
 struct F8Rows {
-  uint4 c[D / 64];
+  uint2 c[D / 32];
   uint32_t e;
 };
 
@@ -90,7 +101,7 @@ __global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const Paged
   constexpr int PG = 4 / CG, TP = PG == 1 ? kChunkStep : 32, NB = TP / 32, NQ = D / 16, ND = D / 32, COLS = CG * kPreWaveCols;
   constexpr int BL = TP / 16, UB = BL / CG;         // blocks of 16 positions of a tile, and those that a wave stages
   constexpr int WS = kWave / BL;                    // steps whose pages a wave holds
-  using L = PreLds<D, TP>;
+  using L = ChunkLds<D, TP>;
   const int at = (int)(blockIdx.x / (uint32_t)p.NKV), h = (int)blockIdx.x - at * p.NKV;
   const PagedShare share = deal_paged<true, false, kChunkStep, 1>(p, COLS, at);
   if (share.b < 0) return;
@@ -102,13 +113,6 @@ __global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const Paged
   const int mine = kPreWaveCols * cg + c, tok = t0 + min(mine >> p.gshift, ntok - 1), hq = (h << p.gshift) + (mine & (p.G - 1));
 
   const float scale = positive_scale(p.scale_log2);
-  bf16x8_t qf[NQ];
-  {
-    const uint16_t* src = p.q + (int64_t)(row.q0 + tok) * p.q_st + (int64_t)hq * p.q_sh + 8 * half;
-#pragma unroll
-    for (int j = 0; j < NQ; ++j) qf[j] = signed_q(*reinterpret_cast<const uint4*>(src + 16 * j), p.scale_log2);
-  }
-
   auto token_end = [&](int t) { return paged_end(p.rows, row, t); };
   const int my_end = token_end(tok), e1 = wave_uniform(token_end(t0 + ntok - 1)), last = e1 - 1;
   const int whole_end = wave_uniform(token_end(t0 + min((kPreWaveCols * cg) >> p.gshift, ntok - 1)));  // of the wave's columns
@@ -179,9 +183,11 @@ __global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const Paged
       const Rsrc rs = span_rsrc((V ? p.vs : p.ks) + page * p.sc_sp + shead, pmask + 1);
       const int at = place(pos_of(j) + 16 * (cg * UB + b) + lane / 4);
 #pragma unroll
-      for (int i = 0; i < D / 64; ++i)
-        x[b].c[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(
-                                                  rsrc, (uint32_t)at * p.kv_ss + (D / 4) * (lane % 4) + 16 * i, 0, 0));
+      for (int i = 0; i < D / 32; i += 2) {
+        const uint4 y = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                      rsrc, (uint32_t)at * p.kv_ss + (D / 4) * (lane % 4) + 8 * i, 0, 0));
+        x[b].c[i] = make_uint2(y.x, y.y), x[b].c[i + 1] = make_uint2(y.z, y.w);
+      }
       x[b].e = __builtin_amdgcn_raw_buffer_load_b8(rs, at, 0, 0);
     }
   };
@@ -191,13 +197,10 @@ __global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const Paged
     for (int b = 0; b < UB; ++b) {
       const int rw = 16 * (cg * UB + b) + lane / 4, swz = V ? L::v_swz(rw) : L::k_swz(rw);
 #pragma unroll
-      for (int i = 0; i < D / 64; ++i)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const uint2 code = u ? make_uint2(x[b].c[i].z, x[b].c[i].w) : make_uint2(x[b].c[i].x, x[b].c[i].y);
-          const int ch = (D / 32) * (lane % 4) + 2 * i + u;
-          *reinterpret_cast<uint4*>(buf + group + rw * L::kRow + 16 * (ch ^ swz)) = bz::f8_values(code, x[b].e);
-        }
+      for (int i = 0; i < D / 32; ++i) {
+        const int ch = (D / 32) * (lane % 4) + i;
+        *reinterpret_cast<uint4*>(buf + group + rw * L::kRow + 16 * (ch ^ swz)) = bz::f8_values(x[b].c[i], x[b].e);
+      }
     }
   };
   constexpr std::false_type isk{};
@@ -234,6 +237,7 @@ __global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const Paged
   constexpr int AHEAD = F8 ? 3 : 2;
   Pages vpage{};
   uint32_t holes = 0;
+  bf16x8_t qf[NQ];
   F8Rows<D> kr[UB], vr[UB];
   // products of K q, pairs of terms beside each, reads ahead (8 bits, D 128: fewer, for the registers)
   constexpr int NK = NB * NQ, PT = 8 * NB / NK, AH = F8 && D == 128 && CG == 4 ? 4 : 8, KA = NK < AH ? NK : AH;
@@ -328,7 +332,14 @@ __global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const Paged
     }
   };
   if (n > 0) {
+    // the table's entries, q and the first tiles are asked for one behind the other, and waited for as they are needed
     fetch(0);
+    uint4 qr[NQ];
+    {
+      const uint16_t* src = p.q + (int64_t)(row.q0 + tok) * p.q_st + (int64_t)hq * p.q_sh + 8 * half;
+#pragma unroll
+      for (int j = 0; j < NQ; ++j) qr[j] = *reinterpret_cast<const uint4*>(src + 16 * j);
+    }
     settle();
     const Pages page0 = page_at(0), page1 = page_at(1);  // (behind the last step: any page, unused)
     holes = odd_at(0) | odd_at(1) << BL;
@@ -346,16 +357,19 @@ __global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const Paged
       if (n > 2) load8(isk, kr, 2, vpage);
       if (n > 1) load8(isv, vr, 1, page1);
     } else {
+      constexpr int LOADS = UB * 16 * L::kRow / 1024;  // of a wave for a tile
+      auto all_but = [](int n) { return 0x0f70 | (n & 15) | (n >> 4) << 14; };
       stage(isk, k_even, 0, page0);
-      vpage = page1;
-    }
-    if constexpr (!F8) __builtin_amdgcn_s_waitcnt(0x0f70);
-    if constexpr (CG > 1) __syncthreads();
-    else asm volatile("" ::: "memory");
-    if constexpr (!F8) {
       if (n > 1) stage(isk, k_odd, 1, page1);
       stage(isv, v_even, 0, page0);
+      vpage = page1;
+      if (n > 1) __builtin_amdgcn_s_waitcnt(all_but(2 * LOADS));  // q and K 0 are there
+      else __builtin_amdgcn_s_waitcnt(all_but(LOADS));
     }
+    if constexpr (CG > 1) __syncthreads();
+    else asm volatile("" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) qf[j] = signed_q(qr[j], p.scale_log2);
 #pragma unroll
     for (int i = 0; i < NK; ++i)
       xa[i % NB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_read(k_even, i), qf[i / NB], i < NB ? f32x16_t{} : xa[i % NB], 0, 0, 0);
