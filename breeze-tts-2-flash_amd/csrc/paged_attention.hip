@@ -154,10 +154,15 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
   }
 
   // The split kernel's, for rows of few tokens (all of them, if there are no others).
-  const bool alike = c->q_start == nullptr && B <= 3;
+  // One token a row, and no dealing: two or three rows, taken to be alike, and batches of so many that rows may stay whole, whose
+  // dealing takes each workgroup a look at all (us, 8 kv heads of 2 q, head_dim 128, dealt / whole: 256 rows of 50 .. 200 36.7 / 26.4, of
+  // 500 .. 2000 209 / 207; 128 rows 18.8 / 16.2, 113 / 113). The longest row alone may take no longer than the batch does.
+  const int row_bytes = f8 ? 2 * D + 2 : 4 * D;  // of a position
+  const bool many = B * NKV >= 4 * cus && longest * row_bytes <= 4 * kOneSplitBytes * (B * NKV / (4 * cus));
+  const bool alike = c->q_start == nullptr && (B <= 3 || many);
   int64_t split_grid = 0;
   if (small) {
-    const int P = f8 ? 32 : 16, row_bytes = f8 ? 2 * D + 2 : 4 * D;
+    const int P = f8 ? 32 : 16;
     const int64_t n = (longest + P - 1) / P;
     p.few = chunks ? few : INT32_MAX;
     p.least = kFewThreads / kWave;
@@ -165,14 +170,14 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
     const int64_t round = std::max<int64_t>(cus / NKV, 1);
     if (alike) {
       const int64_t most = (n + p.least - 1) / p.least;
-      p.splits = n <= p.one_split ? 1 : (int)std::max<int64_t>(std::min({round / B, most, (int64_t)64}), 1);
+      p.splits = many || n <= p.one_split ? 1 : (int)std::max<int64_t>(std::min({round / B, most, (int64_t)64}), 1);
       split_grid = B * p.splits * NKV;
     } else {
       // One round of workgroups, and two for a batch of many rows, whose splits are coarser (us, 8 kv heads of 2 q, head_dim 128, one round /
       // two: 32 rows of 512 .. 8192 of 8 bits 78 / 67, 64 of 128 .. 2048 56 / 52; 8 of 512 .. 8192 30.1 / 29.8; 4 of 1024 .. 16384 of 8 bits 18.7
       // / 21.0; three and four rounds take as long or longer).
       const int64_t units = N / ((chunks ? kLongCols : cols) / G) + B;
-      p.splits = n <= p.one_split ? 0 : (int)(units * 2 > round ? 2 * round : round);
+      p.splits = n <= p.one_split ? 0 : (int)std::min<int64_t>(units * 2 > round ? 2 * round : round, p.part_slots / 2);
       p.lanes = units * 2 > round ? (int)round : 0;
       split_grid = (units * 2 <= p.splits ? p.splits : p.splits + units) * NKV;
     }

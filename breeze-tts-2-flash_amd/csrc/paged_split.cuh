@@ -84,14 +84,11 @@ __device__ __forceinline__ PagedShare deal_paged(const PagedParams& p, int cols,
     PagedRow r;
     int nt, n;  // its column tiles, and the position tiles of the longest
   };
-  auto row_at = [&](int b) {
-    Row x{{0, 0, 0}, 0, 0};
-    if (b < B) {
-      x.r = paged_row(p.rows, b);
-      if (x.r.T > 0 && (x.r.T > p.few) == CHUNK) {
-        x.nt = (x.r.T + (1 << tshift) - 1) >> tshift;
-        x.n = (paged_end(p.rows, x.r, x.r.T - 1) + P - 1) / P;
-      }
+  auto row_at = [&](int b) {  // (loads without a branch, so that those of several rows can be on their way)
+    Row x{paged_row(p.rows, min(b, B - 1)), 0, 0};
+    if (b < B && x.r.T > 0 && (x.r.T > p.few) == CHUNK) {
+      x.nt = (x.r.T + (1 << tshift) - 1) >> tshift;
+      x.n = (paged_end(p.rows, x.r, x.r.T - 1) + P - 1) / P;
     }
     return x;
   };
@@ -101,13 +98,15 @@ __device__ __forceinline__ PagedShare deal_paged(const PagedParams& p, int cols,
     return inv == 0.f || x.n <= p.one_split ? 1 : max(1, (int)__builtin_ceilf((float)x.n * inv));
   };
   if (p.splits > 0) {
-    float total = 0.f, units = 0.f, most = 0.f;
-    for (int b0 = 0; b0 < B; b0 += kWave) {
-      const Row x = b0 == 0 ? first : row_at(b0 + lane);
-      total += wave_sum((float)x.nt * (float)x.n);
-      units += wave_sum((float)x.nt);
-      most = fmaxf(most, wave_max((float)x.n));
+    float total = (float)first.nt * (float)first.n, units = (float)first.nt, most = (float)first.n;
+#pragma unroll 4
+    for (int b0 = kWave; b0 < B; b0 += kWave) {
+      const Row x = row_at(b0 + lane);
+      total += (float)x.nt * (float)x.n;
+      units += (float)x.nt;
+      most = fmaxf(most, (float)x.n);
     }
+    total = wave_sum(total), units = wave_sum(units), most = wave_max(most);
     // (a chunk's splits: two rounds of workgroups where each still has 12 steps, else one: their sums' way through memory costs more)
     const float want = CHUNK && total < 12.f * (float)p.splits ? fmaxf(0.5f * (float)p.splits, 1.f) : (float)p.splits, even = 1.00001f * total;
     // Whole column tiles where those keep the device as busy: `lanes` workgroups of a head at a time, each the longest's time.
@@ -138,8 +137,9 @@ __device__ __forceinline__ PagedShare deal_paged(const PagedParams& p, int cols,
     inv = whole ? 0.f : 0.99999f * __builtin_amdgcn_rcpf(per);
   }
   int seen = 0, parts = 0;
+  Row x = first;
   for (int b0 = 0; b0 < B; b0 += kWave) {
-    const Row x = b0 == 0 ? first : row_at(b0 + lane);
+    const Row next = b0 + kWave < B ? row_at(b0 + kWave + lane) : first;
     const int k = splits_of(x), mine = PER_TILE ? x.nt : x.nt * k, part = k > 1 ? x.nt * k : 0;
     const int last = seen + (int)wave_scan((uint32_t)mine), pl = parts + (int)wave_scan((uint32_t)part);
     const uint64_t hit = __ballot(at < last && at >= last - mine);
@@ -152,6 +152,7 @@ __device__ __forceinline__ PagedShare deal_paged(const PagedParams& p, int cols,
     }
     seen = __builtin_amdgcn_readlane(last, kWave - 1);
     parts = __builtin_amdgcn_readlane(pl, kWave - 1);
+    x = next;
   }
   return {-1, 0, 0, 1, 0, {0, 0, 0}};
 }
