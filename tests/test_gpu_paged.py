@@ -303,6 +303,11 @@ CHUNK_CASES = [
     ([1500], [70], 64, 8, 2, 128), ([0, 900, 77, 300], [200, 1, 2, 1], 16, 2, 2, 128), ([4000, 10], [40, 0], 256, 1, 8, 64),
     ([63, 64, 65], [65, 64, 63], 64, 2, 1, 64), ([700, 20, 0, 5, 1], [9, 300, 1, 1, 17], 16, 4, 4, 128), ([0], [1000], 128, 2, 2, 128),
     ([10] * 70, [20, 1] * 35, 16, 1, 2, 64),
+    # as many columns as the chunk kernels take: one, two and four column groups a workgroup, and positions split
+    ([0, 700], [100, 60], 16, 8, 8, 64), ([1500, 300], [60, 9], 32, 8, 8, 128), ([0, 33, 7], [100, 90, 130], 16, 8, 8, 64),
+    ([200, 90], [150, 140], 64, 8, 8, 128), ([9], [400], 16, 8, 4, 128), ([0, 17], [800, 790], 16, 8, 8, 64),
+    ([40], [1560], 64, 8, 8, 64), ([3000, 77], [110, 100], 16, 8, 4, 128), ([6000], [70], 256, 8, 8, 64), ([5000, 1, 2500], [40, 0, 50], 16, 16, 4, 128),
+    ([2100, 900, 30, 600], [90, 1, 100, 2], 16, 8, 8, 128), ([0, 33, 7], [200, 190, 130], 16, 8, 8, 64), ([0], [1540], 64, 8, 8, 128),
 ]
 
 
@@ -326,23 +331,48 @@ def test_chunks(device, case, bits):
     check(out, q, k, v, b, D ** -0.5, G, False, "few")
 
 
-@pytest.mark.parametrize("T", [1, 40])
+@pytest.mark.parametrize("seed", range(60))
+def test_random_batches(device, seed):
+    """Batches of any rows, page sizes, groups and hints, right or wrong."""
+    rng = np.random.default_rng(1000 + seed)
+    pick = lambda *a: a[rng.integers(len(a))]  # noqa: E731
+    D, bits, page, NKV, G = pick(64, 128), pick(8, 16), pick(16, 32, 64, 512), pick(1, 2, 3, 8), pick(1, 2, 4, 8)
+    rows = int(rng.integers(1, 7))
+    new = [int(pick(0, 1, 1, 2, 5, rng.integers(1, 40), rng.integers(1, 200))) for _ in range(rows)]
+    new[0] = max(new[0], 1)
+    past = [int(pick(0, rng.integers(0, 100), rng.integers(0, 1500))) for _ in range(rows)]
+    b = Batch(rng, past, new, page, NKV, D, device, bits, spare=int(rng.integers(0, 3)), first=int(rng.integers(0, 2)))
+    for _ in range(int(pick(0, 0, 2))):  # a hole
+        b.table[rng.integers(rows), rng.integers(b.table.shape[1])] = -1
+    cache, k, v = filled(b, rng, spread=float(pick(1.0, 100.0)))
+    q = randn(rng, b.N, NKV * G, D)
+    out = torch.full((b.N, NKV * G, D), 9.0, dtype=BF16, device=device)
+    table, lens = b.args()
+    pkg.gqa_paged(q.to(device), cache, table, lens, D ** -0.5, b.starts(), out, max_tokens=int(pick(0, 0, max(new), 1, 10)),
+                  max_seq_len=int(pick(0, max(b.lens), 50, 100000)))
+    torch.cuda.synchronize()
+    check(out, q, k, v, b, D ** -0.5, G, True, str((past, new, page, NKV, G, D, bits)))
+    assert (out[:b.q_start[0]] == 9).all() and (out[b.q_start[-1]:] == 9).all()
+
+
+@pytest.mark.parametrize("T,NKV,G,D,past", [(1, 2, 2, 128, 0), (40, 2, 2, 128, 0), (40, 8, 8, 64, 0), (70, 8, 8, 64, 0), (60, 8, 8, 128, 2500),
+                                          (80, 8, 8, 128, 0)])
 @pytest.mark.parametrize("bits", [8, 16])
-def test_holes_and_bad_pages(device, T, bits):
+def test_holes_and_bad_pages(device, T, NKV, G, D, past, bits):
     """Pages outside the cache in the middle of a row hold nothing; shared pages are read for each; a row of holes gives zeros."""
     rng = np.random.default_rng(T)
-    b = Batch(rng, [600, 300, 200, 90], [T] * 4, 16, 2, 128, device, bits)
+    b = Batch(rng, [600 + past, 300, 200, 90], [T] * 4, 16, NKV, D, device, bits)
     b.table[0, 3:9], b.table[0, 20] = -1, b.pages
     b.table[1, :10] = b.table[0, 9:19]  # shared with row 0
     b.table[2, :] = 2 ** 31 - 1
     b.table[3, 2] = b.table[3, 1]  # twice in one row
     b.table[3, 3] = -2 ** 31
     cache, k, v = filled(b, rng)
-    q = randn(rng, b.N, 4, 128)
+    q = randn(rng, b.N, NKV * G, D)
     table, lens = b.args()
-    out = pkg.gqa_paged(q.to(device), cache, table, lens, 128 ** -0.5, b.starts())
+    out = pkg.gqa_paged(q.to(device), cache, table, lens, D ** -0.5, b.starts())
     torch.cuda.synchronize()
-    check(out, q, k, v, b, 128 ** -0.5, 2, T > 8)
+    check(out, q, k, v, b, D ** -0.5, G, T > 8)
     assert (out[2 * T:3 * T] == 0).all()
 
 
@@ -350,44 +380,46 @@ def test_holes_and_bad_pages(device, T, bits):
 def test_rows_without_positions(device, bits):
     """Lengths of zero, below zero, shorter than the chunk, and past the table."""
     rng = np.random.default_rng(5)
-    for new in ([1, 1, 1, 1, 1], [40, 30, 20, 50, 17]):
-        b = Batch(rng, [100] * 5, new, 32, 1, 64, device, bits)
+    for new, NKV, G in (([1, 1, 1, 1, 1], 1, 2), ([40, 30, 20, 50, 17], 1, 2), ([140, 130, 120, 150, 117], 8, 8), ([900, 700, 1000, 800, 600], 8, 8)):
+        b = Batch(rng, [100] * 5, new, 32, NKV, 64, device, bits)
         b.lens = [0, -7, max(new[2] // 2, 1), b.lens[3], 4000]
         cache, k, v = filled(b, rng)
-        q = randn(rng, b.N, 2, 64)
+        q = randn(rng, b.N, NKV * G, 64)
         table, lens = b.args()
         out = pkg.gqa_paged(q.to(device), cache, table, lens, 0.125, b.starts())
         torch.cuda.synchronize()
-        ref = check(out, q, k, v, b, 0.125, 2, max(new) > 8)
+        ref = check(out, q, k, v, b, 0.125, G, max(new) > 8)
         assert (out[:b.q_start[2]] == 0).all() and (ref[:b.q_start[2]] == 0).all()
 
 
-@pytest.mark.parametrize("T,G,hint", [(1, 2, 0), (5, 2, 0), (60, 2, 0), (33, 4, 0), (5, 2, 5), (10, 2, 10), (13, 4, 13), (60, 2, 1)])
+@pytest.mark.parametrize("T,NKV,G,hint,past", [
+    (1, 2, 2, 0, 130), (5, 2, 2, 0, 130), (60, 2, 2, 0, 130), (33, 2, 4, 0, 130), (5, 2, 2, 5, 130), (10, 2, 2, 10, 130), (13, 2, 4, 13, 130),
+    (60, 2, 2, 1, 130), (100, 8, 8, 0, 130), (40, 8, 8, 0, 3000), (300, 8, 8, 0, 40)])
 @pytest.mark.parametrize("bits", [8, 16])
 @pytest.mark.parametrize("value", [float("nan"), float("inf")])
-def test_later_tokens_values_stay_out(device, T, G, hint, bits, value):
+def test_later_tokens_values_stay_out(device, T, NKV, G, hint, past, bits, value):
     """A non-finite value at a token's own position reaches that token and those behind it, and no other."""
     rng = np.random.default_rng(T + G)
-    b = Batch(rng, [130, 70], [T, T], 16, 2, 128, device, bits)
+    b = Batch(rng, [past, 70], [T, T], 16, NKV, 128, device, bits)
     cache, k, v = filled(b, rng)
     at = T // 2
-    pg, pl = place_of(b.table, 16, b.pages, 0, 130 + at)
+    pg, pl = place_of(b.table, 16, b.pages, 0, past + at)
     v[pg, 1, pl] = 0  # for the oracle, whose products with 0 would spread it; no token compared attends it
     if bits == 8:
         cache.v_scale[pg, 1, pl] = 255
     else:
         cache.v[pg, 1, pl, 3:5] = value
-    q = randn(rng, b.N, 2 * G, 128)
+    q = randn(rng, b.N, NKV * G, 128)
     table, lens = b.args()
     out = pkg.gqa_paged(q.to(device), cache, table, lens, 128 ** -0.5, b.starts(), max_tokens=hint)
     torch.cuda.synchronize()
     ref, spread, reach = paged_attention(f64(q), k, v, b.table, b.lens, b.q_start, 128 ** -0.5)
     got = f64(out)
-    clean = np.ones((b.N, 2 * G), bool)
-    clean[at:T, G:] = False
+    clean = np.ones((b.N, NKV * G), bool)
+    clean[at:T, G:2 * G] = False
     excess = np.abs(got - ref) - attention_bound(ref, spread, reach, 128 ** -0.5, 128, T > 16 // G and hint == 0)
     assert np.isfinite(got[clean]).all() and excess[clean].max() <= 0
-    hit = got[at:T, G:]
+    hit = got[at:T, G:2 * G]
     if bits == 8 or np.isnan(value):
         assert np.isnan(hit[..., 3:5] if bits == 16 else hit).all()
     else:
@@ -396,32 +428,32 @@ def test_later_tokens_values_stay_out(device, T, G, hint, bits, value):
         assert np.isfinite(np.delete(hit, [3, 4], -1)).all()
 
 
-@pytest.mark.parametrize("T", [1, 30])
-def test_scores_without_bounds(device, T):
+@pytest.mark.parametrize("T,NKV,G,past", [(1, 1, 2, 200), (30, 1, 2, 200), (150, 8, 8, 200), (60, 8, 8, 4000)])
+def test_scores_without_bounds(device, T, NKV, G, past):
     """Scores of -inf give zeros where there are no others, a NaN scale gives NaN, a scale of 0 the mean, a negative one its own."""
     rng = np.random.default_rng(T)
-    b = Batch(rng, [200, 0], [T, 0], 32, 1, 64, device)
+    b = Batch(rng, [past, 0], [T, 0], 32, NKV, 64, device)
     cache, k, v = filled(b, rng)
-    q = randn(rng, b.N, 2, 64)
+    q = randn(rng, b.N, NKV * G, 64)
     q[..., 0] = 1
     table, lens = b.args()
     call = lambda c, s: pkg.gqa_paged(q.to(device), c, table, lens, s, b.starts())  # noqa: E731
     for s in (0.0, -0.2):
         out = call(cache, s)
         torch.cuda.synchronize()
-        check(out, q, k, v, b, s, 2, T > 8)
+        check(out, q, k, v, b, s, G, T > 8)
     assert torch.isnan(call(cache, float("nan"))).all()
     down = cache._replace(k=cache.k.clone())
     down.k[..., 0] = float("-inf")
     assert (call(down, 0.2) == 0).all()
 
 
-@pytest.mark.parametrize("T", [1, 3, 50])
+@pytest.mark.parametrize("T,NKV,G", [(1, 2, 2), (3, 2, 2), (50, 2, 2), (100, 8, 8)])
 @pytest.mark.parametrize("bits", [8, 16])
-def test_layouts(device, T, bits):
+def test_layouts(device, T, NKV, G, bits):
     """K and V side by side in one tensor, heads behind positions, strided q and out, a table and lengths in the middle of others."""
     rng = np.random.default_rng(T + bits)
-    NKV, G, D = 2, 2, 64
+    D = 64
     b = Batch(rng, [150, 33, 64], [T] * 3, 16, NKV, D, device, bits)
     cache, k, v = filled(b, rng)
     raw = [x.view(torch.uint8) for x in cache[:2]] if bits == 8 else list(cache[:2])
@@ -513,12 +545,12 @@ def test_long_row_and_far_pages(device):
 
 # ------------------------------------------------------------------------------------------- streams and graphs
 
-@pytest.mark.parametrize("T", [1, 60])
-def test_graph_follows_the_device(device, T):
+@pytest.mark.parametrize("T,NKV,G", [(1, 2, 2), (60, 2, 2), (100, 8, 8)])
+def test_graph_follows_the_device(device, T, NKV, G):
     """A captured step replayed with lengths, tables and tokens changed on the device, with eager work between, each replay against the
     eager result."""
     rng = np.random.default_rng(T)
-    NKV, G, D, page, B = 2, 2, 128, 16, 3
+    D, page, B = 128, 16, 3
     cache = pkg.paged_cache(64, NKV, page, D, device)
     table = ints(np.arange(60).reshape(3, 20).tolist(), device)
     N = B * T
@@ -556,7 +588,8 @@ def test_two_streams_at_once(device):
     """Each stream has a workspace of its own, calls of all sizes share it."""
     rng = np.random.default_rng(1)
     cases = []
-    for past, new, NKV, G, D in (([3000, 50], [1, 1], 2, 4, 128), ([100, 2000], [50, 70], 2, 2, 128), ([5000], [1], 1, 8, 64), ([900] * 9, [3] * 9, 8, 2, 64)):
+    for past, new, NKV, G, D in (([3000, 50], [1, 1], 2, 4, 128), ([100, 2000], [50, 70], 2, 2, 128), ([5000], [1], 1, 8, 64), ([900] * 9, [3] * 9, 8, 2, 64),
+                                  ([3000, 9], [100, 1], 8, 8, 128), ([0], [300], 8, 8, 64)):
         b = Batch(rng, past, new, 16, NKV, D, device)
         cache, _, _ = filled(b, rng)
         q = randn(rng, b.N, NKV * G, D).to(device)
@@ -577,9 +610,9 @@ def test_two_streams_at_once(device):
 
 def test_same_bits_every_time(device):
     rng = np.random.default_rng(2)
-    b = Batch(rng, [7000, 4000, 20, 900], [1, 33, 100, 2], 16, 2, 128, device)
+    b = Batch(rng, [7000, 4000, 20, 900], [1, 133, 100, 2], 16, 8, 128, device)
     cache, _, _ = filled(b, rng)
-    q = randn(rng, b.N, 8, 128).to(device)
+    q = randn(rng, b.N, 32, 128).to(device)
     first = pkg.gqa_paged(q, cache, *b.args(), 128 ** -0.5, b.starts())
     for _ in range(5):
         assert torch.equal(pkg.gqa_paged(q, cache, *b.args(), 128 ** -0.5, b.starts()), first)
