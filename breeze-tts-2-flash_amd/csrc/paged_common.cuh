@@ -5,7 +5,7 @@
 #include "bz_paged_cache.h"
 #include "device_common.cuh"
 
-constexpr int64_t kMaxGrid = INT32_MAX;
+constexpr int64_t kMaxGrid = (1 << 24) - 1;  // of 256 threads: HIP takes fewer than 2^32 in a dimension
 constexpr int64_t kMaxPositions = 1 << 30;  // sums of positions, tokens and tile sizes stay in 32 bits
 
 namespace bz {

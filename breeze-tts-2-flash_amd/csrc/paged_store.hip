@@ -390,7 +390,7 @@ BZ_EXPORT int bz_paged_store(const bz_paged_store_args* a, hipStream_t stream) {
   p.positions = a->positions, p.positions_64 = a->positions_64;
   if (rope) p.turn = turn_params(a->rope, false);
   const int64_t heads = (int64_t)p.NH + 2 * (int64_t)p.NKV;
-  if (heads > kMaxGrid) return BZ_ERR_SHAPE;
+  if (heads > INT32_MAX) return BZ_ERR_SHAPE;
   const int HP = rope && c->tokens * heads >= kManyHeads ? 4 : 1;
   const int64_t per = kPagedThreads / (D / 16), grid = (c->tokens * ((heads + HP - 1) / HP) + per - 1) / per;
   if (grid > kMaxGrid) return BZ_ERR_SHAPE;
@@ -416,8 +416,9 @@ BZ_EXPORT int bz_paged_load(const bz_paged_cache* c, const int32_t* starts, int3
                     c->stride_h, c->stride_s, static_cast<const uint8_t*>(c->k_scale), static_cast<const uint8_t*>(c->v_scale),
                     c->scale_stride_page, c->scale_stride_h, starts, count, static_cast<uint16_t*>(k),
                     static_cast<uint16_t*>(v), x_stride_b, x_stride_h, x_stride_t};
-  const int per = kPagedThreads / (c->head_dim / 8);
-  const dim3 grid((unsigned)(((int64_t)count + per - 1) / per), c->num_kv_heads, c->batch);
+  const int64_t per = kPagedThreads / (c->head_dim / 8), chunks = (count + per - 1) / per;
+  if (chunks > kMaxGrid) return BZ_ERR_SHAPE;
+  const dim3 grid((unsigned)chunks, c->num_kv_heads, c->batch);
   using Fn = void (*)(const PagedLoadParams);
   const Fn fns[2][2] = {{paged_load_kernel<64, false>, paged_load_kernel<64, true>},
                         {paged_load_kernel<128, false>, paged_load_kernel<128, true>}};

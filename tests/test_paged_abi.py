@@ -114,7 +114,7 @@ def test_store_checks(lib, K, over, rope, status):
 @pytest.mark.parametrize("over,status", [
     (dict(x=None), -1), (dict(out=None), -1), (dict(positions=None), -1), (dict(tokens=0), -2), (dict(heads=0), -2), (dict(head_dim=96), -3),
     (dict(x=0x10002), -4), (dict(x_stride_h=4), -4), (dict(out_stride_t=9), -4), (dict(positions=0x50002), -4),
-    (dict(tokens=1 << 30, heads=1 << 10), -2)], ids=str)
+    (dict(tokens=1 << 30, heads=1 << 10), -2), (dict(tokens=1 << 20, heads=1 << 10), -2)], ids=str)
 def test_rope_checks(lib, K, over, status):
     a = K.RopeArgs(x=0x10000, x_stride_t=1024, x_stride_h=128, out=0x20000, out_stride_t=1024, out_stride_h=128, positions=0x50000,
                    tokens=3, heads=8, head_dim=128)
@@ -130,6 +130,7 @@ def test_load_and_workspace_checks(lib, K):
     load = lambda starts=0x10000, n=4, k=0x20000, v=0x30000, st=128: lib.bz_paged_load(  # noqa: E731
         ctypes.byref(c), starts, n, k, v, 8 * 4 * 128, 4 * 128, st, None)
     assert [load(starts=None), load(k=None), load(v=None), load(n=0), load(k=0x20008), load(st=132), load(starts=0x10002)] == [-1, -1, -1, -2, -4, -4, -4]
+    assert load(n=1 << 28) == -2  # 2^32 threads
     n = ctypes.c_size_t(0)
     size = lambda *a: lib.bz_paged_workspace_size(*a, ctypes.byref(n))  # noqa: E731
     assert [size(96, 2, 1), size(64, 3, 1), size(64, 2, -1), lib.bz_paged_workspace_size(64, 2, 1, None)] == [-3, -3, -2, -1]
