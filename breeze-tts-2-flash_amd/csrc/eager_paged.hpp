@@ -119,7 +119,14 @@ void fill_rows(PyObject* seq_lens, PyObject* q_start, int64_t N, const at::Devic
   c.tokens = (int32_t)N;
 }
 
-bool flag_arg(PyObject* o) { return PyObject_IsTrue(o) == 1; }
+bool flag_arg(PyObject* o, const char* name) {
+  const int is = PyObject_IsTrue(o);
+  if (is < 0) {
+    PyErr_Clear();
+    throw Error{std::string(name) + " must be a bool"};
+  }
+  return is != 0;
+}
 
 // A Rope's inv_freq, factor and interleaved.
 void fill_rope(PyObject* const* args, const at::Device& dev, bz_rope& r) {
@@ -130,7 +137,7 @@ void fill_rope(PyObject* const* args, const at::Device& dev, bz_rope& r) {
   r.inv_freq = f.data_ptr<double>(), r.rotary_dim = (int32_t)(2 * f.numel());
   r.factor = float_arg(args[1], "factor");
   require(std::isfinite(r.factor) && r.factor != 0.f, "factor must be finite and not 0");
-  r.interleaved = flag_arg(args[2]);
+  r.interleaved = flag_arg(args[2], "interleaved");
 }
 
 const void* positions_arg(PyObject* o, int64_t N, const at::Device& dev, int32_t& is64) {
@@ -154,7 +161,7 @@ PyObject* rope(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     bz_rope_args a{};
     a.positions = positions_arg(args[1], x.size(0), dev, a.positions_64);
     fill_rope(args + 2, dev, a.rope);
-    a.inverse = flag_arg(args[5]);
+    a.inverse = flag_arg(args[5], "inverse");
     const at::Tensor* given = tensor_or_none(args[6], "out");
     if (given != nullptr) {
       like_heads(*given, "out", x.size(0), x.size(1), x.size(2), dev);

@@ -297,6 +297,47 @@ def test_few_tokens(device, case, bits):
     assert (out[b.q_start[-1]:] == 9).all()
 
 
+@pytest.mark.parametrize("rows,longest,NKV,G,D,hint", [
+    (130, 200, 8, 2, 64, 0), (130, 200, 8, 2, 128, 1), (260, 90, 4, 1, 128, 5000), (70, 40, 32, 1, 64, 40),  # so many that rows stay whole
+    (1, 900, 300, 1, 64, 0), (3, 700, 520, 1, 64, 0), (5, 300, 300, 1, 64, 0), (2, 60, 1100, 1, 64, 0)])  # more kv heads than CUs
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_many_units(device, rows, longest, NKV, G, D, hint, bits, ragged):
+    rng = np.random.default_rng(rows + NKV)
+    past = [int(x) for x in rng.integers(0, longest, rows)]
+    new = [1] * rows
+    if ragged:
+        new[0] = 2
+    b = Batch(rng, past, new, 16, NKV, D, device, bits)
+    cache, k, v = filled(b, rng)
+    q = randn(rng, b.N, NKV * G, D)
+    table, lens = b.args()
+    out = pkg.gqa_paged(q.to(device), cache, table, lens, D ** -0.5, b.starts() if ragged else None, max_tokens=2, max_seq_len=hint)
+    torch.cuda.synchronize()
+    check(out, q, k, v, b, D ** -0.5, G, False)
+
+
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 3.0, float("nan")])
+@pytest.mark.parametrize("T,NKV,G,D,past", [(1, 2, 2, 128, 400), (12, 2, 2, 64, 400), (150, 8, 8, 64, 0), (300, 8, 8, 128, 0), (60, 8, 8, 128, 2500)])
+@pytest.mark.parametrize("bits", [8, 16])
+def test_scales(device, scale, T, NKV, G, D, past, bits):
+    """Scales of either sign and zero; one that is NaN makes every output NaN but those of tokens that attend nothing."""
+    rng = np.random.default_rng(T)
+    b = Batch(rng, [past, 0], [T, T], 32, NKV, D, device, bits)
+    b.lens[1] = T // 2
+    cache, k, v = filled(b, rng)
+    q = randn(rng, b.N, NKV * G, D)
+    table, lens = b.args()
+    out = pkg.gqa_paged(q.to(device), cache, table, lens, scale, b.starts())
+    torch.cuda.synchronize()
+    none = b.q_start[1] + T - T // 2  # the tokens up to here of the second row attend nothing
+    assert (out[b.q_start[1]:none] == 0).all()
+    if scale != scale:
+        assert out[:b.q_start[1]].isnan().all() and out[none:].isnan().all()
+    else:
+        check(out, q, k, v, b, scale, G, True)
+
+
 CHUNK_CASES = [
     # past, new, page, NKV, G, D
     ([0], [129], 16, 1, 1, 128), ([0, 0], [64, 17], 16, 2, 2, 128), ([500, 3, 0], [100, 33, 260], 32, 2, 4, 64),
@@ -660,6 +701,7 @@ def test_refusals(device):
         lambda: pkg.rope(q, pos, pkg.rope_frequencies(128, 1e4, device)), lambda: pkg.rope(q, pos, f._replace(inv_freq=f.inv_freq[:7])),
         lambda: pkg.rope(q[..., :48], pos, f), lambda: pkg.rope(q, pos, f, o[:4]), lambda: pkg.rope(q, pos, f, o[:1].expand(5, 4, 64)),
         lambda: pkg.rope(q[:4], pos[:4], f, q[1:]), lambda: pkg.rope(q.cpu(), pos, f), lambda: pkg.rope(q.view(-1)[4:4 + 256].view(1, 4, 64), pos[:1], f),
+        lambda: pkg.rope(q, pos, f, inverse=pos), lambda: pkg.rope(q, pos, f._replace(interleaved=pos)),
         lambda: pkg.paged_store(k, v, cache, table, lens), lambda: pkg.paged_store(k, v[:4], cache, table, lens, st),
         lambda: pkg.paged_store(k, v, cache, table, lens, st[:2]), lambda: pkg.paged_store(k, v, cache, table, lens[:1], st),
         lambda: pkg.paged_store(k, v, cache, table.long(), lens, st), lambda: pkg.paged_store(k.float(), v, cache, table, lens, st),
