@@ -18,29 +18,38 @@ namespace {
 
 constexpr int kFewThreads = 256;
 // Workspace: the arrival counters, then (max, sum) pairs and sums of 2 * kSlotsPerCu slots a CU, at places that depend on nothing else, so
-// that calls of all sizes can share one. A kernel's splits of all kv heads number at most kSlotsPerCu a CU, and those of rows that
-// are split at most twice that (deal_paged).
+// that calls of all sizes can share one; those of the chunk kernel behind the split kernel's, as one launch may write both. A
+// kernel's splits of all kv heads number at most kSlotsPerCu a CU, and those of rows that are split at most twice that (deal_paged).
 constexpr int kSlotsPerCu = 2;
 
 size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
+struct Parts {  // (max, sum) pairs, sums
+  size_t ml, acc;
+};
 struct Layout {
   int64_t slots;
-  size_t ml, acc, total;
+  Parts split, chunk;
+  size_t total;
 };
 Layout layout(int cus, int D, int cols) {
   Layout y;
   y.slots = (int64_t)2 * kSlotsPerCu * cus;
-  y.ml = (size_t)y.slots * kCounterStride * sizeof(int);
-  y.acc = up256(y.ml + (size_t)y.slots * cols * sizeof(float2));
-  y.total = up256(y.acc + (size_t)y.slots * cols * D * sizeof(float));
+  y.total = (size_t)y.slots * kCounterStride * sizeof(int);
+  auto room = [&](int c) {
+    const Parts x{y.total, up256(y.total + (size_t)y.slots * c * sizeof(float2))};
+    y.total = up256(x.acc + (size_t)y.slots * c * D * sizeof(float));
+    return x;
+  };
+  y.split = room(cols == kChunkCols ? kLongCols : cols);
+  y.chunk = cols == kChunkCols ? room(cols) : y.split;
   return y;
 }
 
 bool group_ok(int G) { return G == 1 || G == 2 || G == 4 || G == 8; }
 
 // Columns of a workgroup, by the most tokens of a row as far as the host knows: 16 or 32 of the split kernel up to 64 columns a row, else
-// 128 of the chunk kernel, with the split kernel for the batch's rows of at most 16 (us, 8 rows of 700 .. 8192, 8 kv heads,
+// 128 of the chunk kernel, with the split kernel's work in it for the batch's rows of at most 16 (us, 8 rows of 700 .. 8192, 8 kv heads,
 // head_dim 128, bf16 / 8 bits: 20 columns 32.9 / 30.6 by two sets of 16, 42.4 / 33.1 by 16 a workgroup, 56.1 / 58.7 by the chunk kernel;
 // 64 columns 48.1 / 41.6, 76.0 / 58.5, 57.1 / 61.0).
 constexpr int kWideCols = 2 * kLongCols, kSplitCols = 64;
@@ -93,11 +102,11 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
     // Short chunks of few heads: the split kernel for all rows. It reads K and V again for each 16 columns, but in one launch (us, split
     // kernel / chunk kernels, 100 tokens alone 6.1 / 8.6, behind 1000 10 .. 14 / 17; 4 kv heads of 2 q, head_dim 128: 300 behind 1000 18.0 /
     // 19.5, 100 behind 6000 22.8 / 26.0, 300 behind 6000 50.9 / 29.8; 2 of 2: 1000 alone 14.9 / 16.0; head_dim 64, 4 of 2: 100 behind 1000
-    // 8.8 / 10.6, 300 12.0 / 11.8). Where the batch may have rows of few tokens as well the chunk kernels take a launch more, about 6 us,
-    // in which the split kernel does 10000 tiles of 16 columns and 16 positions (2 kv heads, head_dim 64, 1151 tokens and four rows of
-    // one: 11.4 / 17.7).
+    // 8.8 / 10.6, 300 12.0 / 11.8). At head_dim 128 from a little more on where the batch may have rows of few tokens as well: a few column
+    // tiles leave CUs idle, which its splits do not (300 behind 1000 and six rows of 600 .. 1300: 18.5 / 23.4; 60 twice behind 2000, 8
+    // bits, and two of 1000 .. 2000 19.3 / 25.7; head_dim 64: 700 tokens of 2 kv heads and four rows 11.3 / 8.8).
     const int64_t most = D == 128 ? 512 + (1 << 21) / length : 1280;
-    if (columns <= (B > 1 ? most + (5 << 19) / length : most)) cols = kLongCols;
+    if (columns <= (B > 1 && D == 128 ? most + (5 << 19) / length : most)) cols = kLongCols;
   } else if (cols == kWideCols && columns * length <= 5 << 19) {
     cols = kLongCols;  // (as few tiles: two sets of columns only make a workgroup slower, 2 rows of 20 tokens behind 500 9.0 / 12.0)
   }
@@ -124,43 +133,18 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
   p.part_slots = (int)(ws.slots / NKV);
   char* const base = static_cast<char*>(a->workspace);
   p.counters = reinterpret_cast<int*>(base);
-  p.part_ml = reinterpret_cast<float2*>(base + ws.ml);
-  p.part_acc = reinterpret_cast<float*>(base + ws.acc);
+  p.part_ml = reinterpret_cast<float2*>(base + ws.split.ml);
+  p.part_acc = reinterpret_cast<float*>(base + ws.split.acc);
   const bool f8 = c->bits == 8;
-  // The chunk kernel's part: its parameters, grid and merge.
-  PagedParams pc = p;
-  int cg = 0;
-  int64_t chunk_grid = 0, merge_grid = 0;
-  if (chunks) {
-    // Workgroups of a chunk kernel with g column groups (of all kv heads; without the tiles that rows' ends leave part empty), and
-    // its column tiles at most.
-    auto tiles = [&](int g) { return (N * G + kPreWaveCols * g - 1) / (kPreWaveCols * g) * NKV; };
-    auto units = [&](int g) { return N / (kPreWaveCols * g / G) + B; };
-    const int64_t steps = longest / kChunkStep + 1;
-    // Few column tiles of 128 over many positions are split over those as well (us, 8 kv heads of 2 q, head_dim 128, whole / split: 1024
-    // tokens over 8192 105 / 82, 2048 over 16384 301 / 263, 256 over 8192 70 / 36); at head_dim 64, where one column group leaves
-    // room for two workgroups a CU, only over very many unless even that leaves CUs idle. Else the widest column tiles that give every
-    // CU work (1024 tokens alone: 26.6 by four groups, split, 18.7 by one; 4096 97 by four, 92 by two).
-    const bool idle = D == 128 || tiles(1) < cus;
-    const bool split = (tiles(4) <= cus && steps >= 32 * (2 * cus / tiles(4))) ||
-                       (tiles(2) < cus && std::min(cus / tiles(4), steps / (idle ? 14 : 64)) > 1);
-    cg = split || tiles(4) >= 3 * cus ? 4 : tiles(2) >= cus ? 2 : 1;
-    pc.few = small ? few : 0;
-    pc.splits = split ? kSlotsPerCu * cus / NKV : 0;
-    pc.least = kPreMinSteps, pc.one_split = kPreMinSteps;
-    pc.merge_cols = units(4) * NKV * (kChunkCols / 16) <= 2 * cus ? 8 : 16;
-    chunk_grid = (units(cg) * 2 <= pc.splits ? pc.splits : pc.splits + units(cg)) * NKV;
-    merge_grid = pc.splits > 0 ? units(4) * NKV * (kChunkCols / pc.merge_cols) : 0;
-  }
-
-  // The split kernel's, for rows of few tokens (all of them, if there are no others).
+  // The split kernel's part, for rows of few tokens (all of them, if there are no others; else its work goes behind that of the chunk
+  // kernel, in one launch).
   // One token a row, and no dealing: two or three rows, taken to be alike, and batches of so many that rows may stay whole, whose
   // dealing takes each workgroup a look at all (us, 8 kv heads of 2 q, head_dim 128, dealt / whole: 256 rows of 50 .. 200 36.7 / 26.4, of
   // 500 .. 2000 209 / 207; 128 rows 18.8 / 16.2, 113 / 113). The longest row alone may take no longer than the batch does.
   const int row_bytes = f8 ? 2 * D + 2 : 4 * D;  // of a position
   const bool many = B * NKV >= 4 * cus && longest * row_bytes <= 4 * kOneSplitBytes * (B * NKV / (4 * cus));
   const bool alike = c->q_start == nullptr && (B <= 3 || many);
-  int64_t split_grid = 0;
+  int64_t split_slots = 0;
   if (small) {
     const int P = f8 ? 32 : 16;
     const int64_t n = (longest + P - 1) / P;
@@ -171,7 +155,7 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
     if (alike) {
       const int64_t most = (n + p.least - 1) / p.least;
       p.splits = many || n <= p.one_split ? 1 : (int)std::max<int64_t>(std::min({round / B, most, (int64_t)64}), 1);
-      split_grid = B * p.splits * NKV;
+      split_slots = B * p.splits;
     } else {
       // One round of workgroups, and two for a batch of many rows, whose splits are coarser (us, 8 kv heads of 2 q, head_dim 128, one round /
       // two: 32 rows of 512 .. 8192 of 8 bits 78 / 67, 64 of 128 .. 2048 56 / 52; 8 of 512 .. 8192 30.1 / 29.8; 4 of 1024 .. 16384 of 8 bits 18.7
@@ -179,31 +163,64 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
       const int64_t units = N / ((chunks ? kLongCols : cols) / G) + B;
       p.splits = n <= p.one_split ? 0 : (int)std::min<int64_t>(units * 2 > round ? 2 * round : round, p.part_slots / 2);
       p.lanes = units * 2 > round ? (int)round : 0;
-      split_grid = (units * 2 <= p.splits ? p.splits : p.splits + units) * NKV;
+      split_slots = units * 2 <= p.splits ? p.splits : p.splits + units;
     }
   }
-  if (std::max({chunk_grid, merge_grid, split_grid}) > kMaxGrid) return BZ_ERR_SHAPE;
-
-  using Fn = void (*)(const PagedParams);
-  static_assert(kPreThreads == kFewThreads, "all by one launch()");
-  auto launch = [&](Fn fn, int64_t grid, const PagedParams& params) {
-    hipLaunchKernelGGL(fn, dim3((unsigned)grid), dim3(kFewThreads), 0, stream, params);
+  auto launch = [&](auto fn, int64_t blocks, const auto&... params) {
+    hipLaunchKernelGGL(fn, dim3((unsigned)blocks), dim3(kFewThreads), 0, stream, params...);
     return hipGetLastError() == hipSuccess ? BZ_OK : BZ_ERR_LAUNCH;
   };
+  p.slots = (int)split_slots;
+  using Fn = void (*)(const PagedParams);
   if (chunks) {
-    const Fn fns[2][2][3] = {{{paged_chunk_kernel<64, false, 1>, paged_chunk_kernel<64, false, 2>, paged_chunk_kernel<64, false, 4>},
-                              {paged_chunk_kernel<64, true, 1>, paged_chunk_kernel<64, true, 2>, paged_chunk_kernel<64, true, 4>}},
-                             {{paged_chunk_kernel<128, false, 1>, paged_chunk_kernel<128, false, 2>, paged_chunk_kernel<128, false, 4>},
-                              {paged_chunk_kernel<128, true, 1>, paged_chunk_kernel<128, true, 2>, paged_chunk_kernel<128, true, 4>}}};
-    rc = launch(fns[D == 128][f8][cg / 2], chunk_grid, pc);
-    if (rc != BZ_OK) return rc;
-    if (merge_grid > 0) {
-      const Fn merges[2][2] = {{paged_merge_kernel<64, false>, paged_merge_kernel<64, true>},
-                               {paged_merge_kernel<128, false>, paged_merge_kernel<128, true>}};
-      rc = launch(merges[D == 128][f8], merge_grid, pc);
-    }
-    if (rc != BZ_OK || !small) return rc;
+    // The chunk kernel's part: its parameters, grid and merge.
+    PagedParams pc = p;
+    pc.part_ml = reinterpret_cast<float2*>(base + ws.chunk.ml);
+    pc.part_acc = reinterpret_cast<float*>(base + ws.chunk.acc);
+    // Workgroups of a chunk kernel with g column groups (of all kv heads; without the tiles that rows' ends leave part empty), and
+    // its column tiles at most.
+    auto tiles = [&](int g) { return (N * G + kPreWaveCols * g - 1) / (kPreWaveCols * g) * NKV; };
+    auto units = [&](int g) { return N / (kPreWaveCols * g / G) + B; };
+    const int64_t steps = longest / kChunkStep + 1;
+    // Few column tiles of 128 over many positions are split over those as well (us, 8 kv heads of 2 q, head_dim 128, whole / split: 1024
+    // tokens over 8192 105 / 82, 2048 over 16384 301 / 263, 256 over 8192 70 / 36); at head_dim 64, where one column group leaves
+    // room for two workgroups a CU, only over very many unless even that leaves CUs idle.
+    const bool idle = D == 128 || tiles(1) < cus;
+    const bool split = (tiles(4) <= cus && steps >= 32 * (2 * cus / tiles(4))) ||
+                       (tiles(2) < cus && std::min(cus / tiles(4), steps / (idle ? 14 : 64)) > 1);
+    // Else four column groups, which read K and V least often, where about a workgroup of the longest row's average length is there for
+    // every CU (us, 8 kv heads of 2 q, two groups / four, head_dim 128: 4096 tokens behind 4096 242 / 219, behind 16384 691 / 588, 6000
+    // alone 181 / 160, but 2048 alone 38 / 46 and 4096 alone 91 / 95; head_dim 64: 4096 behind 4096 144 / 140, 2500 behind 5000 102 / 118),
+    // from half of that on where rows of few tokens fill what is left and one of the two reads more alone (head_dim 128, 16 such rows of
+    // 500 .. 3000 and 3000 tokens 83 / 75, 3 times 1024 47 / 42; head_dim 64, 2048 tokens 28.7 / 31.2). Else two where those give every
+    // CU work, or one, which at head_dim 128 leaves no room for a second workgroup and so none for other rows' (1500 tokens of 4 kv
+    // heads and four rows of 1000 .. 1500: one group 36.2, two 25.4; 1024 tokens alone: 18.7 by one, 26.6 by four, split).
+    const int64_t most = std::min<int64_t>(a->max_tokens > 0 ? std::min<int64_t>(a->max_tokens, N) : N, longest);
+    const double busy = (double)tiles(4) / cus * (1. - 0.5 * (double)most / (double)longest);
+    const bool beside = small && D == 128;
+    const int cg = split || busy >= (beside ? 0.5 : 1.05) ? 4 : tiles(2) >= cus || beside ? 2 : 1;
+    pc.few = small ? few : 0;
+    pc.splits = split ? kSlotsPerCu * cus / NKV : 0;
+    pc.least = kPreMinSteps, pc.one_split = kPreMinSteps;
+    pc.merge_cols = units(4) * NKV * (kChunkCols / 16) <= 2 * cus ? 8 : 16;
+    const int64_t chunk_slots = units(cg) * 2 <= pc.splits ? pc.splits : pc.splits + units(cg);
+    const int64_t merge_grid = pc.splits > 0 ? units(4) * NKV * (kChunkCols / pc.merge_cols) : 0;
+    const int64_t grid = (chunk_slots + split_slots) * NKV;
+    if (std::max(grid, merge_grid) > kMaxGrid) return BZ_ERR_SHAPE;
+    pc.slots = (int)chunk_slots;
+    static_assert(kPreThreads == kFewThreads, "all by one launch()");
+    using Both = void (*)(const PagedParams, const PagedParams);
+    const Both fns[2][2][3] = {{{paged_chunk_kernel<64, false, 1>, paged_chunk_kernel<64, false, 2>, paged_chunk_kernel<64, false, 4>},
+                                {paged_chunk_kernel<64, true, 1>, paged_chunk_kernel<64, true, 2>, paged_chunk_kernel<64, true, 4>}},
+                               {{paged_chunk_kernel<128, false, 1>, paged_chunk_kernel<128, false, 2>, paged_chunk_kernel<128, false, 4>},
+                                {paged_chunk_kernel<128, true, 1>, paged_chunk_kernel<128, true, 2>, paged_chunk_kernel<128, true, 4>}}};
+    rc = launch(fns[D == 128][f8][cg / 2], grid, pc, p);
+    if (rc != BZ_OK || merge_grid == 0) return rc;
+    const Fn merges[2][2] = {{paged_merge_kernel<64, false>, paged_merge_kernel<64, true>},
+                             {paged_merge_kernel<128, false>, paged_merge_kernel<128, true>}};
+    return launch(merges[D == 128][f8], merge_grid, pc);
   }
+  if (split_slots * NKV > kMaxGrid) return BZ_ERR_SHAPE;
   const Fn fns[2][2][3] = {
       {{paged_split_kernel<64, false, false, 1, kFewThreads>, paged_split_kernel<64, false, true, 1, kFewThreads>,
         paged_split_kernel<64, false, true, 2, kFewThreads>},
@@ -213,7 +230,7 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
         paged_split_kernel<128, false, true, 2, kFewThreads>},
        {paged_split_kernel<128, true, false, 1, kFewThreads>, paged_split_kernel<128, true, true, 1, kFewThreads>,
         paged_split_kernel<128, true, true, 2, kFewThreads>}}};
-  return launch(fns[D == 128][f8][alike ? 0 : cols == kWideCols ? 2 : 1], split_grid, p);
+  return launch(fns[D == 128][f8][alike ? 0 : cols == kWideCols ? 2 : 1], split_slots * NKV, p);
 }
 
 }  // extern "C"

@@ -91,18 +91,32 @@ struct F8Rows {
   uint32_t e;
 };
 
-// Grid slots * kv heads, a slot's heads side by side (workgroups go to the XCDs in turn, so with a multiple of 8 kv heads each head's
-// K and V pass through one XCD's L2 alone).
+// Grid (p.slots + few.slots) * kv heads, a slot's heads side by side (workgroups go to the XCDs in turn, so with a multiple of 8 kv heads each
+// head's K and V pass through one XCD's L2 alone). The first p.slots are the chunks'; the others do the split kernel's work on rows of few
+// tokens, from `few`, which fills the CUs that the last chunks leave idle (us, 8 kv heads of 2 q, head_dim 128: chunks of 500 and 400
+// tokens behind 3000 and six rows of 900 .. 5000: a launch of their own 68.5, behind the chunks 56, before them 75.9, in turn with them 64).
 // CG column groups, one a wave, times PG = 4 / CG position groups: 4 x 1 in steps of 64; with 2 x 2 and 1 x 4 a small chunk has
 // more workgroups and fewer steps, each position group taking every PG-th tile of 32, and the groups' accumulators meet in LDS. Only
 // 4 x 1 is split.
+//
+// Matrix and vector instructions of two waves a SIMD bound it (8192 tokens alone, 16 q and 8 kv heads, head_dim 128: FLOPS).
 template <int D, bool F8, int CG>
-__global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const PagedParams p) {
+__global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const PagedParams p, const PagedParams few) {
   constexpr int PG = 4 / CG, TP = PG == 1 ? kChunkStep : 32, NB = TP / 32, NQ = D / 16, ND = D / 32, COLS = CG * kPreWaveCols;
   constexpr int BL = TP / 16, UB = BL / CG;         // blocks of 16 positions of a tile, and those that a wave stages
   constexpr int WS = kWave / BL;                    // steps whose pages a wave holds
   using L = ChunkLds<D, TP>;
+  static_assert(split_floats<D, 1>() * 4 <= PG * L::kBytes, "the rows of few tokens use the same LDS");
+  // arrays of their own, and the steps' parity known at compile time: the compiler then sees that the reads of one do not
+  // depend on the loads in flight to another (it would wait for all of them)
+  __shared__ __align__(16) char k_even[PG * L::kBytes], k_odd[PG * L::kBytes], v_even[PG * L::kBytes], v_odd[PG * L::kBytes];
   const int at = (int)(blockIdx.x / (uint32_t)p.NKV), h = (int)blockIdx.x - at * p.NKV;
+  if (at >= p.slots) {
+    paged_split<D, F8, true, 1, kPreThreads>(few, at - p.slots, h, [&](int u) {
+      return reinterpret_cast<float*>(u == 0 ? k_even : u == 1 ? k_odd : u == 2 ? v_even : v_odd);
+    });
+    return;
+  }
   const PagedShare share = deal_paged<true, false, kChunkStep, 1>(p, COLS, at);
   if (share.b < 0) return;
   const PagedRow& row = share.row;
@@ -123,9 +137,6 @@ __global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const Paged
   const int n = min(cut.per, steps - j0);  // steps of this split
   auto pos_of = [&](int j) { return TP * (PG * (j0 + j) + pg); };
 
-  // arrays of their own, and the steps' parity known at compile time: the compiler then sees that the reads of one do not
-  // depend on the loads in flight to another (it would wait for all of them)
-  __shared__ __align__(16) char k_even[PG * L::kBytes], k_odd[PG * L::kBytes], v_even[PG * L::kBytes], v_odd[PG * L::kBytes];
   const int64_t khead = (int64_t)h * p.kv_sh, shead = (int64_t)h * p.sc_sh;
   const int pshift = p.rows.pshift, pmask = (1 << pshift) - 1;
   const Rsrc table = span_rsrc(p.rows.table + share.b * p.rows.table_st, p.rows.max_pages * 4);

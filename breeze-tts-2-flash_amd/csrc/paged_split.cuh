@@ -29,6 +29,7 @@ struct PagedParams {
   float scale_log2;             // scale * log2(e)
   int few;                      // the split kernel takes the rows of at most `few` new tokens, the chunk kernel the others
   int splits;                   // not dealt: splits of a row; dealt: splits of all rows together (0: rows are not split)
+  int slots;                    // slots in the grid of a dealt kernel
   int lanes;                    // workgroups of a kv head that run at once, where rows may better stay whole (0: they may not)
   int least, one_split;         // tiles of a split at least; up to one_split a row is not split
   int merge_cols;               // columns of a workgroup of the merge kernel
@@ -222,13 +223,15 @@ __device__ __forceinline__ void odd_columns(LongState<D>& st, const uint32_t (&v
   }
 }
 
-// Grid slots * kv heads, a slot's heads side by side; not dealt (DEAL false, rows taken to be alike): slot = row * splits + split,
+// The splits of rows of few tokens: slot `at` of kv head h; not dealt (DEAL false, rows taken to be alike): slot = row * splits + split,
 // one token a row. C sets of 16 columns a workgroup: two where rows have more than 16, so that K and V are read and converted once for
-// both.
-template <int D, bool F8, bool DEAL, int C, int NT>
-__global__ void __launch_bounds__(NT, 2) paged_split_kernel(const PagedParams p) {
+// both. acc_of(u): LDS of split_floats<D, C>() floats for wave u's sums.
+template <int D, int C>
+constexpr int split_floats() { return C * kLongCols * (D + 4); }  // (rows of D + 4: 16-byte stores without bank conflicts)
+
+template <int D, bool F8, bool DEAL, int C, int NT, class Acc>
+__device__ __forceinline__ void paged_split(const PagedParams& p, int at, int h, Acc acc_of) {
   constexpr int NW = NT / kWave, P = F8 ? 32 : 16, NS = P / 16, N = 4 * NS, NJ = D / 32, COLS = C * kLongCols;
-  const int at = (int)(blockIdx.x / (uint32_t)p.NKV), h = (int)blockIdx.x - at * p.NKV;
   const int tid = threadIdx.x, lane = tid % kWave, w = wave_uniform(tid / kWave), r = lane % 16, g = lane / 16;
   PagedShare share;
   if constexpr (DEAL) {
@@ -473,8 +476,8 @@ __global__ void __launch_bounds__(NT, 2) paged_split_kernel(const PagedParams p)
     }
   }
 
-  constexpr int PD = D + 4;  // keeps the 16-byte stores free of bank conflicts
-  __shared__ __align__(16) float s_acc[NW][COLS][PD];
+  constexpr int PD = D + 4;
+  float* const my_acc = acc_of(w);
   __shared__ float s_m[NW][COLS], s_l[NW][COLS];
 #pragma unroll
   for (int c = 0; c < C; ++c) {
@@ -491,7 +494,7 @@ __global__ void __launch_bounds__(NT, 2) paged_split_kernel(const PagedParams p)
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int q = 0; q < D / 16; q += 4)
-          *reinterpret_cast<f32x4_t*>(&s_acc[w][to][D / 16 * (4 * g + i) + q]) =
+          *reinterpret_cast<f32x4_t*>(my_acc + to * PD + D / 16 * (4 * g + i) + q) =
               f32x4_t{st[c].acc[q][i], st[c].acc[q + 1][i], st[c].acc[q + 2][i], st[c].acc[q + 3][i]};
       if (g == 0) {
         s_m[w][to] = st[c].m;
@@ -525,7 +528,7 @@ __global__ void __launch_bounds__(NT, 2) paged_split_kernel(const PagedParams p)
     for (int u = 0; u < NW; ++u) {
       const float f = fast_exp2(s_m[u][c] - mu);
       L = fmaf(f, s_l[u][c], L);
-      const f32x4_t a = *reinterpret_cast<const f32x4_t*>(&s_acc[u][c][d]);
+      const f32x4_t a = *reinterpret_cast<const f32x4_t*>(acc_of(u) + c * PD + d);
 #pragma unroll
       for (int i = 0; i < 4; ++i) A[i] = fmaf(f, a[i], A[i]);
     }
@@ -557,6 +560,14 @@ __global__ void __launch_bounds__(NT, 2) paged_split_kernel(const PagedParams p)
   __syncthreads();
   if (!s_last) return;
   merge_columns<D, NT>(p.part_acc + slot * COLS * D, p.part_ml + slot * COLS, COLS, ncol, nact, write);
+}
+
+// Grid slots * kv heads, a slot's heads side by side.
+template <int D, bool F8, bool DEAL, int C, int NT>
+__global__ void __launch_bounds__(NT, 2) paged_split_kernel(const PagedParams p) {
+  __shared__ __align__(16) float s_acc[NT / kWave][split_floats<D, C>()];
+  const int at = (int)(blockIdx.x / (uint32_t)p.NKV), h = (int)blockIdx.x - at * p.NKV;
+  paged_split<D, F8, DEAL, C, NT>(p, at, h, [&](int u) { return &s_acc[u][0]; });
 }
 
 }  // namespace
