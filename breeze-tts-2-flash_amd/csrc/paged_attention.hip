@@ -102,11 +102,11 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
     // Short chunks of few heads: the split kernel for all rows. It reads K and V again for each 16 columns, but in one launch (us, split
     // kernel / chunk kernels, 100 tokens alone 6.1 / 8.6, behind 1000 10 .. 14 / 17; 4 kv heads of 2 q, head_dim 128: 300 behind 1000 18.0 /
     // 19.5, 100 behind 6000 22.8 / 26.0, 300 behind 6000 50.9 / 29.8; 2 of 2: 1000 alone 14.9 / 16.0; head_dim 64, 4 of 2: 100 behind 1000
-    // 8.8 / 10.6, 300 12.0 / 11.8). At head_dim 128 from a little more on where the batch may have rows of few tokens as well: a few column
-    // tiles leave CUs idle, which its splits do not (300 behind 1000 and six rows of 600 .. 1300: 18.5 / 23.4; 60 twice behind 2000, 8
-    // bits, and two of 1000 .. 2000 19.3 / 25.7; head_dim 64: 700 tokens of 2 kv heads and four rows 11.3 / 8.8).
+    // 8.8 / 10.6, 300 12.0 / 11.8). Up to more columns where the batch may have rows of few tokens as well: a few column tiles leave CUs
+    // idle, which its splits do not (head_dim 128, 300 behind 1000 and six rows of 600 .. 1300 18.5 / 23.4, 60 twice behind 2000, 8 bits,
+    // and two of 1000 .. 2000 19.3 / 25.7; head_dim 64, 200 of 8 heads and four rows 6.2 / 6.9, 700 of 2 kv heads and four 11.1 / 8.9).
     const int64_t most = D == 128 ? 512 + (1 << 21) / length : 1280;
-    if (columns <= (B > 1 && D == 128 ? most + (5 << 19) / length : most)) cols = kLongCols;
+    if (columns <= (B > 1 ? most + (D == 128 ? 5 << 19 : 1 << 18) / length : most)) cols = kLongCols;
   } else if (cols == kWideCols && columns * length <= 5 << 19) {
     cols = kLongCols;  // (as few tiles: two sets of columns only make a workgroup slower, 2 rows of 20 tokens behind 500 9.0 / 12.0)
   }
@@ -160,7 +160,7 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
       // One round of workgroups, and two for a batch of many rows, whose splits are coarser (us, 8 kv heads of 2 q, head_dim 128, one round /
       // two: 32 rows of 512 .. 8192 of 8 bits 78 / 67, 64 of 128 .. 2048 56 / 52; 8 of 512 .. 8192 30.1 / 29.8; 4 of 1024 .. 16384 of 8 bits 18.7
       // / 21.0; three and four rounds take as long or longer).
-      const int64_t units = N / ((chunks ? kLongCols : cols) / G) + B;
+      const int64_t units = chunks ? B : N / (cols / G) + B;  // column tiles at most
       p.splits = n <= p.one_split ? 0 : (int)std::min<int64_t>(units * 2 > round ? 2 * round : round, p.part_slots / 2);
       p.lanes = units * 2 > round ? (int)round : 0;
       split_slots = units * 2 <= p.splits ? p.splits : p.splits + units;

@@ -94,7 +94,7 @@ struct F8Rows {
 // Grid (p.slots + few.slots) * kv heads, a slot's heads side by side (workgroups go to the XCDs in turn, so with a multiple of 8 kv heads each
 // head's K and V pass through one XCD's L2 alone). The first p.slots are the chunks'; the others do the split kernel's work on rows of few
 // tokens, from `few`, which fills the CUs that the last chunks leave idle (us, 8 kv heads of 2 q, head_dim 128: chunks of 500 and 400
-// tokens behind 3000 and six rows of 900 .. 5000: a launch of their own 68.5, behind the chunks 56, before them 75.9, in turn with them 64).
+// tokens behind 3000 and six rows of 900 .. 5000: a launch of their own 68.5, behind the chunks 54, before them 76, in turn with them 64).
 // CG column groups, one a wave, times PG = 4 / CG position groups: 4 x 1 in steps of 64; with 2 x 2 and 1 x 4 a small chunk has
 // more workgroups and fewer steps, each position group taking every PG-th tile of 32, and the groups' accumulators meet in LDS. Only
 // 4 x 1 is split.

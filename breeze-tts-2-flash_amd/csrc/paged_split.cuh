@@ -29,11 +29,11 @@ struct PagedParams {
   float scale_log2;             // scale * log2(e)
   int few;                      // the split kernel takes the rows of at most `few` new tokens, the chunk kernel the others
   int splits;                   // not dealt: splits of a row; dealt: splits of all rows together (0: rows are not split)
-  int slots;                    // slots in the grid of a dealt kernel
   int lanes;                    // workgroups of a kv head that run at once, where rows may better stay whole (0: they may not)
   int least, one_split;         // tiles of a split at least; up to one_split a row is not split
   int merge_cols;               // columns of a workgroup of the merge kernel
   int part_slots;               // splits of a kv head that the workspace has room for
+  int slots;                    // slots of the grid
   float* part_acc;              // [kv head, slot, column, D] unnormalised sums
   float2* part_ml;              // [kv head, slot, column] (max, sum)
   int* counters;                // [kv head, slot] x kCounterStride; the first slot of a column tile counts its splits
