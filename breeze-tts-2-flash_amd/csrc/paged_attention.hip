@@ -106,7 +106,7 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
     // idle, which its splits do not (head_dim 128, 300 behind 1000 and six rows of 600 .. 1300 18.5 / 23.4, 60 twice behind 2000, 8 bits,
     // and two of 1000 .. 2000 19.3 / 25.7; head_dim 64, 200 of 8 heads and four rows 6.2 / 6.9, 700 of 2 kv heads and four 11.1 / 8.9).
     const int64_t most = D == 128 ? 512 + (1 << 21) / length : 1280;
-    if (columns <= (B > 1 ? most + (D == 128 ? 5 << 19 : 1 << 18) / length : most)) cols = kLongCols;
+    if (columns <= (B > 1 ? most + (D == 128 ? 5 << 19 : 1 << 19) / length : most)) cols = kLongCols;
   } else if (cols == kWideCols && columns * length <= 5 << 19) {
     cols = kLongCols;  // (as few tiles: two sets of columns only make a workgroup slower, 2 rows of 20 tokens behind 500 9.0 / 12.0)
   }
@@ -135,9 +135,42 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
   p.counters = reinterpret_cast<int*>(base);
   p.part_ml = reinterpret_cast<float2*>(base + ws.split.ml);
   p.part_acc = reinterpret_cast<float*>(base + ws.split.acc);
+  // The chunk kernel's plan. Workgroups with g column groups (of all kv heads; without the tiles that rows' ends leave part empty), and
+  // its column tiles at most.
   const bool f8 = c->bits == 8;
-  // The split kernel's part, for rows of few tokens (all of them, if there are no others; else its work goes behind that of the chunk
-  // kernel, in one launch).
+  auto tiles = [&](int g) { return (N * G + kPreWaveCols * g - 1) / (kPreWaveCols * g) * NKV; };
+  auto units_of = [&](int g) { return N / (kPreWaveCols * g / G) + B; };
+  int cg = 0;
+  bool split = false, few_first = false;
+  if (chunks) {
+    const int64_t steps = longest / kChunkStep + 1;
+    // Few column tiles of 128 over many positions are split over those as well (us, 8 kv heads of 2 q, head_dim 128, whole / split: 1024
+    // tokens over 8192 105 / 82, 2048 over 16384 301 / 263, 256 over 8192 70 / 36); at head_dim 64, where one column group leaves
+    // room for two workgroups a CU, only over very many unless even that leaves CUs idle.
+    const bool idle = D == 128 || tiles(1) < cus;
+    split = (tiles(4) <= cus && steps >= 32 * (2 * cus / tiles(4))) ||
+            (tiles(2) < cus && std::min(cus / tiles(4), steps / (idle ? 14 : 64)) > 1);
+    // Else four column groups, which read K and V least often, where about a workgroup of the longest row's average length is there for
+    // every CU (us, 8 kv heads of 2 q, two groups / four, head_dim 128: 4096 tokens behind 4096 242 / 219, behind 16384 691 / 588, 6000
+    // alone 181 / 160, but 2048 alone 38 / 46 and 4096 alone 91 / 95; head_dim 64: 4096 behind 4096 144 / 140, 2500 behind 5000 102 / 118),
+    // from half of that on where rows of few tokens fill what is left and one of the two reads more alone (head_dim 128, 16 such rows of
+    // 500 .. 3000 and 3000 tokens 83 / 75, 3 times 1024 47 / 42; head_dim 64, 2048 tokens 28.7 / 31.2). Else two where those give every
+    // CU work, or one, which at head_dim 128 leaves no room for a second workgroup and so none for other rows' (1500 tokens of 4 kv
+    // heads and four rows of 1000 .. 1500: one group 36.2, two 25.4; 1024 tokens alone: 18.7 by one, 26.6 by four, split).
+    const int64_t most = std::min<int64_t>(a->max_tokens > 0 ? std::min<int64_t>(a->max_tokens, N) : N, longest);
+    const double busy = (double)tiles(4) / cus * (1. - 0.5 * (double)most / (double)longest);
+    const bool beside = small && D == 128;
+    cg = split || busy >= (beside ? 0.5 : 1.05) ? 4 : tiles(2) >= cus || beside ? 2 : 1;
+    // Rows of few tokens come behind the chunks, whose longest have to begin at once, and ahead of them where they are most of the work:
+    // an 8-bit batch's positions take about as long as 55 columns of chunks, bf16 ones as 110 (us, 8 kv heads of 2 q, head_dim 128, behind
+    // / ahead: 1000 tokens and 32 rows of 500 .. 4000 72.5 / 67.9, two of 512 and 60 of 100 .. 3000, 8 bits, 61 / 53, but 2048 and 16 of
+    // 500 .. 2000 50 / 60, and 500 and 16 of 900 .. 5000, which leave CUs without a row, 48.5 / 49.5). Splits are shorter than column
+    // tiles, and beside fewer of them those rows go on at the same time (500 behind 4500, 450 behind 2500 and six of 900 .. 5000 68 / 60,
+    // 1024 behind 1024 and 32 of 1000 .. 8000 144 / 126; head_dim 64, 4 kv heads of 4 q, 800 behind 4000 and six of 2000 .. 4800 44 / 48).
+    const int64_t share = (f8 ? 55 : 110) * B;
+    few_first = small && (split ? N * G <= 4 * share : N * G <= share && B * NKV >= cus);
+  }
+  // The split kernel's part, for rows of few tokens (all of them, if there are no others; else its work is in the chunk kernel's launch).
   // One token a row, and no dealing: two or three rows, taken to be alike, and batches of so many that rows may stay whole, whose
   // dealing takes each workgroup a look at all (us, 8 kv heads of 2 q, head_dim 128, dealt / whole: 256 rows of 50 .. 200 36.7 / 26.4, of
   // 500 .. 2000 209 / 207; 128 rows 18.8 / 16.2, 113 / 113). The longest row alone may take no longer than the batch does.
@@ -161,7 +194,8 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
       // two: 32 rows of 512 .. 8192 of 8 bits 78 / 67, 64 of 128 .. 2048 56 / 52; 8 of 512 .. 8192 30.1 / 29.8; 4 of 1024 .. 16384 of 8 bits 18.7
       // / 21.0; three and four rounds take as long or longer).
       const int64_t units = chunks ? B : N / (cols / G) + B;  // column tiles at most
-      p.splits = n <= p.one_split ? 0 : (int)std::min<int64_t>(units * 2 > round ? 2 * round : round, p.part_slots / 2);
+      const int64_t most = units * 2 > round ? 2 * round : few_first ? (round + 1) / 2 : round;  // (half beside a chunk's splits)
+      p.splits = n <= p.one_split ? 0 : (int)std::min<int64_t>(most, p.part_slots / 2);
       p.lanes = units * 2 > round ? (int)round : 0;
       split_slots = units * 2 <= p.splits ? p.splits : p.splits + units;
     }
@@ -177,44 +211,23 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
     PagedParams pc = p;
     pc.part_ml = reinterpret_cast<float2*>(base + ws.chunk.ml);
     pc.part_acc = reinterpret_cast<float*>(base + ws.chunk.acc);
-    // Workgroups of a chunk kernel with g column groups (of all kv heads; without the tiles that rows' ends leave part empty), and
-    // its column tiles at most.
-    auto tiles = [&](int g) { return (N * G + kPreWaveCols * g - 1) / (kPreWaveCols * g) * NKV; };
-    auto units = [&](int g) { return N / (kPreWaveCols * g / G) + B; };
-    const int64_t steps = longest / kChunkStep + 1;
-    // Few column tiles of 128 over many positions are split over those as well (us, 8 kv heads of 2 q, head_dim 128, whole / split: 1024
-    // tokens over 8192 105 / 82, 2048 over 16384 301 / 263, 256 over 8192 70 / 36); at head_dim 64, where one column group leaves
-    // room for two workgroups a CU, only over very many unless even that leaves CUs idle.
-    const bool idle = D == 128 || tiles(1) < cus;
-    const bool split = (tiles(4) <= cus && steps >= 32 * (2 * cus / tiles(4))) ||
-                       (tiles(2) < cus && std::min(cus / tiles(4), steps / (idle ? 14 : 64)) > 1);
-    // Else four column groups, which read K and V least often, where about a workgroup of the longest row's average length is there for
-    // every CU (us, 8 kv heads of 2 q, two groups / four, head_dim 128: 4096 tokens behind 4096 242 / 219, behind 16384 691 / 588, 6000
-    // alone 181 / 160, but 2048 alone 38 / 46 and 4096 alone 91 / 95; head_dim 64: 4096 behind 4096 144 / 140, 2500 behind 5000 102 / 118),
-    // from half of that on where rows of few tokens fill what is left and one of the two reads more alone (head_dim 128, 16 such rows of
-    // 500 .. 3000 and 3000 tokens 83 / 75, 3 times 1024 47 / 42; head_dim 64, 2048 tokens 28.7 / 31.2). Else two where those give every
-    // CU work, or one, which at head_dim 128 leaves no room for a second workgroup and so none for other rows' (1500 tokens of 4 kv
-    // heads and four rows of 1000 .. 1500: one group 36.2, two 25.4; 1024 tokens alone: 18.7 by one, 26.6 by four, split).
-    const int64_t most = std::min<int64_t>(a->max_tokens > 0 ? std::min<int64_t>(a->max_tokens, N) : N, longest);
-    const double busy = (double)tiles(4) / cus * (1. - 0.5 * (double)most / (double)longest);
-    const bool beside = small && D == 128;
-    const int cg = split || busy >= (beside ? 0.5 : 1.05) ? 4 : tiles(2) >= cus || beside ? 2 : 1;
     pc.few = small ? few : 0;
-    pc.splits = split ? kSlotsPerCu * cus / NKV : 0;
+    const int64_t all = kSlotsPerCu * cus / NKV;
+    pc.splits = split ? (int)(few_first && split_slots < all / 2 ? all - split_slots : all) : 0;
     pc.least = kPreMinSteps, pc.one_split = kPreMinSteps;
-    pc.merge_cols = units(4) * NKV * (kChunkCols / 16) <= 2 * cus ? 8 : 16;
-    const int64_t chunk_slots = units(cg) * 2 <= pc.splits ? pc.splits : pc.splits + units(cg);
-    const int64_t merge_grid = pc.splits > 0 ? units(4) * NKV * (kChunkCols / pc.merge_cols) : 0;
+    pc.merge_cols = units_of(4) * NKV * (kChunkCols / 16) <= 2 * cus ? 8 : 16;
+    const int64_t chunk_slots = units_of(cg) * 2 <= pc.splits ? pc.splits : pc.splits + units_of(cg);
+    const int64_t merge_grid = pc.splits > 0 ? units_of(4) * NKV * (kChunkCols / pc.merge_cols) : 0;
     const int64_t grid = (chunk_slots + split_slots) * NKV;
     if (std::max(grid, merge_grid) > kMaxGrid) return BZ_ERR_SHAPE;
     pc.slots = (int)chunk_slots;
     static_assert(kPreThreads == kFewThreads, "all by one launch()");
-    using Both = void (*)(const PagedParams, const PagedParams);
+    using Both = void (*)(const PagedParams, const PagedParams, const int);
     const Both fns[2][2][3] = {{{paged_chunk_kernel<64, false, 1>, paged_chunk_kernel<64, false, 2>, paged_chunk_kernel<64, false, 4>},
                                 {paged_chunk_kernel<64, true, 1>, paged_chunk_kernel<64, true, 2>, paged_chunk_kernel<64, true, 4>}},
                                {{paged_chunk_kernel<128, false, 1>, paged_chunk_kernel<128, false, 2>, paged_chunk_kernel<128, false, 4>},
                                 {paged_chunk_kernel<128, true, 1>, paged_chunk_kernel<128, true, 2>, paged_chunk_kernel<128, true, 4>}}};
-    rc = launch(fns[D == 128][f8][cg / 2], grid, pc, p);
+    rc = launch(fns[D == 128][f8][cg / 2], grid, pc, p, (int)few_first);
     if (rc != BZ_OK || merge_grid == 0) return rc;
     const Fn merges[2][2] = {{paged_merge_kernel<64, false>, paged_merge_kernel<64, true>},
                              {paged_merge_kernel<128, false>, paged_merge_kernel<128, true>}};

@@ -92,16 +92,15 @@ struct F8Rows {
 };
 
 // Grid (p.slots + few.slots) * kv heads, a slot's heads side by side (workgroups go to the XCDs in turn, so with a multiple of 8 kv heads each
-// head's K and V pass through one XCD's L2 alone). The first p.slots are the chunks'; the others do the split kernel's work on rows of few
-// tokens, from `few`, which fills the CUs that the last chunks leave idle (us, 8 kv heads of 2 q, head_dim 128: chunks of 500 and 400
-// tokens behind 3000 and six rows of 900 .. 5000: a launch of their own 68.5, behind the chunks 54, before them 76, in turn with them 64).
+// head's K and V pass through one XCD's L2 alone). p.slots are the chunks'; the others, behind them or (few_first) ahead, do the split
+// kernel's work on rows of few tokens, with the parameters `few`: in a launch of its own that work began when the last chunk had ended.
 // CG column groups, one a wave, times PG = 4 / CG position groups: 4 x 1 in steps of 64; with 2 x 2 and 1 x 4 a small chunk has
 // more workgroups and fewer steps, each position group taking every PG-th tile of 32, and the groups' accumulators meet in LDS. Only
 // 4 x 1 is split.
 //
 // Matrix and vector instructions of two waves a SIMD bound it (8192 tokens alone, 16 q and 8 kv heads, head_dim 128: FLOPS).
 template <int D, bool F8, int CG>
-__global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const PagedParams p, const PagedParams few) {
+__global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const PagedParams p, const PagedParams few, const int few_first) {
   constexpr int PG = 4 / CG, TP = PG == 1 ? kChunkStep : 32, NB = TP / 32, NQ = D / 16, ND = D / 32, COLS = CG * kPreWaveCols;
   constexpr int BL = TP / 16, UB = BL / CG;         // blocks of 16 positions of a tile, and those that a wave stages
   constexpr int WS = kWave / BL;                    // steps whose pages a wave holds
@@ -110,13 +109,15 @@ __global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const Paged
   // arrays of their own, and the steps' parity known at compile time: the compiler then sees that the reads of one do not
   // depend on the loads in flight to another (it would wait for all of them)
   __shared__ __align__(16) char k_even[PG * L::kBytes], k_odd[PG * L::kBytes], v_even[PG * L::kBytes], v_odd[PG * L::kBytes];
-  const int at = (int)(blockIdx.x / (uint32_t)p.NKV), h = (int)blockIdx.x - at * p.NKV;
-  if (at >= p.slots) {
-    paged_split<D, F8, true, 1, kPreThreads>(few, at - p.slots, h, [&](int u) {
+  int at = (int)(blockIdx.x / (uint32_t)p.NKV);
+  const int h = (int)blockIdx.x - at * p.NKV, before = few_first ? few.slots : 0;
+  if (few_first ? at < before : at >= p.slots) {
+    paged_split<D, F8, true, 1, kPreThreads>(few, few_first ? at : at - p.slots, h, [&](int u) {
       return reinterpret_cast<float*>(u == 0 ? k_even : u == 1 ? k_odd : u == 2 ? v_even : v_odd);
     });
     return;
   }
+  at -= before;
   const PagedShare share = deal_paged<true, false, kChunkStep, 1>(p, COLS, at);
   if (share.b < 0) return;
   const PagedRow& row = share.row;

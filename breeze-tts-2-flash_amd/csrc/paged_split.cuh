@@ -13,6 +13,8 @@
 
 namespace bz {
 
+// (Where the fields lie decides how many loads of arguments a kernel begins with: one more int in front of part_acc made every call of the
+// split kernel 0.3 us slower.)
 struct PagedParams {
   PagedRows rows;
   const uint16_t* q;

@@ -637,7 +637,8 @@ def test_two_streams_at_once(device):
         cases.append((q, cache, *b.args(), D ** -0.5, b.starts()))
     wants = [pkg.gqa_paged(*c) for c in cases]
     torch.cuda.synchronize()
-    streams = [torch.cuda.Stream() for _ in range(2)]
+    # a whole turn of torch's pool of 32, so that the streams of later tests, which may look at what a stream has kept, are what they were
+    streams = [torch.cuda.Stream() for _ in range(32)][:2]
     outs = []
     for turn_ in range(10):
         for i, s in enumerate(streams):
