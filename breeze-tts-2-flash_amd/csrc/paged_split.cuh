@@ -5,6 +5,15 @@
 // group's G heads. The row's positions are cut into wave tiles of 16 (bf16) or 32 (8-bit) of them, each in one page (or two, of 16),
 // and the tiles dealt to the row's splits and their waves in turn. Masks, the softmax and the products within a wave are
 // long_cache.cuh's.
+//
+// With running maximum m and sum l of a column (in units of log2: s = scale log2(e) q.k), a tile of scores s_p does
+//   m' = max(m, max s_p), t_p = 2^(s_p - m'), l' = 2^(m - m') l + sum t_p, O' = 2^(m - m') O + sum t_p v_p
+// and two parts of a row join the same way; out = O / l. Each t_p meets V as two bf16 terms, t = hi + lo, off by at most 2^-17 t.
+//
+// Reading K and V once bounds it (bf16, head_dim 128: 512 bytes a position and kv head, for 8 G flops a byte pair): 4 rows of up to 32768, 4
+// kv heads of 8 q, 229 MB in 39.5 us, 5.8 TB/s; 32 rows of 500 .. 8192 of 8 bits, 8 kv heads of 4 q, 289 MB in 59 us, 4.9 TB/s; 8 rows
+// of 700 .. 8192 with up to five tokens each, head_dim 64, 80 MB in 20.5. About 6 us of each are the launch, the lengths', table's and
+// first tiles' round trips and the merge; two rows of 1024 take 5.6, as gqa_decode does.
 #pragma once
 
 #include "bz_paged_cache.h"

@@ -9,7 +9,7 @@ token a row (flash/csrc/bb_attn.cu:416-429).
 The batch's tokens. `page_table` int32 [B, pages a row], `seq_lens` int32 [B] (with the new tokens) and `q_start` int32 [B + 1] say where
 the N tokens of a call belong: row b's are q_start[b] .. q_start[b + 1] - 1, the last positions of the row; position p lies in page
 page_table[b, p / page_size]. q_start None: one token a row. Tokens behind q_start[B] are a batch's padding: nothing of theirs is
-stored, and their rows of an output are left as they were. Page numbers outside the cache (-1) hold nothing. All three are read on
+stored, and their rows of an output are left as they were (in one that the call allocates, whatever its memory held). Page numbers outside the cache (-1) hold nothing. All three are read on
 the device, so a captured graph follows them.
 
 Workspaces: gqa_paged makes one for each device and stream on first use, for calls of all sizes. A call made while its stream is being
@@ -55,7 +55,7 @@ def paged_cache(pages: int, num_kv_heads: int, page_size: int, head_dim: int, de
 def paged_workspace(device: torch.device, head_dim: int, group: int, max_tokens: int = 0) -> torch.Tensor:
     """A new zero-filled workspace for gqa_paged, to be passed as workspace= (a captured graph keeps the one it was captured with, and
     graphs that share one must not run at the same time). group: q heads per kv head. max_tokens: what the calls pass, 1 for calls without
-    q_start; with at most 16 / group far less is needed."""
+    q_start; up to 16 / group a ninth of the bytes is needed, up to 64 / group a quarter."""
     device = torch.device(device)
     idx = device.index if device.index is not None else torch.cuda.current_device()
     n = ctypes.c_size_t(0)

@@ -65,7 +65,8 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freqs: Rope, out: torch.Tenso
     """x turned by its tokens' positions (bz_rope_apply). x: bf16 [tokens, heads, head_dim], head_dim 64 or 128, any strides that are
     multiples of 8 (q and k as views of a projection's output); positions: int32 or int64 [tokens]. out may be x itself. inverse
     turns back: rope(rope(x, p, f), p, f, inverse=True) is x but for two roundings, and keys move from position p to p' by
-    inverse and again. Angles are exact to 2^-30 turns for positions up to 2^22. Returns out."""
+    inverse and again. Angles are worked out and reduced to within half a turn in 64 bits (off by at most 2^-30 turns for positions up to 2^22), and
+    rounded to 32 there (2^-26). Returns out."""
     if torch.compiler.is_compiling():
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
         torch.ops.bz.rope(x, positions, freqs[0], float(freqs[1]), bool(freqs[2]), bool(inverse), out)

@@ -25,7 +25,7 @@ extern "C" {
 
 /* The cache and the batch's rows. K and V [pages, num_kv_heads, page_size, head_dim], sharing strides, the last dimension
    contiguous: bf16 (bits 16) or e4m3 codes (bits 8) with one scale byte E for each vector of head_dim, which stands for
-   2^(E - 127) (255: NaN, every value of the vector), in k_scale and v_scale uint8 [pages, num_kv_heads, page_size], sharing
+   2^(E - 127) (10 to 247 as the stores make them; 255: NaN, every value of the vector), in k_scale and v_scale uint8 [pages, num_kv_heads, page_size], sharing
    strides, the last dimension contiguous. Strides are in bytes; K, V and their strides are multiples of 16, scales and
    theirs of 4. page_size is a power of two from 16 to 1024, head_dim 64 or 128; a page of a head spans less than 2^30 bytes.
    page_table int32 [batch, max_pages], table_stride elements from row to row; max_pages * page_size at most 2^30. */
@@ -73,7 +73,8 @@ int bz_rope_apply(const bz_rope_args* args, hipStream_t stream);
    position in its row, or positions[n] if given; with q_norm_weight / k_norm_weight (bf16 [head_dim]) q / k are normed before
    that: x * rsqrt(mean(x^2) + eps) * weight. All of this is fp32, rounded once, to bf16 or into the 8-bit cache: the scale of a vector
    is the smallest power of two, from 2^-117, with max |x| <= 448 scale, its codes are x / scale rounded to the nearest e4m3 value
-   (ties to even); a vector that holds NaN or an infinity gets scale byte 255. Without rope, q must be NULL and the norms too. */
+   (ties to even; a value of 2^128 - 2^123 or more, under the largest scale, becomes 2^128, which reads as an infinity); a vector
+   that holds NaN or an infinity gets scale byte 255. Without rope, q must be NULL and the norms too. */
 typedef struct bz_paged_store_args {
   bz_paged_cache cache;
   const void *k, *v;
@@ -117,11 +118,12 @@ typedef struct bz_gqa_paged_args {
 /* Causal attention of the new tokens: out[n, h] = sum_p softmax_p(scale q[n, h] . k[p]) v[p] over the positions p of the token's
    row up to its own. A token that attends nothing, or whose scores are all -inf, yields zeros; what is stored at positions that a
    token does not attend (NaN and infinities among it) does not reach its output. Sums are fp32 (sum |V| over a token's positions
-   below 2^119, as in bz_long_cache.h); softmax terms meet V as two bf16 terms each where a row has few tokens (off by at most
-   2^-17 of themselves), as one in a chunk (2^-8, as the output's own rounding). */
+   below 2^119, as in bz_long_cache.h); softmax terms meet V as two bf16 terms each in a row of up to 64 / G tokens (off by at most
+   2^-17 of themselves) and where the batch's chunks are short, else as one (2^-8, as the output's own rounding). */
 int bz_gqa_paged(const bz_gqa_paged_args* args, hipStream_t stream);
 
-/* Workspace bytes of bz_gqa_paged calls with this head_dim: with max_tokens * group <= 16 (few tokens a row) far less. */
+/* Workspace bytes of bz_gqa_paged calls with this head_dim whose rows have up to max_tokens new tokens (0: any): at head_dim 128 and
+   256 CUs 8.8 MB with max_tokens * group <= 16, 17 MB up to 64, else 77 MB; at head_dim 64 half of that. */
 int bz_paged_workspace_size(int32_t head_dim, int32_t group, int32_t max_tokens, size_t* bytes);
 
 #ifdef __cplusplus
