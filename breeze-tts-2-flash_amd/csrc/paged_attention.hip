@@ -49,7 +49,7 @@ Layout layout(int cus, int D, int cols) {
 bool group_ok(int G) { return G == 1 || G == 2 || G == 4 || G == 8; }
 
 // Columns of a workgroup, by the most tokens of a row as far as the host knows: 16 or 32 of the split kernel up to 64 columns a row, else
-// 128 of the chunk kernel, with the split kernel's work in it for the batch's rows of at most 16 (us, 8 rows of 700 .. 8192, 8 kv heads,
+// 128 of the chunk kernel, with the split kernel's work in it for the batch's rows of few columns (us, 8 rows of 700 .. 8192, 8 kv heads,
 // head_dim 128, bf16 / 8 bits: 20 columns 32.9 / 30.6 by two sets of 16, 42.4 / 33.1 by 16 a workgroup, 56.1 / 58.7 by the chunk kernel;
 // 64 columns 48.1 / 41.6, 76.0 / 58.5, 57.1 / 61.0).
 constexpr int kWideCols = 2 * kLongCols, kSplitCols = 64;
@@ -91,7 +91,6 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
   if (rc != BZ_OK) return rc;
 
   const int64_t N = c->tokens, B = c->batch;
-  const int few = few_tokens(G);
   // Columns of a workgroup by the most tokens of a row, as far as the host knows; where the caller says that none has many, the split
   // kernel takes whatever comes, several column tiles a row.
   int cols = columns_of(G, c->q_start == nullptr ? 1 : a->max_tokens > 0 ? std::min<int64_t>(a->max_tokens, N) : N);
@@ -141,6 +140,7 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
   auto tiles = [&](int g) { return (N * G + kPreWaveCols * g - 1) / (kPreWaveCols * g) * NKV; };
   auto units_of = [&](int g) { return N / (kPreWaveCols * g / G) + B; };
   int cg = 0;
+  int few_tiles = 1;  // column tiles of 16 of the rows that count as few
   bool split = false, few_first = false;
   if (chunks) {
     const int64_t steps = longest / kChunkStep + 1;
@@ -161,6 +161,12 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
     const double busy = (double)tiles(4) / cus * (1. - 0.5 * (double)most / (double)longest);
     const bool beside = small && D == 128;
     cg = split || busy >= (beside ? 0.5 : 1.05) ? 4 : tiles(2) >= cus || beside ? 2 : 1;
+    // A row that the chunk kernel takes whole is one workgroup's long way through all its positions, mostly with columns of nobody where it
+    // has few tokens. So up to 64 columns count as few, unless the rows are so many, for their lengths, that reading K and V again for
+    // each 16 columns costs more (us, up to 16 columns / up to 64, head_dim 128, 8 kv heads of 8 q, 500 tokens and eight rows of five behind 4000 .. 8000 155 / 94, behind 500 .. 1000 31 /
+    // 34; 8 bits, 4 of 8, head_dim 64, 700 and four behind 500 .. 1000 18 / 13, behind 4500 47 / 17; 16 rows of 20, 8 of 2, 8 bits, behind
+    // 500 .. 1000 32 / 41, behind 3000 80 / 62; split: 700 and six of 30 behind 500 .. 3000 33 / 39).
+    if (!split && longest >= 20 * B * NKV) few_tiles = kSplitCols / kLongCols;
     // Rows of few tokens come behind the chunks, whose longest have to begin at once, and ahead of them where they are most of the work:
     // an 8-bit batch's positions take about as long as 55 columns of chunks, bf16 ones as 110 (us, 8 kv heads of 2 q, head_dim 128, behind
     // / ahead: 1000 tokens and 32 rows of 500 .. 4000 72.5 / 67.9, two of 512 and 60 of 100 .. 3000, 8 bits, 61 / 53, but 2048 and 16 of
@@ -181,7 +187,7 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
   if (small) {
     const int P = f8 ? 32 : 16;
     const int64_t n = (longest + P - 1) / P;
-    p.few = chunks ? few : INT32_MAX;
+    p.few = chunks ? few_tiles * few_tokens(G) : INT32_MAX;
     p.least = kFewThreads / kWave;
     p.one_split = kOneSplitBytes / row_bytes / P;
     const int64_t round = std::max<int64_t>(cus / NKV, 1);
@@ -193,7 +199,7 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
       // One round of workgroups, and two for a batch of many rows, whose splits are coarser (us, 8 kv heads of 2 q, head_dim 128, one round /
       // two: 32 rows of 512 .. 8192 of 8 bits 78 / 67, 64 of 128 .. 2048 56 / 52; 8 of 512 .. 8192 30.1 / 29.8; 4 of 1024 .. 16384 of 8 bits 18.7
       // / 21.0; three and four rounds take as long or longer).
-      const int64_t units = chunks ? B : N / (cols / G) + B;  // column tiles at most
+      const int64_t units = chunks ? few_tiles * B : N / (cols / G) + B;  // column tiles at most
       const int64_t most = units * 2 > round ? 2 * round : few_first ? (round + 1) / 2 : round;  // (half beside a chunk's splits)
       p.splits = n <= p.one_split ? 0 : (int)std::min<int64_t>(most, p.part_slots / 2);
       p.lanes = units * 2 > round ? (int)round : 0;
@@ -211,7 +217,7 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
     PagedParams pc = p;
     pc.part_ml = reinterpret_cast<float2*>(base + ws.chunk.ml);
     pc.part_acc = reinterpret_cast<float*>(base + ws.chunk.acc);
-    pc.few = small ? few : 0;
+    pc.few = small ? few_tiles * few_tokens(G) : 0;
     const int64_t all = kSlotsPerCu * cus / NKV;
     pc.splits = split ? (int)(few_first && split_slots < all / 2 ? all - split_slots : all) : 0;
     pc.least = kPreMinSteps, pc.one_split = kPreMinSteps;

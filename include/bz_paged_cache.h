@@ -118,8 +118,8 @@ typedef struct bz_gqa_paged_args {
 /* Causal attention of the new tokens: out[n, h] = sum_p softmax_p(scale q[n, h] . k[p]) v[p] over the positions p of the token's
    row up to its own. A token that attends nothing, or whose scores are all -inf, yields zeros; what is stored at positions that a
    token does not attend (NaN and infinities among it) does not reach its output. Sums are fp32 (sum |V| over a token's positions
-   below 2^119, as in bz_long_cache.h); softmax terms meet V as two bf16 terms each in a row of up to 64 / G tokens (off by at most
-   2^-17 of themselves) and where the batch's chunks are short, else as one (2^-8, as the output's own rounding). */
+   below 2^119, as in bz_long_cache.h); softmax terms meet V as two bf16 terms each in rows of up to 16 / G tokens (off by at most
+   2^-17 of themselves), in longer ones as two or as one (2^-8, as the output's own rounding). */
 int bz_gqa_paged(const bz_gqa_paged_args* args, hipStream_t stream);
 
 /* Workspace bytes of bz_gqa_paged calls with this head_dim whose rows have up to max_tokens new tokens (0: any): at head_dim 128 and

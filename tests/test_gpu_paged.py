@@ -372,6 +372,36 @@ def test_chunks(device, case, bits):
     check(out, q, k, v, b, D ** -0.5, G, False, "few")
 
 
+MIXED_CASES = {
+    # chunks and rows of few tokens in one launch; past, new
+    "whole": ([0, 300, 20], [1040, 1, 3]), "whole, many rows": ([0] + [17 * i for i in range(39)], [600] + [1, 2, 3] * 13),
+    "split": ([2500, 300], [900, 1]), "split, beside rows": ([2500, 300, 900], [400, 1, 1]), "four groups": ([0, 100], [2100, 1]),
+    "drafts": ([0, 3000, 2000, 3300], [700, 20, 32, 9]), "drafts, short": ([0] + [40] * 20, [900] + [20, 33] * 10),
+    "few in front": ([700, 0, 1500, 33], [2, 500, 8, 300]),
+}
+
+
+@pytest.mark.parametrize("case", MIXED_CASES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("bits", [8, 16])
+def test_mixed(device, case, D, bits):
+    past, new = MIXED_CASES[case]
+    rng = np.random.default_rng(len(new) + D)
+    b = Batch(rng, past, new, 32, 8, D, device, bits, spare=2)
+    cache, k, v = filled(b, rng)
+    q = randn(rng, b.N, 16, D)
+    out = torch.full((b.N, 16, D), 9.0, dtype=BF16, device=device)
+    table, lens = b.args()
+    pkg.gqa_paged(q.to(device), cache, table, lens, D ** -0.5, b.starts(), out, max_tokens=max(new), max_seq_len=max(b.lens))
+    torch.cuda.synchronize()
+    check(out, q, k, v, b, D ** -0.5, 2)
+    assert (out[b.q_start[-1]:] == 9).all()
+    for _ in range(3):  # the order in which workgroups end changes nothing
+        again = torch.full_like(out, 9.0)
+        pkg.gqa_paged(q.to(device), cache, table, lens, D ** -0.5, b.starts(), again, max_tokens=max(new), max_seq_len=max(b.lens))
+        assert torch.equal(again.view(torch.int16), out.view(torch.int16))
+
+
 @pytest.mark.parametrize("seed", range(60))
 def test_random_batches(device, seed):
     """Batches of any rows, page sizes, groups and hints, right or wrong."""
