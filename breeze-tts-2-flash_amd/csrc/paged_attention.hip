@@ -163,9 +163,10 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
     cg = split || busy >= (beside ? 0.5 : 1.05) ? 4 : tiles(2) >= cus || beside ? 2 : 1;
     // A row that the chunk kernel takes whole is one workgroup's long way through all its positions, mostly with columns of nobody where it
     // has few tokens. So up to 64 columns count as few, unless the rows are so many, for their lengths, that reading K and V again for
-    // each 16 columns costs more (us, up to 16 columns / up to 64, head_dim 128, 8 kv heads of 8 q, 500 tokens and eight rows of five behind 4000 .. 8000 155 / 94, behind 500 .. 1000 31 /
-    // 34; 8 bits, 4 of 8, head_dim 64, 700 and four behind 500 .. 1000 18 / 13, behind 4500 47 / 17; 16 rows of 20, 8 of 2, 8 bits, behind
-    // 500 .. 1000 32 / 41, behind 3000 80 / 62; split: 700 and six of 30 behind 500 .. 3000 33 / 39).
+    // each 16 columns costs more (us, up to 16 columns / up to 64, head_dim 128, 8 kv heads of 8 q: 500 tokens and eight rows of five
+    // behind 4000 .. 8000 155 / 94, behind 500 .. 1000 31 / 34; 8 bits, head_dim 64, 4 of 8: 700 and four of five behind 500 .. 1000 18 /
+    // 13, behind 4500 47 / 17; 8 bits, 8 of 2: 16 rows of 20 behind 500 .. 1000 32 / 41, behind 3000 80 / 62; beside splits, 700 and
+    // six of 30 behind 500 .. 3000 33 / 39).
     if (!split && longest >= 20 * B * NKV) few_tiles = kSplitCols / kLongCols;
     // Rows of few tokens come behind the chunks, whose longest have to begin at once, and ahead of them where they are most of the work:
     // an 8-bit batch's positions take about as long as 55 columns of chunks, bf16 ones as 110 (us, 8 kv heads of 2 q, head_dim 128, behind

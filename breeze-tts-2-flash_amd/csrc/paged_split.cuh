@@ -56,8 +56,6 @@ namespace {
 
 using bz::PagedParams;
 
-constexpr int kPagedCap = 1 << 30;
-
 // A row's new tokens (T of them from token q0 on) and length.
 struct PagedRow {
   int q0, T, len;

@@ -25,7 +25,8 @@ extern "C" {
 
 /* The cache and the batch's rows. K and V [pages, num_kv_heads, page_size, head_dim], sharing strides, the last dimension
    contiguous: bf16 (bits 16) or e4m3 codes (bits 8) with one scale byte E for each vector of head_dim, which stands for
-   2^(E - 127) (10 to 247 as the stores make them; 255: NaN, every value of the vector), in k_scale and v_scale uint8 [pages, num_kv_heads, page_size], sharing
+   2^(E - 127) (10 to 247 as the stores make them; 255: NaN, every value of the vector), in k_scale and v_scale uint8
+   [pages, num_kv_heads, page_size], sharing
    strides, the last dimension contiguous. Strides are in bytes; K, V and their strides are multiples of 16, scales and
    theirs of 4. page_size is a power of two from 16 to 1024, head_dim 64 or 128; a page of a head spans less than 2^30 bytes.
    page_table int32 [batch, max_pages], table_stride elements from row to row; max_pages * page_size at most 2^30. */
