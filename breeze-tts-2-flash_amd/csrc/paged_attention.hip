@@ -110,7 +110,6 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
     cols = kLongCols;  // (as few tiles: two sets of columns only make a workgroup slower, 2 rows of 20 tokens behind 500 9.0 / 12.0)
   }
   const bool chunks = cols == kChunkCols;
-  const bool small = !chunks || B > 1;  // (one row of unknown tokens may have few, but then the chunk kernel takes it)
   const Layout ws = layout(cus, D, cols);
   if (a->workspace == nullptr || a->workspace_bytes < ws.total) return BZ_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(a->workspace) & 255) return BZ_ERR_ALIGNMENT;
@@ -159,7 +158,7 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
     // heads and four rows of 1000 .. 1500: one group 36.2, two 25.4; 1024 tokens alone: 18.7 by one, 26.6 by four, split).
     const int64_t most = std::min<int64_t>(a->max_tokens > 0 ? std::min<int64_t>(a->max_tokens, N) : N, longest);
     const double busy = (double)tiles(4) / cus * (1. - 0.5 * (double)most / (double)longest);
-    const bool beside = small && D == 128;
+    const bool beside = B > 1 && D == 128;
     cg = split || busy >= (beside ? 0.5 : 1.05) ? 4 : tiles(2) >= cus || beside ? 2 : 1;
     // A row that the chunk kernel takes whole is one workgroup's long way through all its positions, mostly with columns of nobody where it
     // has few tokens. So up to 64 columns count as few, unless the rows are so many, for their lengths, that reading K and V again for
@@ -175,9 +174,11 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
     // tiles, and beside fewer of them those rows go on at the same time (500 behind 4500, 450 behind 2500 and six of 900 .. 5000 68 / 60,
     // 1024 behind 1024 and 32 of 1000 .. 8000 144 / 126; head_dim 64, 4 kv heads of 4 q, 800 behind 4000 and six of 2000 .. 4800 44 / 48).
     const int64_t share = (f8 ? 55 : 110) * B;
-    few_first = small && (split ? N * G <= 4 * share : N * G <= share && B * NKV >= cus);
+    few_first = B > 1 && (split ? N * G <= 4 * share : N * G <= share && B * NKV >= cus);
   }
   // The split kernel's part, for rows of few tokens (all of them, if there are no others; else its work is in the chunk kernel's launch).
+  // A batch of one row has that part too, as its tokens may be few and the others padding (us, 8 kv heads of 2 q, head_dim 128: one token
+  // behind 4000 in a batch of 300 13.4, by the chunk kernel 21.0; its slots without work cost a chunk at most 0.5 in 277, and 0.1 in 35).
   // One token a row, and no dealing: two or three rows, taken to be alike, and batches of so many that rows may stay whole, whose
   // dealing takes each workgroup a look at all (us, 8 kv heads of 2 q, head_dim 128, dealt / whole: 256 rows of 50 .. 200 36.7 / 26.4, of
   // 500 .. 2000 209 / 207; 128 rows 18.8 / 16.2, 113 / 113). The longest row alone may take no longer than the batch does.
@@ -185,27 +186,25 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
   const bool many = B * NKV >= 4 * cus && longest * row_bytes <= 4 * kOneSplitBytes * (B * NKV / (4 * cus));
   const bool alike = c->q_start == nullptr && (B <= 3 || many);
   int64_t split_slots = 0;
-  if (small) {
-    const int P = f8 ? 32 : 16;
-    const int64_t n = (longest + P - 1) / P;
-    p.few = chunks ? few_tiles * few_tokens(G) : INT32_MAX;
-    p.least = kFewThreads / kWave;
-    p.one_split = kOneSplitBytes / row_bytes / P;
-    const int64_t round = std::max<int64_t>(cus / NKV, 1);
-    if (alike) {
-      const int64_t most = (n + p.least - 1) / p.least;
-      p.splits = many || n <= p.one_split ? 1 : (int)std::max<int64_t>(std::min({round / B, most, (int64_t)64}), 1);
-      split_slots = B * p.splits;
-    } else {
-      // One round of workgroups, and two for a batch of many rows, whose splits are coarser (us, 8 kv heads of 2 q, head_dim 128, one round /
-      // two: 32 rows of 512 .. 8192 of 8 bits 78 / 67, 64 of 128 .. 2048 56 / 52; 8 of 512 .. 8192 30.1 / 29.8; 4 of 1024 .. 16384 of 8 bits 18.7
-      // / 21.0; three and four rounds take as long or longer).
-      const int64_t units = chunks ? few_tiles * B : N / (cols / G) + B;  // column tiles at most
-      const int64_t most = units * 2 > round ? 2 * round : few_first ? (round + 1) / 2 : round;  // (half beside a chunk's splits)
-      p.splits = n <= p.one_split ? 0 : (int)std::min<int64_t>(most, p.part_slots / 2);
-      p.lanes = units * 2 > round ? (int)round : 0;
-      split_slots = units * 2 <= p.splits ? p.splits : p.splits + units;
-    }
+  const int P = f8 ? 32 : 16;
+  const int64_t n = (longest + P - 1) / P;
+  p.few = chunks ? few_tiles * few_tokens(G) : INT32_MAX;
+  p.least = kFewThreads / kWave;
+  p.one_split = kOneSplitBytes / row_bytes / P;
+  const int64_t round = std::max<int64_t>(cus / NKV, 1);
+  if (alike) {
+    const int64_t most = (n + p.least - 1) / p.least;
+    p.splits = many || n <= p.one_split ? 1 : (int)std::max<int64_t>(std::min({round / B, most, (int64_t)64}), 1);
+    split_slots = B * p.splits;
+  } else {
+    // One round of workgroups, and two for a batch of many rows, whose splits are coarser (us, 8 kv heads of 2 q, head_dim 128, one round /
+    // two: 32 rows of 512 .. 8192 of 8 bits 78 / 67, 64 of 128 .. 2048 56 / 52; 8 of 512 .. 8192 30.1 / 29.8; 4 of 1024 .. 16384 of 8 bits 18.7
+    // / 21.0; three and four rounds take as long or longer).
+    const int64_t units = chunks ? few_tiles * B : N / (cols / G) + B;  // column tiles at most
+    const int64_t most = units * 2 > round ? 2 * round : few_first ? (round + 1) / 2 : round;  // (half beside a chunk's splits)
+    p.splits = n <= p.one_split ? 0 : (int)std::min<int64_t>(most, p.part_slots / 2);
+    p.lanes = units * 2 > round ? (int)round : 0;
+    split_slots = units * 2 <= p.splits ? p.splits : p.splits + units;
   }
   auto launch = [&](auto fn, int64_t blocks, const auto&... params) {
     hipLaunchKernelGGL(fn, dim3((unsigned)blocks), dim3(kFewThreads), 0, stream, params...);
@@ -218,7 +217,6 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
     PagedParams pc = p;
     pc.part_ml = reinterpret_cast<float2*>(base + ws.chunk.ml);
     pc.part_acc = reinterpret_cast<float*>(base + ws.chunk.acc);
-    pc.few = small ? few_tiles * few_tokens(G) : 0;
     const int64_t all = kSlotsPerCu * cus / NKV;
     pc.splits = split ? (int)(few_first && split_slots < all / 2 ? all - split_slots : all) : 0;
     pc.least = kPreMinSteps, pc.one_split = kPreMinSteps;

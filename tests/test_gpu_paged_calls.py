@@ -1,0 +1,67 @@
+"""GPU: calls of the paged cache's operators (include/bz_paged_cache.h) that their documentation allows, or that they refuse, beyond
+those of test_gpu_paged.py (whose batches, caches and bounds these use)."""
+import numpy as np
+import pytest
+import torch
+
+import breeze_tts_2_flash_amd as pkg
+from test_gpu_paged import BF16, Batch, check, filled, ints, randn
+
+pytestmark = pytest.mark.gpu
+
+
+def wide_table(b, pages):
+    """The batch's table with room for `pages` pages a row, none behind those it has."""
+    b.table = np.concatenate([b.table, np.full((len(b.new), pages - b.table.shape[1]), -1, np.int32)], 1)
+    return b
+
+
+# ----------------------------------------------------------------------------------- one row in a bucket of tokens
+
+@pytest.mark.parametrize("T,NKV,G,D,past", [(1, 8, 2, 128, 60), (1, 8, 2, 64, 60), (8, 8, 2, 128, 20), (2, 2, 8, 64, 60), (1, 8, 1, 128, 900),
+                                            (4, 8, 4, 128, 0)])
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("hint", [0, 300])
+def test_single_row_of_few_tokens_in_a_bucket(device, T, NKV, G, D, past, bits, hint):
+    """A row of up to 16 / G tokens meets V as two terms also where it is the only one and the rest is padding."""
+    rng = np.random.default_rng(T + D + past)
+    b = wide_table(Batch(rng, [past], [T], 16, NKV, D, device, bits, spare=300 - T), 256)
+    cache, k, v = filled(b, rng)
+    q = randn(rng, b.N, NKV * G, D)
+    out = torch.full((b.N, NKV * G, D), 9.0, dtype=BF16, device=device)
+    table, lens = b.args()
+    pkg.gqa_paged(q.to(device), cache, table, lens, D ** -0.5, b.starts(), out, max_tokens=hint)
+    torch.cuda.synchronize()
+    check(out, q, k, v, b, D ** -0.5, G, False)
+    assert (out[T:] == 9).all()
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_bucket_of_one_row_captured(device, bits):
+    """One captured step of 300 tokens' room, replayed with one token, a few, and all of them."""
+    rng = np.random.default_rng(bits)
+    NKV, G, D, N = 8, 2, 128, 300
+    b = wide_table(Batch(rng, [500], [N], 16, NKV, D, device, bits), 128)
+    cache, k, v = filled(b, rng)
+    q = randn(rng, N, NKV * G, D)
+    dq, out, ws = q.to(device), torch.zeros(N, NKV * G, D, dtype=BF16, device=device), pkg.paged_workspace(device, D, G)
+    table, lens = b.args()
+    starts = b.starts()
+    call = lambda o, **more: pkg.gqa_paged(dq, cache, table, lens, D ** -0.5, starts, o, **more)  # noqa: E731
+    call(out, workspace=ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(out, workspace=ws)
+    for n, T in ((61, 1), (800, 300), (33, 8), (0, 1), (700, 30), (700, 0), (64, 1)):
+        b.lens, b.new, b.q_start = [n], [T], [0, T]
+        lens.copy_(ints([n], device))
+        starts.copy_(ints([0, T], device))
+        out.fill_(9)
+        want = torch.full_like(out, 9.0)
+        graph.replay()
+        call(want)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        check(out, q, k, v, b, D ** -0.5, G)
+        assert (out[T:] == 9).all()
