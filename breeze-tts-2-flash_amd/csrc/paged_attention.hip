@@ -220,6 +220,7 @@ BZ_EXPORT int bz_gqa_paged(const bz_gqa_paged_args* a, hipStream_t stream) {
     const int64_t all = kSlotsPerCu * cus / NKV;
     pc.splits = split ? (int)(few_first && split_slots < all / 2 ? all - split_slots : all) : 0;
     pc.least = kPreMinSteps, pc.one_split = kPreMinSteps;
+    pc.lanes = 0;  // whether chunks are split was decided above, not by how many rows of few tokens stand beside them
     pc.merge_cols = units_of(4) * NKV * (kChunkCols / 16) <= 2 * cus ? 8 : 16;
     const int64_t chunk_slots = units_of(cg) * 2 <= pc.splits ? pc.splits : pc.splits + units_of(cg);
     const int64_t merge_grid = pc.splits > 0 ? units_of(4) * NKV * (kChunkCols / pc.merge_cols) : 0;

@@ -65,3 +65,23 @@ def test_bucket_of_one_row_captured(device, bits):
         assert torch.equal(out, want)
         check(out, q, k, v, b, D ** -0.5, G)
         assert (out[T:] == 9).all()
+
+
+# --------------------------------------------------------------------------------------- chunks beside many rows
+
+@pytest.mark.parametrize("past,new,NKV,G,D", [([8000] + [300] * 20, [1700] + [1] * 20, 8, 2, 128),
+                                              ([300] * 17 + [5000], [2] * 17 + [800], 4, 4, 128), ([9000] + [300] * 40, [1700] + [1] * 40, 8, 2, 64)])
+@pytest.mark.parametrize("bits", [8, 16])
+def test_a_chunk_is_split_beside_many_rows(device, past, new, NKV, G, D, bits):
+    """A chunk behind a long past is split over positions however many rows of few tokens the batch has: its splits' sums are in the
+    workspace (behind those of the rows of few tokens, which take a ninth of it)."""
+    rng = np.random.default_rng(len(past))
+    b = Batch(rng, past, new, 32, NKV, D, device, bits)
+    cache, k, v = filled(b, rng)
+    q = randn(rng, b.N, NKV * G, D)
+    table, lens = b.args()
+    ws = pkg.paged_workspace(device, D, G)
+    out = pkg.gqa_paged(q.to(device), cache, table, lens, D ** -0.5, b.starts(), max_tokens=max(new), max_seq_len=max(b.lens), workspace=ws)
+    torch.cuda.synchronize()
+    assert ws[ws.numel() // 2:].any()
+    check(out, q, k, v, b, D ** -0.5, G)
