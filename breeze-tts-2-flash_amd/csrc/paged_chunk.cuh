@@ -144,8 +144,9 @@ __global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const Paged
   const Rsrc table = span_rsrc(p.rows.table + share.b * p.rows.table_st, p.rows.max_pages * 4);
 
   // Lane i holds the page of block i of 16 positions, of the 64 blocks (WS steps) of this wave's tiles at hand: that of the block's
-  // first position, or of the last attended one where the block lies behind it. odd: the blocks without one; they are read from
-  // page 0 (any memory that is there) and attended by nobody.
+  // first position, or of the last attended one where the block lies behind it. odd: the blocks without one (-1); they are staged
+  // as zeros, through a span of no bytes, and attended by nobody (read from some page instead, a NaN there would send every column to
+  // paged_careful: 300 tokens behind 700 of 64 heads, a hole and page 0 not yet written, 6414 us in place of 24.5).
   int ids = 0;
   uint64_t odd = 0;
   auto fetch = [&](int j) __attribute__((always_inline)) {
@@ -154,7 +155,7 @@ __global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const Paged
   auto settle = [&]() __attribute__((always_inline)) {
     const bool there = (uint32_t)ids < (uint32_t)p.rows.pages;
     odd = __ballot(!there);
-    ids = there ? ids : 0;
+    ids = there ? ids : -1;
   };
   struct Pages {
     int id[UB];  // of the blocks that this wave stages
@@ -177,7 +178,7 @@ __global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const Paged
     const int p0 = pos_of(j);
 #pragma unroll
     for (int b = 0; b < UB; ++b) {
-      const Rsrc rsrc = span_rsrc((V ? p.v : p.k) + pages.id[b] * p.kv_sp + khead, p.page_bytes);
+      const Rsrc rsrc = span_rsrc((V ? p.v : p.k) + max(pages.id[b], 0) * p.kv_sp + khead, pages.id[b] < 0 ? 0 : p.page_bytes);
 #pragma unroll
       for (int u = 0; u < 16 / RPI; ++u) {
         const int row0 = 16 * (cg * UB + b) + RPI * u, rw = row0 + lane / CH, ch = lane % CH;
@@ -191,9 +192,10 @@ __global__ void __launch_bounds__(kPreThreads, 2) paged_chunk_kernel(const Paged
     constexpr bool V = decltype(isv)::value;
 #pragma unroll
     for (int b = 0; b < UB; ++b) {
-      const int64_t page = pages.id[b];
-      const Rsrc rsrc = span_rsrc((V ? p.v : p.k) + page * p.kv_sp + khead, p.page_bytes);
-      const Rsrc rs = span_rsrc((V ? p.vs : p.ks) + page * p.sc_sp + shead, pmask + 1);
+      const int64_t page = max(pages.id[b], 0);
+      const bool there = pages.id[b] >= 0;
+      const Rsrc rsrc = span_rsrc((V ? p.v : p.k) + page * p.kv_sp + khead, there ? p.page_bytes : 0);
+      const Rsrc rs = span_rsrc((V ? p.vs : p.ks) + page * p.sc_sp + shead, there ? pmask + 1 : 0);
       const int at = place(pos_of(j) + 16 * (cg * UB + b) + lane / 4);
 #pragma unroll
       for (int i = 0; i < D / 32; i += 2) {

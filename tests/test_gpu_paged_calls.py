@@ -85,3 +85,33 @@ def test_a_chunk_is_split_beside_many_rows(device, past, new, NKV, G, D, bits):
     torch.cuda.synchronize()
     assert ws[ws.numel() // 2:].any()
     check(out, q, k, v, b, D ** -0.5, G)
+
+
+# -------------------------------------------------------------------------------------------- holes in the table
+
+@pytest.mark.parametrize("past,new,page,NKV,G,D,hole", [
+    ([700], [300], 16, 8, 8, 128, 5), ([700, 40], [300, 90], 32, 8, 8, 64, 7), ([0], [150], 16, 8, 8, 64, 3), ([300], [110], 64, 8, 8, 128, 2),
+    ([3000], [110], 16, 8, 8, 128, 100), ([40], [300], 16, 8, 2, 128, 21)])
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("which", [-1, 1 << 20])
+def test_a_hole_is_not_read_from_another_page(device, past, new, page, NKV, G, D, hole, bits, which):
+    """What other pages hold (page 0 above all, and what an earlier call left behind on the chip) changes not a bit where the table has a
+    hole, neither -1 nor a number past the cache."""
+    rng = np.random.default_rng(D + hole)
+    b = Batch(rng, past, new, page, NKV, D, device, bits)
+    b.table = np.where(b.table >= 0, b.table + 1, -1).astype(np.int32)  # page 0 is nobody's
+    b.pages += 1
+    b.table[0, hole] = which
+    cache, k, v = filled(b, rng)  # NaN wherever no row lies: in page 0, and where the hole's page would be
+    q = randn(rng, b.N, NKV * G, D)
+    table, lens = b.args()
+    call = lambda c: pkg.gqa_paged(q.to(device), c, table, lens, D ** -0.5, b.starts())  # noqa: E731
+    call(pkg.PagedCache(*(None if x is None else x.clone().view(torch.uint8).fill_(255).view(x.dtype) for x in cache)))  # all NaN
+    out = call(cache)
+    torch.cuda.synchronize()
+    check(out, q, k, v, b, D ** -0.5, G, True)
+    clean = [x.clone() if x is not None else None for x in cache]
+    for x, z in zip(clean, (0, 0, 127, 127)):
+        if x is not None:
+            x.view(torch.uint8)[0] = z
+    assert torch.equal(call(pkg.PagedCache(*clean)), out)
