@@ -119,13 +119,15 @@ void fill_rows(PyObject* seq_lens, PyObject* q_start, int64_t N, const at::Devic
   c.tokens = (int32_t)N;
 }
 
+// True or False (or the ints 1 and 0): not whatever has a truth value, as texts do, and tensors at the price of a synchronisation.
 bool flag_arg(PyObject* o, const char* name) {
-  const int is = PyObject_IsTrue(o);
-  if (is < 0) {
+  if (o == Py_True || o == Py_False) return o == Py_True;
+  const long x = PyLong_CheckExact(o) ? PyLong_AsLong(o) : -1;
+  if (x != 0 && x != 1) {
     PyErr_Clear();
     throw Error{std::string(name) + " must be a bool"};
   }
-  return is != 0;
+  return x == 1;
 }
 
 // A Rope's inv_freq, factor and interleaved.

@@ -25,7 +25,7 @@ import torch
 from . import kernels
 from .attention import _check
 from .long_cache import _again
-from .rotary import Rope
+from .rotary import Rope, _flag
 
 
 class PagedCache(NamedTuple):
@@ -86,8 +86,8 @@ def rope_store(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: PagedCa
     rows (after an eviction, say). Everything is worked out in fp32 and rounded once. out may be q. Returns out, the turned q."""
     if torch.compiler.is_compiling():
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
-        torch.ops.bz.rope_store(q, k, v, *cache, page_table, seq_lens, freqs[0], float(freqs[1]), bool(freqs[2]), q_start, out,
-                                positions, q_norm_weight, k_norm_weight, float(eps))
+        torch.ops.bz.rope_store(q, k, v, *cache, page_table, seq_lens, freqs[0], float(freqs[1]), _flag(freqs[2], "interleaved"), q_start,
+                                out, positions, q_norm_weight, k_norm_weight, float(eps))
         return out
     ck, cv, ks, vs = cache
     return kernels.eager().rope_store(q, k, v, ck, cv, ks, vs, page_table, seq_lens, freqs[0], freqs[1], freqs[2], q_start, out,

@@ -60,6 +60,12 @@ def rope_frequencies(rotary_dim: int, base: float, device, *, interleaved: bool 
     return Rope(f.to(device), scale, interleaved)
 
 
+def _flag(x, name: str) -> bool:
+    """A flag of a traced call, refused where the binding refuses it."""
+    _check(isinstance(x, (bool, int)) and x in (0, 1), f"{name} must be a bool")
+    return bool(x)
+
+
 def rope(x: torch.Tensor, positions: torch.Tensor, freqs: Rope, out: torch.Tensor | None = None, *,
          inverse: bool = False) -> torch.Tensor:
     """x turned by its tokens' positions (bz_rope_apply). x: bf16 [tokens, heads, head_dim], head_dim 64 or 128, any strides that are
@@ -69,6 +75,6 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freqs: Rope, out: torch.Tenso
     rounded to 32 there (2^-26). Returns out."""
     if torch.compiler.is_compiling():
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
-        torch.ops.bz.rope(x, positions, freqs[0], float(freqs[1]), bool(freqs[2]), bool(inverse), out)
+        torch.ops.bz.rope(x, positions, freqs[0], float(freqs[1]), _flag(freqs[2], "interleaved"), _flag(inverse, "inverse"), out)
         return out
     return kernels.eager().rope(x, positions, freqs[0], freqs[1], freqs[2], inverse, out)

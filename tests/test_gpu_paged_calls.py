@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import breeze_tts_2_flash_amd as pkg
-from test_gpu_paged import BF16, Batch, check, filled, ints, randn
+from tests.test_gpu_paged import BF16, Batch, check, filled, ints, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -115,3 +115,31 @@ def test_a_hole_is_not_read_from_another_page(device, past, new, page, NKV, G, D
         if x is not None:
             x.view(torch.uint8)[0] = z
     assert torch.equal(call(pkg.PagedCache(*clean)), out)
+
+
+# --------------------------------------------------------------------------------------------------------- flags
+
+def test_flags_are_bools(device):
+    """inverse and interleaved: True, False, 1 or 0. Texts, lists and tensors are refused, eager or compiled, not taken for their truth."""
+    rng = np.random.default_rng(5)
+    b = Batch(rng, [10], [5], 16, 2, 64, device)
+    q, k, v = (randn(rng, 5, h, 64).to(device) for h in (4, 2, 2))
+    cache, (table, lens), st = b.cache(), b.args(), b.starts()
+    f = pkg.rope_frequencies(64, 1e4, device)
+    pos = torch.arange(5, device=device)
+    held = cache.k.clone()
+    for flag in ("no", "false", "", [], [0], None, 2, -1, 1.0, pos[1:2], pos[:1], 1 << 80):
+        for call in (lambda: pkg.rope(q, pos, f, inverse=flag), lambda: pkg.rope(q, pos, f._replace(interleaved=flag)),
+                     lambda: pkg.rope_store(q, k, v, cache, table, lens, f._replace(interleaved=flag), st)):
+            with pytest.raises(RuntimeError, match="must be a bool"):
+                call()
+    torch.cuda.synchronize()
+    assert torch.equal(cache.k, held)
+    for flag in (False, True):
+        assert torch.equal(pkg.rope(q, pos, f, inverse=flag), pkg.rope(q, pos, f, inverse=int(flag)))
+        assert torch.equal(pkg.rope(q, pos, f._replace(interleaved=flag)), pkg.rope(q, pos, f._replace(interleaved=int(flag))))
+    assert not torch.equal(pkg.rope(q, pos, f, inverse=True), pkg.rope(q, pos, f))
+    compiled = torch.compile(lambda x, flag: pkg.rope(x, pos, f, inverse=flag))
+    assert torch.equal(compiled(q, True), pkg.rope(q, pos, f, inverse=True))
+    with pytest.raises(Exception, match="must be a bool"):
+        compiled(q, "no")
