@@ -14,6 +14,8 @@
 
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "bz_paged_cache.h"
 #include "paged_common.cuh"
 
@@ -247,39 +249,44 @@ struct PagedLoadParams {
   const uint8_t *ks, *vs;
   int64_t sc_sp, sc_sh;
   const int32_t* starts;
-  int count;
+  int count, heads;
   uint16_t *ok, *ov;
   int64_t o_sb, o_sh, o_st;
 };
 
-// Token t of (row, head), 8 dims a lane of K and of V; grid (token chunks, heads, rows).
+// Token t of (row, head), 8 dims a lane of K and of V; grid (token chunks, heads, rows), of either of the latter up to kMaxGridYZ, whose
+// workgroups go on where there are more.
+constexpr int kMaxGridYZ = 65535;  // HIP's
 template <int D, bool F8>
 __global__ void __launch_bounds__(kPagedThreads) paged_load_kernel(const PagedLoadParams p) {
   constexpr int LPR = D / 8;
-  const int h = blockIdx.y, b = blockIdx.z;
   const int64_t t = (int64_t)blockIdx.x * (kPagedThreads / LPR) + threadIdx.x / LPR;
   const int c = threadIdx.x % LPR;
   if (t >= p.count) return;
-  const int64_t pos = p.starts[b] + t;
-  uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-  const int page = pos > INT32_MAX ? -1 : bz::page_of(p.rows, b, (int)pos);
-  if (page >= 0) {
-    const int at = (int)pos & ((1 << p.rows.pshift) - 1);
-    const int64_t off = page * p.kv_sp + h * p.kv_sh + at * p.kv_ss;
-    if constexpr (F8) {
-      const int64_t so = page * p.sc_sp + h * p.sc_sh + at;
-      const uint2 ck = *reinterpret_cast<const uint2*>(p.k + off + 8 * c), cv = *reinterpret_cast<const uint2*>(p.v + off + 8 * c);
-      const uint32_t ek = p.ks[so], ev = p.vs[so];
-      x[0] = bz::f8_values(ck, ek);
-      x[1] = bz::f8_values(cv, ev);
-    } else {
-      x[0] = *reinterpret_cast<const uint4*>(p.k + off + 16 * c);
-      x[1] = *reinterpret_cast<const uint4*>(p.v + off + 16 * c);
+  for (int b = blockIdx.z; b < p.rows.B; b += gridDim.z) {
+    const int64_t pos = p.starts[b] + t;
+    const int page = pos > INT32_MAX ? -1 : bz::page_of(p.rows, b, (int)pos);
+    for (int h = blockIdx.y; h < p.heads; h += gridDim.y) {
+      uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+      if (page >= 0) {
+        const int at = (int)pos & ((1 << p.rows.pshift) - 1);
+        const int64_t off = page * p.kv_sp + h * p.kv_sh + at * p.kv_ss;
+        if constexpr (F8) {
+          const int64_t so = page * p.sc_sp + h * p.sc_sh + at;
+          const uint2 ck = *reinterpret_cast<const uint2*>(p.k + off + 8 * c), cv = *reinterpret_cast<const uint2*>(p.v + off + 8 * c);
+          const uint32_t ek = p.ks[so], ev = p.vs[so];
+          x[0] = bz::f8_values(ck, ek);
+          x[1] = bz::f8_values(cv, ev);
+        } else {
+          x[0] = *reinterpret_cast<const uint4*>(p.k + off + 16 * c);
+          x[1] = *reinterpret_cast<const uint4*>(p.v + off + 16 * c);
+        }
+      }
+      const int64_t o = b * p.o_sb + h * p.o_sh + t * p.o_st + 8 * c;
+      *reinterpret_cast<uint4*>(p.ok + o) = x[0];
+      *reinterpret_cast<uint4*>(p.ov + o) = x[1];
     }
   }
-  const int64_t o = b * p.o_sb + h * p.o_sh + t * p.o_st + 8 * c;
-  *reinterpret_cast<uint4*>(p.ok + o) = x[0];
-  *reinterpret_cast<uint4*>(p.ov + o) = x[1];
 }
 
 bool aligned(const void* p, int64_t strides) { return !(reinterpret_cast<uintptr_t>(p) & 15) && !(strides & 7); }
@@ -409,16 +416,16 @@ BZ_EXPORT int bz_paged_load(const bz_paged_cache* c, const int32_t* starts, int3
   if (c == nullptr || starts == nullptr || k == nullptr || v == nullptr) return BZ_ERR_NULL;
   const int rc = bz::check_paged(c, false);
   if (rc != BZ_OK) return rc;
-  if (count <= 0 || count > kMaxPositions || c->batch > 65535 || c->num_kv_heads > 65535) return BZ_ERR_SHAPE;
+  if (count <= 0 || count > kMaxPositions) return BZ_ERR_SHAPE;
   if (!aligned(k, x_stride_b | x_stride_h | x_stride_t) || !aligned(v, 0) || (reinterpret_cast<uintptr_t>(starts) & 3))
     return BZ_ERR_ALIGNMENT;
   PagedLoadParams p{bz::paged_rows(c), static_cast<const char*>(c->k), static_cast<const char*>(c->v), c->stride_page,
                     c->stride_h, c->stride_s, static_cast<const uint8_t*>(c->k_scale), static_cast<const uint8_t*>(c->v_scale),
-                    c->scale_stride_page, c->scale_stride_h, starts, count, static_cast<uint16_t*>(k),
+                    c->scale_stride_page, c->scale_stride_h, starts, count, c->num_kv_heads, static_cast<uint16_t*>(k),
                     static_cast<uint16_t*>(v), x_stride_b, x_stride_h, x_stride_t};
   const int64_t per = kPagedThreads / (c->head_dim / 8), chunks = (count + per - 1) / per;
   if (chunks > kMaxGrid) return BZ_ERR_SHAPE;
-  const dim3 grid((unsigned)chunks, c->num_kv_heads, c->batch);
+  const dim3 grid((unsigned)chunks, std::min(c->num_kv_heads, kMaxGridYZ), std::min(c->batch, kMaxGridYZ));
   using Fn = void (*)(const PagedLoadParams);
   const Fn fns[2][2] = {{paged_load_kernel<64, false>, paged_load_kernel<64, true>},
                         {paged_load_kernel<128, false>, paged_load_kernel<128, true>}};

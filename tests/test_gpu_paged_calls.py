@@ -143,3 +143,29 @@ def test_flags_are_bools(device):
     assert torch.equal(compiled(q, True), pkg.rope(q, pos, f, inverse=True))
     with pytest.raises(Exception, match="must be a bool"):
         compiled(q, "no")
+
+
+# ---------------------------------------------------------------------------------------------------- many rows
+
+@pytest.mark.parametrize("rows,heads,D", [(65535, 1, 64), (65536, 1, 64), (70001, 2, 128), (2, 65537, 64)])
+@pytest.mark.parametrize("bits", [8, 16])
+def test_load_of_many_rows_and_heads(device, rows, heads, D, bits):
+    """As many rows as the stores and the attention take, each at a place of its own; rows without a page are zeros."""
+    pages = 3 if heads > 2 else 1000
+    gen = torch.Generator(device=device).manual_seed(rows)
+    cache = pkg.paged_cache(pages, heads, 16, D, device, torch.float8_e4m3fn if bits == 8 else BF16)
+    values = []
+    for i in range(2):
+        x = torch.randint(-15, 16, cache.k.shape, generator=gen, device=device).to(BF16)  # every value one of e4m3's
+        cache[i].copy_(x)
+        values.append(x)
+    table = torch.randint(-1, pages, (rows, 2), generator=gen, device=device, dtype=torch.int32)
+    starts = torch.randint(0, 30, (rows,), generator=gen, device=device, dtype=torch.int32)
+    k, v = pkg.paged_load(cache, table, starts, 3)
+    assert k.shape == (rows, heads, 3, D)
+    for t in range(3):
+        pos = (starts + t).long()
+        page = torch.where(pos < 32, table.gather(1, (pos // 16).clamp(max=1)[:, None])[:, 0], -1)
+        for out, x in ((k, values[0]), (v, values[1])):
+            want = x[page.clamp(min=0).long(), :, pos % 16].masked_fill(page[:, None, None] < 0, 0)
+            assert torch.equal(out[:, :, t], want)
