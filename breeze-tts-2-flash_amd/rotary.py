@@ -33,8 +33,8 @@ def rope_frequencies(rotary_dim: int, base: float, device, *, interleaved: bool 
       "linear"  every angle divided by factor (positions interpolated)
       "ntk"     base times factor^(R / (R - 2)), R = rotary_dim: the lowest frequency is divided by factor, the highest kept
       "yarn"    pairs that turn at least beta_fast times within the `trained` positions kept, those that turn at most beta_slow
-                times interpolated, between them (by pair number, from the floor of one bound to the ceiling of the other) a
-                mixture; cos and sin times 0.1 ln(factor) + 1 (Peng et al. 2023, sections 3.2 to 3.4)
+                times interpolated, between them (by pair number, from the floor of one bound to the ceiling of the other, within
+                0 and R - 1) a mixture; cos and sin times 0.1 ln(factor) + 1 (Peng et al. 2023, sections 3.2 to 3.4)
 
     rotary_dim: a multiple of 16 up to the head's dims."""
     _check(rotary_dim > 0 and rotary_dim % 16 == 0, f"rotary_dim must be a positive multiple of 16, got {rotary_dim}")
@@ -55,6 +55,8 @@ def rope_frequencies(rotary_dim: int, base: float, device, *, interleaved: bool 
         at = [rotary_dim * math.log(trained / (2 * math.pi * beta)) / (2 * math.log(base)) for beta in (beta_fast, beta_slow)]
         low, high = max(math.floor(at[0]), 0), min(math.ceil(at[1]), rotary_dim - 1)
         mix = ((torch.arange(rotary_dim // 2, dtype=torch.float64) - low) / max(high - low, 1e-3)).clamp(0, 1)
+        if at[1] <= 0:  # not even pair 0 turns more than beta_slow times
+            mix = torch.ones_like(f)
         f = f * (1 - mix) + f / factor * mix
         scale = 0.1 * math.log(factor) + 1
     return Rope(f.to(device), scale, interleaved)
