@@ -169,3 +169,34 @@ def test_load_of_many_rows_and_heads(device, rows, heads, D, bits):
         for out, x in ((k, values[0]), (v, values[1])):
             want = x[page.clamp(min=0).long(), :, pos % 16].masked_fill(page[:, None, None] < 0, 0)
             assert torch.equal(out[:, :, t], want)
+
+
+# ------------------------------------------------------------------------------------ each row by its own bound
+
+@pytest.mark.parametrize("seed", range(80))
+def test_random_batches_by_each_rows_bound(device, seed):
+    """Batches of any rows, page sizes, groups, holes and hints: rows of up to 16 / G tokens by the bound of two terms whatever the hint, all
+    of them where the hint gives the batch to the kernel for few tokens, and only the others by that of one."""
+    rng = np.random.default_rng(5000 + seed)
+    pick = lambda *a: a[rng.integers(len(a))]  # noqa: E731
+    D, bits, page, NKV, G = pick(64, 128), pick(8, 16), pick(16, 32, 64, 512), pick(1, 2, 3, 8), pick(1, 2, 4, 8)
+    rows = int(pick(1, 1, 2, 3, 6, 30))
+    new = [int(pick(0, 1, 1, 2, 5, rng.integers(1, 40), rng.integers(1, 200) if rows < 9 else 3)) for _ in range(rows)]
+    new[0] = max(new[0], 1)
+    past = [int(pick(0, rng.integers(0, 100), rng.integers(0, 1500))) for _ in range(rows)]
+    b = Batch(rng, past, new, page, NKV, D, device, bits, spare=int(pick(0, 2, 300)), first=int(rng.integers(0, 2)))
+    if rng.integers(2):
+        wide_table(b, b.table.shape[1] + 4096 // page)
+    for _ in range(int(pick(0, 0, 2))):  # a hole
+        b.table[rng.integers(rows), rng.integers(b.table.shape[1])] = -1
+    cache, k, v = filled(b, rng, spread=float(pick(1.0, 100.0)))
+    q = randn(rng, b.N, NKV * G, D)
+    out = torch.full((b.N, NKV * G, D), 9.0, dtype=BF16, device=device)
+    table, lens = b.args()
+    hint = int(pick(0, 0, max(new), 1, 10))
+    pkg.gqa_paged(q.to(device), cache, table, lens, D ** -0.5, b.starts(), out, max_tokens=hint,
+                  max_seq_len=int(pick(0, max(b.lens), 50, 100000)))
+    torch.cuda.synchronize()
+    few = 0 < min(hint or b.N, b.N) * G <= 64
+    check(out, q, k, v, b, D ** -0.5, G, False if few else None, str((past, new, page, NKV, G, D, bits, hint)))
+    assert (out[:b.q_start[0]] == 9).all() and (out[b.q_start[-1]:] == 9).all()
