@@ -10,10 +10,11 @@
 //   m' = max(m, max s_p), t_p = 2^(s_p - m'), l' = 2^(m - m') l + sum t_p, O' = 2^(m - m') O + sum t_p v_p
 // and two parts of a row join the same way; out = O / l. Each t_p meets V as two bf16 terms, t = hi + lo, off by at most 2^-17 t.
 //
-// Reading K and V once bounds it (bf16, head_dim 128: 512 bytes a position and kv head, for 8 G flops a byte pair): 4 rows of up to 32768, 4
-// kv heads of 8 q, 229 MB in 39.5 us, 5.8 TB/s; 32 rows of 500 .. 8192 of 8 bits, 8 kv heads of 4 q, 289 MB in 59 us, 4.9 TB/s; 8 rows
-// of 700 .. 8192 with up to five tokens each, head_dim 64, 80 MB in 20.5. About 6 us of each are the launch, the lengths', table's and
-// first tiles' round trips and the merge; two rows of 1024 take 5.6, as gqa_decode does.
+// Reading K and V once bounds it (bf16, head_dim 128: 512 bytes a position and kv head for 512 G flops, 768 G as V meets two terms; a
+// large product and a large copy meet at 244 flops a byte): 4 rows of up to 32768, 4 kv heads of 8 q, 229 MB in 39.5 us, 5.8 TB/s; 32
+// rows of 300 .. 8192 of 8 bits, 8 kv heads of 2 q, 289 MB in 59 us, 4.9 TB/s; 8 rows of 700 .. 8192 with up to five tokens each,
+// head_dim 64, 80 MB in 20.5. About 6 us of each are the launch, the lengths', table's and first tiles' round trips and the merge; two
+// rows of 1024 take 5.6, as gqa_decode does.
 #pragma once
 
 #include "bz_paged_cache.h"
@@ -276,7 +277,6 @@ __device__ __forceinline__ void paged_split(const PagedParams& p, int at, int h,
   const int j0 = share.split * NW + w, stride = nact * NW, count = j0 < n ? (n - j0 + stride - 1) / stride : 0;
 
   const Rsrc table = span_rsrc(p.rows.table + share.b * p.rows.table_st, p.rows.max_pages * 4);
-  constexpr bool TWO = NS == 2;
   int ids[NS];
   auto fetch = [&](int i0) {
     const int64_t pos = (int64_t)P * (j0 + (int64_t)(i0 + lane) * stride);

@@ -115,7 +115,8 @@ def gqa_paged(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor, seq_
     """Causal GQA attention of every row's new tokens over its pages (bz_gqa_paged): one token a row (a decode step), a few (a
     verified draft), a prompt's chunk, or all of these in one batch. q: bf16 [N, NH, D], NH / NKV of 1, 2, 4 or 8; a token at position
     p of its row attends [0, p]. max_tokens, max_seq_len: about the most new tokens and positions of a row, where known; they steer
-    the launch alone. A token that attends nothing gets zeros; nothing stored at positions a token does not attend reaches its
+    the launch, and with it the order of sums and whether softmax terms of rows of more than NKV 16 / NH tokens meet V as two bf16 terms or
+    as one. A token that attends nothing gets zeros; nothing stored at positions a token does not attend reaches its
     output. Returns out [N, NH, D]."""
     if torch.compiler.is_compiling():
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out

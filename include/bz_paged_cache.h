@@ -101,8 +101,9 @@ int bz_paged_load(const bz_paged_cache* cache, const int32_t* starts, int32_t co
 
 /* Arguments of bz_gqa_paged. q, out bf16 [tokens, num_q_heads, head_dim], q 16-byte aligned with strides of multiples of 8
    elements; q head h reads kv head h / G, G = num_q_heads / num_kv_heads of 1, 2, 4 or 8. max_tokens (0: unknown) and max_seq_len
-   (0: max_pages * page_size): about the most new tokens and positions of a row; they steer the launch and change no result but
-   the order of its sums. workspace: bz_paged_workspace_size bytes, 256-byte aligned, zero-filled once; it serves every later call
+   (0: max_pages * page_size): about the most new tokens and positions of a row, right or wrong. They steer the launch: they change
+   the order of a result's sums and, for rows of more than 16 / G tokens, whether softmax terms meet V as two bf16 terms or as one
+   (below). workspace: bz_paged_workspace_size bytes, 256-byte aligned, zero-filled once; it serves every later call
    of any sizes that needs no more, and two calls that share one must be ordered on one stream. */
 typedef struct bz_gqa_paged_args {
   bz_paged_cache cache;
@@ -120,7 +121,8 @@ typedef struct bz_gqa_paged_args {
    row up to its own. A token that attends nothing, or whose scores are all -inf, yields zeros; what is stored at positions that a
    token does not attend (NaN and infinities among it) does not reach its output. Sums are fp32 (sum |V| over a token's positions
    below 2^119, as in bz_long_cache.h); softmax terms meet V as two bf16 terms each in rows of up to 16 / G tokens (off by at most
-   2^-17 of themselves), in longer ones as two or as one (2^-8, as the output's own rounding). */
+   2^-17 of themselves), in longer ones as two or as one (2^-8, as the output's own rounding), by the batch's sizes and the hints;
+   max_tokens of up to 64 / G makes it two in all rows. */
 int bz_gqa_paged(const bz_gqa_paged_args* args, hipStream_t stream);
 
 /* Workspace bytes of bz_gqa_paged calls with this head_dim whose rows have up to max_tokens new tokens (0: any): at head_dim 128 and
