@@ -200,3 +200,44 @@ def test_random_batches_by_each_rows_bound(device, seed):
     few = 0 < min(hint or b.N, b.N) * G <= 64
     check(out, q, k, v, b, D ** -0.5, G, False if few else None, str((past, new, page, NKV, G, D, bits, hint)))
     assert (out[:b.q_start[0]] == 9).all() and (out[b.q_start[-1]:] == 9).all()
+
+
+# ------------------------------------------------------------------------------------------ many heads, many rows
+
+@pytest.mark.parametrize("past,new,spare,NKV,G,D,bits", [
+    ([50], [100], 0, 300, 1, 128, 8), ([50], [3], 97, 300, 1, 128, 8), ([700], [1], 99, 520, 1, 64, 16), ([9], [90], 30, 1100, 1, 64, 16),
+    ([5000], [100], 0, 200, 1, 64, 16), ([5000, 300], [100, 1], 0, 200, 1, 64, 16), ([5000], [2], 90, 200, 1, 64, 16),
+    ([4500], [30], 100, 130, 2, 128, 16)])
+def test_chunks_of_many_heads(device, past, new, spare, NKV, G, D, bits):
+    """Fewer splits a head than rows or column tiles, or none."""
+    rng = np.random.default_rng(NKV)
+    b = Batch(rng, past, new, 64, NKV, D, device, bits, spare=spare)
+    cache, k, v = filled(b, rng)
+    q = randn(rng, b.N, NKV * G, D)
+    out = torch.full((b.N, NKV * G, D), 9.0, dtype=BF16, device=device)
+    table, lens = b.args()
+    pkg.gqa_paged(q.to(device), cache, table, lens, D ** -0.5, b.starts(), out)
+    torch.cuda.synchronize()
+    check(out, q, k, v, b, D ** -0.5, G)
+    assert (out[b.q_start[-1]:] == 9).all()
+
+
+@pytest.mark.parametrize("rows,chunk,NKV,G,D", [(1100, 300, 2, 2, 64), (700, 0, 8, 1, 64), (300, 500, 8, 4, 128), (2500, 0, 1, 4, 64)])
+@pytest.mark.parametrize("bits", [8, 16])
+def test_ragged_batches_of_many_rows(device, rows, chunk, NKV, G, D, bits):
+    """Rows without tokens, of one, and of a few, in any order, beside a chunk or not."""
+    rng = np.random.default_rng(rows)
+    new = [int(x) for x in rng.integers(0, 4, rows)]
+    if chunk:
+        new[rows // 3] = chunk
+    past = [int(x) for x in rng.integers(0, 90, rows)]
+    past[rows // 2] = 2000
+    b = Batch(rng, past, new, 16, NKV, D, device, bits, spare=5)
+    cache, k, v = filled(b, rng)
+    q = randn(rng, b.N, NKV * G, D)
+    out = torch.full((b.N, NKV * G, D), 9.0, dtype=BF16, device=device)
+    table, lens = b.args()
+    pkg.gqa_paged(q.to(device), cache, table, lens, D ** -0.5, b.starts(), out)
+    torch.cuda.synchronize()
+    check(out, q, k, v, b, D ** -0.5, G)
+    assert (out[b.q_start[-1]:] == 9).all()
